@@ -302,6 +302,44 @@ int ifl_coupling_bwd(const float* z, const float* dzout, const float* dld, const
                      float eps, int branch, int c0, int n, float* dz, float* dh_ring, float* dlogs_part, int B, int h, int w,
                      int C, void* stream);
 
+/* ---- 8-bit blocks: activation checkpoints in 8 bits and products of 8-bit operands (no counterpart in the reference) ----
+ * Format: a row's values in blocks of 128 (the last may be shorter).  A block has one scale 2^e (E8M0 byte e + 127, scales[row *
+ * lds + block]); its codes (codes[row * ldc + column], one byte each) are OCP e4m3 or e5m2: with m = the largest finite |x| and
+ * F = 448 (e4m3) or 57344 (e5m2), e is the smallest integer >= -126 with m <= F 2^e, and a code is x 2^-e rounded to nearest
+ * even.  NaN is NaN; infinity is infinity in e5m2 and NaN in e4m3; neither counts for m.
+ *
+ * ifl_block8_quantize: x (IFL_T_*), element (r, c) at x + r row_stride + c col_stride, one of the two strides 1.  Bytes of a
+ * code row from `cols` to the next multiple of 16 (or ldc) are written as zeros.  rows = 0 does nothing.
+ * ifl_block8_dequantize: out[r * ldo + c] = code * 2^e (* chan[c] unless NULL), rounded once to otype.
+ * ifl_block8_matmul: out[m * ldo + n] = sum_k A[m][k] B[n][k] + bias[n] (bias may be NULL), A [M][K] and B [N][K] in 8-bit blocks,
+ * code rows 16-byte aligned (ld multiples of 16); sums in float32, rounded once to otype.
+ * ifl_block8_wgrad: dw[n * ldw + k] = chan[k] sum_m dy[m * ldy + n] A[m][k] (chan may be NULL) and db[n] = sum_m dy[m * ldy + n]; dw or
+ * db may be NULL.  Sums of exact products in float32, in an order that depends on the sizes only.  scratch:
+ * ifl_block8_wgrad_scratch_floats floats (NULL if 0).  M = 0 gives zeros.                                              */
+enum { IFL_T_F32 = 0, IFL_T_BF16 = 1, IFL_T_F16 = 2 };
+enum { IFL_Q_E4M3 = 0, IFL_Q_E5M2 = 1 };
+int ifl_block8_quantize(const void* x, int xtype, int64_t row_stride, int64_t col_stride, uint8_t* codes, int64_t ldc, uint8_t* scales,
+                        int64_t lds, int64_t rows, int64_t cols, int fmt, void* stream);
+int ifl_block8_dequantize(const uint8_t* codes, int64_t ldc, const uint8_t* scales, int64_t lds, int fmt, const float* chan, void* out,
+                          int otype, int64_t ldo, int64_t rows, int64_t cols, void* stream);
+int ifl_block8_matmul(const uint8_t* a, int64_t lda, const uint8_t* sa, int64_t lsa, int fa, const uint8_t* b, int64_t ldb,
+                      const uint8_t* sb, int64_t lsb, int fb, const void* bias, int btype, void* out, int otype, int64_t ldo,
+                      int64_t M, int64_t N, int64_t K, void* stream);
+int64_t ifl_block8_wgrad_scratch_floats(int64_t M, int64_t N, int64_t K);
+int ifl_block8_wgrad(const void* dy, int dytype, int64_t ldy, const uint8_t* codes, int64_t ldc, const uint8_t* scales, int64_t lds,
+                     int fmt, const float* chan, void* dw, int dwtype, int64_t ldw, void* db, int dbtype, float* scratch, int64_t M,
+                     int64_t N, int64_t K, void* stream);
+/* ActNorm + ReLU of the coupling networks (as ifl_an_relu_*) with an 8-bit checkpoint: v = relu(x + bias), y = v exp(logs) on
+ * ringed planes [B][h+2][w+2][C], C a multiple of 32, at most 1024.  codes [B][h+2][w+2][C] and scales [B][h+2][w+2][ceil(C/128)]
+ * receive v in 8-bit blocks (e4m3); a positive v never gets the code 0.  Interior pixels of x and dy are read; y, dx and the
+ * checkpoint are written whole, zeros on the ring.  The backward: dx = dy exp(logs) where the code is not 0, dbias = sum dx,
+ * dlogs = sum dy v8 exp(logs) over the pixels (partials: ifl_an_relu8_blocks * 2 C floats).                             */
+int64_t ifl_an_relu8_blocks(int B, int h, int w, int C);
+int ifl_an_relu8_fwd(const float* x, float* y, uint8_t* codes, uint8_t* scales, const float* bias, const float* logs, int B, int h,
+                     int w, int C, void* stream);
+int ifl_an_relu8_bwd(const float* dy, const uint8_t* codes, const uint8_t* scales, const float* logs, float* dx, float* dbias,
+                     float* dlogs, float* partials, int B, int h, int w, int C, void* stream);
+
 /* ---- gradient-enabled pass of one flow level (training: train.py:73,129 through FlowUpsamplerNet.encode) ----
  * Replaces, for the encode direction, what torch autograd does over FlowStep.normal_flow (FlowStep.py:114-151) in the
  * reference: ifl_train_level_fwd runs the level's steps and keeps the activations in the caller's buffers,

@@ -1,0 +1,179 @@
+// block8.h -- the 8-bit block format shared by block8.hip, matmul8.hip and wgrad8.hip.
+//
+// A row's values in blocks of 128 (the last may be shorter).  A block has one scale 2^e, stored as the E8M0 byte e + 127; its
+// codes are OCP e4m3 or e5m2:
+//     m = max finite |x|,   e = the smallest integer >= -126 with m <= F 2^e  (F = 448 = 1.75 2^8, or 57344 = 1.75 2^15),
+//     code = x 2^-e rounded to nearest even.
+// A power of two costs a floating code no precision, is exact to apply and to undo (a code times its scale is exact in bf16),
+// makes codes independent of how they were computed, and is what the scaled matrix instructions take (one byte per row and
+// 32 values).  |x| 2^-e <= F, so rounding never saturates.  NaN has the code NaN; infinity keeps its sign in e5m2 and is NaN in
+// e4m3, which has none; neither takes part in m, so the other values of the block are what they would be without it.
+#pragma once
+#include "ifl_common.h"
+
+#define B8_BLK 128
+
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+// element types at the boundary (IFL_T_*)
+template <int T> struct B8Type;
+template <> struct B8Type<IFL_T_F32> { typedef float type; };
+template <> struct B8Type<IFL_T_BF16> { typedef __bf16 type; };
+template <> struct B8Type<IFL_T_F16> { typedef _Float16 type; };
+static inline int b8_size(int t) { return t == IFL_T_F32 ? 4 : 2; }
+
+// 8 consecutive elements as floats; `left` of them exist.  VEC: 16-byte aligned.
+template <class T, bool VEC>
+__device__ __forceinline__ void b8_load8(const T* __restrict__ p, int left, float v[8]) {
+    if (VEC && left >= 8) {
+        if constexpr (sizeof(T) == 4) {
+            const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
+        } else {
+            typedef T T8 __attribute__((ext_vector_type(8)));
+            const T8 a = *(const T8*)p;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = (float)a[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < left ? (float)p[i] : 0.f;
+    }
+}
+
+template <class T, bool VEC>
+__device__ __forceinline__ void b8_store8(T* __restrict__ p, int left, const float v[8]) {
+    if (VEC && left >= 8) {
+        if constexpr (sizeof(T) == 4) {
+            const f32x4 a = {v[0], v[1], v[2], v[3]}, b = {v[4], v[5], v[6], v[7]};
+            *(f32x4*)p = a;
+            *(f32x4*)(p + 4) = b;
+        } else {
+            typedef T T8 __attribute__((ext_vector_type(8)));
+            T8 a;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) a[i] = (T)v[i];
+            *(T8*)p = a;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) if (i < left) p[i] = (T)v[i];
+    }
+}
+
+__device__ __forceinline__ bool b8_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
+
+// largest finite magnitude of 8 values, as its bits (magnitudes order as unsigned integers)
+__device__ __forceinline__ uint32_t b8_amax_bits(const float v[8]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t u = __float_as_uint(v[i]) & 0x7fffffffu;
+        m = max(m, u < 0x7f800000u ? u : 0u);
+    }
+    return m;
+}
+
+// maximum over groups of LANES neighbouring lanes (4, 8 or 16), in every lane: exchanges inside a row of 16 by DPP
+template <int LANES>
+__device__ __forceinline__ uint32_t b8_group_max(uint32_t m) {
+    m = max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0xB1, 0xf, 0xf, true));                        // lane ^ 1
+    m = max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0x4E, 0xf, 0xf, true));                        // lane ^ 2
+    if (LANES >= 8) m = max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0x141, 0xf, 0xf, true));       // mirror within 8
+    if (LANES >= 16) m = max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0x140, 0xf, 0xf, true));      // mirror within 16
+    return m;
+}
+
+// E8M0 byte of a block whose largest magnitude has these bits: its exponent, one more where the mantissa is over 1.75
+__device__ __forceinline__ int b8_scale_byte(uint32_t amax, int fmt) {
+    const int e = (int)((amax + 0x1fffffu) >> 23) - (fmt == IFL_Q_E4M3 ? 8 : 15);
+    return e < 1 ? 1 : e;
+}
+// 2^(127 - byte): what values are multiplied by before rounding (byte from b8_scale_byte: 1 .. 248)
+__device__ __forceinline__ float b8_inv_scale(int byte) { return __uint_as_float((uint32_t)(254 - byte) << 23); }
+// 2^(byte - 127) for any byte: 0 is 2^-127 (subnormal), 255 is NaN
+__device__ __forceinline__ float b8_scale(int byte) {
+    return __uint_as_float(byte == 0 ? 0x00400000u : byte == 255 ? 0x7fc00000u : (uint32_t)byte << 23);
+}
+
+// codes of 8 values already multiplied by 2^-e
+__device__ __forceinline__ i32x2 b8_encode8(const float v[8], int fmt) {
+    i32x2 r = {0, 0};
+    if (fmt == IFL_Q_E4M3) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            r[h] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * h], v[4 * h + 1], r[h], false);
+            r[h] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * h + 2], v[4 * h + 3], r[h], true);
+        }
+    } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            r[h] = __builtin_amdgcn_cvt_pk_bf8_f32(v[4 * h], v[4 * h + 1], r[h], false);
+            r[h] = __builtin_amdgcn_cvt_pk_bf8_f32(v[4 * h + 2], v[4 * h + 3], r[h], true);
+        }
+    }
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) odd |= !b8_finite(v[i]);
+    if (odd) {                                      // (what the conversion makes of infinities depends on a mode bit: set here)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (!b8_finite(v[i])) {
+                const uint32_t u = __float_as_uint(v[i]);
+                const uint32_t c = (u >> 24 & 0x80u) | ((fmt == IFL_Q_E4M3 || (u & 0x7fffffu)) ? 0x7fu : 0x7cu);
+                r[i >> 2] = (int)(((uint32_t)r[i >> 2] & ~(0xffu << 8 * (i & 3))) | c << 8 * (i & 3));
+            }
+        }
+    }
+    return r;
+}
+
+__device__ __forceinline__ void b8_decode4(int w, int fmt, float* v) {
+    const f32x2 a = fmt == IFL_Q_E4M3 ? __builtin_amdgcn_cvt_pk_f32_fp8(w, false) : __builtin_amdgcn_cvt_pk_f32_bf8(w, false);
+    const f32x2 b = fmt == IFL_Q_E4M3 ? __builtin_amdgcn_cvt_pk_f32_fp8(w, true) : __builtin_amdgcn_cvt_pk_f32_bf8(w, true);
+    v[0] = a[0]; v[1] = a[1]; v[2] = b[0]; v[3] = b[1];
+}
+
+// 8 codes of a row from column c on, `left` of them exist; VEC: 8-byte aligned
+template <bool VEC>
+__device__ __forceinline__ i32x2 b8_load_codes(const uint8_t* __restrict__ p, int left) {
+    if (VEC && left >= 8) return *(const i32x2*)p;
+    i32x2 r = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) if (i < left) r[i >> 2] |= (int)((uint32_t)p[i] << 8 * (i & 3));
+    return r;
+}
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+// 8 codes times their block's scale (a byte) as bf16: exact, as a code has at most 4 significant bits
+template <int FMT>
+__device__ __forceinline__ bf16x8 b8_bf16x8(int w0, int w1, int byte) {
+    const float s = __uint_as_float(byte == 0 ? 0x00400000u : (uint32_t)byte << 23);
+    if (byte == 255) w0 = w1 = 0x7f7f7f7f;                               // a scale that is NaN: codes that are
+    bf16x2 p[4];
+    if constexpr (FMT == IFL_Q_E4M3) {
+        p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, s, false); p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, s, true);
+        p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, s, false); p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, s, true);
+    } else {
+        p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w0, s, false); p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w0, s, true);
+        p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w1, s, false); p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w1, s, true);
+    }
+    bf16x8 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { r[2 * i] = p[i][0]; r[2 * i + 1] = p[i][1]; }
+    return r;
+}
+
+// dispatch on an element type: body sees `T`
+#define B8_DISPATCH(type, ...) \
+    do { if ((type) == IFL_T_F32) { typedef float T; __VA_ARGS__; } \
+         else if ((type) == IFL_T_BF16) { typedef __bf16 T; __VA_ARGS__; } \
+         else { typedef _Float16 T; __VA_ARGS__; } } while (0)
+
+static inline bool b8_type_ok(int t) { return t == IFL_T_F32 || t == IFL_T_BF16 || t == IFL_T_F16; }
+static inline bool b8_fmt_ok(int f) { return f == IFL_Q_E4M3 || f == IFL_Q_E5M2; }

@@ -1,0 +1,365 @@
+// block8.hip -- activations in 8-bit blocks: quantize, restore, and the coupling networks' ActNorm + ReLU whose backward pass
+// reads an 8-bit checkpoint instead of two float32 tensors.  All of it is bound by memory traffic: one pass over the data, a
+// block's maximum inside a group of 4, 8 or 16 lanes (8 values each), no LDS.
+#include "block8.h"
+
+namespace {
+
+// ------------------------------------------------------------------------------------------------ quantize, rows contiguous
+// Group of LANES lanes = one block of a row; kg (a power of two) groups side by side along a row, the rest along rows.  Four
+// rows per group are in flight at once: their loads are issued before the first is used.
+template <class T, int LANES, bool VEC>
+__global__ __launch_bounds__(256)
+void quantize_kernel(const T* __restrict__ x, int64_t rs, uint8_t* __restrict__ codes, int64_t ldc, uint8_t* __restrict__ scales,
+                     int64_t lds, int64_t rows, int cols, int pad, int wide, int kg_log, int fmt)
+{
+    constexpr int U = 4, GPB = 256 / LANES;
+    const int lane = threadIdx.x % LANES, grp = threadIdx.x / LANES;
+    const int gk = grp & ((1 << kg_log) - 1), gr = grp >> kg_log, rpb = GPB >> kg_log;
+    const int KB = (cols + B8_BLK - 1) / B8_BLK;
+    const int64_t step = (int64_t)gridDim.x * rpb;
+    for (int64_t r0 = (int64_t)blockIdx.x * rpb + gr; r0 < rows; r0 += U * step) {
+        for (int kb = gk; kb < KB; kb += 1 << kg_log) {
+            const int c = kb * B8_BLK + lane * 8;
+            float v[U][8];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t r = r0 + u * step;
+                b8_load8<T, VEC>(x + r * rs + c, r < rows ? cols - c : 0, v[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t r = r0 + u * step;
+                if (r >= rows) break;                                   // (the same for all lanes of a group)
+                const int sb = b8_scale_byte(b8_group_max<LANES>(b8_amax_bits(v[u])), fmt);
+                const float inv = b8_inv_scale(sb);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[u][i] *= inv;
+                const i32x2 w = b8_encode8(v[u], fmt);
+                uint8_t* q = codes + r * ldc + c;
+                if (wide && c + 8 <= pad) *(i32x2*)q = w;
+                else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) if (c + i < pad) q[i] = (uint8_t)((uint32_t)w[i >> 2] >> 8 * (i & 3));
+                }
+                if (lane == 0) scales[r * lds + kb] = (uint8_t)sb;
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ quantize, columns contiguous
+// x[r][c] at x + r + c * cs (a transposed view).  Workgroup = 64 rows x one block of 128 columns: lanes run along the rows
+// (contiguous in memory), a thread holds 32 columns of its row, the four threads of a row meet in LDS for the maximum and
+// write 32 code bytes each.
+template <class T>
+__global__ __launch_bounds__(256)
+void quantize_t_kernel(const T* __restrict__ x, int64_t cs, uint8_t* __restrict__ codes, int64_t ldc, uint8_t* __restrict__ scales,
+                       int64_t lds, int64_t rows, int cols, int pad, int wide, int fmt)
+{
+    __shared__ uint32_t red[4][64];
+    const int lr = threadIdx.x & 63, g = threadIdx.x >> 6;
+    const int64_t r = (int64_t)blockIdx.x * 64 + lr;
+    const int kb = blockIdx.y, c0 = kb * B8_BLK + g * 32;
+    const int64_t rc = r < rows ? r : rows - 1;
+    float v[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = c0 + i < cols ? (float)x[rc + (int64_t)(c0 + i) * cs] : 0.f;
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = max(m, b8_amax_bits(v + 8 * i));
+    red[g][lr] = m;
+    __syncthreads();
+    m = max(max(red[0][lr], red[1][lr]), max(red[2][lr], red[3][lr]));
+    if (r >= rows) return;
+    const int sb = b8_scale_byte(m, fmt);
+    const float inv = b8_inv_scale(sb);
+    uint8_t* q = codes + r * ldc + c0;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        i32x4 w;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float* u = v + 16 * j + 8 * h;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) u[i] *= inv;
+            const i32x2 e = b8_encode8(u, fmt);
+            w[2 * h] = e[0]; w[2 * h + 1] = e[1];
+        }
+        if (wide && c0 + 16 * j + 16 <= pad) *(i32x4*)(q + 16 * j) = w;
+        else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) if (c0 + 16 * j + i < pad) q[16 * j + i] = (uint8_t)((uint32_t)w[i >> 2] >> 8 * (i & 3));
+        }
+    }
+    if (g == 0) scales[r * lds + kb] = (uint8_t)sb;
+}
+
+// ------------------------------------------------------------------------------------------------ restore
+// out = code * 2^e (* chan[c]): a thread takes 8 columns, tpr (a power of two) threads along a row; four rows in flight.
+template <class T, bool VEC>
+__global__ __launch_bounds__(256)
+void dequantize_kernel(const uint8_t* __restrict__ codes, int64_t ldc, const uint8_t* __restrict__ scales, int64_t lds, int fmt,
+                       const float* __restrict__ chan, T* __restrict__ out, int64_t ldo, int64_t rows, int cols, int tpr_log)
+{
+    constexpr int U = 4;
+    const int rpb = 256 >> tpr_log;
+    const int64_t step = (int64_t)gridDim.x * rpb;
+    for (int64_t r0 = (int64_t)blockIdx.x * rpb + (threadIdx.x >> tpr_log); r0 < rows; r0 += U * step) {
+        for (int c = (threadIdx.x & ((1 << tpr_log) - 1)) * 8; c < cols; c += 8 << tpr_log) {
+            i32x2 w[U];
+            int sb[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t r = r0 + u * step;
+                w[u] = b8_load_codes<VEC>(codes + r * ldc + c, r < rows ? cols - c : 0);
+                sb[u] = r < rows ? scales[r * lds + c / B8_BLK] : 0;
+            }
+            float f[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = chan && c + i < cols ? chan[c + i] : 1.f;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t r = r0 + u * step;
+                if (r >= rows) break;
+                float v[8];
+                b8_decode4(w[u][0], fmt, v);
+                b8_decode4(w[u][1], fmt, v + 4);
+                const float s = b8_scale(sb[u]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) { v[i] *= s; if (chan) v[i] *= f[i]; }
+                b8_store8<T, VEC>(out + r * ldo + c, cols - c, v);
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ ActNorm + ReLU, 8-bit checkpoint
+// v = relu(x + bias), y = v exp(logs); the checkpoint is v in 8 bits, one scale per pixel and 128 channels.  v and not y: x +
+// bias is one rounded addition whatever computes it, so the codes do not hang on an exp's last bit, and the backward pass and the
+// next convolution's weight gradient multiply by exp(logs) in float32.  A positive v never gets the code 0 (the smallest
+// subnormal instead): the code's zeros ARE the ReLU's mask.  Ring pixels of y and of the codes are written as zeros.
+template <int LANES>
+__global__ __launch_bounds__(256)
+void an_relu8_fwd_kernel(const float* __restrict__ x, float* __restrict__ y, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
+                         const float* __restrict__ bias, const float* __restrict__ logs, uint32_t npx, int h2, int w2, int C, int kg)
+{
+    constexpr int GPB = 256 / LANES;
+    const int lane = threadIdx.x % LANES, grp = threadIdx.x / LANES;
+    const int KB = (C + B8_BLK - 1) / B8_BLK;
+    const int gk = grp % kg, gr = grp / kg, ppb = GPB / kg;             // kg groups per pixel, ppb pixels per pass
+    if (gr >= ppb) return;
+    const int c = gk * B8_BLK + lane * 8;
+    const bool here = c < C;                                             // (C is a multiple of 8)
+    float b[8], s[8];
+    b8_load8<float, false>(bias + (here ? c : 0), 8, b);
+    b8_load8<float, false>(logs + (here ? c : 0), 8, s);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[i] = expf(s[i]);
+    for (uint32_t p = blockIdx.x * ppb + gr; p < npx; p += gridDim.x * ppb) {
+        const uint32_t line = p / (uint32_t)w2, px = p - line * w2, py = line % (uint32_t)h2;
+        const bool inside = px > 0 && px < (uint32_t)w2 - 1 && py > 0 && py < (uint32_t)h2 - 1;
+        const int64_t o = (int64_t)p * C + c;
+        float v[8];
+        b8_load8<float, true>(x + o, here && inside ? 8 : 0, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float t = v[i] + b[i];
+            v[i] = here && inside && !(t <= 0.f) ? t : 0.f;              // (NaN stays NaN, as torch's relu leaves it)
+        }
+        const int sb = b8_scale_byte(b8_group_max<LANES>(b8_amax_bits(v)), IFL_Q_E4M3);
+        const float inv = b8_inv_scale(sb);
+        float q[8], r[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { q[i] = v[i] * inv; r[i] = v[i] == 0.f ? 0.f : v[i] * s[i]; }
+        i32x2 w = b8_encode8(q, IFL_Q_E4M3);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) if (v[i] > 0.f && ((uint32_t)w[i >> 2] >> 8 * (i & 3) & 0xffu) == 0u) w[i >> 2] |= 1 << 8 * (i & 3);
+        if (here) {
+            b8_store8<float, true>(y + o, 8, r);
+            *(i32x2*)(codes + o) = w;
+            if (lane == 0) scales[(int64_t)p * KB + gk] = (uint8_t)sb;
+        }
+    }
+}
+
+// dx = g s [code != 0];  part[blk][0:C] = sum g [..], part[blk][C:2C] = sum g v8 over the block's pixels (both still without
+// the factor s, which the reduction applies).  A block walks a contiguous range of pixels; a thread keeps its 8 channels.
+__global__ __launch_bounds__(256)
+void an_relu8_bwd_kernel(const float* __restrict__ g, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
+                         const float* __restrict__ logs, float* __restrict__ dx, float* __restrict__ part, uint32_t npx,
+                         uint32_t px_per_block, int h2, int w2, int C)
+{
+    extern __shared__ float sm[];                                        // [pixel lane][2][C]
+    const int lpp = C / 8, ppb = 256 / lpp, KB = (C + B8_BLK - 1) / B8_BLK;
+    const int pl = threadIdx.x / lpp, c = (threadIdx.x - pl * lpp) * 8;
+    float sg[8], sv[8], s[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { sg[i] = sv[i] = 0.f; s[i] = expf(logs[c + i]); }
+    const uint32_t end = min(npx, (blockIdx.x + 1) * px_per_block);
+    if (pl < ppb) {
+        for (uint32_t p = blockIdx.x * px_per_block + pl; p < end; p += ppb) {
+            const uint32_t line = p / (uint32_t)w2, px = p - line * w2, py = line % (uint32_t)h2;
+            const bool inside = px > 0 && px < (uint32_t)w2 - 1 && py > 0 && py < (uint32_t)h2 - 1;
+            const int64_t o = (int64_t)p * C + c;
+            float d[8], v[8], r[8];
+            b8_load8<float, true>(g + o, inside ? 8 : 0, d);
+            const i32x2 w = *(const i32x2*)(codes + o);
+            const float sc = b8_scale(scales[(int64_t)p * KB + c / B8_BLK]);
+            b8_decode4(w[0], IFL_Q_E4M3, v);
+            b8_decode4(w[1], IFL_Q_E4M3, v + 4);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float e = v[i] == 0.f ? 0.f : d[i];
+                r[i] = e * s[i];
+                sg[i] += e;
+                sv[i] = fmaf(e, v[i] * sc, sv[i]);
+            }
+            b8_store8<float, true>(dx + o, 8, r);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { sm[(pl * 2) * C + c + i] = sg[i]; sm[(pl * 2 + 1) * C + c + i] = sv[i]; }
+    }
+    __syncthreads();
+    for (int k = threadIdx.x; k < 2 * C; k += 256) {
+        float t = 0.f;
+        for (int i = 0; i < ppb; ++i) t += sm[i * 2 * C + k];
+        part[(int64_t)blockIdx.x * 2 * C + k] = t;
+    }
+}
+
+// out[k] = exp(logs[k mod C]) sum over blocks of part[blk][k]: a wave per k, blocks 64 apart per lane, then the lanes in a
+// fixed order
+__global__ __launch_bounds__(256)
+void an_relu8_reduce_kernel(const float* __restrict__ part, int nblk, const float* __restrict__ logs, float* __restrict__ dbias,
+                            float* __restrict__ dlogs, int C)
+{
+    const int k = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (k >= 2 * C) return;
+    float t = 0.f;
+    for (int b = lane; b < nblk; b += 64) t += part[(int64_t)b * 2 * C + k];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
+    if (lane == 0) { const int c = k < C ? k : k - C; (k < C ? dbias : dlogs)[c] = t * expf(logs[c]); }
+}
+
+int log2_up(int64_t n, int most) { int l = 0; while (l < most && (1 << l) < n) ++l; return l; }
+bool aligned(const void* p, int64_t stride_bytes, int a) { return (uintptr_t)p % a == 0 && stride_bytes % a == 0; }
+
+constexpr int AN8_BLOCKS = 1024;                                         // most blocks (partial sums) of the backward pass
+
+}  // namespace
+
+extern "C" int ifl_block8_quantize(const void* x, int xtype, int64_t row_stride, int64_t col_stride, uint8_t* codes, int64_t ldc,
+                                   uint8_t* scales, int64_t lds, int64_t rows, int64_t cols, int fmt, void* stream)
+{
+    IFL_CHECK_ARG(b8_type_ok(xtype), IFL_EINVAL, "block8_quantize: element type %d", xtype);
+    IFL_CHECK_ARG(b8_fmt_ok(fmt), IFL_EINVAL, "block8_quantize: format %d", fmt);
+    IFL_CHECK_ARG(rows >= 0 && cols >= 1 && cols <= 0x7ffffc00, IFL_EINVAL, "block8_quantize: %lld x %lld", (long long)rows, (long long)cols);
+    if (rows == 0) return 0;
+    const int KB = ifl_cdiv((int)cols, B8_BLK);
+    IFL_CHECK_ARG(x && codes && scales, IFL_EINVAL, "block8_quantize: null pointer");
+    IFL_CHECK_ARG(ldc >= cols && lds >= KB, IFL_EINVAL, "block8_quantize: row strides %lld, %lld for %lld columns", (long long)ldc, (long long)lds, (long long)cols);
+    IFL_CHECK_ARG(col_stride == 1 || row_stride == 1 || rows == 1, IFL_EINVAL, "block8_quantize: strides %lld, %lld: one of them has to be 1", (long long)row_stride, (long long)col_stride);
+    const int64_t pad64 = (cols + 15) / 16 * 16;
+    const int pad = (int)(pad64 < ldc ? pad64 : ldc);
+    const int es = b8_size(xtype);
+    hipStream_t st = (hipStream_t)stream;
+    if (col_stride != 1) {
+        const int64_t gx = (rows + 63) / 64;
+        IFL_CHECK_ARG(gx <= 0x7fffffff && KB <= 65535, IFL_ENOTSUP, "block8_quantize: transposed %lld x %lld", (long long)rows, (long long)cols);
+        B8_DISPATCH(xtype, hipLaunchKernelGGL(HIP_KERNEL_NAME(quantize_t_kernel<T>), dim3((unsigned)gx, KB), dim3(256), 0, st, (const T*)x, col_stride, codes, ldc, scales,
+                                              lds, rows, (int)cols, pad, (int)aligned(codes, ldc, 16), fmt));
+        IFL_LAUNCH_CHECK();
+        return 0;
+    }
+    const bool vec = aligned(x, row_stride * es, 16);
+    const int wide = aligned(codes, ldc, 8);
+    const int lanes = cols <= 32 ? 4 : cols <= 64 ? 8 : 16;
+    const int gpb_log = lanes == 4 ? 6 : lanes == 8 ? 5 : 4;
+    const int kgl = log2_up(KB, gpb_log);
+    const int64_t rpb = 1 << (gpb_log - kgl);
+    int64_t grid = (rows + 4 * rpb - 1) / (4 * rpb);
+    if (grid < 1024) grid = (rows + rpb - 1) / rpb < 1024 ? (rows + rpb - 1) / rpb : 1024;      // few rows: spread them before stacking them
+    if (grid > 65536) grid = 65536;
+#define Q8_GO(L, V) hipLaunchKernelGGL(HIP_KERNEL_NAME(quantize_kernel<T, L, V>), dim3((unsigned)grid), dim3(256), 0, st, (const T*)x, row_stride, codes, ldc, scales, lds, rows, (int)cols, pad, wide, kgl, fmt)
+#define Q8_LANES(V) do { if (lanes == 4) Q8_GO(4, V); else if (lanes == 8) Q8_GO(8, V); else Q8_GO(16, V); } while (0)
+    B8_DISPATCH(xtype, if (vec) Q8_LANES(true); else Q8_LANES(false));
+    IFL_LAUNCH_CHECK();
+    return 0;
+}
+
+extern "C" int ifl_block8_dequantize(const uint8_t* codes, int64_t ldc, const uint8_t* scales, int64_t lds, int fmt, const float* chan,
+                                     void* out, int otype, int64_t ldo, int64_t rows, int64_t cols, void* stream)
+{
+    IFL_CHECK_ARG(b8_type_ok(otype), IFL_EINVAL, "block8_dequantize: element type %d", otype);
+    IFL_CHECK_ARG(b8_fmt_ok(fmt), IFL_EINVAL, "block8_dequantize: format %d", fmt);
+    IFL_CHECK_ARG(rows >= 0 && cols >= 1 && cols <= 0x7ffffc00, IFL_EINVAL, "block8_dequantize: %lld x %lld", (long long)rows, (long long)cols);
+    if (rows == 0) return 0;
+    IFL_CHECK_ARG(codes && scales && out, IFL_EINVAL, "block8_dequantize: null pointer");
+    IFL_CHECK_ARG(ldc >= cols && ldo >= cols && lds >= ifl_cdiv((int)cols, B8_BLK), IFL_EINVAL, "block8_dequantize: row strides");
+    const bool vec = aligned(codes, ldc, 8) && aligned(out, ldo * b8_size(otype), 16);
+    const int tl = log2_up((cols + 7) / 8, 8);
+    const int64_t rpb = 256 >> tl;
+    int64_t grid = (rows + 4 * rpb - 1) / (4 * rpb);
+    if (grid < 1024) grid = (rows + rpb - 1) / rpb < 1024 ? (rows + rpb - 1) / rpb : 1024;
+    if (grid > 65536) grid = 65536;
+#define D8_GO(V) hipLaunchKernelGGL(HIP_KERNEL_NAME(dequantize_kernel<T, V>), dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, codes, ldc, scales, lds, fmt, chan, (T*)out, ldo, rows, (int)cols, tl)
+    B8_DISPATCH(otype, if (vec) D8_GO(true); else D8_GO(false));
+    IFL_LAUNCH_CHECK();
+    return 0;
+}
+
+static int an_relu8_check(const char* what, int B, int h, int w, int C)
+{
+    IFL_CHECK_ARG(B >= 1 && h >= 1 && w >= 1, IFL_EINVAL, "%s: bad shape %d x %d x %d", what, B, h, w);
+    IFL_CHECK_ARG(C >= 32 && C % 32 == 0 && C <= 1024, IFL_ENOTSUP, "%s: C=%d (a multiple of 32, at most 1024)", what, C);
+    IFL_CHECK_ARG((int64_t)B * (h + 2) * (w + 2) <= 0x7fffffff - 65536 * 64, IFL_ENOTSUP, "%s: more than 2^31 pixels", what);
+    return 0;
+}
+
+extern "C" int ifl_an_relu8_fwd(const float* x, float* y, uint8_t* codes, uint8_t* scales, const float* bias, const float* logs, int B,
+                                int h, int w, int C, void* stream)
+{
+    if (int rc = an_relu8_check("an_relu8_fwd", B, h, w, C)) return rc;
+    IFL_CHECK_ARG(x && y && codes && scales && bias && logs, IFL_EINVAL, "an_relu8_fwd: null pointer");
+    IFL_CHECK_ARG(aligned(x, 0, 16) && aligned(y, 0, 16) && aligned(codes, 0, 8), IFL_EINVAL, "an_relu8_fwd: alignment");
+    const uint32_t npx = (uint32_t)B * (h + 2) * (w + 2);
+    const int lanes = C <= 32 ? 4 : C <= 64 ? 8 : 16, kg = ifl_cdiv(C, B8_BLK), ppb = 256 / lanes / kg;
+    uint32_t grid = (npx + ppb - 1) / ppb;
+    if (grid > 8192) grid = 8192;
+#define AN8_GO(L) hipLaunchKernelGGL(HIP_KERNEL_NAME(an_relu8_fwd_kernel<L>), dim3(grid), dim3(256), 0, (hipStream_t)stream, x, y, codes, scales, bias, logs, npx, h + 2, w + 2, C, kg)
+    if (lanes == 4) AN8_GO(4); else if (lanes == 8) AN8_GO(8); else AN8_GO(16);
+    IFL_LAUNCH_CHECK();
+    return 0;
+}
+
+static uint32_t an_relu8_px_per_block(uint32_t npx, int C)
+{
+    const uint32_t ppb = 256 / (C / 8);
+    const uint32_t p = (npx + AN8_BLOCKS - 1) / AN8_BLOCKS;
+    return (p + ppb - 1) / ppb * ppb;
+}
+
+extern "C" int64_t ifl_an_relu8_blocks(int B, int h, int w, int C)
+{
+    if (an_relu8_check("an_relu8_blocks", B, h, w, C)) return 0;
+    const uint32_t npx = (uint32_t)B * (h + 2) * (w + 2), p = an_relu8_px_per_block(npx, C);
+    return (npx + p - 1) / p;
+}
+
+extern "C" int ifl_an_relu8_bwd(const float* dy, const uint8_t* codes, const uint8_t* scales, const float* logs, float* dx, float* dbias,
+                                float* dlogs, float* partials, int B, int h, int w, int C, void* stream)
+{
+    if (int rc = an_relu8_check("an_relu8_bwd", B, h, w, C)) return rc;
+    IFL_CHECK_ARG(dy && codes && scales && logs && dx && dbias && dlogs && partials, IFL_EINVAL, "an_relu8_bwd: null pointer");
+    IFL_CHECK_ARG(aligned(dy, 0, 16) && aligned(dx, 0, 16) && aligned(codes, 0, 8), IFL_EINVAL, "an_relu8_bwd: alignment");
+    const uint32_t npx = (uint32_t)B * (h + 2) * (w + 2), ppx = an_relu8_px_per_block(npx, C);
+    const int nblk = (int)((npx + ppx - 1) / ppx);
+    const int sm = 256 / (C / 8) * 2 * C * 4;
+    hipLaunchKernelGGL(an_relu8_bwd_kernel, dim3(nblk), dim3(256), sm, (hipStream_t)stream, dy, codes, scales, logs, dx, partials, npx, ppx, h + 2, w + 2, C);
+    IFL_LAUNCH_CHECK();
+    hipLaunchKernelGGL(an_relu8_reduce_kernel, dim3(ifl_cdiv(2 * C, 4)), dim3(256), 0, (hipStream_t)stream, partials, nblk, logs, dbias, dlogs, C);
+    IFL_LAUNCH_CHECK();
+    return 0;
+}

@@ -16,12 +16,33 @@ gradient-enabled pass of a module in training mode whose bias is still all zero.
 """
 from __future__ import annotations
 
+import os
+
 import torch
 import torch.nn.functional as F
 
 from . import hip
 from . import train_ops as T
 from .synth import N_RRDB_CH
+
+
+# 8-bit activation checkpoints of the coupling networks (set_activation_checkpoints)
+_checkpoint8 = [os.environ.get("IFL_CHECKPOINT8", "0") == "1"]
+
+
+def set_activation_checkpoints(bits=None) -> int:
+    """How gradient-enabled passes keep the coupling networks' hidden activations for the backward pass: 32 (default) as float32,
+    8 in 8-bit blocks with a scale per pixel and 128 channels (`train_ops.an_relu8_ring`; environment IFL_CHECKPOINT8=1).  With 8
+    a pass is evaluated layer by layer and keeps 65 bytes per pixel and hidden layer instead of 512 (the level drivers hold their
+    activations in float32 arenas); outputs and the gradients of everything a network's input depends on are those of the float32
+    path, the weight, `logs` and conditioning-weight gradients behind a checkpoint are those of its values, each within 2^-4 of the
+    activation.  `None` only queries.  Takes effect for passes that start afterwards.  Returns the previous setting."""
+    prev = 8 if _checkpoint8[0] else 32
+    if bits is not None:
+        if bits not in (8, 32):
+            raise ValueError(f"activation checkpoints in {bits!r} bits: 8 or 32")
+        _checkpoint8[0] = bits == 8
+    return prev
 
 
 FUSED_LEVELS = True      # encode on the level drivers of train_fused.py when they apply (tests switch it off to compare)
@@ -95,15 +116,18 @@ def invconv(ic, x_cl, logdet=None, reverse=False):
 
 
 # ------------------------------------------------------------------------------------------------ coupling networks
-def _conv_actnorm_relu(conv, srcs, reals):
-    """flow.Conv2d (no bias) + its ActNorm + the following ReLU, ringed in and out.  Data-dependent initialisation of the
-    ActNorm (flow.py:57-63) from the convolution's interior on the first training pass."""
-    p = T.conv2d_ring(srcs, reals, conv.weight)
+def _conv_actnorm_relu(conv, srcs, reals, checkpoints=None):
+    """flow.Conv2d (no bias) + its ActNorm + the following ReLU, ringed in and out; also the 8-bit checkpoint of the result where
+    those are on, else None.  Data-dependent initialisation of the ActNorm (flow.py:57-63) from the convolution's interior on the
+    first training pass."""
+    p = T.conv2d_ring(srcs, reals, conv.weight, checkpoints=checkpoints)
     an = conv.actnorm
     if not an.inited:
         actnorm_init(an, p[:, 1:-1, 1:-1, :].detach())
     assert p.shape[-1] == an.num_features, (tuple(p.shape), an.num_features)
-    return T.an_relu_ring(p, an.bias, an.logs)
+    if _checkpoint8[0] and torch.is_grad_enabled():
+        return T.an_relu8_ring(p, an.bias, an.logs)
+    return T.an_relu_ring(p, an.bias, an.logs), None
 
 
 def coupling_nn(seq, srcs, reals):
@@ -112,9 +136,9 @@ def coupling_nn(seq, srcs, reals):
     convolution (conv + bias, before the exp(3 logs) factor of flow.py:80-82, which the coupling kernel applies) as a ringed
     tensor with pad32(Cout) channels."""
     c1, c2, c3 = seq[0], seq[2], seq[4]
-    a1 = _conv_actnorm_relu(c1, srcs, reals)                                                    # flow.py:25-64
-    a2 = _conv_actnorm_relu(c2, [a1], [a1.shape[-1]])
-    return T.conv2d_ring([a2], [a2.shape[-1]], c3.weight, c3.bias)
+    a1, ck1 = _conv_actnorm_relu(c1, srcs, reals)                                               # flow.py:25-64
+    a2, ck2 = _conv_actnorm_relu(c2, [a1], [a1.shape[-1]], [ck1])
+    return T.conv2d_ring([a2], [a2.shape[-1]], c3.weight, c3.bias, [ck2])
 
 
 def coupling(aff, z_cl, logdet, reverse, ft_ring):
@@ -217,13 +241,14 @@ def run(fu, src, rrdbResults, logdet, test_input_size, decode, epses=None, y_one
         return rings[level]
 
     ld = _as_logdet(logdet, B, src.device)
-    if not decode and FUSED_LEVELS:
+    fused = FUSED_LEVELS and not _checkpoint8[0]
+    if not decode and fused:
         from . import train_fused
         if train_fused.usable(fu, feats):
             out = train_fused.run_encode(fu, src, feats, ld)
             if out is not None:
                 return out
-    if decode and FUSED_LEVELS:
+    if decode and fused:
         from . import train_fused
         if train_fused.usable(fu, feats) and src.shape[1] == fu.C:
             out = train_fused.run_decode(fu, src, feats, ld)

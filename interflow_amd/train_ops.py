@@ -16,7 +16,7 @@ import torch
 import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
-from . import hip
+from . import block8, hip
 
 
 def pad32(c: int) -> int:
@@ -106,7 +106,7 @@ def _launch_conv(srcs, wpacked, bias, out, cout, taps, B, h, w):
 
 class _ConvRing(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, weight, bias, real_channels, *srcs):
+    def forward(ctx, weight, bias, real_channels, checkpoints, *srcs):
         srcs = [hip._dev_f32(s, "conv source") for s in srcs]
         B, hp, wp_, _ = srcs[0].shape
         h, w = hp - 2, wp_ - 2
@@ -121,14 +121,22 @@ class _ConvRing(torch.autograd.Function):
         bpad = F.pad(bias.detach().float(), (0, cout_pad - cout)).contiguous() if bias is not None else None
         out = torch.zeros(B, hp, wp_, cout_pad, dtype=torch.float32, device=srcs[0].device)
         _launch_conv(srcs, _packed(weight, splits, cout_pad, False), bpad, out, cout_pad, taps, B, h, w)
-        ctx.save_for_backward(weight, *srcs)
+        # a source with a checkpoint is kept as its 8-bit codes, block scales and channel factors
+        kept = []
+        for s, ck in zip(srcs, checkpoints or [None] * len(srcs)):
+            kept += [s] if ck is None else [ck.codes, ck.scales, ck.chan]
+        ctx.save_for_backward(weight, *kept)
+        ctx.in8 = [ck is not None for ck in checkpoints] if checkpoints else [False] * len(srcs)
         ctx.meta = (splits, cout, cout_pad, taps, B, h, w, bias is not None)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gout):
-        weight, *srcs = ctx.saved_tensors
+        weight, *kept = ctx.saved_tensors
+        kept, srcs = list(kept), []
+        for in8 in ctx.in8:
+            srcs.append(Checkpoint8(kept.pop(0), kept.pop(0), kept.pop(0)) if in8 else kept.pop(0))
         splits, cout, cout_pad, taps, B, h, w, has_bias = ctx.meta
         L = hip.lib()
         # a fresh contiguous [B, h+2, w+2, cout_pad] buffer (the kernels index it as such, whatever strides gout has):
@@ -137,12 +145,21 @@ class _ConvRing(torch.autograd.Function):
         assert g.is_contiguous()
         g[:, 1:-1, 1:-1, :cout] = gout[:, 1:-1, 1:-1, :cout]
         cin_pad = sum(p for _, p in splits)
-        grads = [None, None, None]
+        grads = [None, None, None, None]
         if ctx.needs_input_grad[0]:
             dW = torch.zeros(cout_pad, cin_pad, taps, dtype=torch.float32, device=g.device)
             c0 = 0
             with torch.cuda.device(g.device):
                 for s in srcs:
+                    if isinstance(s, Checkpoint8):
+                        if taps == 1:
+                            # the ring's codes and gradients are zeros: all pixels of the planes are rows of one product
+                            dw8, _ = block8._wgrad(g.view(-1, cout_pad), s.codes.view(-1, s.shape[3]), s.scales.view(-1, s.scales.shape[3]), s.chan,
+                                                   torch.float32, None)
+                            dW[:, c0:c0 + s.shape[3], 0] = dw8
+                            c0 += s.shape[3]
+                            continue
+                        s = s.restore()
                     hip.check(L.ifl_conv2d_wgrad(hip._ptr(s), s.shape[3], 0, s.shape[3], hip._ptr(g), cout_pad, 0, cout_pad,
                                                  hip._ptr(dW), cin_pad, c0 // 32, taps, B, h, w, hip._stream()),
                               "ifl_conv2d_wgrad")
@@ -154,14 +171,14 @@ class _ConvRing(torch.autograd.Function):
             grads[0] = torch.cat(parts, 1).reshape(weight.shape).to(weight.dtype)
         if has_bias and ctx.needs_input_grad[1]:
             grads[1] = g[:, 1:-1, 1:-1, :cout].sum(dim=(0, 1, 2))
-        need_src = [ctx.needs_input_grad[3 + i] for i in range(len(srcs))]
+        need_src = [ctx.needs_input_grad[4 + i] for i in range(len(srcs))]
         if any(need_src):
             # data gradient = the same convolution with W^T, spatially flipped:  Wt[ci][co][tap] = W[co][ci][taps-1-tap]
             wts = _packed(weight, splits, cout_pad, True)
             for i, s in enumerate(srcs):
                 padded = s.shape[3]
                 if need_src[i]:
-                    gi = torch.zeros(s.shape, dtype=torch.float32, device=s.device)
+                    gi = torch.zeros(s.shape, dtype=torch.float32, device=g.device)
                     _launch_conv([g], wts[i], None, gi, padded, taps, B, h, w)
                     grads.append(gi)
                 else:
@@ -171,12 +188,18 @@ class _ConvRing(torch.autograd.Function):
         return tuple(grads)
 
 
-def conv2d_ring(srcs, real_channels, weight, bias=None):
+def conv2d_ring(srcs, real_channels, weight, bias=None, checkpoints=None):
     """Stride-1 'same' convolution (3x3 or 1x1) of the channel-wise concatenation of `srcs` (ringed channels-last tensors
     whose channel counts are multiples of 32; the first `real_channels[i]` channels of source i are the reference's
     channels, the rest zero) with `weight` [Cout, sum(real), k, k] (+ bias).  Returns a ringed tensor with pad32(Cout)
-    channels (zero ring, zero padded channels)."""
-    return _ConvRing.apply(weight, bias, tuple(real_channels), *srcs)
+    channels (zero ring, zero padded channels).
+    `checkpoints`: per source a `Checkpoint8` of it (from `an_relu8_ring`) or None.  A source with one is not kept for the
+    backward pass; its part of the weight gradient is computed from the checkpoint's values."""
+    if checkpoints is not None:
+        assert len(checkpoints) == len(srcs)
+        for s, ck in zip(srcs, checkpoints):
+            assert ck is None or tuple(ck.shape) == tuple(s.shape), (tuple(ck.shape), tuple(s.shape))
+    return _ConvRing.apply(weight, bias, tuple(real_channels), checkpoints, *srcs)
 
 
 # ------------------------------------------------------------------------------------------------ fused per-pixel operators
@@ -216,6 +239,125 @@ class _AnRelu(torch.autograd.Function):
 def an_relu_ring(x_ring, bias, logs):
     """ReLU(ActNorm(x)) of flow.Conv2d + the following nn.ReLU, ringed 64-channel tensors in and out."""
     return _AnRelu.apply(x_ring, bias, logs)
+
+
+class Checkpoint8:
+    """An activation of `an_relu8_ring` in 8 bits: values v in 8-bit blocks (block8: e4m3, a scale per pixel and 128 channels) and
+    the factor per channel that makes them y = v exp(logs).  codes [B, h+2, w+2, C], scales [B, h+2, w+2, ceil(C / 128)], chan [C]."""
+    __slots__ = ("codes", "scales", "_chan", "_logs")
+
+    def __init__(self, codes, scales, chan=None, logs=None):
+        self.codes, self.scales, self._chan, self._logs = codes, scales, chan, logs
+
+    @property
+    def shape(self):
+        return self.codes.shape
+
+    @property
+    def chan(self):
+        if self._chan is None:
+            self._chan = torch.exp(self._logs)
+        return self._chan
+
+    def restore(self):
+        """The ringed float32 activation that the checkpoint stands for."""
+        P, C = self.codes[..., 0].numel(), self.codes.shape[3]
+        out = torch.empty(self.codes.shape, dtype=torch.float32, device=self.codes.device)
+        block8._call("ifl_block8_dequantize", self.codes.device, self.codes.data_ptr(), C, self.scales.data_ptr(), self.scales.shape[3], 0,
+                     self.chan.data_ptr(), out.data_ptr(), 0, C, P, C)
+        return out
+
+
+def _aligned(t):
+    """A contiguous tensor whose data starts on 16 bytes (a view may start anywhere)."""
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+class _AnRelu8(torch.autograd.Function):
+    """y = relu((x + bias) * exp(logs)) on a ringed tensor; the backward reads an 8-bit checkpoint (ifl_an_relu8_fwd / _bwd)."""
+
+    @staticmethod
+    def forward(ctx, x, bias, logs):
+        x = _aligned(hip._dev_f32(x, "an_relu8 input"))
+        B, hp, wp_, C = x.shape
+        b, l = bias.detach().reshape(-1).float().contiguous(), logs.detach().reshape(-1).float().contiguous()
+        assert b.numel() == C and l.numel() == C, (tuple(bias.shape), tuple(logs.shape), C)
+        block8._same_device(x.device, b, l)
+        y = torch.empty_like(x)
+        codes = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+        scales = torch.empty((B, hp, wp_, -(-C // block8.BLOCK)), dtype=torch.float8_e8m0fnu, device=x.device)
+        block8._call("ifl_an_relu8_fwd", x.device, x.data_ptr(), y.data_ptr(), codes.data_ptr(), scales.data_ptr(), b.data_ptr(), l.data_ptr(),
+                     B, hp - 2, wp_ - 2, C)
+        ctx.save_for_backward(codes, scales, l)
+        ctx.shapes = (bias.shape, logs.shape)
+        ctx.mark_non_differentiable(codes, scales)
+        return y, codes, scales
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy, _codes, _scales):
+        codes, scales, l = ctx.saved_tensors
+        B, hp, wp_, C = codes.shape
+        gy = _aligned(hip._dev_f32(gy, "an_relu8 gradient"))
+        dx = torch.empty_like(gy)
+        db, dl = torch.empty_like(l), torch.empty_like(l)
+        part = torch.empty(hip.lib().ifl_an_relu8_blocks(B, hp - 2, wp_ - 2, C) * 2 * C, dtype=torch.float32, device=gy.device)
+        block8._call("ifl_an_relu8_bwd", gy.device, gy.data_ptr(), codes.data_ptr(), scales.data_ptr(), l.data_ptr(), dx.data_ptr(), db.data_ptr(),
+                     dl.data_ptr(), part.data_ptr(), B, hp - 2, wp_ - 2, C)
+        return dx, db.reshape(ctx.shapes[0]), dl.reshape(ctx.shapes[1])
+
+
+def an_relu8_ring(x_ring, bias, logs):
+    """`an_relu_ring` with an 8-bit activation checkpoint: (y, Checkpoint8 of y).  The backward pass keeps C bytes (and one scale
+    per 128 channels) of a pixel instead of x's 4 C: dx is exact (the checkpoint's zeros are the ReLU's mask), the gradient of
+    logs is that of the checkpoint's values.  Ringed tensors, channels a multiple of 32, at most 1024.  Hand the checkpoint to the
+    convolution that reads y (`conv2d_ring(checkpoints=...)`) and y itself is not kept either."""
+    assert x_ring.dim() == 4 and x_ring.shape[1] >= 3 and x_ring.shape[2] >= 3, tuple(x_ring.shape)
+    y, codes, scales = _AnRelu8.apply(x_ring, bias, logs)
+    return y, Checkpoint8(codes, scales, logs=logs.detach().reshape(-1).float())
+
+
+class _Linear8(torch.autograd.Function):
+    """y = Q(x) Q(w)^T + bias; the backward has Q(x) for a checkpoint (block8.py)."""
+
+    @staticmethod
+    def forward(ctx, x, w, bias, grad_fmt):
+        x2 = x.reshape(-1, x.shape[-1])
+        q = block8.quantize(x2)
+        y = block8.matmul(q, block8.quantize(w), bias, x.dtype)
+        ctx.save_for_backward(q.codes if ctx.needs_input_grad[1] else None, q.scales if ctx.needs_input_grad[1] else None, w)
+        ctx.meta = (x.shape, x.dtype, bias.dtype if bias is not None else None, grad_fmt)
+        return y.view(*x.shape[:-1], w.shape[0])
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        codes, scales, w = ctx.saved_tensors
+        shape, dtype, bias_dtype, grad_fmt = ctx.meta
+        g = g.reshape(-1, w.shape[0])
+        if not block8._rows_apart(g):
+            g = g.contiguous()
+        dx = None
+        if ctx.needs_input_grad[0]:
+            dx = block8.matmul(block8.quantize(g, grad_fmt), block8.quantize(w.t()), None, dtype).view(shape)
+        need_w, need_b = ctx.needs_input_grad[1], ctx.needs_input_grad[2]
+        dw, db = block8._wgrad(g, codes, scales, None, w.dtype if need_w else None, bias_dtype if need_b else None)
+        return dx, dw, db, None
+
+
+def linear8(x, weight, bias=None, grad_fmt: str = "e4m3"):
+    """x [..., K] times weight [N, K]^T (+ bias [N]) -> [..., N] in x's type, on the 8-bit matrix cores, with gradients.
+    Forward: x and weight are quantized along K in blocks of 128 (e4m3); x's 8-bit blocks are the checkpoint.  Backward: dx is the
+    product of the quantized gradient (`grad_fmt`, along N) and the weight quantized along N; dw multiplies the gradient as it is
+    with the checkpoint (exact products); the bias' gradient is the gradient's column sum.  Sums are float32.  x and the gradient
+    float32, bfloat16 or float16; weight and bias each any of them (a float32 master weight under bfloat16 activations)."""
+    block8._real(x, "linear8 input")
+    block8._real(weight, "linear8 weight")
+    assert x.dim() >= 1 and weight.dim() == 2 and x.shape[-1] == weight.shape[1] and weight.numel() > 0, (tuple(x.shape), tuple(weight.shape))
+    if grad_fmt not in block8._FMT:
+        raise ValueError(f"linear8: grad_fmt has to be 'e4m3' or 'e5m2', got {grad_fmt!r}")
+    block8._same_device(x.device, weight)
+    return _Linear8.apply(x, weight, bias, grad_fmt)
 
 
 class _Coupling(torch.autograd.Function):
