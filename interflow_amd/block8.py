@@ -183,9 +183,11 @@ def matmul(a: Block8, b: Block8, bias=None, dtype=torch.bfloat16) -> torch.Tenso
     _same_device(a_c.device, b_c)
     bias, bt = _bias(bias, N, a_c.device)
     out = torch.empty((M, N), dtype=_dtype(dtype, "matmul"), device=a_c.device)
+    n = hip.lib().ifl_block8_matmul_scratch_floats(M, N, K, _TYPE[dtype])
+    scratch = torch.empty((n,), dtype=torch.float32, device=out.device) if n else None
     _call("ifl_block8_matmul", a_c.device, a_c.data_ptr(), _up(_ld(a_c), 16), a_s.data_ptr(), _up(_ld(a_s), 4), _FMT_OF[a_c.dtype], b_c.data_ptr(),
           _up(_ld(b_c), 16), b_s.data_ptr(), _up(_ld(b_s), 4), _FMT_OF[b_c.dtype], bias.data_ptr() if bias is not None else None, bt,
-          out.data_ptr(), _TYPE[dtype], N, M, N, K)
+          out.data_ptr(), _TYPE[dtype], N, scratch.data_ptr() if n else None, M, N, K)
     return out
 
 
@@ -197,8 +199,20 @@ def linear(x, w: Block8, bias=None) -> torch.Tensor:
         raise TypeError("linear: the weights have to be a Block8 (block8.quantize)")
     assert x.dim() >= 1 and x.shape[-1] == w.shape[1], (tuple(x.shape), tuple(w.shape))
     _same_device(x.device, w)
-    y = matmul(quantize(x.reshape(-1, x.shape[-1])), w, bias, x.dtype)
-    return y if x.dim() == 2 else y.view(*x.shape[:-1], w.shape[0])
+    K, N = x.shape[-1], w.shape[0]
+    b_c, b_s = _operand(w, "weights")
+    bias, bt = _bias(bias, N, x.device)
+    x2 = x.reshape(-1, K)
+    if not _rows_apart(x2):
+        x2 = x2.contiguous()
+    M = x2.shape[0]
+    out = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=x.device)
+    t = _TYPE[x.dtype]
+    n = hip.lib().ifl_block8_linear_scratch_bytes(M, N, K, t)
+    scratch = torch.empty((n,), dtype=torch.uint8, device=x.device) if n else None
+    _call("ifl_block8_linear", x.device, x2.data_ptr(), t, _ld(x2), b_c.data_ptr(), _up(_ld(b_c), 16), b_s.data_ptr(), _up(_ld(b_s), 4),
+          _FMT_OF[b_c.dtype], bias.data_ptr() if bias is not None else None, bt, out.data_ptr(), N, scratch.data_ptr() if n else None, M, N, K)
+    return out
 
 
 def weight_grad(dy, q: Block8, dtype=torch.float32, bias_dtype=None, weight: bool = True):

@@ -20,20 +20,27 @@ struct MM8 {
     const uint8_t *a, *b, *sa, *sb;
     int64_t lda, ldb, lsa, lsb;
     const void* bias; int btype;
-    void* out; int64_t ldo;
+    void* out; int otype; int64_t ldo;
     int64_t M, N; int K;
+    const void* x; int64_t ldx;          // skinny kernel with its own quantization: the m side as it is
+    float* part; int split, ksteps;      // float32 partial sums [split][M][N], K steps of 128 per part
+    int tiles_m, tiles_n, per_xcd;
 };
 
 __device__ __forceinline__ float mm8_bias(const MM8& q, int64_t n) {
     return !q.bias ? 0.f : q.btype == IFL_T_F32 ? ((const float*)q.bias)[n] : q.btype == IFL_T_BF16 ? (float)((const __bf16*)q.bias)[n] : (float)((const _Float16*)q.bias)[n];
 }
 
-// 16 bytes of a row from k on, zero where k >= K
+// 16 bytes of a row from k on, zero where k >= K (rows are whole 16 bytes in memory)
 __device__ __forceinline__ i32x4 mm8_load16(const uint8_t* __restrict__ row, int k, int K) {
-    if (k + 16 <= K) return *(const i32x4*)(row + k);
-    i32x4 r = {0, 0, 0, 0};
+    i32x4 r = *(const i32x4*)(row + (k < K ? k : 0));
+    if (k + 16 > K) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) if (k + i < K) r[i >> 2] |= (int)((uint32_t)row[k + i] << 8 * (i & 3));
+        for (int i = 0; i < 4; ++i) {
+            const int left = K - k - 4 * i;
+            r[i] = left >= 4 ? r[i] : left <= 0 ? 0 : (int)((uint32_t)r[i] & ((1u << 8 * left) - 1));
+        }
+    }
     return r;
 }
 
@@ -49,67 +56,443 @@ __device__ __forceinline__ f32x4 mm8_mfma(i32x8 b, i32x8 a, f32x4 c, int sb, int
     }
 }
 
-// Wave = 32 n x 32 m, operands straight from memory.
-template <int FA, int FB, class T>
-__global__ __launch_bounds__(256)
-void mm8_direct_kernel(MM8 q)
-{
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, g = lane >> 4;
-    const int64_t n0 = (int64_t)blockIdx.x * 64 + (wave & 1) * 32, m0 = (int64_t)blockIdx.y * 64 + (wave >> 1) * 32;
-    const uint8_t *pb[2], *pa[2], *psb[2], *psa[2];
+__device__ __forceinline__ i32x8 mm8_join(i32x4 a, i32x4 b) {
+    i32x8 r;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int64_t n = min(n0 + 16 * i + r16, q.N - 1), m = min(m0 + 16 * i + r16, q.M - 1);
-        pb[i] = q.b + n * q.ldb; psb[i] = q.sb + n * q.lsb;
-        pa[i] = q.a + m * q.lda; psa[i] = q.sa + m * q.lsa;
+    for (int i = 0; i < 4; ++i) { r[i] = a[i]; r[4 + i] = b[i]; }
+    return r;
+}
+
+// n values of one row of the result from column n on; wide: 16-byte stores fit
+template <class T, int CNT>
+__device__ __forceinline__ void mm8_store(const MM8& q, int64_t m, int64_t n, const float v[CNT], bool wide) {
+    T* p = (T*)q.out + m * q.ldo + n;
+    constexpr int V = 16 / sizeof(T);
+    if (wide && n + CNT <= q.N && CNT % V == 0) {
+        typedef T TV __attribute__((ext_vector_type(V)));
+#pragma unroll
+        for (int i = 0; i < CNT / V; ++i) {
+            TV t;
+#pragma unroll
+            for (int e = 0; e < V; ++e) t[e] = (T)v[i * V + e];
+            ((TV*)p)[i] = t;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < CNT; ++i) if (n + i < q.N) p[i] = (T)v[i];
     }
-    f32x4 acc[2][2] = {};
-    for (int k = 0, kb = 0; k < q.K; k += B8_BLK, ++kb) {
-        i32x8 a[2], b[2];
-        int sa[2], sb[2];
+}
+
+// ------------------------------------------------------------------------------------------------ tiles
+// Workgroup = TN x TM of the result, K in steps of 128 bytes through two LDS buffers: while one is multiplied, the other is
+// filled by loads that go straight to LDS (16 bytes a lane, no registers).  Those write LDS in lane order, so rows lie 128 bytes
+// apart and it is the SOURCE that is permuted: position p of row r holds the 16 bytes p ^ s(r), s(r) = (r ^ r >> 2) & 7, which
+// makes every 16-byte fragment read free of bank conflicts.  Rows past the end repeat the last one (their results are not
+// stored); a last step that K does not fill goes through registers with zeros behind K.
+//
+// Waves WN x WM; a wave has NF x MF fragments of 16 x 16.  Row r of n-fragment f is row 16 G (f / G) + 4 G (r / 4) + 4 (f % G) +
+// r % 4 of the wave's (G = 4, or NF if less): so the four values a lane gets from each of G fragments are 4 G neighbours of
+// one output row.
+//
+// Workgroups go to the 8 XCDs in turn; an XCD takes a contiguous run of tiles, in groups of 8 along m, so that the 32 tiles
+// it works on at a time share rows of both operands in its own L2.
+template <int TN, int TM, int WN, int WM, int FA, int FB, bool EXACT, bool SPLIT>
+__global__ __launch_bounds__(64 * WN * WM)
+void mm8_tile_kernel(MM8 q)
+{
+    constexpr int NW = WN * WM, NF = TN / WN / 16, MF = TM / WM / 16, G = NF < 4 ? NF : 4;
+    constexpr int CH = (TN + TM) * 8, PER = CH / (64 * NW);              // 16-byte pieces of a step, per thread
+    __shared__ __attribute__((aligned(16))) uint8_t buf0[(TN + TM) * 128];
+    __shared__ __attribute__((aligned(16))) uint8_t buf1[(TN + TM) * 128];
+    __shared__ uint32_t sc[2][TN + TM];                                  // scale bytes of four steps, per row
+    const int tiles = q.tiles_m * q.tiles_n;
+    const int t = (blockIdx.x & 7) * q.per_xcd + (blockIdx.x >> 3);
+    if (t >= tiles) return;
+    const int gsz = 8 * q.tiles_n, grp = t / gsz, rest = t - grp * gsz;
+    const int gm = min(8, q.tiles_m - grp * 8);
+    const int tm = grp * 8 + rest % gm, tn = rest / gm;
+    const int64_t n0 = (int64_t)tn * TN, m0 = (int64_t)tm * TM;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, g = lane >> 4;
+    const int wn = wave % WN, wm = wave / WN;
+
+    // where this thread's pieces come from: 32-bit offsets from the tile's first rows
+    uint32_t off[PER];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const i32x4 a0 = mm8_load16(pa[i], k + 16 * g, q.K), a1 = mm8_load16(pa[i], k + 64 + 16 * g, q.K);
-            const i32x4 b0 = mm8_load16(pb[i], k + 16 * g, q.K), b1 = mm8_load16(pb[i], k + 64 + 16 * g, q.K);
+    for (int i = 0; i < PER; ++i) {
+        const int p = (i * NW + wave) * 64 + lane, row = p >> 3, ch = (p & 7) ^ ((row ^ row >> 2) & 7);
+        const bool nside = row < TN;
+        const int64_t left = nside ? q.N - 1 - n0 : q.M - 1 - m0;
+        const int r = nside ? row : row - TN;
+        off[i] = (uint32_t)((int64_t)(r < left ? r : (int)left) * (nside ? q.ldb : q.lda)) + ch * 16;
+    }
+    const uint8_t* bb = q.b + n0 * q.ldb;
+    const uint8_t* ab = q.a + m0 * q.lda;
+    const int k_first = SPLIT ? blockIdx.y * q.ksteps : 0;
+    const int all = (q.K + B8_BLK - 1) / B8_BLK, k_end = SPLIT ? min(all, k_first + q.ksteps) : all;
+
+    auto fill = [&](uint8_t* buf, int ks) {
+        const int k0 = ks * B8_BLK;
+        if (k0 + B8_BLK <= q.K) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) { a[i][e] = a0[e]; a[i][4 + e] = a1[e]; b[i][e] = b0[e]; b[i][4 + e] = b1[e]; }
-            sa[i] = psa[i][kb]; sb[i] = psb[i][kb];
+            for (int i = 0; i < PER; ++i) {
+                const uint8_t* src = ((i * NW * 64) >> 3 < TN ? bb : ab) + k0;      // (a piece's side is the same for all waves)
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + off[i]),
+                                                 (__attribute__((address_space(3))) void*)(buf + (i * NW + wave) * 1024), 16, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const int p = (i * NW + wave) * 64 + lane, row = p >> 3, ch = (p & 7) ^ ((row ^ row >> 2) & 7);
+                const uint8_t* src = ((i * NW * 64) >> 3 < TN ? bb : ab) + (off[i] - ch * 16);
+                *(i32x4*)(buf + p * 16) = mm8_load16(src, k0 + ch * 16, q.K);
+            }
+        }
+    };
+
+    // fragment addresses.  Rows of one lane's fragments differ by constants, and so do, after an XOR, their swizzled positions:
+    // s(row) = s0 ^ f % 4 ^ 4 (f & 1) on the n side, s0 ^ 4 (f & 1) on the m side.
+    const int nrow0 = wn * NF * 16 + 4 * G * (r16 >> 2) + (r16 & 3), mrow0 = TN + wm * MF * 16 + r16;
+    const int ns = (r16 & 3) ^ ((r16 >> 2) & 1) << 2, ms = (r16 & 7) ^ r16 >> 2;
+    auto npos = [&](int f, int c) {
+        const int row = nrow0 + 16 * G * (f / G) + 4 * (f % G);
+        const int s = G == 4 ? ns ^ (f % G) ^ (f & 1) << 2 : (row ^ row >> 2) & 7;
+        return row * 128 + ((g + 4 * c) ^ s) * 16;
+    };
+    auto mpos = [&](int f, int c) { return (mrow0 + 16 * f) * 128 + ((g + 4 * c) ^ ms ^ (f & 1) << 2) * 16; };
+
+    // a thread's row of the scales (the tile has at most as many rows as threads)
+    const int srow = threadIdx.x;
+    const bool has_s = srow < TN + TM;
+    const uint8_t* sp = srow < TN ? q.sb + min(n0 + srow, q.N - 1) * q.lsb : q.sa + min(m0 + (srow - TN), q.M - 1) * q.lsa;
+    uint32_t snext = 0;
+
+    f32x4 acc[NF][MF] = {};
+    auto multiply = [&](const uint8_t* buf, int ks) {
+        const uint8_t* s = (const uint8_t*)sc[(ks >> 2) & 1] + (ks & 3);
+        i32x8 a[MF];
+        int ca[MF];
+#pragma unroll
+        for (int j = 0; j < MF; ++j) {
+            a[j] = mm8_join(*(const i32x4*)(buf + mpos(j, 0)), *(const i32x4*)(buf + mpos(j, 1)));
+            ca[j] = s[4 * (mrow0 + 16 * j)];
         }
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < NF; ++i) {
+            const i32x8 b = mm8_join(*(const i32x4*)(buf + npos(i, 0)), *(const i32x4*)(buf + npos(i, 1)));
+            const int cb = s[4 * (nrow0 + 16 * G * (i / G) + 4 * (i % G))];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) acc[i][j] = mm8_mfma<FA, FB, sizeof(T) == 4>(b[i], a[j], acc[i][j], sb[i], sa[j]);
+            for (int j = 0; j < MF; ++j) acc[i][j] = mm8_mfma<FA, FB, EXACT>(b, a[j], acc[i][j], cb, ca[j]);
+        }
+    };
+    // behind step ks: the scales of the next four steps are asked for at the first of these four and put into LDS at the last
+    auto scales = [&](int ks) {
+        if ((ks & 3) == 0 && ks + 4 < k_end && has_s) snext = ((const uint32_t*)sp)[(ks >> 2) + 1];
+        if ((ks & 3) == 3 && has_s) sc[((ks >> 2) + 1) & 1][srow] = snext;
+    };
+    auto turn = [&]() {
+        __builtin_amdgcn_s_waitcnt(0x0f70);                              // vmcnt(0): this wave's pieces of the next step are in LDS
+        __syncthreads();
+    };
+
+    if (has_s) sc[(k_first >> 2) & 1][srow] = ((const uint32_t*)sp)[k_first >> 2];        // (k_first is a multiple of 4)
+    fill(buf0, k_first);
+    turn();
+    for (int ks = k_first; ks < k_end; ks += 2) {
+        if (ks + 1 < k_end) fill(buf1, ks + 1);
+        scales(ks);
+        multiply(buf0, ks);
+        turn();
+        if (ks + 1 < k_end) {
+            if (ks + 2 < k_end) fill(buf0, ks + 2);
+            scales(ks + 1);
+            multiply(buf1, ks + 1);
+            turn();
+        }
+    }
+
+    const int64_t nw = n0 + wn * NF * 16 + 4 * G * g;
+    if constexpr (SPLIT) {
+        float* out = q.part + (int64_t)blockIdx.y * q.M * q.N;
+#pragma unroll
+        for (int j = 0; j < MF; ++j) {
+            const int64_t m = m0 + wm * MF * 16 + 16 * j + r16;
+            if (m < q.M) {
+#pragma unroll
+                for (int i = 0; i < NF; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int64_t n = nw + 16 * G * (i / G) + 4 * (i % G) + e;
+                        if (n < q.N) out[m * q.N + n] = acc[i][j][e];
+                    }
+            }
+        }
+    } else {
+        const int es = q.otype == IFL_T_F32 ? 4 : 2;
+        const bool wide = ((uintptr_t)q.out | (uint64_t)(q.ldo * es)) % 16 == 0;
+#pragma unroll
+        for (int h = 0; h < NF / G; ++h) {
+            float bias[4 * G];
+#pragma unroll
+            for (int i = 0; i < 4 * G; ++i) bias[i] = nw + 16 * G * h + i < q.N ? mm8_bias(q, nw + 16 * G * h + i) : 0.f;
+#pragma unroll
+            for (int j = 0; j < MF; ++j) {
+                const int64_t m = m0 + wm * MF * 16 + 16 * j + r16;
+                float v[4 * G];
+#pragma unroll
+                for (int i = 0; i < 4 * G; ++i) v[i] = acc[h * G + i / 4][j][i % 4] + bias[i];
+                if (m < q.M) {
+                    if constexpr (EXACT) mm8_store<float, 4 * G>(q, m, nw + 16 * G * h, v, wide);
+                    else if (q.otype == IFL_T_BF16) mm8_store<__bf16, 4 * G>(q, m, nw + 16 * G * h, v, wide);
+                    else mm8_store<_Float16, 4 * G>(q, m, nw + 16 * G * h, v, wide);
+                }
+            }
+        }
+    }
+}
+
+// out = sum of the parts, in order, + bias
+template <class T>
+__global__ __launch_bounds__(256)
+void mm8_join_kernel(MM8 q)
+{
+    const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x, m = blockIdx.y;
+    if (n >= q.N) return;
+    const float* p = q.part + m * q.N + n;
+    float t = p[0];
+    for (int s = 1; s < q.split; ++s) t += p[(int64_t)s * q.M * q.N];
+    ((T*)q.out)[m * q.ldo + n] = (T)(t + mm8_bias(q, n));
+}
+
+// ------------------------------------------------------------------------------------------------ few rows
+// M <= 16 MF: bound by reading B once, so nothing is staged.  Workgroup = 16 n; its 8 waves take every eighth step of K, four of
+// their steps' loads in flight at a time, and meet in LDS.  OWN: the m side is not quantized yet: each workgroup quantizes all of
+// it (M K values, 32 a thread at most) into LDS, which saves a launch.
+constexpr int SK_WAVES = 8, SK_OWN = 16384;                              // OWN: most bytes of codes in LDS
+
+template <int MF, int FA, int FB, bool EXACT, bool OWN, class TX>
+__global__ __launch_bounds__(64 * SK_WAVES)
+void mm8_skinny_kernel(MM8 q)
+{
+    __shared__ float red[SK_WAVES][16 * 16 * MF];
+    extern __shared__ __attribute__((aligned(16))) uint8_t own[];        // [M][KP] codes, then [M][KB] scale bytes
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, g = lane >> 4;
+    const int KB = (q.K + B8_BLK - 1) / B8_BLK, KP = KB * B8_BLK;
+    const int64_t n0 = (int64_t)blockIdx.x * 16;
+    const int64_t n = min(n0 + r16, q.N - 1);
+    const uint8_t *pb = q.b + n * q.ldb, *psb = q.sb + n * q.lsb;
+    constexpr int U = 4;
+    i32x8 b[U];
+    int cb[U];
+    auto load = [&](int ks0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int ks = ks0 + u * SK_WAVES;
+            if (ks < KB) {
+                const int k = ks * B8_BLK + 16 * g;
+                b[u] = mm8_join(mm8_load16(pb, k, q.K), mm8_load16(pb, k + 64, q.K));
+                cb[u] = psb[ks];
+            }
+        }
+    };
+    load(wave);                                                          // (the first loads run while the m side is quantized)
+    if constexpr (OWN) {
+        const int l16 = threadIdx.x & 15;
+        for (int i = threadIdx.x >> 4; i < (int)q.M * KB; i += 64 * SK_WAVES / 16) {
+            const int m = i / KB, kb = i - m * KB, c = kb * B8_BLK + l16 * 8;
+            float v[8];
+            b8_load8<TX, false>((const TX*)q.x + m * q.ldx + c, q.K - c, v);
+            const int s = b8_scale_byte(b8_group_max<16>(b8_amax_bits(v)), IFL_Q_E4M3);
+            const float inv = b8_inv_scale(s);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] *= inv;
+            *(i32x2*)(own + m * KP + c) = b8_encode8(v, IFL_Q_E4M3);
+            if (l16 == 0) own[(int)q.M * KP + i] = (uint8_t)s;
+        }
+        __syncthreads();
+    }
+    f32x4 acc[MF] = {};
+    for (int ks0 = wave; ks0 < KB; ks0 += U * SK_WAVES) {
+        if (ks0 != wave) load(ks0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int ks = ks0 + u * SK_WAVES;
+            if (ks >= KB) break;
+            const int k = ks * B8_BLK + 16 * g;
+#pragma unroll
+            for (int j = 0; j < MF; ++j) {
+                const int m = min(16 * j + r16, (int)q.M - 1);
+                i32x8 a;
+                int ca;
+                if constexpr (OWN) {
+                    a = mm8_join(*(const i32x4*)(own + m * KP + k), *(const i32x4*)(own + m * KP + k + 64));
+                    ca = own[(int)q.M * KP + m * KB + ks];
+                } else {
+                    const uint8_t* pa = q.a + m * q.lda;
+                    a = mm8_join(mm8_load16(pa, k, q.K), mm8_load16(pa, k + 64, q.K));
+                    ca = q.sa[m * q.lsa + ks];
+                }
+                acc[j] = mm8_mfma<FA, FB, EXACT>(b[u], a, acc[j], cb[u], ca);
+            }
+        }
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < MF; ++j)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int e = 0; e < 4; ++e) red[wave][(16 * j + r16) * 16 + 4 * g + e] = acc[j][e];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * 16 * MF; i += 64 * SK_WAVES) {
+        const int m = i >> 4;
+        const int64_t nn = n0 + (i & 15);
+        float t = red[0][i];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int64_t n = n0 + 16 * i + 4 * g + e, m = m0 + 16 * j + r16;
-                if (n < q.N && m < q.M) ((T*)q.out)[m * q.ldo + n] = (T)(acc[i][j][e] + mm8_bias(q, n));
-            }
+        for (int w = 1; w < SK_WAVES; ++w) t += red[w][i];
+        if (m < q.M && nn < q.N) {
+            t += mm8_bias(q, nn);
+            if constexpr (EXACT) ((float*)q.out)[m * q.ldo + nn] = t;
+            else if (q.otype == IFL_T_BF16) ((__bf16*)q.out)[m * q.ldo + nn] = (__bf16)t;
+            else ((_Float16*)q.out)[m * q.ldo + nn] = (_Float16)t;
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ which of them
+// Few rows: the skinny kernel.  Else the largest tile that still gives the 256 CUs work (measured: DESIGN), float32 results at most
+// 128 (their fragments are held as bf16); a product of few tiles and a long K is split along K.
+struct Plan { int kind, tile, split, ksteps; };
+Plan mm8_plan(int64_t M, int64_t N, int64_t K, int otype)
+{
+    Plan p = {0, 0, 1, 0};
+    if (M <= 32) { p.kind = M <= 16 ? 1 : 2; return p; }
+    auto tiles = [&](int t) { return ((M + t - 1) / t) * ((N + t - 1) / t); };
+    p.tile = 64;
+    if (otype != IFL_T_F32 && tiles(256) >= 192) p.tile = 256;
+    else if (tiles(128) >= 192) p.tile = 128;
+    const int64_t n = tiles(p.tile), steps = (K + B8_BLK - 1) / B8_BLK;
+    if (p.tile == 64 && n <= 128 && steps >= 8) {
+        int64_t s = 256 / n;
+        if (s > steps / 4) s = steps / 4;
+        if (s > 16) s = 16;
+        if (s > 1) { p.ksteps = (int)(((steps + s - 1) / s + 3) / 4 * 4); p.split = (int)((steps + p.ksteps - 1) / p.ksteps); }
+    }
+    if (p.split <= 1) { p.split = 1; p.ksteps = (int)steps; }
+    return p;
+}
+
+template <int FA, int FB>
+int mm8_launch(MM8 q, const Plan& p, hipStream_t st)
+{
+    const bool f32 = q.otype == IFL_T_F32;
+    if (p.kind) {
+        const dim3 grid((unsigned)((q.N + 15) / 16)), block(64 * SK_WAVES);
+#define MM8_SK(MF, EX) hipLaunchKernelGGL(HIP_KERNEL_NAME(mm8_skinny_kernel<MF, FA, FB, EX, false, float>), grid, block, 0, st, q)
+        if (p.kind == 1) { if (f32) MM8_SK(1, true); else MM8_SK(1, false); }
+        else { if (f32) MM8_SK(2, true); else MM8_SK(2, false); }
+        IFL_LAUNCH_CHECK();
+        return 0;
+    }
+    q.tiles_m = (int)((q.M + p.tile - 1) / p.tile);
+    q.tiles_n = (int)((q.N + p.tile - 1) / p.tile);
+    q.per_xcd = (q.tiles_m * q.tiles_n + 7) / 8;
+    q.split = p.split; q.ksteps = p.ksteps;
+    const dim3 grid(8 * q.per_xcd, p.split);
+#define MM8_TILE(T, WN, WM, EX, SP) hipLaunchKernelGGL(HIP_KERNEL_NAME(mm8_tile_kernel<T, T, WN, WM, FA, FB, EX, SP>), grid, dim3(64 * WN * WM), 0, st, q)
+    if (p.tile == 256) MM8_TILE(256, 2, 4, false, false);
+    else if (p.tile == 128) { if (f32) MM8_TILE(128, 2, 2, true, false); else MM8_TILE(128, 2, 2, false, false); }
+    else if (p.split == 1) { if (f32) MM8_TILE(64, 2, 2, true, false); else MM8_TILE(64, 2, 2, false, false); }
+    else { if (f32) MM8_TILE(64, 2, 2, true, true); else MM8_TILE(64, 2, 2, false, true); }
+    IFL_LAUNCH_CHECK();
+    if (p.split > 1) {
+        const dim3 jg((unsigned)((q.N + 255) / 256), (unsigned)q.M);
+        B8_DISPATCH(q.otype, hipLaunchKernelGGL(HIP_KERNEL_NAME(mm8_join_kernel<T>), jg, dim3(256), 0, st, q));
+        IFL_LAUNCH_CHECK();
+    }
+    return 0;
+}
+
+int mm8_check(int64_t M, int64_t N, int64_t K, const uint8_t* b, int64_t ldb, const uint8_t* sb, int64_t lsb, const void* bias, int btype,
+              const void* out, int otype, int64_t ldo)
+{
+    IFL_CHECK_ARG(b8_type_ok(otype) && (!bias || b8_type_ok(btype)), IFL_EINVAL, "block8 product: element types");
+    IFL_CHECK_ARG(M >= 0 && N >= 1 && K >= 1, IFL_EINVAL, "block8 product: %lld x %lld x %lld", (long long)M, (long long)N, (long long)K);
+    IFL_CHECK_ARG(K <= 0x7ffffc00 && M <= 0x3fffffff && N <= 0x3fffffff, IFL_ENOTSUP, "block8 product: %lld x %lld x %lld", (long long)M, (long long)N, (long long)K);
+    if (M == 0) return 0;
+    const int KB = ifl_cdiv((int)K, B8_BLK);
+    IFL_CHECK_ARG(b && sb && out, IFL_EINVAL, "block8 product: null pointer");
+    IFL_CHECK_ARG(ldb >= K && lsb >= KB && ldo >= N, IFL_EINVAL, "block8 product: row strides");
+    IFL_CHECK_ARG(ldb % 16 == 0 && (uintptr_t)b % 16 == 0 && lsb % 4 == 0 && (uintptr_t)sb % 4 == 0, IFL_EINVAL,
+                  "block8 product: codes in rows of whole, aligned 16 bytes, scales of whole, aligned 4");
+    IFL_CHECK_ARG(ldb < (1 << 23), IFL_ENOTSUP, "block8 product: rows of %lld bytes", (long long)ldb);
+    return 0;
 }
 
 }  // namespace
 
+extern "C" int64_t ifl_block8_matmul_scratch_floats(int64_t M, int64_t N, int64_t K, int otype)
+{
+    if (M < 1 || N < 1 || K < 1) return 0;
+    const Plan p = mm8_plan(M, N, K, otype);
+    return p.split > 1 ? p.split * M * N : 0;
+}
+
 extern "C" int ifl_block8_matmul(const uint8_t* a, int64_t lda, const uint8_t* sa, int64_t lsa, int fa, const uint8_t* b, int64_t ldb,
                                  const uint8_t* sb, int64_t lsb, int fb, const void* bias, int btype, void* out, int otype, int64_t ldo,
-                                 int64_t M, int64_t N, int64_t K, void* stream)
+                                 float* scratch, int64_t M, int64_t N, int64_t K, void* stream)
 {
     IFL_CHECK_ARG(b8_fmt_ok(fa) && b8_fmt_ok(fb), IFL_EINVAL, "block8_matmul: formats %d, %d", fa, fb);
-    IFL_CHECK_ARG(b8_type_ok(otype) && (!bias || b8_type_ok(btype)), IFL_EINVAL, "block8_matmul: element types");
-    IFL_CHECK_ARG(M >= 0 && N >= 1 && K >= 1 && K <= 0x7ffffc00, IFL_EINVAL, "block8_matmul: %lld x %lld x %lld", (long long)M, (long long)N, (long long)K);
+    if (int rc = mm8_check(M, N, K, b, ldb, sb, lsb, bias, btype, out, otype, ldo)) return rc;
     if (M == 0) return 0;
-    const int KB = ifl_cdiv((int)K, B8_BLK);
-    IFL_CHECK_ARG(a && b && sa && sb && out, IFL_EINVAL, "block8_matmul: null pointer");
-    IFL_CHECK_ARG(lda >= K && ldb >= K && lsa >= KB && lsb >= KB && ldo >= N, IFL_EINVAL, "block8_matmul: row strides");
-    IFL_CHECK_ARG(lda % 16 == 0 && ldb % 16 == 0 && (uintptr_t)a % 16 == 0 && (uintptr_t)b % 16 == 0, IFL_EINVAL, "block8_matmul: codes in rows of whole, aligned 16 bytes");
-    IFL_CHECK_ARG((M + 63) / 64 <= 65535 && (N + 63) / 64 <= 0x7fffffff, IFL_ENOTSUP, "block8_matmul: %lld x %lld", (long long)M, (long long)N);
-    const MM8 q = {a, b, sa, sb, lda, ldb, lsa, lsb, bias, btype, out, ldo, M, N, (int)K};
-    const dim3 grid((unsigned)((N + 63) / 64), (unsigned)((M + 63) / 64));
-#define MM8_GO(FA, FB) B8_DISPATCH(otype, hipLaunchKernelGGL(HIP_KERNEL_NAME(mm8_direct_kernel<FA, FB, T>), grid, dim3(256), 0, (hipStream_t)stream, q))
-    if (fa == 0 && fb == 0) MM8_GO(0, 0); else if (fa == 0) MM8_GO(0, 1); else if (fb == 0) MM8_GO(1, 0); else MM8_GO(1, 1);
-    IFL_LAUNCH_CHECK();
-    return 0;
+    IFL_CHECK_ARG(a && sa, IFL_EINVAL, "block8_matmul: null pointer");
+    IFL_CHECK_ARG(lda >= K && lsa >= ifl_cdiv((int)K, B8_BLK), IFL_EINVAL, "block8_matmul: row strides");
+    IFL_CHECK_ARG(lda % 16 == 0 && (uintptr_t)a % 16 == 0 && lsa % 4 == 0 && (uintptr_t)sa % 4 == 0, IFL_EINVAL,
+                  "block8_matmul: codes in rows of whole, aligned 16 bytes, scales of whole, aligned 4");
+    IFL_CHECK_ARG(lda < (1 << 23), IFL_ENOTSUP, "block8_matmul: rows of %lld bytes", (long long)lda);
+    const Plan p = mm8_plan(M, N, K, otype);
+    IFL_CHECK_ARG(p.split == 1 || scratch, IFL_EINVAL, "block8_matmul: no scratch");
+    MM8 q = {};
+    q.a = a; q.b = b; q.sa = sa; q.sb = sb; q.lda = lda; q.ldb = ldb; q.lsa = lsa; q.lsb = lsb; q.bias = bias; q.btype = btype;
+    q.out = out; q.otype = otype; q.ldo = ldo; q.M = M; q.N = N; q.K = (int)K; q.part = scratch;
+    hipStream_t st = (hipStream_t)stream;
+    if (fa == 0 && fb == 0) return mm8_launch<0, 0>(q, p, st);
+    if (fa == 0) return mm8_launch<0, 1>(q, p, st);
+    if (fb == 0) return mm8_launch<1, 0>(q, p, st);
+    return mm8_launch<1, 1>(q, p, st);
+}
+
+extern "C" int64_t ifl_block8_linear_scratch_bytes(int64_t M, int64_t N, int64_t K, int otype)
+{
+    if (M < 1 || N < 1 || K < 1) return 0;
+    if (M * K <= SK_OWN / 2 && M <= 16) return 0;
+    return M * ((K + 15) / 16 * 16) + M * ((K + 511) / 512 * 4) + 4 * ifl_block8_matmul_scratch_floats(M, N, K, otype) + 16;
+}
+
+extern "C" int ifl_block8_linear(const void* x, int xtype, int64_t ldx, const uint8_t* b, int64_t ldb, const uint8_t* sb, int64_t lsb, int fb,
+                                 const void* bias, int btype, void* out, int64_t ldo, void* scratch, int64_t M, int64_t N, int64_t K,
+                                 void* stream)
+{
+    IFL_CHECK_ARG(b8_fmt_ok(fb) && b8_type_ok(xtype), IFL_EINVAL, "block8_linear: types");
+    if (int rc = mm8_check(M, N, K, b, ldb, sb, lsb, bias, btype, out, xtype, ldo)) return rc;
+    if (M == 0) return 0;
+    IFL_CHECK_ARG(x && (M == 1 || ldx >= K), IFL_EINVAL, "block8_linear: x");
+    hipStream_t st = (hipStream_t)stream;
+    if (M * K <= SK_OWN / 2 && M <= 16) {
+        MM8 q = {};
+        q.b = b; q.sb = sb; q.ldb = ldb; q.lsb = lsb; q.bias = bias; q.btype = btype; q.out = out; q.otype = xtype; q.ldo = ldo;
+        q.M = M; q.N = N; q.K = (int)K; q.x = x; q.ldx = ldx;
+        const int KB = ifl_cdiv((int)K, B8_BLK), sm = (int)M * KB * B8_BLK + (int)M * KB;
+        const dim3 grid((unsigned)((N + 15) / 16)), block(64 * SK_WAVES);
+#define MM8_OWN(FB) do { \
+            if (xtype == IFL_T_F32) hipLaunchKernelGGL(HIP_KERNEL_NAME(mm8_skinny_kernel<1, 0, FB, true, true, float>), grid, block, sm, st, q); \
+            else if (xtype == IFL_T_BF16) hipLaunchKernelGGL(HIP_KERNEL_NAME(mm8_skinny_kernel<1, 0, FB, false, true, __bf16>), grid, block, sm, st, q); \
+            else hipLaunchKernelGGL(HIP_KERNEL_NAME(mm8_skinny_kernel<1, 0, FB, false, true, _Float16>), grid, block, sm, st, q); } while (0)
+        if (fb == 0) MM8_OWN(0); else MM8_OWN(1);
+        IFL_LAUNCH_CHECK();
+        return 0;
+    }
+    IFL_CHECK_ARG(scratch && (uintptr_t)scratch % 16 == 0, IFL_EINVAL, "block8_linear: scratch");
+    const int64_t lda = (K + 15) / 16 * 16, lsa = (K + 511) / 512 * 4;
+    uint8_t* codes = (uint8_t*)scratch;
+    uint8_t* scales = codes + M * lda;
+    float* part = (float*)(scales + M * lsa);                            // (both sizes are multiples of 4)
+    if (int rc = ifl_block8_quantize(x, xtype, ldx, 1, codes, lda, scales, lsa, M, K, IFL_Q_E4M3, stream)) return rc;
+    return ifl_block8_matmul(codes, lda, scales, lsa, IFL_Q_E4M3, b, ldb, sb, lsb, fb, bias, btype, out, xtype, ldo, part, M, N, K, stream);
 }

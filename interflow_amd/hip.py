@@ -142,7 +142,12 @@ def lib():
     vp, ll = c_void_p, c_int64
     L.ifl_block8_quantize.argtypes = [vp, c_int, ll, ll, vp, ll, vp, ll, ll, ll, c_int, vp]
     L.ifl_block8_dequantize.argtypes = [vp, ll, vp, ll, c_int, vp, vp, c_int, ll, ll, ll, vp]
-    L.ifl_block8_matmul.argtypes = [vp, ll, vp, ll, c_int, vp, ll, vp, ll, c_int, vp, c_int, vp, c_int, ll, ll, ll, ll, vp]
+    L.ifl_block8_matmul.argtypes = [vp, ll, vp, ll, c_int, vp, ll, vp, ll, c_int, vp, c_int, vp, c_int, ll, vp, ll, ll, ll, vp]
+    L.ifl_block8_matmul_scratch_floats.argtypes = [ll, ll, ll, c_int]
+    L.ifl_block8_matmul_scratch_floats.restype = ll
+    L.ifl_block8_linear.argtypes = [vp, c_int, ll, vp, ll, vp, ll, c_int, vp, c_int, vp, ll, vp, ll, ll, ll, vp]
+    L.ifl_block8_linear_scratch_bytes.argtypes = [ll, ll, ll, c_int]
+    L.ifl_block8_linear_scratch_bytes.restype = ll
     L.ifl_block8_wgrad_scratch_floats.argtypes = [ll, ll, ll]
     L.ifl_block8_wgrad_scratch_floats.restype = ll
     L.ifl_block8_wgrad.argtypes = [vp, c_int, ll, vp, ll, vp, ll, c_int, vp, vp, c_int, ll, vp, c_int, vp, ll, ll, ll, vp]
@@ -150,7 +155,7 @@ def lib():
     L.ifl_an_relu8_blocks.restype = ll
     L.ifl_an_relu8_fwd.argtypes = [vp, vp, vp, vp, vp, vp, c_int, c_int, c_int, c_int, vp]
     L.ifl_an_relu8_bwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, c_int, c_int, c_int, c_int, vp]
-    for name in ("ifl_block8_quantize", "ifl_block8_dequantize", "ifl_block8_matmul", "ifl_block8_wgrad", "ifl_an_relu8_fwd", "ifl_an_relu8_bwd"):
+    for name in ("ifl_block8_quantize", "ifl_block8_dequantize", "ifl_block8_matmul", "ifl_block8_linear", "ifl_block8_wgrad", "ifl_an_relu8_fwd", "ifl_an_relu8_bwd"):
         getattr(L, name).restype = c_int
     L.ifl_prof_enable.argtypes = [c_int]
     L.ifl_prof_enable.restype = c_int
@@ -174,7 +179,8 @@ EXPORTS = ("ifl_version", "ifl_last_error", "ifl_step_param_floats", "ifl_step_f
            "ifl_an_relu_blocks", "ifl_an_relu_fwd", "ifl_an_relu_bwd", "ifl_coupling_blocks", "ifl_coupling_fwd", "ifl_coupling_bwd", "ifl_resize_sep",
            "ifl_adam_table", "ifl_wino4_untile", "ifl_rrdb_train_ws_bytes", "ifl_rrdb_train_ws_init", "ifl_rrdb_train_fwd", "ifl_rrdb_train_bwd", "ifl_pack_table", "ifl_affine_px_blocks", "ifl_train_level_fwd", "ifl_train_level_bwd", "ifl_train_vg_floats",
            "ifl_train_bulk_conv1", "ifl_wino4_tiles", "ifl_wino4_kmajor", "ifl_wino4_dw", "ifl_conv2d_wgrad_batched", "ifl_conv2d_batched",
-           "ifl_block8_quantize", "ifl_block8_dequantize", "ifl_block8_matmul", "ifl_block8_wgrad_scratch_floats", "ifl_block8_wgrad",
+           "ifl_block8_quantize", "ifl_block8_dequantize", "ifl_block8_matmul", "ifl_block8_matmul_scratch_floats",
+           "ifl_block8_linear", "ifl_block8_linear_scratch_bytes", "ifl_block8_wgrad_scratch_floats", "ifl_block8_wgrad",
            "ifl_an_relu8_blocks", "ifl_an_relu8_fwd", "ifl_an_relu8_bwd")
 
 K_CONV1_FT_L1, K_CONV1_FT_L2, K_CONV1_FINISH, K_CONV3_F, K_CONV3_ENC, K_CONV3_DEC, K_ANIC = range(7)

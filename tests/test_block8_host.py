@@ -83,11 +83,11 @@ def test_checkpoint_switch():
     ("ifl_block8_dequantize", (16, 63, 16, 1, 0, None, 16, 0, 64, 1, 64, None)),
     ("ifl_block8_dequantize", (16, 64, 16, 1, 0, None, 16, 3, 64, 1, 64, None)),
     ("ifl_block8_dequantize", (16, 64, 16, 1, 0, None, None, 0, 64, 1, 64, None)),
-    ("ifl_block8_matmul", (16, 64, 16, 4, 0, 16, 64, 16, 4, 2, None, 0, 16, 0, 8, 1, 8, 64, None)),
-    ("ifl_block8_matmul", (16, 72, 16, 4, 0, 16, 64, 16, 4, 0, None, 0, 16, 0, 8, 1, 8, 64, None)),
-    ("ifl_block8_matmul", (8, 64, 16, 4, 0, 16, 64, 16, 4, 0, None, 0, 16, 0, 8, 1, 8, 64, None)),
-    ("ifl_block8_matmul", (16, 64, 16, 4, 0, 16, 64, 16, 4, 0, None, 0, 16, 0, 7, 1, 8, 64, None)),
-    ("ifl_block8_matmul", (16, 64, 16, 4, 0, 16, 64, 16, 4, 0, None, 0, 16, 0, 8, 1, 0, 64, None)),
+    ("ifl_block8_matmul", (16, 64, 16, 4, 0, 16, 64, 16, 4, 2, None, 0, 16, 0, 8, None, 1, 8, 64, None)),
+    ("ifl_block8_matmul", (16, 72, 16, 4, 0, 16, 64, 16, 4, 0, None, 0, 16, 0, 8, None, 1, 8, 64, None)),
+    ("ifl_block8_matmul", (8, 64, 16, 4, 0, 16, 64, 16, 4, 0, None, 0, 16, 0, 8, None, 1, 8, 64, None)),
+    ("ifl_block8_matmul", (16, 64, 16, 4, 0, 16, 64, 16, 4, 0, None, 0, 16, 0, 7, None, 1, 8, 64, None)),
+    ("ifl_block8_matmul", (16, 64, 16, 4, 0, 16, 64, 16, 4, 0, None, 0, 16, 0, 8, None, 1, 0, 64, None)),
     ("ifl_block8_wgrad", (16, 0, 8, 16, 64, 16, 1, 0, None, None, 0, 64, None, 0, None, 4, 8, 64, None)),
     ("ifl_block8_wgrad", (16, 0, 7, 16, 64, 16, 1, 0, None, 16, 0, 64, None, 0, None, 4, 8, 64, None)),
     ("ifl_block8_wgrad", (16, 5, 8, 16, 64, 16, 1, 0, None, 16, 0, 64, None, 0, None, 4, 8, 64, None)),
