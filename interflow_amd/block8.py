@@ -148,7 +148,7 @@ def dequantize(q: Block8, dtype=torch.float32) -> torch.Tensor:
 def _operand(q, name):
     """(codes, scales) as the product reads them: aligned rows of whole 16 and 4 bytes; copies where they are not."""
     if not isinstance(q, Block8):
-        raise TypeError(f"matmul {name}: expected a Block8")
+        raise TypeError(f"{name}: expected a Block8")
     codes, scales = q.codes, q.scales
     if _ld(codes) % 16 or codes.data_ptr() % 16:
         if codes.shape[0] != 1 or codes.data_ptr() % 16:
@@ -225,7 +225,8 @@ def weight_grad(dy, q: Block8, dtype=torch.float32, bias_dtype=None, weight: boo
     _same_device(dy.device, q)
     if not _rows_apart(dy):
         dy = dy.contiguous()
-    return _wgrad(dy, q.codes, q.scales, None, _dtype(dtype, "weight_grad") if weight else None,
+    codes, scales = _operand(q, "checkpoint") if weight else (None, None)
+    return _wgrad(dy, codes, scales, None, _dtype(dtype, "weight_grad") if weight else None,
                   _dtype(bias_dtype, "weight_grad") if bias_dtype is not None else None)
 
 
@@ -238,7 +239,7 @@ def _wgrad(dy, codes, scales, chan, dtype, bias_dtype):
         if bias_dtype is None:
             return None, None
         db = torch.empty((N,), dtype=bias_dtype, device=dev)
-        n = hip.lib().ifl_block8_wgrad_scratch_floats(M, N, 0)
+        n = hip.lib().ifl_block8_wgrad_scratch_floats(M, N, 0, _TYPE[dy.dtype])
         scratch = torch.empty((n,), dtype=torch.float32, device=dev) if n else None
         _call("ifl_block8_wgrad", dev, dy.data_ptr(), _TYPE[dy.dtype], _ld(dy), None, 0, None, 0, 0, None, None, 0, 0, db.data_ptr(), _TYPE[bias_dtype],
               scratch.data_ptr() if n else None, M, N, 0)
@@ -246,7 +247,7 @@ def _wgrad(dy, codes, scales, chan, dtype, bias_dtype):
     K = codes.shape[1]
     dw = torch.empty((N, K), dtype=dtype, device=dev)
     db = torch.empty((N,), dtype=bias_dtype, device=dev) if bias_dtype is not None else None
-    n = hip.lib().ifl_block8_wgrad_scratch_floats(M, N, K)
+    n = hip.lib().ifl_block8_wgrad_scratch_floats(M, N, K, _TYPE[dy.dtype])
     scratch = torch.empty((n,), dtype=torch.float32, device=dev) if n else None
     _call("ifl_block8_wgrad", dev, dy.data_ptr(), _TYPE[dy.dtype], _ld(dy), codes.data_ptr(), _ld(codes), scales.data_ptr(), _ld(scales),
           _FMT_OF[codes.dtype], chan.data_ptr() if chan is not None else None, dw.data_ptr(), _TYPE[dtype], K,

@@ -86,8 +86,9 @@ __device__ __forceinline__ void mm8_store(const MM8& q, int64_t m, int64_t n, co
 // ------------------------------------------------------------------------------------------------ tiles
 // Workgroup = TN x TM of the result, K in steps of 128 bytes through two LDS buffers: while one is multiplied, the other is
 // filled by loads that go straight to LDS (16 bytes a lane, no registers).  Those write LDS in lane order, so rows lie 128 bytes
-// apart and it is the SOURCE that is permuted: position p of row r holds the 16 bytes p ^ s(r), s(r) = (r ^ r >> 2) & 7, which
-// makes every 16-byte fragment read free of bank conflicts.  Rows past the end repeat the last one (their results are not
+// apart and it is the SOURCE that is permuted: position p of row r holds the 16 bytes p ^ s(r).  s takes 8 different values in the
+// rows that 8 neighbouring lanes read, so no fragment read has bank conflicts, and the same value in all fragments of a
+// lane, so that their addresses differ by constants.  Rows past the end repeat the last one (their results are not
 // stored); a last step that K does not fill goes through registers with zeros behind K.
 //
 // Waves WN x WM; a wave has NF x MF fragments of 16 x 16.  Row r of n-fragment f is row 16 G (f / G) + 4 G (r / 4) + 4 (f % G) +
@@ -97,118 +98,174 @@ __device__ __forceinline__ void mm8_store(const MM8& q, int64_t m, int64_t n, co
 // Workgroups go to the 8 XCDs in turn; an XCD takes a contiguous run of tiles, in groups of 8 along m, so that the 32 tiles
 // it works on at a time share rows of both operands in its own L2.
 template <int TN, int TM, int WN, int WM, int FA, int FB, bool EXACT, bool SPLIT>
-__global__ __launch_bounds__(64 * WN * WM)
+__global__ __launch_bounds__(64 * WN * WM, 1)
 void mm8_tile_kernel(MM8 q)
 {
     constexpr int NW = WN * WM, NF = TN / WN / 16, MF = TM / WM / 16, G = NF < 4 ? NF : 4;
     constexpr int CH = (TN + TM) * 8, PER = CH / (64 * NW);              // 16-byte pieces of a step, per thread
+    constexpr int D = 1, R = 2 * D;                                          // n-fragments read ahead, and the registers they rotate through
+    static_assert(NF % R == 0 && D < R, "");
     __shared__ __attribute__((aligned(16))) uint8_t buf0[(TN + TM) * 128];
     __shared__ __attribute__((aligned(16))) uint8_t buf1[(TN + TM) * 128];
-    __shared__ uint32_t sc[2][TN + TM];                                  // scale bytes of four steps, per row
+    constexpr int SR = (TN + TM + 64 * NW - 1) / (64 * NW);              // rows of scales per thread
+    __shared__ uint32_t sc[2][SR * 64 * NW];                                  // scale bytes of four steps, per row
     const int tiles = q.tiles_m * q.tiles_n;
     const int t = (blockIdx.x & 7) * q.per_xcd + (blockIdx.x >> 3);
     if (t >= tiles) return;
     const int gsz = 8 * q.tiles_n, grp = t / gsz, rest = t - grp * gsz;
     const int gm = min(8, q.tiles_m - grp * 8);
-    const int tm = grp * 8 + rest % gm, tn = rest / gm;
+    const int tm = __builtin_amdgcn_readfirstlane(grp * 8 + rest % gm), tn = __builtin_amdgcn_readfirstlane(rest / gm);
     const int64_t n0 = (int64_t)tn * TN, m0 = (int64_t)tm * TM;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, g = lane >> 4;
     const int wn = wave % WN, wm = wave / WN;
 
+    // s(r): n side its bits 0, 1 and the one that r16's bit 2 goes to; m side bits 0 .. 2
+    auto swz = [&](int row, bool nside) { return nside ? (row & 3) | (row / (4 * G) & 1) << 2 : row & 7; };
     // where this thread's pieces come from: 32-bit offsets from the tile's first rows
+    auto piece = [&](int i, bool nside, int& ch) {
+        const int p = (i * NW + wave) * 64 + lane, row = p >> 3, r = nside ? row : row - TN;
+        ch = (p & 7) ^ swz(r, nside);
+        const int64_t left = nside ? q.N - 1 - n0 : q.M - 1 - m0;
+        return (uint32_t)((int64_t)(r < left ? r : (int)left) * (nside ? q.ldb : q.lda));
+    };
     uint32_t off[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        const int p = (i * NW + wave) * 64 + lane, row = p >> 3, ch = (p & 7) ^ ((row ^ row >> 2) & 7);
-        const bool nside = row < TN;
-        const int64_t left = nside ? q.N - 1 - n0 : q.M - 1 - m0;
-        const int r = nside ? row : row - TN;
-        off[i] = (uint32_t)((int64_t)(r < left ? r : (int)left) * (nside ? q.ldb : q.lda)) + ch * 16;
+        int ch;
+        off[i] = piece(i, (i * NW * 64) >> 3 < TN, ch);
+        off[i] += ch * 16;
     }
     const uint8_t* bb = q.b + n0 * q.ldb;
     const uint8_t* ab = q.a + m0 * q.lda;
     const int k_first = SPLIT ? blockIdx.y * q.ksteps : 0;
     const int all = (q.K + B8_BLK - 1) / B8_BLK, k_end = SPLIT ? min(all, k_first + q.ksteps) : all;
 
+    const int whole = min(k_end, q.K / B8_BLK);                          // steps that K fills
     auto fill = [&](uint8_t* buf, int ks) {
-        const int k0 = ks * B8_BLK;
-        if (k0 + B8_BLK <= q.K) {
+        int k0 = __builtin_amdgcn_readfirstlane(ks) * B8_BLK;
+        asm volatile("" : "+s"(k0));                                     // (a scalar offset at every step: sums per lane would be kept in registers)
+        const uint8_t *bk = bb + k0, *ak = ab + k0;
 #pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                const uint8_t* src = ((i * NW * 64) >> 3 < TN ? bb : ab) + k0;      // (a piece's side is the same for all waves)
-                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + off[i]),
-                                                 (__attribute__((address_space(3))) void*)(buf + (i * NW + wave) * 1024), 16, 0, 0);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                const int p = (i * NW + wave) * 64 + lane, row = p >> 3, ch = (p & 7) ^ ((row ^ row >> 2) & 7);
-                const uint8_t* src = ((i * NW * 64) >> 3 < TN ? bb : ab) + (off[i] - ch * 16);
-                *(i32x4*)(buf + p * 16) = mm8_load16(src, k0 + ch * 16, q.K);
-            }
+        for (int i = 0; i < PER; ++i) {
+            const uint8_t* src = (i * NW * 64) >> 3 < TN ? bk : ak;      // (a piece's side is the same for all waves)
+            uint32_t o = off[i];
+            asm volatile("" : "+v"(o));                                  // (a 32-bit offset at the load, not a 64-bit one kept for it)
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + o),
+                                             (__attribute__((address_space(3))) void*)(buf + (i * NW + wave) * 1024), 16, 0, 0);
+        }
+    };
+    auto fill_last = [&](uint8_t* buf, int ks) {
+#pragma unroll 1
+        for (int i = 0; i < PER; ++i) {
+            const bool nside = (i * NW * 64) >> 3 < TN;
+            int ch;
+            const uint32_t o = piece(i, nside, ch);
+            *(i32x4*)(buf + ((i * NW + wave) * 64 + lane) * 16) = mm8_load16((nside ? bb : ab) + o, ks * B8_BLK + ch * 16, q.K);
         }
     };
 
-    // fragment addresses.  Rows of one lane's fragments differ by constants, and so do, after an XOR, their swizzled positions:
-    // s(row) = s0 ^ f % 4 ^ 4 (f & 1) on the n side, s0 ^ 4 (f & 1) on the m side.
-    const int nrow0 = wn * NF * 16 + 4 * G * (r16 >> 2) + (r16 & 3), mrow0 = TN + wm * MF * 16 + r16;
-    const int ns = (r16 & 3) ^ ((r16 >> 2) & 1) << 2, ms = (r16 & 7) ^ r16 >> 2;
-    auto npos = [&](int f, int c) {
-        const int row = nrow0 + 16 * G * (f / G) + 4 * (f % G);
-        const int s = G == 4 ? ns ^ (f % G) ^ (f & 1) << 2 : (row ^ row >> 2) & 7;
-        return row * 128 + ((g + 4 * c) ^ s) * 16;
-    };
-    auto mpos = [&](int f, int c) { return (mrow0 + 16 * f) * 128 + ((g + 4 * c) ^ ms ^ (f & 1) << 2) * 16; };
+    // fragment addresses of this lane in LDS, but for constants: its two 16-byte pieces of fragment 0 of either side
+    const int nrow0 = wn * NF * 16 + 4 * G * (r16 >> 2) + (r16 & 3), mrow0 = wm * MF * 16 + r16;
+    const int nat[2] = {nrow0 * 128 + (g ^ swz(nrow0, true)) * 16, nrow0 * 128 + ((g + 4) ^ swz(nrow0, true)) * 16};
+    const int mat[2] = {(TN + mrow0) * 128 + (g ^ swz(mrow0, false)) * 16, (TN + mrow0) * 128 + ((g + 4) ^ swz(mrow0, false)) * 16};
+    auto nrow = [](int f) { return 16 * G * (f / G) + 4 * (f % G); };
 
-    // a thread's row of the scales (the tile has at most as many rows as threads)
-    const int srow = threadIdx.x;
-    const bool has_s = srow < TN + TM;
-    const uint8_t* sp = srow < TN ? q.sb + min(n0 + srow, q.N - 1) * q.lsb : q.sa + min(m0 + (srow - TN), q.M - 1) * q.lsa;
-    uint32_t snext = 0;
+    // a thread's rows of the scales (threads past the tile's rows repeat one): n side first
+    const uint8_t* sp[SR];
+#pragma unroll
+    for (int i = 0; i < SR; ++i) {
+        const int r = i * 64 * NW + threadIdx.x;
+        sp[i] = r < TN ? q.sb + min(n0 + r, q.N - 1) * q.lsb : q.sa + min(m0 + (r - TN), q.M - 1) * q.lsa;
+    }
+    uint32_t snext[SR];
 
     f32x4 acc[NF][MF] = {};
-    auto multiply = [&](const uint8_t* buf, int ks) {
+    i32x8 a[1][MF], b[R];
+    int ca[1][MF], cb[R];
+    // (Addresses are made anew for each fragment: the second buffer's are out of an instruction's offset range, and the compiler
+    // would keep one register for each of them.)
+    auto fresh = [](int x) { asm volatile("" : "+v"(x)); return x; };
+    auto read_a = [&](const uint8_t* buf, int ks, int o) {
         const uint8_t* s = (const uint8_t*)sc[(ks >> 2) & 1] + (ks & 3);
-        i32x8 a[MF];
-        int ca[MF];
 #pragma unroll
         for (int j = 0; j < MF; ++j) {
-            a[j] = mm8_join(*(const i32x4*)(buf + mpos(j, 0)), *(const i32x4*)(buf + mpos(j, 1)));
-            ca[j] = s[4 * (mrow0 + 16 * j)];
-        }
-#pragma unroll
-        for (int i = 0; i < NF; ++i) {
-            const i32x8 b = mm8_join(*(const i32x4*)(buf + npos(i, 0)), *(const i32x4*)(buf + npos(i, 1)));
-            const int cb = s[4 * (nrow0 + 16 * G * (i / G) + 4 * (i % G))];
-#pragma unroll
-            for (int j = 0; j < MF; ++j) acc[i][j] = mm8_mfma<FA, FB, EXACT>(b, a[j], acc[i][j], cb, ca[j]);
+            a[o][j] = mm8_join(*(const i32x4*)(buf + fresh(mat[0]) + 2048 * j), *(const i32x4*)(buf + fresh(mat[1]) + 2048 * j));
+            ca[o][j] = s[4 * (TN + mrow0 + 16 * j)];
         }
     };
-    // behind step ks: the scales of the next four steps are asked for at the first of these four and put into LDS at the last
-    auto scales = [&](int ks) {
-        if ((ks & 3) == 0 && ks + 4 < k_end && has_s) snext = ((const uint32_t*)sp)[(ks >> 2) + 1];
-        if ((ks & 3) == 3 && has_s) sc[((ks >> 2) + 1) & 1][srow] = snext;
+    auto read_b = [&](const uint8_t* buf, int ks, int i) {
+        const uint8_t* s = (const uint8_t*)sc[(ks >> 2) & 1] + (ks & 3);
+        b[i % R] = mm8_join(*(const i32x4*)(buf + fresh(nat[0]) + 128 * nrow(i)), *(const i32x4*)(buf + fresh(nat[1]) + 128 * nrow(i)));
+        cb[i % R] = s[4 * (nrow0 + nrow(i))];
     };
     auto turn = [&]() {
-        __builtin_amdgcn_s_waitcnt(0x0f70);                              // vmcnt(0): this wave's pieces of the next step are in LDS
+        __builtin_amdgcn_s_waitcnt(0x0070);                              // vmcnt(0), lgkmcnt(0)
         __syncthreads();
     };
+    // One step: NF groups of MF products.  Fragments of the n side are read D groups ahead.  Before the last D groups everything
+    // this step needs is in registers, and the next step's bytes have had the time of NF - D groups to arrive: there the
+    // workgroup meets, this step's buffer is handed to the step after the next, and the next step's first fragments are read
+    // while the last D groups run.
+    // (No branches inside, the compiler would move products past them: behind the last steps it is the last whole step that is
+    // loaded again, unused.)
+    auto step = [&](uint8_t* cur, const uint8_t* nxt, int ks, int o) {
+#pragma unroll
+        for (int i = 0; i < NF; ++i) {
+            if (i + D < NF) read_b(cur, ks, i + D);
+            if (i == NF - D) {
+                turn();
+                fill(cur, min(ks + 2, whole - 1));
+            }
+            if (i >= NF - D) read_b(nxt, ks + 1, i + D - NF);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int j = 0; j < MF; ++j) acc[i][j] = mm8_mfma<FA, FB, EXACT>(b[i % R], a[0][j], acc[i][j], cb[i % R], ca[0][j]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        read_a(nxt, ks + 1, 0);
+    };
 
-    if (has_s) sc[(k_first >> 2) & 1][srow] = ((const uint32_t*)sp)[k_first >> 2];        // (k_first is a multiple of 4)
-    fill(buf0, k_first);
-    turn();
-    for (int ks = k_first; ks < k_end; ks += 2) {
-        if (ks + 1 < k_end) fill(buf1, ks + 1);
-        scales(ks);
-        multiply(buf0, ks);
+    const int last = (k_end - 1) >> 2;
+    auto ask = [&](int grp) {
+#pragma unroll
+        for (int i = 0; i < SR; ++i) snext[i] = ((const uint32_t*)sp[i])[min(grp, last)];
+    };
+    auto put = [&](int grp) {
+#pragma unroll
+        for (int i = 0; i < SR; ++i) sc[grp & 1][i * 64 * NW + threadIdx.x] = snext[i];
+    };
+    ask(k_first >> 2);                                                   // (k_first is a multiple of 4)
+    put(k_first >> 2);
+    int ks = k_first;
+    if (ks < whole) {
+        fill(buf0, ks);
         turn();
-        if (ks + 1 < k_end) {
-            if (ks + 2 < k_end) fill(buf0, ks + 2);
-            scales(ks + 1);
-            multiply(buf1, ks + 1);
-            turn();
+        fill(buf1, min(ks + 1, whole - 1));
+        read_a(buf0, ks, 0);
+#pragma unroll
+        for (int e = 0; e < D; ++e) read_b(buf0, ks, e);
+        // scales of the next four steps are asked for and put into LDS in every pair of steps, needed or not: no branch
+        for (; ks + 1 < whole; ks += 2) {
+            ask((ks >> 2) + 1);
+            step(buf0, buf1, ks, 0);
+            put((ks >> 2) + 1);
+            step(buf1, buf0, ks + 1, 1);
+        }
+        if (ks < whole) step(buf0, buf1, ks, 0);
+    }
+    if (k_end > whole) {                                                 // a last step that K does not fill
+        turn();
+        fill_last(buf0, whole);
+        turn();
+        read_a(buf0, whole, 0);
+#pragma unroll
+        for (int i = 0; i < NF; ++i) {
+            read_b(buf0, whole, i);
+#pragma unroll
+            for (int j = 0; j < MF; ++j) acc[i][j] = mm8_mfma<FA, FB, EXACT>(b[i % R], a[0][j], acc[i][j], cb[i % R], ca[0][j]);
         }
     }
+    __builtin_amdgcn_s_waitcnt(0x0f70);
 
     const int64_t nw = n0 + wn * NF * 16 + 4 * G * g;
     if constexpr (SPLIT) {

@@ -1,84 +1,392 @@
 // wgrad8.hip -- the weight gradient of a product whose input was kept in 8-bit blocks (block8.h):
 //     dw[n][k] = chan[k] sum_m dy[m][n] code[m][k] 2^e[m][k / 128],      db[n] = sum_m dy[m][n]
-// The sum runs over the rows of both operands, whose scales change from row to row, so the 8-bit instructions cannot apply them;
-// a code times its scale is exact in bf16.
+// The sum runs over the rows of both operands, whose scales change from row to row, so the 8-bit instructions cannot apply them.
+// A code times its scale is exact in bf16, and so is a bf16 gradient; a float16 gradient is the sum of two bf16 terms and a
+// float32 one of three (its 24 significant bits in pieces of 8).  So every product goes exactly through
+// v_mfma_f32_16x16x32_bf16 (one, two or three of them), which keeps 24 bits of the sums.
 #include "block8.h"
 
 namespace {
 
-template <class T, class TW>
-__global__ __launch_bounds__(256)
-void wgrad8_simple_kernel(const T* __restrict__ dy, int64_t ldy, const uint8_t* __restrict__ codes, int64_t ldc, const uint8_t* __restrict__ scales,
-                          int64_t lds, int fmt, const float* __restrict__ chan, TW* __restrict__ dw, int64_t ldw, int64_t M, int N, int K)
-{
-    __shared__ float sy[16][64 + 4], sx[16][64 + 4];
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const int k0 = blockIdx.x * 64, n0 = blockIdx.y * 64;
-    float acc[4][4] = {};
-    for (int64_t m0 = 0; m0 < M; m0 += 16) {
-        for (int i = threadIdx.x; i < 16 * 64; i += 256) {
-            const int r = i >> 6, c = i & 63;
-            const int64_t m = m0 + r;
-            sy[r][c] = m < M && n0 + c < N ? (float)dy[m * ldy + n0 + c] : 0.f;
-            float v[4] = {0.f, 0.f, 0.f, 0.f};
-            if (m < M && k0 + c < K) { b8_decode4(codes[m * ldc + k0 + c], fmt, v); v[0] *= b8_scale(scales[m * lds + (k0 + c) / B8_BLK]); }
-            sx[r][c] = v[0];
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+
+struct WG8 {
+    const void* dy; int64_t ldy;
+    const uint8_t* codes; int64_t ldc;
+    const uint8_t* scales; int64_t lds;
+    const float* chan;
+    void* dw; int64_t ldw; int dwtype;
+    float* part; int split, steps;       // float32 partial sums [split][N][K], steps of 64 rows per part
+    int64_t M; int N, K;
+    int tiles_n, tiles_k, per_xcd;
+    int ywide;                           // whole 16-byte loads of dy
+};
+
+// One, two or three bf16 terms whose sum is the value, as floats with 16 low zero bits: its leading 8 significant bits, the next 8,
+// the rest.  What is not finite is the first term alone.
+template <int NP>
+__device__ __forceinline__ void wg8_terms(float x, float t[NP]) {
+    if constexpr (NP == 1) t[0] = x;                                     // (from bf16)
+    else {
+        x = __builtin_canonicalizef(x);                                  // (a NaN has a high bit set)
+        t[0] = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+        float r = x - t[0];
+        r = r == r ? r : 0.f;
+#pragma unroll
+        for (int i = 1; i < NP; ++i) {
+            t[i] = __uint_as_float(__float_as_uint(r) & 0xffff0000u);
+            r -= t[i];
         }
-        __syncthreads();
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sy[r][ty * 4 + i], sx[r][tx * 4 + j], acc[i][j]);
-        __syncthreads();
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int n = n0 + ty * 4 + i, k = k0 + tx * 4 + j;
-            if (n < N && k < K) dw[(int64_t)n * ldw + k] = (TW)(chan ? acc[i][j] * chan[k] : acc[i][j]);
-        }
 }
 
-// column sums: a workgroup takes 64 columns, its four waves every fourth row, joined in LDS
-template <class T, class TW>
+template <class TW>
+__device__ __forceinline__ void wg8_store16(TW* d, int left, const float v[16]) {
+    if (left >= 16 && (uintptr_t)d % 16 == 0) { b8_store8<TW, true>(d, 8, v); b8_store8<TW, true>(d + 8, 8, v + 8); }
+    else { b8_store8<TW, false>(d, left, v); if (left > 8) b8_store8<TW, false>(d + 8, left - 8, v + 8); }
+}
+
+// Workgroup = TN x TK of dw over a range of rows, MS at a time through two LDS buffers (rows of dy and of the restored codes as they
+// lie in memory); the fragments, which run along m, come out of LDS transposed (ds_read_b64_tr_b16: 16 lanes read 4 rows of
+// 16 values and get columns).  The instruction's first operand is the k side: a lane ends up with 4 neighbouring k of one n.
+//
+// A fragment read touches, per group of 16 lanes, 4 rows and 4 pieces of 8 bytes of each.  n side: the four pieces are one granule
+// of 32 bytes, granule i of row m at place i ^ (m & 7).  k side: piece f % 4 of four neighbouring granules, so that a lane's four
+// fragments are 16 neighbouring k; piece j of granule i of row m at piece j ^ (m & 3) of place i ^ (m & 4).  Both: no bank conflicts.
+//
+// bf16 gradients go straight to LDS (DMA); others, and whatever is not aligned or is cut off, through registers, loaded one
+// step ahead.
+template <class T, int NP, int TN, int TK, int WN, int WK, int MS, int FMT, bool DMA>
+__global__ __launch_bounds__(64 * WN * WK)
+void wgrad8_kernel(WG8 q)
+{
+    constexpr int NT = 64 * WN * WK, NF = TN / WN / 16, KF = TK / WK / 16;
+    constexpr int YROW = TN * 2, XROW = TK * 2, YPL = MS * YROW;       // bytes
+    constexpr int YP = MS * TN / 8 / NT, XP = MS * TK / 16 / NT;     // pieces (8 values of dy, 16 codes) per thread
+    static_assert(KF % 4 == 0 && YP * NT * 8 == MS * TN && XP * NT * 16 == MS * TK, "");
+    __shared__ __attribute__((aligned(16))) uint8_t y0[NP * YPL], y1[NP * YPL], x0[MS * XROW], x1[MS * XROW];
+    const int all = q.tiles_n * q.tiles_k * q.split;
+    const int id = (blockIdx.x & 7) * q.per_xcd + (blockIdx.x >> 3);
+    if (id >= all) return;
+    const int part = id / (q.tiles_n * q.tiles_k), tile = id - part * (q.tiles_n * q.tiles_k);
+    const int tn = tile / q.tiles_k, tk = tile - tn * q.tiles_k;
+    const int n0 = tn * TN, k0 = tk * TK;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, g = lane >> 4;
+    const int wk = wave % WK, wn = wave / WK;
+    const int64_t mb = (int64_t)part * q.steps * MS, me = min(q.M, mb + (int64_t)q.steps * MS);
+    const int steps = (int)((me - mb + MS - 1) / MS);
+
+    // ---- staging: registers of the step that is on its way
+    float yr[DMA ? 1 : YP][8];
+    i32x4 xr[XP];
+    int xs[XP];
+    const T* dy = (const T*)q.dy;
+    // (what is cut off is loaded from a place that exists and made zero when it is stored: a load that is used or branched around at
+    // once would be waited for at once)
+    auto y_load = [&](int64_t m0) {
+        if constexpr (!DMA) {
+#pragma unroll
+            for (int i = 0; i < YP; ++i) {
+                const int p = i * NT + tid, r = p / (TN / 8), n = n0 + p % (TN / 8) * 8;
+                const T* src = dy + min(m0 + r, me - 1) * q.ldy;
+                if (q.ywide) b8_load8<T, true>(src + (n < q.N ? n : 0), 8, yr[i]);
+                else b8_load8<T, false>(src + n, q.N - n, yr[i]);
+            }
+        }
+    };
+    auto y_dma = [&](uint8_t* buf, int64_t m0) {
+        if constexpr (DMA) {
+            const uint8_t* base = (const uint8_t*)(dy + m0 * q.ldy + n0);
+#pragma unroll
+            for (int i = 0; i < YP; ++i) {
+                const int p = i * NT + tid, r = p / (TN / 8), c = p % (TN / 8);
+                const int s = ((c >> 1) ^ (r & 7)) * 2 + (c & 1);
+                const int n = n0 + s * 8 < q.N ? s * 16 : 0;             // (columns past the end: any, their results are not stored)
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(base + (uint32_t)(r * (int)q.ldy * 2 + n)),
+                                                 (__attribute__((address_space(3))) void*)(buf + (i * NT + wave * 64) * 16), 16, 0, 0);
+            }
+        }
+    };
+    auto y_store = [&](uint8_t* buf, int64_t m0) {
+        if constexpr (!DMA) {
+#pragma unroll
+            for (int i = 0; i < YP; ++i) {
+                const int p = i * NT + tid, r = p / (TN / 8), c = p % (TN / 8);
+                float t[8][NP];
+                const bool in = m0 + r < me && n0 + c * 8 < q.N;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) wg8_terms<NP>(in ? yr[i][e] : 0.f, t[e]);
+#pragma unroll
+                for (int k = 0; k < NP; ++k) {
+                    i32x4 w;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[e] = (int)__builtin_amdgcn_perm(__float_as_uint(t[2 * e + 1][k]), __float_as_uint(t[2 * e][k]), 0x07060302u);   // the high halves
+                    *(i32x4*)(buf + k * YPL + r * YROW + ((c >> 1) ^ (r & 7)) * 32 + (c & 1) * 16) = w;
+                }
+            }
+        }
+    };
+    auto x_load = [&](int64_t m0) {
+#pragma unroll
+        for (int i = 0; i < XP; ++i) {
+            const int p = i * NT + tid, r = p / (TK / 16), k = k0 + p % (TK / 16) * 16;
+            const int64_t m = min(m0 + r, me - 1);
+            const int kc = k < q.K ? k : 0;
+            xr[i] = *(const i32x4*)(q.codes + m * q.ldc + kc);
+            xs[i] = q.scales[m * q.lds + kc / B8_BLK];
+        }
+    };
+    auto x_store = [&](uint8_t* buf, int64_t m0) {
+#pragma unroll
+        for (int i = 0; i < XP; ++i) {
+            const int p = i * NT + tid, r = p / (TK / 16), c = p % (TK / 16);
+            const int left = m0 + r < me ? q.K - k0 - c * 16 : 0;
+            if (left < 16) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int l = left - 4 * e;
+                    xr[i][e] = l >= 4 ? xr[i][e] : l <= 0 ? 0 : (int)((uint32_t)xr[i][e] & ((1u << 8 * l) - 1));
+                }
+                if (left <= 0) xs[i] = 127;
+            }
+            const bf16x8 lo = b8_bf16x8<FMT>(xr[i][0], xr[i][1], xs[i]), hi = b8_bf16x8<FMT>(xr[i][2], xr[i][3], xs[i]);
+            const i32x4 a = __builtin_bit_cast(i32x4, lo), b = __builtin_bit_cast(i32x4, hi);
+            const bool odd = r & 1;                                      // piece j at j ^ (r & 3): first within 16 bytes, then the halves
+            const i32x4 u = {odd ? a[2] : a[0], odd ? a[3] : a[1], odd ? a[0] : a[2], odd ? a[1] : a[3]};
+            const i32x4 v = {odd ? b[2] : b[0], odd ? b[3] : b[1], odd ? b[0] : b[2], odd ? b[1] : b[3]};
+            uint8_t* d = buf + r * XROW + (c ^ (r & 4)) * 32;
+            *(i32x4*)(d + (r & 2 ? 16 : 0)) = u;
+            *(i32x4*)(d + (r & 2 ? 0 : 16)) = v;
+        }
+    };
+
+    // ---- fragments
+    const int mrow = 4 * g + (r16 >> 2), q4 = r16 & 3;
+    auto y_frag = [&](const uint8_t* buf, int pl, int f, int h) {
+        const uint8_t* a = buf + pl * YPL + (32 * h + mrow) * YROW + ((wn * NF + f) ^ (mrow & 7)) * 32 + q4 * 8;
+        const s16x4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a));
+        const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a + 16 * YROW));
+        return __builtin_bit_cast(bf16x8, __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    auto x_frag = [&](const uint8_t* buf, int f, int h) {
+        const uint8_t* a = buf + (32 * h + mrow) * XROW + (((wk * KF / 4 + f / 4) * 4 + q4) ^ (mrow & 4)) * 32 + ((f & 3) ^ (mrow & 3)) * 8;
+        const s16x4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a));
+        const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a + 16 * XROW));
+        return __builtin_bit_cast(bf16x8, __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    f32x4 acc[KF][NF] = {};
+    auto multiply = [&](const uint8_t* yb, const uint8_t* xb) {
+#pragma unroll
+        for (int h = 0; h < MS / 32; ++h) {
+            bf16x8 y[NF][NP];
+#pragma unroll
+            for (int f = 0; f < NF; ++f)
+#pragma unroll
+                for (int k = 0; k < NP; ++k) y[f][k] = y_frag(yb, k, f, h);
+#pragma unroll
+            for (int i = 0; i < KF; ++i) {
+                const bf16x8 x = x_frag(xb, i, h);
+#pragma unroll
+                for (int f = 0; f < NF; ++f)
+#pragma unroll
+                    for (int k = 0; k < NP; ++k) acc[i][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y[f][k], acc[i][f], 0, 0, 0);
+            }
+        }
+    };
+    auto turn = [&]() {
+        __builtin_amdgcn_s_waitcnt(0x0f70);                              // vmcnt(0): the loads that go to LDS are there
+        __syncthreads();
+    };
+
+    y_load(mb); x_load(mb);
+    y_dma(y0, mb); y_store(y0, mb); x_store(x0, mb);
+    turn();
+    for (int s = 0; s < steps; s += 2) {
+        const bool more = s + 1 < steps, more2 = s + 2 < steps;
+        const int64_t m1 = mb + (int64_t)(s + 1) * MS, m2 = m1 + MS;
+        if (more) { y_load(m1); x_load(m1); y_dma(y1, m1); }
+        multiply(y0, x0);
+        if (more) { y_store(y1, m1); x_store(x1, m1); }
+        turn();
+        if (more) {
+            if (more2) { y_load(m2); x_load(m2); y_dma(y0, m2); }
+            multiply(y1, x1);
+            if (more2) { y_store(y0, m2); x_store(x0, m2); }
+            turn();
+        }
+    }
+
+    const int kw = k0 + wk * KF * 16 + 16 * g, nw = n0 + wn * NF * 16 + r16;
+#pragma unroll
+    for (int h = 0; h < KF / 4; ++h) {
+        const int k = kw + 64 * h;
+        float ch[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) ch[e] = q.chan && k + e < q.K && q.split == 1 ? q.chan[k + e] : 1.f;
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+            const int n = nw + 16 * f;
+            float v[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] = acc[4 * h + e / 4][f][e % 4] * ch[e];
+            if (n < q.N && k < q.K) {
+                if (q.split > 1) {
+                    float* d = q.part + ((int64_t)part * q.N + n) * q.K + k;
+                    wg8_store16(d, q.K - k, v);
+                } else {
+                    const int64_t at = (int64_t)n * q.ldw + k;
+                    if (q.dwtype == IFL_T_F32) wg8_store16((float*)q.dw + at, q.K - k, v);
+                    else if (q.dwtype == IFL_T_BF16) wg8_store16((__bf16*)q.dw + at, q.K - k, v);
+                    else wg8_store16((_Float16*)q.dw + at, q.K - k, v);
+                }
+            }
+        }
+    }
+}
+
+// dw = chan * sum of the parts, in order
+template <class TW>
 __global__ __launch_bounds__(256)
-void colsum_kernel(const T* __restrict__ dy, int64_t ldy, TW* __restrict__ db, int64_t M, int N)
+void wgrad8_join_kernel(WG8 q)
+{
+    const int64_t nk = (int64_t)q.N * q.K;
+    if (q.K % 4 == 0) {
+        for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < nk; i += (int64_t)gridDim.x * 1024) {
+            f32x4 t = *(const f32x4*)(q.part + i);
+            for (int s = 1; s < q.split; ++s) t += *(const f32x4*)(q.part + s * nk + i);
+            const int n = (int)(i / q.K), k = (int)(i - (int64_t)n * q.K);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) ((TW*)q.dw)[(int64_t)n * q.ldw + k + e] = (TW)(q.chan ? t[e] * q.chan[k + e] : t[e]);
+        }
+    } else {
+        for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < nk; i += (int64_t)gridDim.x * 256) {
+            float t = q.part[i];
+            for (int s = 1; s < q.split; ++s) t += q.part[s * nk + i];
+            const int n = (int)(i / q.K), k = (int)(i - (int64_t)n * q.K);
+            ((TW*)q.dw)[(int64_t)n * q.ldw + k] = (TW)(q.chan ? t * q.chan[k] : t);
+        }
+    }
+}
+
+template <class TW>
+__global__ void fill_zero_kernel(TW* p, int64_t ld, int rows, int cols)
+{
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < (int64_t)rows * cols; i += (int64_t)gridDim.x * blockDim.x) p[i / cols * ld + i % cols] = (TW)0.f;
+}
+
+// Column sums, first pass: a workgroup takes 64 columns of a range of rows, its four waves every fourth row.  part[blk][N]
+template <class T>
+__global__ __launch_bounds__(256)
+void colsum_kernel(const T* __restrict__ dy, int64_t ldy, float* __restrict__ part, int64_t M, int N, int64_t rows_per)
 {
     __shared__ float red[4][64];
     const int c = threadIdx.x & 63, r = threadIdx.x >> 6, n = blockIdx.x * 64 + c;
+    const int64_t end = min(M, (int64_t)(blockIdx.y + 1) * rows_per);
     float t = 0.f;
-    if (n < N) for (int64_t m = r; m < M; m += 4) t += (float)dy[m * ldy + n];
+    if (n < N) {
+#pragma unroll 8
+        for (int64_t m = (int64_t)blockIdx.y * rows_per + r; m < end; m += 4) t += (float)dy[m * ldy + n];
+    }
     red[r][c] = t;
     __syncthreads();
-    if (r == 0 && n < N) db[n] = (TW)((red[0][c] + red[1][c]) + (red[2][c] + red[3][c]));
+    if (r == 0 && n < N) part[(int64_t)blockIdx.y * N + n] = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
+}
+template <class TW>
+__global__ __launch_bounds__(64)
+void colsum_join_kernel(const float* __restrict__ part, TW* __restrict__ db, int N, int parts)
+{
+    const int n = blockIdx.x * 64 + threadIdx.x;
+    if (n >= N) return;
+    float t = 0.f;
+    for (int s = 0; s < parts; ++s) t += part[(int64_t)s * N + n];
+    db[n] = (TW)t;
+}
+
+// Tiles of 256 x 256 for bf16 gradients of large layers, else 128 x 128; 128 x 256 where a gradient has two or three terms (they
+// take that much more LDS).  The rows are split until about 256 workgroups are at work, each with two steps at least.
+struct WPlan { int tn, tk, ms, split, steps, cs_parts; int64_t cs_rows; };
+WPlan wg8_plan(int64_t M, int64_t N, int64_t K, int dytype)
+{
+    WPlan p = {128, 128, 64, 1, 0, 1, 0};
+    auto tiles = [&](int64_t a, int64_t b) { return ((N + a - 1) / a) * ((K + b - 1) / b); };
+    if (dytype != IFL_T_BF16) { p.tk = 256; p.ms = 32; }
+    else if (tiles(256, 256) >= 32) p.tn = p.tk = 256;
+    const int64_t steps = (M + p.ms - 1) / p.ms, n = tiles(p.tn, p.tk);
+    int64_t s = n >= 192 ? 1 : 256 / n;
+    if (s > steps / 2) s = steps / 2;
+    if (s > 64) s = 64;
+    if (s < 1) s = 1;
+    p.steps = (int)((steps + s - 1) / s);
+    p.split = p.steps ? (int)((steps + p.steps - 1) / p.steps) : 1;
+    const int64_t cols = (N + 63) / 64;
+    int64_t c = 512 / cols;
+    if (c > M / 32) c = M / 32;
+    if (c > 256) c = 256;
+    if (c < 1) c = 1;
+    p.cs_rows = (M + c - 1) / c;
+    p.cs_parts = p.cs_rows ? (int)((M + p.cs_rows - 1) / p.cs_rows) : 1;
+    return p;
 }
 
 }  // namespace
 
-extern "C" int64_t ifl_block8_wgrad_scratch_floats(int64_t M, int64_t N, int64_t K) { (void)M; (void)N; (void)K; return 0; }
+extern "C" int64_t ifl_block8_wgrad_scratch_floats(int64_t M, int64_t N, int64_t K, int dytype)
+{
+    if (M < 1 || N < 1 || K < 0) return 0;
+    const WPlan p = wg8_plan(M, N, K > 0 ? K : 1, dytype);
+    return (K > 0 && p.split > 1 ? p.split * N * K : 0) + (int64_t)p.cs_parts * N;
+}
 
 extern "C" int ifl_block8_wgrad(const void* dy, int dytype, int64_t ldy, const uint8_t* codes, int64_t ldc, const uint8_t* scales,
                                 int64_t lds, int fmt, const float* chan, void* dw, int dwtype, int64_t ldw, void* db, int dbtype,
                                 float* scratch, int64_t M, int64_t N, int64_t K, void* stream)
 {
-    (void)scratch;
     IFL_CHECK_ARG(b8_fmt_ok(fmt) && b8_type_ok(dytype) && (!dw || b8_type_ok(dwtype)) && (!db || b8_type_ok(dbtype)), IFL_EINVAL, "block8_wgrad: types");
-    IFL_CHECK_ARG(M >= 0 && N >= 1 && (K >= 1 || !dw) && N <= 0x3fffffff && K <= 0x3fffffff, IFL_EINVAL, "block8_wgrad: %lld x %lld x %lld", (long long)M, (long long)N, (long long)K);
-    IFL_CHECK_ARG((dw || db) && (M == 0 || dy) && (M == 0 || !dw || (codes && scales)), IFL_EINVAL, "block8_wgrad: null pointer");
-    IFL_CHECK_ARG(ldy >= N && (!dw || (ldc >= K && lds >= ifl_cdiv((int)K, B8_BLK) && ldw >= K)), IFL_EINVAL, "block8_wgrad: row strides");
-    IFL_CHECK_ARG((N + 63) / 64 <= 65535, IFL_ENOTSUP, "block8_wgrad: N=%lld", (long long)N);
+    IFL_CHECK_ARG(M >= 0 && N >= 1 && (K >= 1 || !dw), IFL_EINVAL, "block8_wgrad: %lld x %lld x %lld", (long long)M, (long long)N, (long long)K);
+    IFL_CHECK_ARG(N <= 0x3fffff && K <= 0x3fffff && M < ((int64_t)1 << 40), IFL_ENOTSUP, "block8_wgrad: %lld x %lld x %lld", (long long)M, (long long)N, (long long)K);
+    IFL_CHECK_ARG((dw || db) && (M == 0 || (dy && scratch)) && (M == 0 || !dw || (codes && scales)), IFL_EINVAL, "block8_wgrad: null pointer");
+    IFL_CHECK_ARG((M <= 1 || ldy >= N) && (!dw || ((M <= 1 || (ldc >= K && lds >= ifl_cdiv((int)K, B8_BLK))) && ldw >= K)), IFL_EINVAL, "block8_wgrad: row strides");
+    IFL_CHECK_ARG(!dw || M == 0 || ((uintptr_t)codes % 16 == 0 && (M == 1 || ldc % 16 == 0)), IFL_EINVAL, "block8_wgrad: codes in rows of whole, aligned 16 bytes");
+    IFL_CHECK_ARG(ldy < (1 << 23), IFL_ENOTSUP, "block8_wgrad: rows of %lld gradients", (long long)ldy);
     hipStream_t st = (hipStream_t)stream;
-#define WG8(TWCODE, ...) do { if ((TWCODE) == IFL_T_F32) { typedef float TW; __VA_ARGS__; } else if ((TWCODE) == IFL_T_BF16) { typedef __bf16 TW; __VA_ARGS__; } else { typedef _Float16 TW; __VA_ARGS__; } } while (0)
+    if (M == 0) {
+        if (dw) { B8_DISPATCH(dwtype, hipLaunchKernelGGL(HIP_KERNEL_NAME(fill_zero_kernel<T>), dim3(256), dim3(256), 0, st, (T*)dw, ldw, (int)N, (int)K)); IFL_LAUNCH_CHECK(); }
+        if (db) { B8_DISPATCH(dbtype, hipLaunchKernelGGL(HIP_KERNEL_NAME(fill_zero_kernel<T>), dim3(16), dim3(256), 0, st, (T*)db, N, 1, (int)N)); IFL_LAUNCH_CHECK(); }
+        return 0;
+    }
+    const WPlan p = wg8_plan(M, N, K > 0 ? K : 1, dytype);
+    const int es = b8_size(dytype);
     if (dw) {
-        B8_DISPATCH(dytype, WG8(dwtype, hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_simple_kernel<T, TW>), dim3((unsigned)((K + 63) / 64), (unsigned)((N + 63) / 64)), dim3(256), 0, st,
-                                                           (const T*)dy, ldy, codes, ldc, scales, lds, fmt, chan, (TW*)dw, ldw, M, (int)N, (int)K)));
+        WG8 q = {};
+        q.dy = dy; q.ldy = ldy; q.codes = codes; q.ldc = ldc; q.scales = scales; q.lds = lds; q.chan = chan; q.dw = dw; q.ldw = ldw;
+        q.dwtype = dwtype; q.part = scratch; q.split = p.split; q.steps = p.steps; q.M = M; q.N = (int)N; q.K = (int)K;
+        q.tiles_n = (int)((N + p.tn - 1) / p.tn); q.tiles_k = (int)((K + p.tk - 1) / p.tk);
+        q.per_xcd = (q.tiles_n * q.tiles_k * p.split + 7) / 8;
+        q.ywide = (uintptr_t)dy % 16 == 0 && ldy * es % 16 == 0 && N % 8 == 0;
+        const bool dma = dytype == IFL_T_BF16 && q.ywide && M % p.ms == 0;
+        const dim3 grid(8 * q.per_xcd);
+#define WG8_K(T, NP, TN, TK, WN, WK, MS, F, D) hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_kernel<T, NP, TN, TK, WN, WK, MS, F, D>), grid, dim3(64 * WN * WK), 0, st, q)
+#define WG8_F(F) do { \
+            if (dytype == IFL_T_F32) WG8_K(float, 3, 128, 256, 2, 4, 32, F, false); \
+            else if (dytype == IFL_T_F16) WG8_K(_Float16, 2, 128, 256, 2, 4, 32, F, false); \
+            else if (p.tn == 256) { if (dma) WG8_K(__bf16, 1, 256, 256, 4, 2, 64, F, true); else WG8_K(__bf16, 1, 256, 256, 4, 2, 64, F, false); } \
+            else { if (dma) WG8_K(__bf16, 1, 128, 128, 2, 2, 64, F, true); else WG8_K(__bf16, 1, 128, 128, 2, 2, 64, F, false); } } while (0)
+        if (fmt == IFL_Q_E4M3) WG8_F(0); else WG8_F(1);
         IFL_LAUNCH_CHECK();
+        if (p.split > 1) {
+            const int64_t quads = (N * K + 3) / 4;
+            const unsigned jg = (unsigned)(quads / 256 + 1 < 4096 ? quads / 256 + 1 : 4096);
+            B8_DISPATCH(dwtype, hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_join_kernel<T>), dim3(jg), dim3(256), 0, st, q));
+            IFL_LAUNCH_CHECK();
+        }
     }
     if (db) {
-        B8_DISPATCH(dytype, WG8(dbtype, hipLaunchKernelGGL(HIP_KERNEL_NAME(colsum_kernel<T, TW>), dim3((unsigned)((N + 63) / 64)), dim3(256), 0, st, (const T*)dy, ldy, (TW*)db, M, (int)N)));
+        float* part = scratch + (dw && p.split > 1 ? (int64_t)p.split * N * K : 0);
+        const unsigned cols = (unsigned)((N + 63) / 64);
+        B8_DISPATCH(dytype, hipLaunchKernelGGL(HIP_KERNEL_NAME(colsum_kernel<T>), dim3(cols, p.cs_parts), dim3(256), 0, st, (const T*)dy, ldy, part, M, (int)N, p.cs_rows));
+        IFL_LAUNCH_CHECK();
+        B8_DISPATCH(dbtype, hipLaunchKernelGGL(HIP_KERNEL_NAME(colsum_join_kernel<T>), dim3(cols), dim3(64), 0, st, part, (T*)db, (int)N, p.cs_parts));
         IFL_LAUNCH_CHECK();
     }
     return 0;

@@ -148,7 +148,7 @@ def lib():
     L.ifl_block8_linear.argtypes = [vp, c_int, ll, vp, ll, vp, ll, c_int, vp, c_int, vp, ll, vp, ll, ll, ll, vp]
     L.ifl_block8_linear_scratch_bytes.argtypes = [ll, ll, ll, c_int]
     L.ifl_block8_linear_scratch_bytes.restype = ll
-    L.ifl_block8_wgrad_scratch_floats.argtypes = [ll, ll, ll]
+    L.ifl_block8_wgrad_scratch_floats.argtypes = [ll, ll, ll, c_int]
     L.ifl_block8_wgrad_scratch_floats.restype = ll
     L.ifl_block8_wgrad.argtypes = [vp, c_int, ll, vp, ll, vp, ll, c_int, vp, vp, c_int, ll, vp, c_int, vp, ll, ll, ll, vp]
     L.ifl_an_relu8_blocks.argtypes = [c_int, c_int, c_int, c_int]

@@ -89,8 +89,11 @@ def test_checkpoint_switch():
     ("ifl_block8_matmul", (16, 64, 16, 4, 0, 16, 64, 16, 4, 0, None, 0, 16, 0, 7, None, 1, 8, 64, None)),
     ("ifl_block8_matmul", (16, 64, 16, 4, 0, 16, 64, 16, 4, 0, None, 0, 16, 0, 8, None, 1, 0, 64, None)),
     ("ifl_block8_wgrad", (16, 0, 8, 16, 64, 16, 1, 0, None, None, 0, 64, None, 0, None, 4, 8, 64, None)),
-    ("ifl_block8_wgrad", (16, 0, 7, 16, 64, 16, 1, 0, None, 16, 0, 64, None, 0, None, 4, 8, 64, None)),
+    ("ifl_block8_wgrad", (16, 0, 7, 16, 64, 16, 1, 0, None, 16, 0, 64, None, 0, 16, 4, 8, 64, None)),
     ("ifl_block8_wgrad", (16, 5, 8, 16, 64, 16, 1, 0, None, 16, 0, 64, None, 0, None, 4, 8, 64, None)),
+    ("ifl_block8_wgrad", (16, 0, 8, 16, 64, 16, 1, 0, None, 16, 0, 64, None, 0, None, 4, 8, 64, None)),
+    ("ifl_block8_wgrad", (16, 0, 8, 8, 64, 16, 1, 0, None, 16, 0, 64, None, 0, 16, 4, 8, 64, None)),
+    ("ifl_block8_wgrad", (16, 0, 8, 16, 72, 16, 1, 0, None, 16, 0, 64, None, 0, 16, 4, 8, 64, None)),
     ("ifl_an_relu8_fwd", (16, 16, 16, 16, 16, 16, 0, 4, 4, 64, None)),
     ("ifl_an_relu8_fwd", (4, 16, 16, 16, 16, 16, 1, 4, 4, 64, None)),
     ("ifl_an_relu8_bwd", (16, 16, 16, 16, 16, None, 16, 16, 1, 4, 4, 64, None)),
