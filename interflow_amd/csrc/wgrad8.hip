@@ -11,6 +11,8 @@ namespace {
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 
+template <bool V> struct Flag { static constexpr bool value = V; };
+
 struct WG8 {
     const void* dy; int64_t ldy;
     const uint8_t* codes; int64_t ldc;
@@ -62,9 +64,10 @@ __global__ __launch_bounds__(64 * WN * WK)
 void wgrad8_kernel(WG8 q)
 {
     constexpr int NT = 64 * WN * WK, NF = TN / WN / 16, KF = TK / WK / 16;
+    constexpr int GR = KF * MS / 32, D = 2, R = 4;          // groups of a step, x fragments read ahead and held
     constexpr int YROW = TN * 2, XROW = TK * 2, YPL = MS * YROW;       // bytes
     constexpr int YP = MS * TN / 8 / NT, XP = MS * TK / 16 / NT;     // pieces (8 values of dy, 16 codes) per thread
-    static_assert(KF % 4 == 0 && YP * NT * 8 == MS * TN && XP * NT * 16 == MS * TK, "");
+    static_assert(YP * NT * 8 == MS * TN && XP * NT * 16 == MS * TK && NF == 4 && (KF == 4 || KF == 8) && GR % R == 0, "");
     __shared__ __attribute__((aligned(16))) uint8_t y0[NP * YPL], y1[NP * YPL], x0[MS * XROW], x1[MS * XROW];
     const int all = q.tiles_n * q.tiles_k * q.split;
     const int id = (blockIdx.x & 7) * q.per_xcd + (blockIdx.x >> 3);
@@ -86,24 +89,34 @@ void wgrad8_kernel(WG8 q)
     // once would be waited for at once)
     auto y_load = [&](int64_t m0) {
         if constexpr (!DMA) {
+            const T* base = dy + m0 * q.ldy;
+            const int rows = (int)min((int64_t)MS, me - m0) - 1;
 #pragma unroll
             for (int i = 0; i < YP; ++i) {
-                const int p = i * NT + tid, r = p / (TN / 8), n = n0 + p % (TN / 8) * 8;
-                const T* src = dy + min(m0 + r, me - 1) * q.ldy;
-                if (q.ywide) b8_load8<T, true>(src + (n < q.N ? n : 0), 8, yr[i]);
-                else b8_load8<T, false>(src + n, q.N - n, yr[i]);
+                const int p = i * NT + tid, n = n0 + p % (TN / 8) * 8;
+                const uint32_t at = (uint32_t)(min(p / (TN / 8), rows) * (int)q.ldy);
+                if (q.ywide) b8_load8<T, true>(base + (at + (n < q.N ? n : 0)), 8, yr[i]);
+                else b8_load8<T, false>(base + (at + n), q.N - n, yr[i]);
             }
         }
     };
+    // (fresh: an address or offset that is made again at its use instead of being held in registers of its own)
+    auto fresh = [](auto x) { asm volatile("" : "+v"(x)); return x; };
+    uint32_t ycol = 0;
+    if constexpr (DMA) {
+        const int r = tid / (TN / 8), c = tid % (TN / 8), s = ((c >> 1) ^ (r & 7)) * 2 + (c & 1);
+        ycol = n0 + s * 8 < q.N ? s * 16 : 0;                            // (columns past the end: any, their results are not stored)
+    }
     auto y_dma = [&](uint8_t* buf, int64_t m0) {
         if constexpr (DMA) {
             const uint8_t* base = (const uint8_t*)(dy + m0 * q.ldy + n0);
+            const int rows = (int)min((int64_t)MS, me - m0) - 1;
 #pragma unroll
             for (int i = 0; i < YP; ++i) {
-                const int p = i * NT + tid, r = p / (TN / 8), c = p % (TN / 8);
-                const int s = ((c >> 1) ^ (r & 7)) * 2 + (c & 1);
-                const int n = n0 + s * 8 < q.N ? s * 16 : 0;             // (columns past the end: any, their results are not stored)
-                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(base + (uint32_t)(r * (int)q.ldy * 2 + n)),
+                // a thread's pieces lie NT / (TN / 8) rows, a multiple of 8, apart: the same column in all of them
+                static_assert(NT / (TN / 8) % 8 == 0, "");
+                const uint32_t o = fresh(ycol) + (uint32_t)(min(fresh(tid) / (TN / 8) + i * (NT / (TN / 8)), rows) * 2 * (int)q.ldy);
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(base + o),
                                                  (__attribute__((address_space(3))) void*)(buf + (i * NT + wave * 64) * 16), 16, 0, 0);
             }
         }
@@ -128,18 +141,18 @@ void wgrad8_kernel(WG8 q)
         }
     };
     auto x_load = [&](int64_t m0) {
+        const uint8_t *base = q.codes + m0 * q.ldc, *sbase = q.scales + m0 * q.lds;
+        const int rows = (int)min((int64_t)MS, me - m0) - 1;
 #pragma unroll
         for (int i = 0; i < XP; ++i) {
-            const int p = i * NT + tid, r = p / (TK / 16), k = k0 + p % (TK / 16) * 16;
-            const int64_t m = min(m0 + r, me - 1);
-            const int kc = k < q.K ? k : 0;
-            xr[i] = *(const i32x4*)(q.codes + m * q.ldc + kc);
-            xs[i] = q.scales[m * q.lds + kc / B8_BLK];
+            const int p = i * NT + tid, k = k0 + p % (TK / 16) * 16;
+            const int r = min(p / (TK / 16), rows), kc = k < q.K ? k : 0;
+            xr[i] = *(const i32x4*)(base + (uint32_t)(r * (int)q.ldc + kc));
+            xs[i] = sbase[(uint32_t)(r * (int)q.lds + kc / B8_BLK)];
         }
     };
-    auto x_store = [&](uint8_t* buf, int64_t m0) {
-#pragma unroll
-        for (int i = 0; i < XP; ++i) {
+    auto x_store = [&](uint8_t* buf, int64_t m0, int i) {
+        {
             const int p = i * NT + tid, r = p / (TK / 16), c = p % (TK / 16);
             const int left = m0 + r < me ? q.K - k0 - c * 16 : 0;
             if (left < 16) {
@@ -163,59 +176,108 @@ void wgrad8_kernel(WG8 q)
 
     // ---- fragments
     const int mrow = 4 * g + (r16 >> 2), q4 = r16 & 3;
-    auto y_frag = [&](const uint8_t* buf, int pl, int f, int h) {
-        const uint8_t* a = buf + pl * YPL + (32 * h + mrow) * YROW + ((wn * NF + f) ^ (mrow & 7)) * 32 + q4 * 8;
+    // (places are XORs of a lane's own and of a fragment's constants)
+    const int ya = mrow * YROW + ((wn * NF) ^ (mrow & 7)) * 32 + q4 * 8;
+    const int xa = mrow * XROW + ((wk * KF + q4) ^ (mrow & 4)) * 32 + (mrow & 3) * 8;
+    auto tr8 = [&](const uint8_t* a, int rows16) {
         const s16x4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a));
-        const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a + 16 * YROW));
+        const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a + rows16));
         return __builtin_bit_cast(bf16x8, __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7));
     };
-    auto x_frag = [&](const uint8_t* buf, int f, int h) {
-        const uint8_t* a = buf + (32 * h + mrow) * XROW + (((wk * KF / 4 + f / 4) * 4 + q4) ^ (mrow & 4)) * 32 + ((f & 3) ^ (mrow & 3)) * 8;
-        const s16x4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a));
-        const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a + 16 * XROW));
-        return __builtin_bit_cast(bf16x8, __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7));
-    };
+    auto y_frag = [&](const uint8_t* buf, int pl, int f, int h) { return tr8(buf + (fresh(ya) ^ f << 5) + (pl * YPL + 32 * h * YROW), 16 * YROW); };
+    auto x_frag = [&](const uint8_t* buf, int f, int h) { return tr8(buf + (fresh(xa) ^ ((f & 3) << 3 | (f >> 2) << 7)) + 32 * h * XROW, 16 * XROW); };
+    // One step: GR groups (an x fragment with all y fragments of its 32 rows), x fragments read D groups ahead, y fragments 32 rows
+    // ahead.  The next step's rows that come through registers are stored before group GR - D; those registers are then loaded
+    // for the step after it.  At group GR - D everything of this step is in registers, and what goes straight to LDS has had the
+    // time since the step's start: there the workgroup meets and goes on reading in the next step's buffer.
     f32x4 acc[KF][NF] = {};
-    auto multiply = [&](const uint8_t* yb, const uint8_t* xb) {
+    bf16x8 y[2][NF][NP], x[R];
+    auto read_y = [&](const uint8_t* yb, int h, int o) {
 #pragma unroll
-        for (int h = 0; h < MS / 32; ++h) {
-            bf16x8 y[NF][NP];
+        for (int f = 0; f < NF; ++f)
 #pragma unroll
-            for (int f = 0; f < NF; ++f)
+            for (int k = 0; k < NP; ++k) y[o][f][k] = y_frag(yb, k, f, h);
+    };
+    auto products = [&](int i, int o) {
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int k = 0; k < NP; ++k) y[f][k] = y_frag(yb, k, f, h);
+        for (int f = 0; f < NF; ++f)
 #pragma unroll
-            for (int i = 0; i < KF; ++i) {
-                const bf16x8 x = x_frag(xb, i, h);
+            for (int k = 0; k < NP; ++k)
+                acc[i % KF][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[i % R], y[o][f][k], acc[i % KF][f], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // (not __syncthreads: that would also wait for the loads on their way to registers)
+    auto turn = [&]() {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    auto landed = [&]() { if constexpr (DMA) asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); };
+    const int64_t mlast = mb + (int64_t)(steps - 1) * MS;                // (behind the last step it is loaded again, unused)
+    // behind a load that goes straight to LDS: rows past the end, made zero where this thread has just put them
+    auto y_cut = [&](uint8_t* buf, int64_t m0) {
+        if constexpr (DMA) {
+            if (m0 + MS > me) {
 #pragma unroll
-                for (int f = 0; f < NF; ++f)
-#pragma unroll
-                    for (int k = 0; k < NP; ++k) acc[i][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y[f][k], acc[i][f], 0, 0, 0);
+                for (int i = 0; i < YP; ++i)
+                    if (m0 + (i * NT + tid) / (TN / 8) >= me) *(i32x4*)(buf + (i * NT + tid) * 16) = i32x4{0, 0, 0, 0};
             }
         }
     };
-    auto turn = [&]() {
-        __builtin_amdgcn_s_waitcnt(0x0f70);                              // vmcnt(0): the loads that go to LDS are there
-        __syncthreads();
+    // (CHECK: the next step may be cut off.  In the others no branches: the compiler would move products past them.)
+    auto step = [&](auto CHECK, auto ODD, uint8_t* yc, uint8_t* xc, uint8_t* yn, uint8_t* xn, int64_t m) {
+        constexpr int H = MS / 32;
+        const int64_t m1 = min(m + MS, mlast), m2 = min(m + 2 * MS, mlast);
+        y_dma(yn, m1);
+#pragma unroll
+        for (int i = 0; i < GR; ++i) {
+            const int h = i / KF, o = (h + (H & 1) * ODD.value) & 1;
+            constexpr int S = GR - D - 1;                                // the last group before the meeting
+            if (i + D < GR) x[(i + D) % R] = x_frag(xc, (i + D) % KF, (i + D) / KF);
+#pragma unroll
+            for (int e = 0; e < XP; ++e) if (i == S - 2 * (XP - 1 - e)) x_store(xn, m1, e);
+            if (i == S) {
+                y_store(yn, m1);
+                landed();
+                if constexpr (CHECK.value) y_cut(yn, m1);
+                x_load(m2);
+                y_load(m2);
+            }
+            if (i == GR - D) {
+                turn();
+                read_y(yn, 0, o ^ 1);
+            }
+            if (i + D >= GR) x[(i + D) % R] = x_frag(xn, i + D - GR, 0);
+            if (i % KF == KF - 4 && h + 1 < H) read_y(yc, h + 1, o ^ 1);
+            products(i, o);
+        }
     };
 
-    y_load(mb); x_load(mb);
-    y_dma(y0, mb); y_store(y0, mb); x_store(x0, mb);
+    x_load(mb);
+    y_load(mb);
+    y_dma(y0, mb);
+    y_store(y0, mb);
+#pragma unroll
+    for (int e = 0; e < XP; ++e) x_store(x0, mb, e);
+    landed();
+    y_cut(y0, mb);
+    x_load(min(mb + MS, mlast));
+    y_load(min(mb + MS, mlast));
     turn();
-    for (int s = 0; s < steps; s += 2) {
-        const bool more = s + 1 < steps, more2 = s + 2 < steps;
-        const int64_t m1 = mb + (int64_t)(s + 1) * MS, m2 = m1 + MS;
-        if (more) { y_load(m1); x_load(m1); y_dma(y1, m1); }
-        multiply(y0, x0);
-        if (more) { y_store(y1, m1); x_store(x1, m1); }
-        turn();
-        if (more) {
-            if (more2) { y_load(m2); x_load(m2); y_dma(y0, m2); }
-            multiply(y1, x1);
-            if (more2) { y_store(y0, m2); x_store(x0, m2); }
-            turn();
-        }
+    read_y(y0, 0, 0);
+#pragma unroll
+    for (int e = 0; e < D; ++e) x[e] = x_frag(x0, e, 0);
+    int64_t m = mb;
+    int s = 0;
+    for (; s + 3 < steps; s += 2, m += 2 * MS) {
+        step(Flag<false>(), Flag<false>(), y0, x0, y1, x1, m);
+        step(Flag<false>(), Flag<true>(), y1, x1, y0, x0, m + MS);
     }
+    step(Flag<true>(), Flag<false>(), y0, x0, y1, x1, m);
+    if (s + 1 < steps) step(Flag<true>(), Flag<true>(), y1, x1, y0, x0, m + MS);
+    if (s + 2 < steps) step(Flag<true>(), Flag<false>(), y0, x0, y1, x1, m + 2 * MS);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
     const int kw = k0 + wk * KF * 16 + 16 * g, nw = n0 + wn * NF * 16 + r16;
 #pragma unroll
@@ -245,27 +307,28 @@ void wgrad8_kernel(WG8 q)
     }
 }
 
-// dw = chan * sum of the parts, in order
-template <class TW>
+// dw = chan * sum of the parts, in order: four parts' values are on their way at a time
+template <class TW, int V>
 __global__ __launch_bounds__(256)
 void wgrad8_join_kernel(WG8 q)
 {
+    typedef float FV __attribute__((ext_vector_type(V)));
     const int64_t nk = (int64_t)q.N * q.K;
-    if (q.K % 4 == 0) {
-        for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < nk; i += (int64_t)gridDim.x * 1024) {
-            f32x4 t = *(const f32x4*)(q.part + i);
-            for (int s = 1; s < q.split; ++s) t += *(const f32x4*)(q.part + s * nk + i);
-            const int n = (int)(i / q.K), k = (int)(i - (int64_t)n * q.K);
+    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V; i < nk; i += (int64_t)gridDim.x * 256 * V) {
+        FV t = 0.f;
+        int s = 0;
+        for (; s + 4 <= q.split; s += 4) {
+            FV u[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) ((TW*)q.dw)[(int64_t)n * q.ldw + k + e] = (TW)(q.chan ? t[e] * q.chan[k + e] : t[e]);
+            for (int e = 0; e < 4; ++e) u[e] = *(const FV*)(q.part + (s + e) * nk + i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) t += u[e];
         }
-    } else {
-        for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < nk; i += (int64_t)gridDim.x * 256) {
-            float t = q.part[i];
-            for (int s = 1; s < q.split; ++s) t += q.part[s * nk + i];
-            const int n = (int)(i / q.K), k = (int)(i - (int64_t)n * q.K);
-            ((TW*)q.dw)[(int64_t)n * q.ldw + k] = (TW)(q.chan ? t * q.chan[k] : t);
-        }
+        for (; s < q.split; ++s) t += *(const FV*)(q.part + s * nk + i);
+        const int n = (int)(i / q.K), k = (int)(i - (int64_t)n * q.K);
+        TW* d = (TW*)q.dw + (int64_t)n * q.ldw + k;
+#pragma unroll
+        for (int e = 0; e < V; ++e) d[e] = (TW)(q.chan ? t[e] * q.chan[k + e] : t[e]);
     }
 }
 
@@ -292,26 +355,37 @@ void colsum_kernel(const T* __restrict__ dy, int64_t ldy, float* __restrict__ pa
     __syncthreads();
     if (r == 0 && n < N) part[(int64_t)blockIdx.y * N + n] = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
 }
+// second pass: a workgroup takes 16 columns, 16 threads of each every 16th part, joined in LDS in a fixed order
 template <class TW>
-__global__ __launch_bounds__(64)
+__global__ __launch_bounds__(256)
 void colsum_join_kernel(const float* __restrict__ part, TW* __restrict__ db, int N, int parts)
 {
-    const int n = blockIdx.x * 64 + threadIdx.x;
-    if (n >= N) return;
+    __shared__ float red[16][17];
+    const int c = threadIdx.x & 15, r = threadIdx.x >> 4, n = blockIdx.x * 16 + c;
     float t = 0.f;
-    for (int s = 0; s < parts; ++s) t += part[(int64_t)s * N + n];
-    db[n] = (TW)t;
+    if (n < N) {
+#pragma unroll 4
+        for (int s = r; s < parts; s += 16) t += part[(int64_t)s * N + n];
+    }
+    red[r][c] = t;
+    __syncthreads();
+    if (r == 0 && n < N) {
+#pragma unroll
+        for (int i = 1; i < 16; ++i) t += red[i][c];
+        db[n] = (TW)t;
+    }
 }
 
-// Tiles of 256 x 256 for bf16 gradients of large layers, else 128 x 128; 128 x 256 where a gradient has two or three terms (they
-// take that much more LDS).  The rows are split until about 256 workgroups are at work, each with two steps at least.
+// bf16 gradients: tiles of 256 x 256 for large layers if they can go straight to LDS, else 128 x 128; gradients of two or three terms,
+// which take that much more LDS: 128 x 256.  The rows are split until about 256 workgroups are at work, each with two steps at
+// least.
 struct WPlan { int tn, tk, ms, split, steps, cs_parts; int64_t cs_rows; };
-WPlan wg8_plan(int64_t M, int64_t N, int64_t K, int dytype)
+WPlan wg8_plan(int64_t M, int64_t N, int64_t K, int dytype, bool dma)
 {
     WPlan p = {128, 128, 64, 1, 0, 1, 0};
     auto tiles = [&](int64_t a, int64_t b) { return ((N + a - 1) / a) * ((K + b - 1) / b); };
     if (dytype != IFL_T_BF16) { p.tk = 256; p.ms = 32; }
-    else if (tiles(256, 256) >= 32) p.tn = p.tk = 256;
+    else if (dma && tiles(256, 256) >= 32) p.tn = p.tk = 256;
     const int64_t steps = (M + p.ms - 1) / p.ms, n = tiles(p.tn, p.tk);
     int64_t s = n >= 192 ? 1 : 256 / n;
     if (s > steps / 2) s = steps / 2;
@@ -334,8 +408,9 @@ WPlan wg8_plan(int64_t M, int64_t N, int64_t K, int dytype)
 extern "C" int64_t ifl_block8_wgrad_scratch_floats(int64_t M, int64_t N, int64_t K, int dytype)
 {
     if (M < 1 || N < 1 || K < 0) return 0;
-    const WPlan p = wg8_plan(M, N, K > 0 ? K : 1, dytype);
-    return (K > 0 && p.split > 1 ? p.split * N * K : 0) + (int64_t)p.cs_parts * N;
+    const WPlan p = wg8_plan(M, N, K > 0 ? K : 1, dytype, false), d = wg8_plan(M, N, K > 0 ? K : 1, dytype, true);
+    const int64_t s = p.split > d.split ? p.split : d.split;
+    return (K > 0 && s > 1 ? s * N * K : 0) + (int64_t)p.cs_parts * N;
 }
 
 extern "C" int ifl_block8_wgrad(const void* dy, int dytype, int64_t ldy, const uint8_t* codes, int64_t ldc, const uint8_t* scales,
@@ -348,36 +423,39 @@ extern "C" int ifl_block8_wgrad(const void* dy, int dytype, int64_t ldy, const u
     IFL_CHECK_ARG((dw || db) && (M == 0 || (dy && scratch)) && (M == 0 || !dw || (codes && scales)), IFL_EINVAL, "block8_wgrad: null pointer");
     IFL_CHECK_ARG((M <= 1 || ldy >= N) && (!dw || ((M <= 1 || (ldc >= K && lds >= ifl_cdiv((int)K, B8_BLK))) && ldw >= K)), IFL_EINVAL, "block8_wgrad: row strides");
     IFL_CHECK_ARG(!dw || M == 0 || ((uintptr_t)codes % 16 == 0 && (M == 1 || ldc % 16 == 0)), IFL_EINVAL, "block8_wgrad: codes in rows of whole, aligned 16 bytes");
-    IFL_CHECK_ARG(ldy < (1 << 23), IFL_ENOTSUP, "block8_wgrad: rows of %lld gradients", (long long)ldy);
+    IFL_CHECK_ARG(ldy < (1 << 23) && ldc < (1 << 23) && lds < (1 << 23), IFL_ENOTSUP, "block8_wgrad: rows of %lld gradients, %lld codes", (long long)ldy, (long long)ldc);
     hipStream_t st = (hipStream_t)stream;
     if (M == 0) {
         if (dw) { B8_DISPATCH(dwtype, hipLaunchKernelGGL(HIP_KERNEL_NAME(fill_zero_kernel<T>), dim3(256), dim3(256), 0, st, (T*)dw, ldw, (int)N, (int)K)); IFL_LAUNCH_CHECK(); }
         if (db) { B8_DISPATCH(dbtype, hipLaunchKernelGGL(HIP_KERNEL_NAME(fill_zero_kernel<T>), dim3(16), dim3(256), 0, st, (T*)db, N, 1, (int)N)); IFL_LAUNCH_CHECK(); }
         return 0;
     }
-    const WPlan p = wg8_plan(M, N, K > 0 ? K : 1, dytype);
-    const int es = b8_size(dytype);
+    const bool ywide = (uintptr_t)dy % 16 == 0 && (M == 1 || ldy * b8_size(dytype) % 16 == 0) && N % 8 == 0;
+    const bool dma = dytype == IFL_T_BF16 && ywide;
+    const WPlan p = wg8_plan(M, N, K > 0 ? K : 1, dytype, dma);
     if (dw) {
         WG8 q = {};
         q.dy = dy; q.ldy = ldy; q.codes = codes; q.ldc = ldc; q.scales = scales; q.lds = lds; q.chan = chan; q.dw = dw; q.ldw = ldw;
         q.dwtype = dwtype; q.part = scratch; q.split = p.split; q.steps = p.steps; q.M = M; q.N = (int)N; q.K = (int)K;
         q.tiles_n = (int)((N + p.tn - 1) / p.tn); q.tiles_k = (int)((K + p.tk - 1) / p.tk);
         q.per_xcd = (q.tiles_n * q.tiles_k * p.split + 7) / 8;
-        q.ywide = (uintptr_t)dy % 16 == 0 && ldy * es % 16 == 0 && N % 8 == 0;
-        const bool dma = dytype == IFL_T_BF16 && q.ywide && M % p.ms == 0;
+        q.ywide = ywide;
         const dim3 grid(8 * q.per_xcd);
 #define WG8_K(T, NP, TN, TK, WN, WK, MS, F, D) hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_kernel<T, NP, TN, TK, WN, WK, MS, F, D>), grid, dim3(64 * WN * WK), 0, st, q)
 #define WG8_F(F) do { \
             if (dytype == IFL_T_F32) WG8_K(float, 3, 128, 256, 2, 4, 32, F, false); \
             else if (dytype == IFL_T_F16) WG8_K(_Float16, 2, 128, 256, 2, 4, 32, F, false); \
-            else if (p.tn == 256) { if (dma) WG8_K(__bf16, 1, 256, 256, 4, 2, 64, F, true); else WG8_K(__bf16, 1, 256, 256, 4, 2, 64, F, false); } \
+            else if (p.tn == 256) WG8_K(__bf16, 1, 256, 256, 4, 2, 64, F, true); \
             else { if (dma) WG8_K(__bf16, 1, 128, 128, 2, 2, 64, F, true); else WG8_K(__bf16, 1, 128, 128, 2, 2, 64, F, false); } } while (0)
         if (fmt == IFL_Q_E4M3) WG8_F(0); else WG8_F(1);
         IFL_LAUNCH_CHECK();
         if (p.split > 1) {
-            const int64_t quads = (N * K + 3) / 4;
-            const unsigned jg = (unsigned)(quads / 256 + 1 < 4096 ? quads / 256 + 1 : 4096);
-            B8_DISPATCH(dwtype, hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_join_kernel<T>), dim3(jg), dim3(256), 0, st, q));
+            // four values per thread where the parts are large, else one: the parts' loads are what it waits for
+            const bool v4 = K % 4 == 0 && N * K >= 1 << 18;
+            const int64_t jobs = (v4 ? N * K / 4 : N * K) / 256 + 1;
+            const unsigned jg = (unsigned)(jobs < 4096 ? jobs : 4096);
+            B8_DISPATCH(dwtype, if (v4) hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_join_kernel<T, 4>), dim3(jg), dim3(256), 0, st, q);
+                        else hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_join_kernel<T, 1>), dim3(jg), dim3(256), 0, st, q));
             IFL_LAUNCH_CHECK();
         }
     }
@@ -386,7 +464,7 @@ extern "C" int ifl_block8_wgrad(const void* dy, int dytype, int64_t ldy, const u
         const unsigned cols = (unsigned)((N + 63) / 64);
         B8_DISPATCH(dytype, hipLaunchKernelGGL(HIP_KERNEL_NAME(colsum_kernel<T>), dim3(cols, p.cs_parts), dim3(256), 0, st, (const T*)dy, ldy, part, M, (int)N, p.cs_rows));
         IFL_LAUNCH_CHECK();
-        B8_DISPATCH(dbtype, hipLaunchKernelGGL(HIP_KERNEL_NAME(colsum_join_kernel<T>), dim3(cols), dim3(64), 0, st, part, (T*)db, (int)N, p.cs_parts));
+        B8_DISPATCH(dbtype, hipLaunchKernelGGL(HIP_KERNEL_NAME(colsum_join_kernel<T>), dim3((unsigned)((N + 15) / 16)), dim3(256), 0, st, part, (T*)db, (int)N, p.cs_parts));
         IFL_LAUNCH_CHECK();
     }
     return 0;

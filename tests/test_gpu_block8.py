@@ -184,7 +184,8 @@ def test_matmul_nan_and_infinity_stay_in_their_rows():
     assert not bool(y[:, 7].isfinite().any())
 
 
-@pytest.mark.parametrize("M, N, K", [(1, 1, 1), (1, 5, 300), (7, 3, 64), (50, 64, 64), (64, 130, 96), (200, 64, 320), (333, 77, 129), (1000, 256, 512), (4097, 40, 200), (3000, 320, 130)])
+@pytest.mark.parametrize("M, N, K", [(1, 1, 1), (1, 5, 300), (7, 3, 64), (50, 64, 64), (64, 130, 96), (200, 64, 320), (333, 77, 129), (1000, 256, 512), (4097, 40, 200), (3000, 320, 130),
+                                     (777, 2048, 1040), (65, 2056, 1030), (5000, 2048, 1024)])
 @pytest.mark.parametrize("dtype", list(DT))
 def test_weight_grad(M, N, K, dtype):
     g = gen(M + N + K)
@@ -199,6 +200,23 @@ def test_weight_grad(M, N, K, dtype):
         close(db, dy.double().sum(0), M, dy.double().abs().sum(0), (M, N, K))
     again, _ = block8.weight_grad(dy, q, torch.float32)
     assert torch.equal(again, block8.weight_grad(dy, q, torch.float32)[0])
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("M, N, K", [(71, 64, 64), (71, 2048, 1040), (71, 9, 64)])
+def test_weight_grad_nan_and_infinity(M, N, K, dtype):
+    """What is not finite in a gradient or in a checkpoint reaches its own row or column of dw, in the last rows too, and nothing else."""
+    g = gen(40)
+    q = block8.quantize(torch.ones(M, K).cuda() + torch.rand(M, K, generator=g).cuda())
+    dy = rand(g, M, N, dtype=DT[dtype])
+    dy[M - 1, 3], dy[M - 2, 5], dy[0, 7] = math.inf, math.nan, -math.inf
+    dw, _ = block8.weight_grad(dy, q)
+    assert bool((dw[3] == math.inf).all()) and bool(dw[5].isnan().all()) and bool((dw[7] == -math.inf).all())
+    assert bool(dw[[i for i in range(N) if i not in (3, 5, 7)]].isfinite().all())
+    x = torch.ones(M, K).cuda()
+    x[M - 1, 6] = math.nan
+    dw, _ = block8.weight_grad(rand(g, M, N, dtype=DT[dtype]), block8.quantize(x))
+    assert bool(dw[:, 6].isnan().all()) and bool(dw[:, [i for i in range(K) if i != 6]].isfinite().all())
 
 
 def test_weight_grad_is_exact_in_float32():
