@@ -337,6 +337,19 @@ int64_t ifl_block8_wgrad_scratch_floats(int64_t M, int64_t N, int64_t K, int dyt
 int ifl_block8_wgrad(const void* dy, int dytype, int64_t ldy, const uint8_t* codes, int64_t ldc, const uint8_t* scales, int64_t lds,
                      int fmt, const float* chan, void* dw, int dwtype, int64_t ldw, void* db, int dbtype, float* scratch, int64_t M,
                      int64_t N, int64_t K, void* stream);
+/* The layer y = Q(x) Q(w)^T + bias in training, one call per direction.  Forward: x [M][K] and w [N][K] (element (r, c) at
+ * r *_rs + c *_cs, one of the two 1) are quantized along K (e4m3); codes [M][K rounded up to 16] and scales [M][ceil(K / 512) * 4]
+ * receive x's blocks, the checkpoint; y [M][N] of x's type.  Backward, from dy [M][N] (x's type, columns contiguous): dx [M][K] =
+ * Q(dy) Q(w^T)^T, dy quantized along N as gfmt, w^T along N (e4m3); dw [N][K] of w's type and db [N] as ifl_block8_wgrad from the
+ * checkpoint; each of the three may be NULL.  scratch: the size functions' bytes, 16-byte aligned.                    */
+int ifl_linear8_fwd(const void* x, int xtype, int64_t x_rs, int64_t x_cs, const void* w, int wtype, int64_t w_rs, int64_t w_cs,
+                    const void* bias, int btype, uint8_t* codes, uint8_t* scales, void* y, void* scratch, int64_t M, int64_t N,
+                    int64_t K, void* stream);
+int64_t ifl_linear8_fwd_scratch_bytes(int64_t M, int64_t N, int64_t K, int xtype);
+int ifl_linear8_bwd(const void* dy, int xtype, int64_t ldy, const uint8_t* codes, const uint8_t* scales, const void* w, int wtype,
+                    int64_t w_rs, int64_t w_cs, int gfmt, void* dx, void* dw, void* db, int dbtype, void* scratch, int64_t M,
+                    int64_t N, int64_t K, void* stream);
+int64_t ifl_linear8_bwd_scratch_bytes(int64_t M, int64_t N, int64_t K, int xtype, int need_dx, int need_dw);
 /* ActNorm + ReLU of the coupling networks (as ifl_an_relu_*) with an 8-bit checkpoint: v = relu(x + bias), y = v exp(logs) on
  * ringed planes [B][h+2][w+2][C], C a multiple of 32, at most 1024.  codes [B][h+2][w+2][C] and scales [B][h+2][w+2][ceil(C/128)]
  * receive v in 8-bit blocks (e4m3); a positive v never gets the code 0.  Interior pixels of x and dy are read; y, dx and the

@@ -18,8 +18,11 @@ import torch
 
 from . import hip
 
+_raw_stream = torch._C._cuda_getCurrentRawStream        # (a current_stream() object costs a small call more than its launch)
+_get_device = torch._C._cuda_getDevice
+
 BLOCK = 128
-_FMT = {"e4m3": (0, torch.float8_e4m3fn), "e5m2": (1, torch.float8_e5m2)}
+_FMT = {"e4m3": 0, "e5m2": 1}
 _FMT_OF = {torch.float8_e4m3fn: 0, torch.float8_e5m2: 1}
 _TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
@@ -33,66 +36,61 @@ def _on_gpu(t, name):
 
 
 def _real(t, name):
-    _on_gpu(t, name)
-    if t.dtype not in _TYPE:
+    """The element type's code."""
+    code = _TYPE.get(t.dtype) if isinstance(t, torch.Tensor) and t.is_cuda else None
+    if code is None:
+        _on_gpu(t, name)
         raise TypeError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
-    return t
+    return code
 
 
 def _dtype(dtype, what):
-    if dtype not in _TYPE:
+    code = _TYPE.get(dtype)
+    if code is None:
         raise TypeError(f"{what}: dtype has to be float32, bfloat16 or float16, got {dtype}")
-    return dtype
+    return code
+
+
+def _format(fmt, what):
+    code = _FMT.get(fmt)
+    if code is None:
+        raise ValueError(f"{what}: the format has to be 'e4m3' or 'e5m2', got {fmt!r}")
+    return code
 
 
 def _same_device(dev, *ts):
     for t in ts:
-        if t is not None:
-            assert t.device == dev, f"tensors on {dev} and {t.device}"
+        assert t is None or t.get_device() == dev, f"tensors on cuda:{dev} and {t.device}"
+
+
+_fns = {}
 
 
 def _call(what, dev, *args):
-    """One library call on the current stream of `dev`."""
-    fn = getattr(hip.lib(), what)
-    if torch.cuda.current_device() == dev.index:
-        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    """One library call on the current stream of device number `dev`."""
+    fn = _fns.get(what)
+    if fn is None:
+        fn = _fns[what] = getattr(hip.lib(), what)
+    if _get_device() == dev:
+        rc = fn(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+            rc = fn(*args, _raw_stream(dev))
     if rc:
         hip.check(rc, what)
 
 
-class Block8:
-    """A matrix in 8-bit blocks: `codes` [rows, cols] (torch.float8_e4m3fn or float8_e5m2) and `scales` [rows, ceil(cols / 128)]
-    (torch.float8_e8m0fnu), columns contiguous, rows any distance apart.  Made by `quantize`, or from tensors of that form."""
-    __slots__ = ("codes", "scales")
+def _size(what, *args):
+    """A size that the library names; what it refuses raises."""
+    fn = _fns.get(what)
+    if fn is None:
+        fn = _fns[what] = getattr(hip.lib(), what)
+    return fn(*args)
 
-    def __init__(self, codes, scales):
-        _on_gpu(codes, "Block8 codes")
-        _on_gpu(scales, "Block8 scales")
-        if codes.dtype not in _FMT_OF or scales.dtype != torch.float8_e8m0fnu:
-            raise TypeError(f"Block8: codes in float8_e4m3fn or float8_e5m2 and scales in float8_e8m0fnu, got {codes.dtype} and {scales.dtype}")
-        assert codes.dim() == 2 and scales.dim() == 2 and codes.shape[1] >= 1, (tuple(codes.shape), tuple(scales.shape))
-        assert scales.shape == (codes.shape[0], -(-codes.shape[1] // BLOCK)), (tuple(codes.shape), tuple(scales.shape))
-        _same_device(codes.device, scales)
-        self.codes = codes if _rows_apart(codes) else codes.contiguous()
-        self.scales = scales if _rows_apart(scales) else scales.contiguous()
 
-    @property
-    def shape(self):
-        return self.codes.shape
-
-    @property
-    def device(self):
-        return self.codes.device
-
-    @property
-    def fmt(self):
-        return "e4m3" if self.codes.dtype == torch.float8_e4m3fn else "e5m2"
-
-    def __repr__(self):
-        return f"Block8({self.codes.shape[0]} x {self.codes.shape[1]}, {self.fmt}, {self.device})"
+def _scratch(n, dev):
+    """n bytes, or nothing."""
+    return torch.empty((n,), dtype=torch.uint8, device=dev) if n else None
 
 
 def _rows_apart(t):
@@ -105,113 +103,167 @@ def _ld(t):
     return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
 
 
-def _alloc(rows, cols, fmt, dev):
-    """Codes in rows of whole 16 bytes, scales in rows of whole 4: what the product's wide loads want."""
-    codes = torch.empty((rows, (cols + 15) // 16 * 16), dtype=_FMT[fmt][1], device=dev)
-    scales = torch.empty((rows, (cols + 511) // 512 * 4), dtype=torch.float8_e8m0fnu, device=dev)
-    q = Block8.__new__(Block8)
-    q.codes, q.scales = codes[:, :cols], scales[:, :(cols + 127) // 128]
-    return q
+class Block8:
+    """A matrix in 8-bit blocks: `codes` [rows, cols] (torch.float8_e4m3fn or float8_e5m2) and `scales` [rows, ceil(cols / 128)]
+    (torch.float8_e8m0fnu), columns contiguous, rows any distance apart.  Made by `quantize`, or from tensors of that form."""
+    __slots__ = ("rows", "cols", "_f", "_dev", "_raw", "_codes", "_scales", "_cp", "_ldc", "_sp", "_lds")
+
+    def __init__(self, codes, scales):
+        _on_gpu(codes, "Block8 codes")
+        _on_gpu(scales, "Block8 scales")
+        f = _FMT_OF.get(codes.dtype)
+        if f is None or scales.dtype != torch.float8_e8m0fnu:
+            raise TypeError(f"Block8: codes in float8_e4m3fn or float8_e5m2 and scales in float8_e8m0fnu, got {codes.dtype} and {scales.dtype}")
+        assert codes.dim() == 2 and scales.dim() == 2 and codes.shape[1] >= 1, (tuple(codes.shape), tuple(scales.shape))
+        rows, cols = codes.shape
+        assert scales.shape == (rows, -(-cols // BLOCK)), (tuple(codes.shape), tuple(scales.shape))
+        self._dev = codes.get_device()
+        _same_device(self._dev, scales)
+        self._codes = codes = codes if _rows_apart(codes) else codes.contiguous()
+        self._scales = scales = scales if _rows_apart(scales) else scales.contiguous()
+        self.rows, self.cols, self._f, self._raw = rows, cols, f, None
+        self._cp, self._ldc, self._sp, self._lds = codes.data_ptr(), _ld(codes), scales.data_ptr(), _ld(scales)
+
+    @classmethod
+    def _new(cls, rows, cols, f, dev, raw=None):
+        """Room for rows x cols: one allocation, codes in rows of whole 16 bytes and behind them scales in rows of whole 4, which is
+        what the product's wide loads want."""
+        q = cls.__new__(cls)
+        ldc, lds = (cols + 15) // 16 * 16, (cols + 511) // 512 * 4
+        q._raw = raw = torch.empty((rows * (ldc + lds),), dtype=torch.uint8, device=dev) if raw is None else raw
+        q.rows, q.cols, q._f, q._dev, q._codes, q._scales = rows, cols, f, raw.get_device(), None, None
+        q._cp, q._ldc, q._lds = raw.data_ptr(), ldc, lds
+        q._sp = q._cp + rows * ldc
+        return q
+
+    @property
+    def codes(self):
+        if self._codes is None:
+            c = self._raw[:self.rows * self._ldc].view(self.rows, self._ldc)
+            self._codes = c.view(torch.float8_e5m2 if self._f else torch.float8_e4m3fn)[:, :self.cols]
+        return self._codes
+
+    @property
+    def scales(self):
+        if self._scales is None:
+            s = self._raw[self.rows * self._ldc:].view(self.rows, self._lds)
+            self._scales = s.view(torch.float8_e8m0fnu)[:, :(self.cols + 127) // 128]
+        return self._scales
+
+    @property
+    def shape(self):
+        return torch.Size((self.rows, self.cols))
+
+    @property
+    def device(self):
+        return torch.device("cuda", self._dev)
+
+    @property
+    def fmt(self):
+        return "e5m2" if self._f else "e4m3"
+
+    def __repr__(self):
+        return f"Block8({self.rows} x {self.cols}, {self.fmt}, {self.device})"
+
+    def _aligned(self):
+        """Itself, or a copy whose rows are whole, aligned 16 and 4 bytes (a single row's length does not matter)."""
+        one = self.rows <= 1
+        if self._cp % 16 == 0 and self._sp % 4 == 0 and (one or (self._ldc % 16 == 0 and self._lds % 4 == 0)):
+            return self
+        q = Block8._new(self.rows, self.cols, self._f, self.device)
+        q.codes.view(torch.uint8).copy_(self.codes.view(torch.uint8))
+        q.scales.view(torch.uint8).copy_(self.scales.view(torch.uint8))
+        return q
 
 
-def quantize(x, fmt: str = "e4m3") -> Block8:
-    """x [rows, cols] (float32, bfloat16 or float16, any strides; a transposed view is read as it is) in 8-bit blocks."""
-    _real(x, "quantize input")
-    if fmt not in _FMT:
-        raise ValueError(f"quantize: fmt has to be 'e4m3' or 'e5m2', got {fmt!r}")
-    assert x.dim() == 2 and x.shape[1] >= 1, tuple(x.shape)
-    rows, cols = x.shape
-    rs, cs = x.stride()
-    if cs == 1 or cols == 1:
-        cs = 1
-    elif rs != 1 and rows > 1 or cs == 0:
-        x = x.contiguous()
-        rs, cs = cols, 1
-    elif rows == 1:
-        rs = 1
-    q = _alloc(rows, cols, fmt, x.device)
-    _call("ifl_block8_quantize", x.device, x.data_ptr(), _TYPE[x.dtype], rs, cs, q.codes.data_ptr(), _ld(q.codes), q.scales.data_ptr(),
-          _ld(q.scales), rows, cols, _FMT[fmt][0])
-    return q
-
-
-def dequantize(q: Block8, dtype=torch.float32) -> torch.Tensor:
-    """The values [rows, cols] that `q` stands for, rounded once to `dtype` (float16 overflows to infinity above 65504)."""
-    if not isinstance(q, Block8):
-        raise TypeError("dequantize: expected a Block8")
-    out = torch.empty(q.shape, dtype=_dtype(dtype, "dequantize"), device=q.device)
-    _call("ifl_block8_dequantize", q.device, q.codes.data_ptr(), _ld(q.codes), q.scales.data_ptr(), _ld(q.scales), _FMT_OF[q.codes.dtype], None,
-          out.data_ptr(), _TYPE[dtype], out.shape[1], out.shape[0], out.shape[1])
-    return out
-
-
-def _operand(q, name):
-    """(codes, scales) as the product reads them: aligned rows of whole 16 and 4 bytes; copies where they are not."""
+def _b8(q, name):
     if not isinstance(q, Block8):
         raise TypeError(f"{name}: expected a Block8")
-    codes, scales = q.codes, q.scales
-    if _ld(codes) % 16 or codes.data_ptr() % 16:
-        if codes.shape[0] != 1 or codes.data_ptr() % 16:
-            codes = torch.empty((codes.shape[0], (codes.shape[1] + 15) // 16 * 16), dtype=codes.dtype, device=codes.device)[:, :codes.shape[1]]
-            codes.view(torch.uint8).copy_(q.codes.view(torch.uint8))
-    if _ld(scales) % 4 or scales.data_ptr() % 4:
-        scales = torch.empty((scales.shape[0], (scales.shape[1] + 3) // 4 * 4), dtype=scales.dtype, device=scales.device)[:, :scales.shape[1]]
-        scales.view(torch.uint8).copy_(q.scales.view(torch.uint8))
-    return codes, scales
+    return q
 
 
 def _up(n, k):
     return (n + k - 1) // k * k
 
 
+def _matrix(x):
+    """(x, row stride, column stride) of a 2-dimensional x as the library reads it: one of the strides is 1."""
+    rows, cols = x.shape
+    rs, cs = x.stride()
+    if cs == 1 or cols == 1:
+        return x, rs, 1
+    if rows == 1 and cs:
+        return x, 1, cs
+    if rs == 1 and cs:
+        return x, 1, cs
+    return x.contiguous(), cols, 1
+
+
+def quantize(x, fmt: str = "e4m3") -> Block8:
+    """x [rows, cols] (float32, bfloat16 or float16, any strides; a transposed view is read as it is) in 8-bit blocks."""
+    t = _real(x, "quantize input")
+    f = _format(fmt, "quantize")
+    assert x.dim() == 2 and x.shape[1] >= 1, tuple(x.shape)
+    rows, cols = x.shape
+    x, rs, cs = _matrix(x)
+    q = Block8._new(rows, cols, f, x.device)
+    _call("ifl_block8_quantize", q._dev, x.data_ptr(), t, rs, cs, q._cp, q._ldc, q._sp, q._lds, rows, cols, f)
+    return q
+
+
+def dequantize(q: Block8, dtype=torch.float32) -> torch.Tensor:
+    """The values [rows, cols] that `q` stands for, rounded once to `dtype` (float16 overflows to infinity above 65504)."""
+    _b8(q, "dequantize")
+    t = _dtype(dtype, "dequantize")
+    out = torch.empty((q.rows, q.cols), dtype=dtype, device=q.device)
+    _call("ifl_block8_dequantize", q._dev, q._cp, q._ldc, q._sp, q._lds, q._f, None, out.data_ptr(), t, q.cols, q.rows, q.cols)
+    return out
+
+
 def _bias(bias, n, dev):
+    """(bias, its address, its type)"""
     if bias is None:
-        return None, 0
-    _real(bias, "bias")
+        return None, None, 0
+    t = _real(bias, "bias")
     assert bias.shape == (n,), (tuple(bias.shape), n)
     _same_device(dev, bias)
-    return bias.contiguous(), _TYPE[bias.dtype]
+    bias = bias.contiguous()
+    return bias, bias.data_ptr(), t
 
 
 def matmul(a: Block8, b: Block8, bias=None, dtype=torch.bfloat16) -> torch.Tensor:
     """a [M, K] times b [N, K]^T (+ bias [N]) -> [M, N] of `dtype`.  Formats may differ.  Sums are float32, rounded once."""
-    a_c, a_s = _operand(a, "a")
-    b_c, b_s = _operand(b, "b")
-    M, K = a_c.shape
-    N = b_c.shape[0]
-    assert b_c.shape[1] == K and N >= 1, (tuple(a.shape), tuple(b.shape))
-    _same_device(a_c.device, b_c)
-    bias, bt = _bias(bias, N, a_c.device)
-    out = torch.empty((M, N), dtype=_dtype(dtype, "matmul"), device=a_c.device)
-    n = hip.lib().ifl_block8_matmul_scratch_floats(M, N, K, _TYPE[dtype])
-    scratch = torch.empty((n,), dtype=torch.float32, device=out.device) if n else None
-    _call("ifl_block8_matmul", a_c.device, a_c.data_ptr(), _up(_ld(a_c), 16), a_s.data_ptr(), _up(_ld(a_s), 4), _FMT_OF[a_c.dtype], b_c.data_ptr(),
-          _up(_ld(b_c), 16), b_s.data_ptr(), _up(_ld(b_s), 4), _FMT_OF[b_c.dtype], bias.data_ptr() if bias is not None else None, bt,
-          out.data_ptr(), _TYPE[dtype], N, scratch.data_ptr() if n else None, M, N, K)
+    a, b = _b8(a, "matmul a")._aligned(), _b8(b, "matmul b")._aligned()
+    M, K, N, dev = a.rows, a.cols, b.rows, a._dev
+    assert b.cols == K and N >= 1, (tuple(a.shape), tuple(b.shape))
+    assert b._dev == dev, f"{a} and {b}"
+    bias, bp, bt = _bias(bias, N, dev)
+    t = _dtype(dtype, "matmul")
+    out = torch.empty((M, N), dtype=dtype, device=a.device)
+    scratch = _scratch(4 * _size("ifl_block8_matmul_scratch_floats", M, N, K, t), out.device)
+    _call("ifl_block8_matmul", dev, a._cp, _up(a._ldc, 16), a._sp, _up(a._lds, 4), a._f, b._cp, _up(b._ldc, 16), b._sp, _up(b._lds, 4), b._f, bp, bt,
+          out.data_ptr(), t, N, scratch.data_ptr() if scratch is not None else None, M, N, K)
     return out
 
 
 def linear(x, w: Block8, bias=None) -> torch.Tensor:
     """x [..., K] (float32, bfloat16 or float16) through a layer whose weights w [N, K] are kept in 8-bit blocks: x is quantized
     along its last dimension (e4m3) and multiplied -> [..., N] of x's type."""
-    _real(x, "linear input")
-    if not isinstance(w, Block8):
-        raise TypeError("linear: the weights have to be a Block8 (block8.quantize)")
-    assert x.dim() >= 1 and x.shape[-1] == w.shape[1], (tuple(x.shape), tuple(w.shape))
-    _same_device(x.device, w)
-    K, N = x.shape[-1], w.shape[0]
-    b_c, b_s = _operand(w, "weights")
-    bias, bt = _bias(bias, N, x.device)
-    x2 = x.reshape(-1, K)
+    t = _real(x, "linear input")
+    w = _b8(w, "linear weights")._aligned()
+    shape, K, N = x.shape, w.cols, w.rows
+    assert len(shape) >= 1 and shape[-1] == K and N >= 1, (tuple(shape), tuple(w.shape))
+    dev = x.get_device()
+    assert w._dev == dev, f"x on cuda:{dev}, weights {w}"
+    bias, bp, bt = _bias(bias, N, dev)
+    x2 = x if len(shape) == 2 else x.reshape(-1, K)
     if not _rows_apart(x2):
         x2 = x2.contiguous()
     M = x2.shape[0]
-    out = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=x.device)
-    t = _TYPE[x.dtype]
-    n = hip.lib().ifl_block8_linear_scratch_bytes(M, N, K, t)
-    scratch = torch.empty((n,), dtype=torch.uint8, device=x.device) if n else None
-    _call("ifl_block8_linear", x.device, x2.data_ptr(), t, _ld(x2), b_c.data_ptr(), _up(_ld(b_c), 16), b_s.data_ptr(), _up(_ld(b_s), 4),
-          _FMT_OF[b_c.dtype], bias.data_ptr() if bias is not None else None, bt, out.data_ptr(), N, scratch.data_ptr() if n else None, M, N, K)
+    out = torch.empty((*shape[:-1], N), dtype=x.dtype, device=x.device)
+    scratch = _scratch(_size("ifl_block8_linear_scratch_bytes", M, N, K, t), out.device)
+    _call("ifl_block8_linear", dev, x2.data_ptr(), t, _ld(x2), w._cp, _up(w._ldc, 16), w._sp, _up(w._lds, 4), w._f, bp, bt, out.data_ptr(), N,
+          scratch.data_ptr() if scratch is not None else None, M, N, K)
     return out
 
 
@@ -219,38 +271,63 @@ def weight_grad(dy, q: Block8, dtype=torch.float32, bias_dtype=None, weight: boo
     """(dw, db): dy [M, N]^T times the checkpoint q [M, K] -> dw [N, K] of `dtype` (None unless `weight`), and dy's column sums
     [N] of `bias_dtype` (None without one).  Products are exact and sums float32, in an order that depends on the sizes only."""
     _real(dy, "weight_grad dy")
-    if not isinstance(q, Block8):
-        raise TypeError("weight_grad: expected a Block8")
-    assert dy.dim() == 2 and dy.shape[0] == q.shape[0] and dy.shape[1] >= 1, (tuple(dy.shape), tuple(q.shape))
-    _same_device(dy.device, q)
+    _b8(q, "weight_grad checkpoint")
+    assert dy.dim() == 2 and dy.shape[0] == q.rows and dy.shape[1] >= 1, (tuple(dy.shape), tuple(q.shape))
+    _same_device(q._dev, dy)
     if not _rows_apart(dy):
         dy = dy.contiguous()
-    codes, scales = _operand(q, "checkpoint") if weight else (None, None)
-    return _wgrad(dy, codes, scales, None, _dtype(dtype, "weight_grad") if weight else None,
-                  _dtype(bias_dtype, "weight_grad") if bias_dtype is not None else None)
+    if weight:
+        _dtype(dtype, "weight_grad")
+    if bias_dtype is not None:
+        _dtype(bias_dtype, "weight_grad")
+    if not weight and bias_dtype is None:
+        return None, None
+    q = q._aligned() if weight else q
+    return _wgrad(dy, q._cp, _up(q._ldc, 16), q._sp, q._lds, q._f, q.cols, None, dtype if weight else None, bias_dtype)
 
 
-def _wgrad(dy, codes, scales, chan, dtype, bias_dtype):
-    """dy [M, N], codes [M, K], scales [M, ceil(K / 128)] with contiguous columns, chan float32 [K] or None; without `dtype` the
-    column sums alone (no codes)."""
+def _wgrad(dy, cp, ldc, sp, lds, f, K, chan, dtype, bias_dtype):
+    """dy [M, N], contiguous columns; codes [M, K] and scales by their addresses and row strides; chan float32 [K] or None."""
     M, N = dy.shape
-    dev = dy.device
-    if dtype is None:
-        if bias_dtype is None:
-            return None, None
-        db = torch.empty((N,), dtype=bias_dtype, device=dev)
-        n = hip.lib().ifl_block8_wgrad_scratch_floats(M, N, 0, _TYPE[dy.dtype])
-        scratch = torch.empty((n,), dtype=torch.float32, device=dev) if n else None
-        _call("ifl_block8_wgrad", dev, dy.data_ptr(), _TYPE[dy.dtype], _ld(dy), None, 0, None, 0, 0, None, None, 0, 0, db.data_ptr(), _TYPE[bias_dtype],
-              scratch.data_ptr() if n else None, M, N, 0)
-        return None, db
-    K = codes.shape[1]
-    dw = torch.empty((N, K), dtype=dtype, device=dev)
-    db = torch.empty((N,), dtype=bias_dtype, device=dev) if bias_dtype is not None else None
-    n = hip.lib().ifl_block8_wgrad_scratch_floats(M, N, K, _TYPE[dy.dtype])
-    scratch = torch.empty((n,), dtype=torch.float32, device=dev) if n else None
-    _call("ifl_block8_wgrad", dev, dy.data_ptr(), _TYPE[dy.dtype], _ld(dy), codes.data_ptr(), _ld(codes), scales.data_ptr(), _ld(scales),
-          _FMT_OF[codes.dtype], chan.data_ptr() if chan is not None else None, dw.data_ptr(), _TYPE[dtype], K,
-          db.data_ptr() if db is not None else None, _TYPE[bias_dtype] if db is not None else 0,
-          scratch.data_ptr() if n else None, M, N, K)
+    dev = dy.get_device()
+    dw = torch.empty((N, K), dtype=dtype, device=dy.device) if dtype is not None else None
+    db = torch.empty((N,), dtype=bias_dtype, device=dy.device) if bias_dtype is not None else None
+    scratch = _scratch(4 * _size("ifl_block8_wgrad_scratch_floats", M, N, K if dw is not None else 0, _TYPE[dy.dtype]), dy.device)
+    _call("ifl_block8_wgrad", dev, dy.data_ptr(), _TYPE[dy.dtype], _ld(dy), cp, ldc, sp, lds, f, chan.data_ptr() if chan is not None else None,
+          dw.data_ptr() if dw is not None else None, _TYPE[dtype] if dw is not None else 0, K, db.data_ptr() if db is not None else None,
+          _TYPE[bias_dtype] if db is not None else 0, scratch.data_ptr() if scratch is not None else None, M, N, K if dw is not None else 0)
     return dw, db
+
+
+# ------------------------------------------------------------------------------------------------ the layer in training
+def _linear_fwd(x2, w, bias, keep: bool):
+    """(y [M, N], x's 8-bit blocks as one tensor, if they are to be kept): quantize x and w along K and multiply."""
+    M, K = x2.shape
+    N = w.shape[0]
+    t, wt = _TYPE[x2.dtype], _TYPE[w.dtype]
+    x2, rs, cs = _matrix(x2)
+    w, wrs, wcs = _matrix(w)
+    bias, bp, bt = _bias(bias, N, x2.get_device())
+    y = torch.empty((M, N), dtype=x2.dtype, device=x2.device)
+    q = Block8._new(M, K, 0, x2.device)
+    scratch = _scratch(_size("ifl_linear8_fwd_scratch_bytes", M, N, K, t), x2.device)
+    _call("ifl_linear8_fwd", q._dev, x2.data_ptr(), t, rs, cs, w.data_ptr(), wt, wrs, wcs, bp, bt, q._cp, q._sp, y.data_ptr(),
+          scratch.data_ptr(), M, N, K)
+    return y, q._raw if keep else None
+
+
+def _linear_bwd(g, raw, w, need_x, need_w, bias_dtype, f):
+    """(dx, dw, db) of `_linear_fwd`; g [M, N] contiguous columns, raw the kept blocks of x."""
+    M, N = g.shape
+    K = w.shape[1]
+    t, wt, dev = _TYPE[g.dtype], _TYPE[w.dtype], g.device
+    w, wrs, wcs = _matrix(w)
+    dx = torch.empty((M, K), dtype=g.dtype, device=dev) if need_x else None
+    dw = torch.empty((N, K), dtype=w.dtype, device=dev) if need_w else None
+    db = torch.empty((N,), dtype=bias_dtype, device=dev) if bias_dtype is not None else None
+    scratch = _scratch(_size("ifl_linear8_bwd_scratch_bytes", M, N, K, t, int(need_x), int(need_w)), dev)
+    cp = raw.data_ptr() if need_w else None
+    _call("ifl_linear8_bwd", g.get_device(), g.data_ptr(), t, _ld(g), cp, cp + M * _up(K, 16) if need_w else None, w.data_ptr(), wt, wrs, wcs, f,
+          dx.data_ptr() if need_x else None, dw.data_ptr() if need_w else None, db.data_ptr() if db is not None else None,
+          _TYPE[bias_dtype] if db is not None else 0, scratch.data_ptr(), M, N, K)
+    return dx, dw, db

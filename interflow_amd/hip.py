@@ -151,11 +151,17 @@ def lib():
     L.ifl_block8_wgrad_scratch_floats.argtypes = [ll, ll, ll, c_int]
     L.ifl_block8_wgrad_scratch_floats.restype = ll
     L.ifl_block8_wgrad.argtypes = [vp, c_int, ll, vp, ll, vp, ll, c_int, vp, vp, c_int, ll, vp, c_int, vp, ll, ll, ll, vp]
+    L.ifl_linear8_fwd.argtypes = [vp, c_int, ll, ll, vp, c_int, ll, ll, vp, c_int, vp, vp, vp, vp, ll, ll, ll, vp]
+    L.ifl_linear8_fwd_scratch_bytes.argtypes = [ll, ll, ll, c_int]
+    L.ifl_linear8_fwd_scratch_bytes.restype = ll
+    L.ifl_linear8_bwd.argtypes = [vp, c_int, ll, vp, vp, vp, c_int, ll, ll, c_int, vp, vp, vp, c_int, vp, ll, ll, ll, vp]
+    L.ifl_linear8_bwd_scratch_bytes.argtypes = [ll, ll, ll, c_int, c_int, c_int]
+    L.ifl_linear8_bwd_scratch_bytes.restype = ll
     L.ifl_an_relu8_blocks.argtypes = [c_int, c_int, c_int, c_int]
     L.ifl_an_relu8_blocks.restype = ll
     L.ifl_an_relu8_fwd.argtypes = [vp, vp, vp, vp, vp, vp, c_int, c_int, c_int, c_int, vp]
     L.ifl_an_relu8_bwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, c_int, c_int, c_int, c_int, vp]
-    for name in ("ifl_block8_quantize", "ifl_block8_dequantize", "ifl_block8_matmul", "ifl_block8_linear", "ifl_block8_wgrad", "ifl_an_relu8_fwd", "ifl_an_relu8_bwd"):
+    for name in ("ifl_block8_quantize", "ifl_block8_dequantize", "ifl_block8_matmul", "ifl_block8_linear", "ifl_block8_wgrad", "ifl_linear8_fwd", "ifl_linear8_bwd", "ifl_an_relu8_fwd", "ifl_an_relu8_bwd"):
         getattr(L, name).restype = c_int
     L.ifl_prof_enable.argtypes = [c_int]
     L.ifl_prof_enable.restype = c_int
@@ -181,6 +187,7 @@ EXPORTS = ("ifl_version", "ifl_last_error", "ifl_step_param_floats", "ifl_step_f
            "ifl_train_bulk_conv1", "ifl_wino4_tiles", "ifl_wino4_kmajor", "ifl_wino4_dw", "ifl_conv2d_wgrad_batched", "ifl_conv2d_batched",
            "ifl_block8_quantize", "ifl_block8_dequantize", "ifl_block8_matmul", "ifl_block8_matmul_scratch_floats",
            "ifl_block8_linear", "ifl_block8_linear_scratch_bytes", "ifl_block8_wgrad_scratch_floats", "ifl_block8_wgrad",
+           "ifl_linear8_fwd", "ifl_linear8_fwd_scratch_bytes", "ifl_linear8_bwd", "ifl_linear8_bwd_scratch_bytes",
            "ifl_an_relu8_blocks", "ifl_an_relu8_fwd", "ifl_an_relu8_bwd")
 
 K_CONV1_FT_L1, K_CONV1_FT_L2, K_CONV1_FINISH, K_CONV3_F, K_CONV3_ENC, K_CONV3_DEC, K_ANIC = range(7)

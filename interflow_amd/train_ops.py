@@ -154,8 +154,8 @@ class _ConvRing(torch.autograd.Function):
                     if isinstance(s, Checkpoint8):
                         if taps == 1:
                             # the ring's codes and gradients are zeros: all pixels of the planes are rows of one product
-                            dw8, _ = block8._wgrad(g.view(-1, cout_pad), s.codes.view(-1, s.shape[3]), s.scales.view(-1, s.scales.shape[3]), s.chan,
-                                                   torch.float32, None)
+                            dw8, _ = block8._wgrad(g.view(-1, cout_pad), s.codes.data_ptr(), s.shape[3], s.scales.data_ptr(), s.scales.shape[3], 0,
+                                                   s.shape[3], s.chan, torch.float32, None)
                             dW[:, c0:c0 + s.shape[3], 0] = dw8
                             c0 += s.shape[3]
                             continue
@@ -263,7 +263,7 @@ class Checkpoint8:
         """The ringed float32 activation that the checkpoint stands for."""
         P, C = self.codes[..., 0].numel(), self.codes.shape[3]
         out = torch.empty(self.codes.shape, dtype=torch.float32, device=self.codes.device)
-        block8._call("ifl_block8_dequantize", self.codes.device, self.codes.data_ptr(), C, self.scales.data_ptr(), self.scales.shape[3], 0,
+        block8._call("ifl_block8_dequantize", self.codes.get_device(), self.codes.data_ptr(), C, self.scales.data_ptr(), self.scales.shape[3], 0,
                      self.chan.data_ptr(), out.data_ptr(), 0, C, P, C)
         return out
 
@@ -282,11 +282,11 @@ class _AnRelu8(torch.autograd.Function):
         B, hp, wp_, C = x.shape
         b, l = bias.detach().reshape(-1).float().contiguous(), logs.detach().reshape(-1).float().contiguous()
         assert b.numel() == C and l.numel() == C, (tuple(bias.shape), tuple(logs.shape), C)
-        block8._same_device(x.device, b, l)
+        block8._same_device(x.get_device(), b, l)
         y = torch.empty_like(x)
         codes = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
         scales = torch.empty((B, hp, wp_, -(-C // block8.BLOCK)), dtype=torch.float8_e8m0fnu, device=x.device)
-        block8._call("ifl_an_relu8_fwd", x.device, x.data_ptr(), y.data_ptr(), codes.data_ptr(), scales.data_ptr(), b.data_ptr(), l.data_ptr(),
+        block8._call("ifl_an_relu8_fwd", x.get_device(), x.data_ptr(), y.data_ptr(), codes.data_ptr(), scales.data_ptr(), b.data_ptr(), l.data_ptr(),
                      B, hp - 2, wp_ - 2, C)
         ctx.save_for_backward(codes, scales, l)
         ctx.shapes = (bias.shape, logs.shape)
@@ -302,7 +302,7 @@ class _AnRelu8(torch.autograd.Function):
         dx = torch.empty_like(gy)
         db, dl = torch.empty_like(l), torch.empty_like(l)
         part = torch.empty(hip.lib().ifl_an_relu8_blocks(B, hp - 2, wp_ - 2, C) * 2 * C, dtype=torch.float32, device=gy.device)
-        block8._call("ifl_an_relu8_bwd", gy.device, gy.data_ptr(), codes.data_ptr(), scales.data_ptr(), l.data_ptr(), dx.data_ptr(), db.data_ptr(),
+        block8._call("ifl_an_relu8_bwd", gy.get_device(), gy.data_ptr(), codes.data_ptr(), scales.data_ptr(), l.data_ptr(), dx.data_ptr(), db.data_ptr(),
                      dl.data_ptr(), part.data_ptr(), B, hp - 2, wp_ - 2, C)
         return dx, db.reshape(ctx.shapes[0]), dl.reshape(ctx.shapes[1])
 
@@ -321,28 +321,24 @@ class _Linear8(torch.autograd.Function):
     """y = Q(x) Q(w)^T + bias; the backward has Q(x) for a checkpoint (block8.py)."""
 
     @staticmethod
-    def forward(ctx, x, w, bias, grad_fmt):
-        x2 = x.reshape(-1, x.shape[-1])
-        q = block8.quantize(x2)
-        y = block8.matmul(q, block8.quantize(w), bias, x.dtype)
-        ctx.save_for_backward(q.codes if ctx.needs_input_grad[1] else None, q.scales if ctx.needs_input_grad[1] else None, w)
-        ctx.meta = (x.shape, x.dtype, bias.dtype if bias is not None else None, grad_fmt)
-        return y.view(*x.shape[:-1], w.shape[0])
+    def forward(ctx, x, w, bias, f):
+        shape = x.shape
+        y, raw = block8._linear_fwd(x if len(shape) == 2 else x.reshape(-1, shape[-1]), w, bias, ctx.needs_input_grad[1])
+        ctx.save_for_backward(raw, w)
+        ctx.meta = (shape, bias.dtype if bias is not None else None, f)
+        return y if len(shape) == 2 else y.view(*shape[:-1], w.shape[0])
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        codes, scales, w = ctx.saved_tensors
-        shape, dtype, bias_dtype, grad_fmt = ctx.meta
+        raw, w = ctx.saved_tensors
+        shape, bias_dtype, f = ctx.meta
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
         g = g.reshape(-1, w.shape[0])
         if not block8._rows_apart(g):
             g = g.contiguous()
-        dx = None
-        if ctx.needs_input_grad[0]:
-            dx = block8.matmul(block8.quantize(g, grad_fmt), block8.quantize(w.t()), None, dtype).view(shape)
-        need_w, need_b = ctx.needs_input_grad[1], ctx.needs_input_grad[2]
-        dw, db = block8._wgrad(g, codes, scales, None, w.dtype if need_w else None, bias_dtype if need_b else None)
-        return dx, dw, db, None
+        dx, dw, db = block8._linear_bwd(g, raw, w, need_x, need_w, bias_dtype if need_b else None, f)
+        return dx if dx is None or len(shape) == 2 else dx.view(shape), dw, db, None
 
 
 def linear8(x, weight, bias=None, grad_fmt: str = "e4m3"):
@@ -354,10 +350,8 @@ def linear8(x, weight, bias=None, grad_fmt: str = "e4m3"):
     block8._real(x, "linear8 input")
     block8._real(weight, "linear8 weight")
     assert x.dim() >= 1 and weight.dim() == 2 and x.shape[-1] == weight.shape[1] and weight.numel() > 0, (tuple(x.shape), tuple(weight.shape))
-    if grad_fmt not in block8._FMT:
-        raise ValueError(f"linear8: grad_fmt has to be 'e4m3' or 'e5m2', got {grad_fmt!r}")
-    block8._same_device(x.device, weight)
-    return _Linear8.apply(x, weight, bias, grad_fmt)
+    block8._same_device(x.get_device(), weight)
+    return _Linear8.apply(x, weight, bias, block8._format(grad_fmt, "linear8 grad_fmt"))
 
 
 class _Coupling(torch.autograd.Function):
