@@ -92,8 +92,9 @@ __device__ __forceinline__ void mm8_store(const MM8& q, int64_t m, int64_t n, co
 // stored); a last step that K does not fill goes through registers with zeros behind K.
 //
 // Waves WN x WM; a wave has NF x MF fragments of 16 x 16.  Row r of n-fragment f is row 16 G (f / G) + 4 G (r / 4) + 4 (f % G) +
-// r % 4 of the wave's (G = 4, or NF if less): so the four values a lane gets from each of G fragments are 4 G neighbours of
-// one output row.
+// r % 4 of the wave's: so the four values a lane gets from each of G fragments are 4 G neighbours of one output row, 32 bytes
+// of 16-bit results (G = 4, or NF if less), 16 of float32 (G = 1: four lanes' 16-byte stores then fill 64 bytes of a row; with
+// G = 4 each store left gaps for the next: 169 us instead of 144 at 16384 x 2048 x 2048).
 //
 // Workgroups go to the 8 XCDs in turn; an XCD takes a contiguous run of tiles, in groups of 8 along m, so that the 32 tiles
 // it works on at a time share rows of both operands in its own L2.
@@ -101,7 +102,7 @@ template <int TN, int TM, int WN, int WM, int FA, int FB, bool EXACT, bool SPLIT
 __global__ __launch_bounds__(64 * WN * WM, 1)
 void mm8_tile_kernel(MM8 q)
 {
-    constexpr int NW = WN * WM, NF = TN / WN / 16, MF = TM / WM / 16, G = NF < 4 ? NF : 4;
+    constexpr int NW = WN * WM, NF = TN / WN / 16, MF = TM / WM / 16, G = EXACT ? 1 : NF < 4 ? NF : 4;
     constexpr int CH = (TN + TM) * 8, PER = CH / (64 * NW);              // 16-byte pieces of a step, per thread
     constexpr int D = 1, R = 2 * D;                                          // n-fragments read ahead, and the registers they rotate through
     static_assert(NF % R == 0 && D < R, "");
