@@ -124,9 +124,9 @@ class _ConvRing(torch.autograd.Function):
         # a source with a checkpoint is kept as its 8-bit codes, block scales and channel factors
         kept = []
         for s, ck in zip(srcs, checkpoints or [None] * len(srcs)):
-            kept += [s] if ck is None else [ck.codes, ck.scales, ck.chan]
+            kept += [s] if ck is None else [ck.raw, ck.chan]
         ctx.save_for_backward(weight, *kept)
-        ctx.in8 = [ck is not None for ck in checkpoints] if checkpoints else [False] * len(srcs)
+        ctx.in8 = [ck.shape if ck is not None else None for ck in checkpoints] if checkpoints else [None] * len(srcs)
         ctx.meta = (splits, cout, cout_pad, taps, B, h, w, bias is not None)
         return out
 
@@ -136,7 +136,7 @@ class _ConvRing(torch.autograd.Function):
         weight, *kept = ctx.saved_tensors
         kept, srcs = list(kept), []
         for in8 in ctx.in8:
-            srcs.append(Checkpoint8(kept.pop(0), kept.pop(0), kept.pop(0)) if in8 else kept.pop(0))
+            srcs.append(Checkpoint8(kept.pop(0), in8, kept.pop(0)) if in8 is not None else kept.pop(0))
         splits, cout, cout_pad, taps, B, h, w, has_bias = ctx.meta
         L = hip.lib()
         # a fresh contiguous [B, h+2, w+2, cout_pad] buffer (the kernels index it as such, whatever strides gout has):
@@ -154,8 +154,7 @@ class _ConvRing(torch.autograd.Function):
                     if isinstance(s, Checkpoint8):
                         if taps == 1:
                             # the ring's codes and gradients are zeros: all pixels of the planes are rows of one product
-                            dw8, _ = block8._wgrad(g.view(-1, cout_pad), s.codes.data_ptr(), s.shape[3], s.scales.data_ptr(), s.scales.shape[3], 0,
-                                                   s.shape[3], s.chan, torch.float32, None)
+                            dw8, _ = block8._wgrad(g.view(-1, cout_pad), *s._where(), 0, s.shape[3], s.chan, torch.float32, None)
                             dW[:, c0:c0 + s.shape[3], 0] = dw8
                             c0 += s.shape[3]
                             continue
@@ -243,34 +242,61 @@ def an_relu_ring(x_ring, bias, logs):
 
 class Checkpoint8:
     """An activation of `an_relu8_ring` in 8 bits: values v in 8-bit blocks (block8: e4m3, a scale per pixel and 128 channels) and
-    the factor per channel that makes them y = v exp(logs).  codes [B, h+2, w+2, C], scales [B, h+2, w+2, ceil(C / 128)], chan [C]."""
-    __slots__ = ("codes", "scales", "_chan", "_logs")
+    the factor per channel that makes them y = v exp(logs).  codes [B, h+2, w+2, C], scales [B, h+2, w+2, ceil(C / 128)], chan [C].
+    `raw` is both in one tensor of bytes, codes first."""
+    __slots__ = ("raw", "shape", "_chan", "_logs", "_version")
 
-    def __init__(self, codes, scales, chan=None, logs=None):
-        self.codes, self.scales, self._chan, self._logs = codes, scales, chan, logs
+    def __init__(self, raw, shape, chan=None, logs=None):
+        self.raw, self.shape, self._chan, self._logs = raw, shape, chan, logs
+        if logs is not None:
+            self._version = None if logs.is_inference() else logs._version
+            if self._version is None:
+                self._chan = torch.exp(logs.reshape(-1).float())
+
+    @staticmethod
+    def room(shape, dev):
+        px, C = shape[0] * shape[1] * shape[2], shape[3]
+        return torch.empty((px * (C + -(-C // block8.BLOCK)),), dtype=torch.uint8, device=dev)
 
     @property
-    def shape(self):
-        return self.codes.shape
+    def codes(self):
+        return self.raw[:self.shape.numel()].view(torch.float8_e4m3fn).view(self.shape)
+
+    @property
+    def scales(self):
+        return self.raw[self.shape.numel():].view(torch.float8_e8m0fnu).view(*self.shape[:3], -1)
 
     @property
     def chan(self):
         if self._chan is None:
-            self._chan = torch.exp(self._logs)
+            if self._logs._version != self._version:
+                raise RuntimeError("an activation checkpoint's logs were changed in place before its channel factors were first used")
+            self._chan = torch.exp(self._logs.detach().reshape(-1).float())
         return self._chan
+
+    def _where(self):
+        """(address of the codes, their row stride, address of the scales, their row stride)"""
+        p, C = self.raw.data_ptr(), self.shape[3]
+        return p, C, p + self.shape.numel(), -(-C // block8.BLOCK)
 
     def restore(self):
         """The ringed float32 activation that the checkpoint stands for."""
-        P, C = self.codes[..., 0].numel(), self.codes.shape[3]
-        out = torch.empty(self.codes.shape, dtype=torch.float32, device=self.codes.device)
-        block8._call("ifl_block8_dequantize", self.codes.get_device(), self.codes.data_ptr(), C, self.scales.data_ptr(), self.scales.shape[3], 0,
-                     self.chan.data_ptr(), out.data_ptr(), 0, C, P, C)
+        C = self.shape[3]
+        out = torch.empty(self.shape, dtype=torch.float32, device=self.raw.device)
+        block8._call("ifl_block8_dequantize", self.raw.get_device(), *self._where(), 0, self.chan.data_ptr(), out.data_ptr(), 0, C, out.numel() // C, C)
         return out
 
 
 def _aligned(t):
     """A contiguous tensor whose data starts on 16 bytes (a view may start anywhere)."""
     return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _plain_f32(t):
+    """A parameter as contiguous float32: itself, if it is."""
+    if t.dtype == torch.float32 and t.is_contiguous():
+        return t
+    return t.detach().float().contiguous()
 
 
 class _AnRelu8(torch.autograd.Function):
@@ -280,31 +306,36 @@ class _AnRelu8(torch.autograd.Function):
     def forward(ctx, x, bias, logs):
         x = _aligned(hip._dev_f32(x, "an_relu8 input"))
         B, hp, wp_, C = x.shape
-        b, l = bias.detach().reshape(-1).float().contiguous(), logs.detach().reshape(-1).float().contiguous()
+        b, l = _plain_f32(bias), _plain_f32(logs)
         assert b.numel() == C and l.numel() == C, (tuple(bias.shape), tuple(logs.shape), C)
-        block8._same_device(x.get_device(), b, l)
+        dev = x.get_device()
+        block8._same_device(dev, b, l)
         y = torch.empty_like(x)
-        codes = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
-        scales = torch.empty((B, hp, wp_, -(-C // block8.BLOCK)), dtype=torch.float8_e8m0fnu, device=x.device)
-        block8._call("ifl_an_relu8_fwd", x.get_device(), x.data_ptr(), y.data_ptr(), codes.data_ptr(), scales.data_ptr(), b.data_ptr(), l.data_ptr(),
-                     B, hp - 2, wp_ - 2, C)
-        ctx.save_for_backward(codes, scales, l)
-        ctx.shapes = (bias.shape, logs.shape)
-        ctx.mark_non_differentiable(codes, scales)
-        return y, codes, scales
+        raw = Checkpoint8.room(x.shape, x.device)
+        p = raw.data_ptr()
+        block8._call("ifl_an_relu8_fwd", dev, x.data_ptr(), y.data_ptr(), p, p + x.numel(), b.data_ptr(), l.data_ptr(), B, hp - 2, wp_ - 2, C)
+        ctx.save_for_backward(raw, l)
+        ctx.shapes = (x.shape, bias.shape, logs.shape)
+        ctx.mark_non_differentiable(raw)
+        ctx.set_materialize_grads(False)
+        return y, raw
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, gy, _codes, _scales):
-        codes, scales, l = ctx.saved_tensors
-        B, hp, wp_, C = codes.shape
+    def backward(ctx, gy, _raw):
+        if gy is None:
+            return None, None, None
+        raw, l = ctx.saved_tensors
+        shape, bshape, lshape = ctx.shapes
+        B, hp, wp_, C = shape
         gy = _aligned(hip._dev_f32(gy, "an_relu8 gradient"))
         dx = torch.empty_like(gy)
-        db, dl = torch.empty_like(l), torch.empty_like(l)
-        part = torch.empty(hip.lib().ifl_an_relu8_blocks(B, hp - 2, wp_ - 2, C) * 2 * C, dtype=torch.float32, device=gy.device)
-        block8._call("ifl_an_relu8_bwd", gy.get_device(), gy.data_ptr(), codes.data_ptr(), scales.data_ptr(), l.data_ptr(), dx.data_ptr(), db.data_ptr(),
-                     dl.data_ptr(), part.data_ptr(), B, hp - 2, wp_ - 2, C)
-        return dx, db.reshape(ctx.shapes[0]), dl.reshape(ctx.shapes[1])
+        db, dl = torch.empty(bshape, dtype=torch.float32, device=gy.device), torch.empty(lshape, dtype=torch.float32, device=gy.device)
+        part = torch.empty((block8._size("ifl_an_relu8_blocks", B, hp - 2, wp_ - 2, C) * 2 * C,), dtype=torch.float32, device=gy.device)
+        p = raw.data_ptr()
+        block8._call("ifl_an_relu8_bwd", gy.get_device(), gy.data_ptr(), p, p + gy.numel(), l.data_ptr(), dx.data_ptr(), db.data_ptr(), dl.data_ptr(),
+                     part.data_ptr(), B, hp - 2, wp_ - 2, C)
+        return dx, db, dl
 
 
 def an_relu8_ring(x_ring, bias, logs):
@@ -313,8 +344,8 @@ def an_relu8_ring(x_ring, bias, logs):
     logs is that of the checkpoint's values.  Ringed tensors, channels a multiple of 32, at most 1024.  Hand the checkpoint to the
     convolution that reads y (`conv2d_ring(checkpoints=...)`) and y itself is not kept either."""
     assert x_ring.dim() == 4 and x_ring.shape[1] >= 3 and x_ring.shape[2] >= 3, tuple(x_ring.shape)
-    y, codes, scales = _AnRelu8.apply(x_ring, bias, logs)
-    return y, Checkpoint8(codes, scales, logs=logs.detach().reshape(-1).float())
+    y, raw = _AnRelu8.apply(x_ring, bias, logs)
+    return y, Checkpoint8(raw, x_ring.shape, logs=logs)
 
 
 class _Linear8(torch.autograd.Function):
