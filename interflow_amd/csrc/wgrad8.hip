@@ -4,25 +4,35 @@
 // A code times its scale is exact in bf16, and so is a bf16 gradient; a float16 gradient is the sum of two bf16 terms and a
 // float32 one of three (its 24 significant bits in pieces of 8).  So every product goes exactly through
 // v_mfma_f32_16x16x32_bf16 (one, two or three of them), which keeps 24 bits of the sums.
+//
+// Three launches: codes restored to bf16 and gradients split into their terms, with dy's column sums (memory-bound, one pass); the
+// product; the parts of a split sum joined.  Restoring and splitting inside the product, where every workgroup of a row of
+// tiles repeats it, was the slower way: its arithmetic does not fit beside the matrix instructions (2048 x 2048 over 65536 rows,
+// bf16: 615 us with it, 390 without; float32: 1644 and 841).
 #include "block8.h"
 
 namespace {
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-
-template <bool V> struct Flag { static constexpr bool value = V; };
 
 struct WG8 {
+    // the caller's
     const void* dy; int64_t ldy;
     const uint8_t* codes; int64_t ldc;
     const uint8_t* scales; int64_t lds;
     const float* chan;
     void* dw; int64_t ldw; int dwtype;
-    float* part; int split, steps;       // float32 partial sums [split][N][K], steps of 64 rows per part
-    int64_t M; int N, K;
+    void* db; int dbtype;
+    int64_t M; int N, K, fmt;
+    int want_x;                          // 0: column sums alone
+    // scratch
+    uint16_t* xb; int64_t kp;            // restored codes [rows up to a multiple of 32][kp], zeros behind row M
+    uint16_t* yb; int64_t np, yplane;    // terms of dy [NP][rows up to a multiple of 32][np]; of bf16 read in place: its last M % 32 rows
+    int in_place;
+    float* part; int split, steps;       // float32 partial sums [split][N][K], steps of 32 rows per part
+    float* cs; int cs_parts; int64_t cs_rows, y_row0;        // partial column sums [cs_parts][N], of cs_rows rows from y_row0 on
     int tiles_n, tiles_k, per_xcd;
-    int ywide;                           // whole 16-byte loads of dy
+    int x_blocks, x_tpr_log, y_cols;     // first launch: workgroups that restore codes, threads along a row; of 256 columns of dy
 };
 
 // One, two or three bf16 terms whose sum is the value, as floats with 16 low zero bits: its leading 8 significant bits, the next 8,
@@ -44,291 +54,296 @@ __device__ __forceinline__ void wg8_terms(float x, float t[NP]) {
 }
 
 template <class TW>
-__device__ __forceinline__ void wg8_store16(TW* d, int left, const float v[16]) {
-    if (left >= 16 && (uintptr_t)d % 16 == 0) { b8_store8<TW, true>(d, 8, v); b8_store8<TW, true>(d + 8, 8, v + 8); }
-    else { b8_store8<TW, false>(d, left, v); if (left > 8) b8_store8<TW, false>(d + 8, left - 8, v + 8); }
+__device__ __forceinline__ void wg8_store4(TW* d, int left, const float v[4]) {
+    typedef TW TW4 __attribute__((ext_vector_type(4)));
+    if (left >= 4 && (uintptr_t)d % sizeof(TW4) == 0) {
+        TW4 w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = (TW)v[e];
+        *(TW4*)d = w;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) if (e < left) d[e] = (TW)v[e];
+    }
 }
 
-// Workgroup = TN x TK of dw over a range of rows, MS at a time through two LDS buffers (rows of dy and of the restored codes as they
-// lie in memory); the fragments, which run along m, come out of LDS transposed (ds_read_b64_tr_b16: 16 lanes read 4 rows of
-// 16 values and get columns).  The instruction's first operand is the k side: a lane ends up with 4 neighbouring k of one n.
-//
-// A fragment read touches, per group of 16 lanes, 4 rows and 4 pieces of 8 bytes of each.  n side: the four pieces are one granule
-// of 32 bytes, granule i of row m at place i ^ (m & 7).  k side: piece f % 4 of four neighbouring granules, so that a lane's four
-// fragments are 16 neighbouring k; piece j of granule i of row m at piece j ^ (m & 3) of place i ^ (m & 4).  Both: no bank conflicts.
-//
-// bf16 gradients go straight to LDS (DMA); others, and whatever is not aligned or is cut off, through registers, loaded one
-// step ahead.
-template <class T, int NP, int TN, int TK, int WN, int WK, int MS, int FMT, bool DMA>
-__global__ __launch_bounds__(64 * WN * WK)
-void wgrad8_kernel(WG8 q)
-{
-    constexpr int NT = 64 * WN * WK, NF = TN / WN / 16, KF = TK / WK / 16;
-    constexpr int GR = KF * MS / 32, D = 2, R = 4;          // groups of a step, x fragments read ahead and held
-    constexpr int YROW = TN * 2, XROW = TK * 2, YPL = MS * YROW;       // bytes
-    constexpr int YP = MS * TN / 8 / NT, XP = MS * TK / 16 / NT;     // pieces (8 values of dy, 16 codes) per thread
-    static_assert(YP * NT * 8 == MS * TN && XP * NT * 16 == MS * TK && NF == 4 && (KF == 4 || KF == 8) && GR % R == 0, "");
-    __shared__ __attribute__((aligned(16))) uint8_t y0[NP * YPL], y1[NP * YPL], x0[MS * XROW], x1[MS * XROW];
-    const int all = q.tiles_n * q.tiles_k * q.split;
-    const int id = (blockIdx.x & 7) * q.per_xcd + (blockIdx.x >> 3);
-    if (id >= all) return;
-    const int part = id / (q.tiles_n * q.tiles_k), tile = id - part * (q.tiles_n * q.tiles_k);
-    const int tn = tile / q.tiles_k, tk = tile - tn * q.tiles_k;
-    const int n0 = tn * TN, k0 = tk * TK;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, g = lane >> 4;
-    const int wk = wave % WK, wn = wave / WK;
-    const int64_t mb = (int64_t)part * q.steps * MS, me = min(q.M, mb + (int64_t)q.steps * MS);
-    const int steps = (int)((me - mb + MS - 1) / MS);
+constexpr int MS = 32;                                                  // rows per step: the depth of one product
 
-    // ---- staging: registers of the step that is on its way
-    float yr[DMA ? 1 : YP][8];
-    i32x4 xr[XP];
-    int xs[XP];
-    const T* dy = (const T*)q.dy;
-    // (what is cut off is loaded from a place that exists and made zero when it is stored: a load that is used or branched around at
-    // once would be waited for at once)
-    auto y_load = [&](int64_t m0) {
-        if constexpr (!DMA) {
-            const T* base = dy + m0 * q.ldy;
-            const int rows = (int)min((int64_t)MS, me - m0) - 1;
+// ------------------------------------------------------------------------------------------------ first launch
+// Workgroups 0 .. x_blocks - 1 restore codes, 8 a thread.  The others take 256 columns (8 a thread) of cs_rows rows of dy: eight
+// threads' rows in turn, column sums on the way, joined in LDS in a fixed order.
+template <class T, int NP, bool VEC>
+__global__ __launch_bounds__(256)
+void wgrad8_prepare_kernel(WG8 q)
+{
+    const int64_t mp = (q.M + MS - 1) / MS * MS;
+    if ((int)blockIdx.x < q.x_blocks) {
+        const int rpb = 256 >> q.x_tpr_log;
+        const int64_t step = (int64_t)q.x_blocks * rpb;
+        constexpr int U = 4;
+        for (int64_t r0 = (int64_t)blockIdx.x * rpb + (threadIdx.x >> q.x_tpr_log); r0 < mp; r0 += U * step) {
+            for (int c = (threadIdx.x & ((1 << q.x_tpr_log) - 1)) * 8; c < q.kp; c += 8 << q.x_tpr_log) {
+                i32x2 w[U];
+                int sb[U];
 #pragma unroll
-            for (int i = 0; i < YP; ++i) {
-                const int p = i * NT + tid, n = n0 + p % (TN / 8) * 8;
-                const uint32_t at = (uint32_t)(min(p / (TN / 8), rows) * (int)q.ldy);
-                if (q.ywide) b8_load8<T, true>(base + (at + (n < q.N ? n : 0)), 8, yr[i]);
-                else b8_load8<T, false>(base + (at + n), q.N - n, yr[i]);
+                for (int u = 0; u < U; ++u) {
+                    const int64_t r = r0 + u * step;
+                    const bool in = r < q.M && c < q.K;                  // (rows are whole 16 bytes)
+                    w[u] = in ? *(const i32x2*)(q.codes + r * q.ldc + c) : i32x2{0, 0};
+                    sb[u] = in ? q.scales[r * q.lds + c / B8_BLK] : 127;
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int64_t r = r0 + u * step;
+                    if (r < mp) *(bf16x8*)(q.xb + r * q.kp + c) = q.fmt == IFL_Q_E4M3 ? b8_bf16x8<IFL_Q_E4M3>(w[u][0], w[u][1], sb[u]) : b8_bf16x8<IFL_Q_E5M2>(w[u][0], w[u][1], sb[u]);
+                }
             }
         }
-    };
-    // (fresh: an address or offset that is made again at its use instead of being held in registers of its own)
-    auto fresh = [](auto x) { asm volatile("" : "+v"(x)); return x; };
-    uint32_t ycol = 0;
-    if constexpr (DMA) {
-        const int r = tid / (TN / 8), c = tid % (TN / 8), s = ((c >> 1) ^ (r & 7)) * 2 + (c & 1);
-        ycol = n0 + s * 8 < q.N ? s * 16 : 0;                            // (columns past the end: any, their results are not stored)
+        return;
     }
-    auto y_dma = [&](uint8_t* buf, int64_t m0) {
-        if constexpr (DMA) {
-            const uint8_t* base = (const uint8_t*)(dy + m0 * q.ldy + n0);
-            const int rows = (int)min((int64_t)MS, me - m0) - 1;
+    __shared__ float red[8][256 + 8];
+    const int b = blockIdx.x - q.x_blocks, part = b / q.y_cols, cb = b - part * q.y_cols;
+    const int c = cb * 256 + (threadIdx.x & 31) * 8, rl = threadIdx.x >> 5;
+    const int64_t first = q.y_row0 + (int64_t)part * q.cs_rows, last = min(mp, first + q.cs_rows);
+    const int64_t m32 = q.M / MS * MS;
+    const T* dy = (const T*)q.dy;
+    float sum[8] = {};
+    for (int64_t r0 = first + rl; r0 < last; r0 += 32) {
+        float v[4][8];
 #pragma unroll
-            for (int i = 0; i < YP; ++i) {
-                // a thread's pieces lie NT / (TN / 8) rows, a multiple of 8, apart: the same column in all of them
-                static_assert(NT / (TN / 8) % 8 == 0, "");
-                const uint32_t o = fresh(ycol) + (uint32_t)(min(fresh(tid) / (TN / 8) + i * (NT / (TN / 8)), rows) * 2 * (int)q.ldy);
-                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(base + o),
-                                                 (__attribute__((address_space(3))) void*)(buf + (i * NT + wave * 64) * 16), 16, 0, 0);
-            }
+        for (int u = 0; u < 4; ++u) {
+            const int64_t r = r0 + 8 * u;
+            b8_load8<T, VEC>(dy + (r < q.M ? r : 0) * q.ldy + c, r < q.M && r < last ? q.N - c : 0, v[u]);
         }
-    };
-    auto y_store = [&](uint8_t* buf, int64_t m0) {
-        if constexpr (!DMA) {
 #pragma unroll
-            for (int i = 0; i < YP; ++i) {
-                const int p = i * NT + tid, r = p / (TN / 8), c = p % (TN / 8);
+        for (int u = 0; u < 4; ++u) {
+            const int64_t r = r0 + 8 * u;
+            if (r >= last) break;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[i] += v[u][i];
+            // terms of what is not read in place: everything, or the rows behind the last 32 whole ones
+            if (q.want_x && c < q.np && (!q.in_place || r >= m32)) {
                 float t[8][NP];
-                const bool in = m0 + r < me && n0 + c * 8 < q.N;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) wg8_terms<NP>(in ? yr[i][e] : 0.f, t[e]);
+                for (int i = 0; i < 8; ++i) wg8_terms<NP>(v[u][i], t[i]);
 #pragma unroll
                 for (int k = 0; k < NP; ++k) {
                     i32x4 w;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) w[e] = (int)__builtin_amdgcn_perm(__float_as_uint(t[2 * e + 1][k]), __float_as_uint(t[2 * e][k]), 0x07060302u);   // the high halves
-                    *(i32x4*)(buf + k * YPL + r * YROW + ((c >> 1) ^ (r & 7)) * 32 + (c & 1) * 16) = w;
+                    *(i32x4*)(q.yb + k * q.yplane + (q.in_place ? r - m32 : r) * q.np + c) = w;
                 }
             }
         }
-    };
-    auto x_load = [&](int64_t m0) {
-        const uint8_t *base = q.codes + m0 * q.ldc, *sbase = q.scales + m0 * q.lds;
-        const int rows = (int)min((int64_t)MS, me - m0) - 1;
+    }
+    if (!q.db) return;
 #pragma unroll
-        for (int i = 0; i < XP; ++i) {
-            const int p = i * NT + tid, k = k0 + p % (TK / 16) * 16;
-            const int r = min(p / (TK / 16), rows), kc = k < q.K ? k : 0;
-            xr[i] = *(const i32x4*)(base + (uint32_t)(r * (int)q.ldc + kc));
-            xs[i] = sbase[(uint32_t)(r * (int)q.lds + kc / B8_BLK)];
-        }
-    };
-    auto x_store = [&](uint8_t* buf, int64_t m0, int i) {
-        {
-            const int p = i * NT + tid, r = p / (TK / 16), c = p % (TK / 16);
-            const int left = m0 + r < me ? q.K - k0 - c * 16 : 0;
-            if (left < 16) {
+    for (int i = 0; i < 8; ++i) red[rl][(threadIdx.x & 31) * 8 + i] = sum[i];
+    __syncthreads();
+    float t = red[0][threadIdx.x];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int l = left - 4 * e;
-                    xr[i][e] = l >= 4 ? xr[i][e] : l <= 0 ? 0 : (int)((uint32_t)xr[i][e] & ((1u << 8 * l) - 1));
-                }
-                if (left <= 0) xs[i] = 127;
-            }
-            const bf16x8 lo = b8_bf16x8<FMT>(xr[i][0], xr[i][1], xs[i]), hi = b8_bf16x8<FMT>(xr[i][2], xr[i][3], xs[i]);
-            const i32x4 a = __builtin_bit_cast(i32x4, lo), b = __builtin_bit_cast(i32x4, hi);
-            const bool odd = r & 1;                                      // piece j at j ^ (r & 3): first within 16 bytes, then the halves
-            const i32x4 u = {odd ? a[2] : a[0], odd ? a[3] : a[1], odd ? a[0] : a[2], odd ? a[1] : a[3]};
-            const i32x4 v = {odd ? b[2] : b[0], odd ? b[3] : b[1], odd ? b[0] : b[2], odd ? b[1] : b[3]};
-            uint8_t* d = buf + r * XROW + (c ^ (r & 4)) * 32;
-            *(i32x4*)(d + (r & 2 ? 16 : 0)) = u;
-            *(i32x4*)(d + (r & 2 ? 0 : 16)) = v;
+    for (int i = 1; i < 8; ++i) t += red[i][threadIdx.x];
+    if (cb * 256 + (int)threadIdx.x < q.N) q.cs[(int64_t)part * q.N + cb * 256 + threadIdx.x] = t;
+}
+
+// ------------------------------------------------------------------------------------------------ the product
+// Workgroup = TN x TK of dw over a range of rows, 32 at a time.  Rows of both operands lie in LDS as they do in memory; the fragments,
+// which run along m, come out of LDS transposed (ds_read_b64_tr_b16: 16 lanes read 4 rows of 16 values and get columns).  The
+// instruction's first operand is the k side: a lane ends up with 4 neighbouring k of one n.
+//
+// A fragment read touches, per group of 16 lanes, 4 rows and 4 pieces of 8 bytes of each: one granule of 32 bytes, granule i of row m at
+// place i ^ (m & 7), which leaves no bank conflicts.  Loads go straight to LDS in lane order, so it is the source that is permuted.
+//
+// A step is a term of dy with 32 rows (the terms of the same rows follow one another and share the k side's fragments).  It has two
+// phases.  MEM: the loads of the step three ahead are issued (rings of four), this step's fragments are read.  COMPUTE: its
+// products, nothing else.  With 8 waves the second four run one phase behind the first, so that of the two waves on a SIMD one
+// multiplies while the other one reads: the workgroup meets after every phase.  Three steps are about 1.5 us, what rows that
+// all workgroups ask for at the same time take to come from memory.
+template <int V> struct Int { static constexpr int value = V; };
+
+template <int NP, int TN, int TK, int WN, int WK>
+__global__ __launch_bounds__(64 * WN * WK)
+void wgrad8_kernel(WG8 q)
+{
+    constexpr int NW = WN * WK, NT = 64 * NW, NF = TN / WN / 16, KF = TK / WK / 16;
+    constexpr bool TURNS = NW == 8;
+    constexpr int YROW = TN * 2, XROW = TK * 2, YB = MS * YROW, XB = MS * XROW;          // bytes
+    constexpr int YP = YB / 16 / NT, XP = XB / 16 / NT;                  // 16-byte pieces per thread
+    static_assert(YP == 2 && XP == 2 && NF == 4 && (KF == 4 || KF == 8), "");
+    __shared__ __attribute__((aligned(16))) uint8_t ys[4 * YB], xs[4 * XB];
+    const int all = q.tiles_n * q.tiles_k * q.split;
+    const int id = (blockIdx.x & 7) * q.per_xcd + (blockIdx.x >> 3);
+    if (id >= all) return;
+    const int part = __builtin_amdgcn_readfirstlane(id / (q.tiles_n * q.tiles_k)), tile = id - part * (q.tiles_n * q.tiles_k);
+    const int tn = __builtin_amdgcn_readfirstlane(tile / q.tiles_k), tk = tile - tn * q.tiles_k;
+    const int n0 = tn * TN, k0 = tk * TK;
+    const uint32_t tid = threadIdx.x;
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, g = lane >> 4;
+    const int wk = wave % WK, wn = wave / WK;
+    const int s0 = part * q.steps, rows_steps = (int)((q.M + MS - 1) / MS), steps = (min(rows_steps, s0 + q.steps) - s0) * NP;
+    // (fresh: an address or offset that is made again at its use instead of being held in registers of its own)
+    auto fresh = [](auto x) { asm volatile("" : "+v"(x)); return x; };
+
+    // ---- loads: 64 lanes' 16 bytes each, from base + their offsets, to LDS in lane order.  By hand: the compiler waits for all loads
+    // wherever it thinks that one might have written what is read.  (The instruction reads M0 one wait state after it is written.)
+    auto to_lds = [&](const void* base, uint32_t o, const uint8_t* to) {
+        const uint32_t at = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)to;
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(at), "v"(o), "s"(base) : "memory", "m0");
+    };
+    // a thread's pieces: a column (past the end: any, its results are not stored), rows that lie a multiple of 8 apart
+    constexpr int YSTEP = NT / (TN / 8), XSTEP = NT / (TK / 8);
+    static_assert(YSTEP % 8 == 0 && XSTEP % 8 == 0, "");
+    const int64_t ldy = q.in_place ? q.ldy : q.np;
+    uint32_t yo, xo;
+    {
+        const int r = tid / (TN / 8), c = ((tid % (TN / 8) >> 1) ^ (r & 7)) * 2 + (tid & 1);
+        yo = (n0 + c * 8 < q.np ? n0 * 2 + c * 16 : 0) + (uint32_t)(r * 2 * (int)ldy);
+        const int rx = tid / (TK / 8), cx = ((tid % (TK / 8) >> 1) ^ (rx & 7)) * 2 + (tid & 1);
+        xo = (k0 + cx * 8 < q.kp ? k0 * 2 + cx * 16 : 0) + (uint32_t)(rx * 2 * (int)q.kp);
+    }
+    const int m32 = (int)(q.M / MS);
+    // step t: term PL of rows 32 (s0 + t / NP) on; behind the last step it is loaded again, unused
+    auto load = [&](auto PL, int t, int ry, int rx) {
+        const int s = s0 + min(t, steps - 1) / NP;
+        // of rows read in place the last ones, which do not fill a step, were copied to a place with zeros behind them: np apart there
+        const uint16_t* y = q.in_place ? (const uint16_t*)q.dy + (int64_t)s * MS * ldy : q.yb + PL.value * q.yplane + (int64_t)s * MS * ldy;
+        const bool cut = q.in_place && s >= m32;
+        y = cut ? q.yb : y;
+        const int dl = cut ? (int)(q.np - ldy) * 2 : 0;                  // (rows of the copy are closer together)
+#pragma unroll
+        for (int i = 0; i < YP; ++i)
+            to_lds(y, fresh(yo) + (uint32_t)(((int)(fresh(tid) / (TN / 8)) + i * YSTEP) * dl + i * YSTEP * 2 * (int)ldy), ys + ry * YB + (i * NT + wave * 64) * 16);
+        if constexpr (PL.value == 0) {
+            const uint16_t* x = q.xb + (int64_t)s * MS * q.kp;
+#pragma unroll
+            for (int i = 0; i < XP; ++i) to_lds(x, fresh(xo) + (uint32_t)(i * XSTEP * 2 * (int)q.kp), xs + rx * XB + (i * NT + wave * 64) * 16);
         }
     };
 
-    // ---- fragments
+    // ---- fragments (places are XORs of a lane's own and of a fragment's constants)
     const int mrow = 4 * g + (r16 >> 2), q4 = r16 & 3;
-    // (places are XORs of a lane's own and of a fragment's constants)
-    const int ya = mrow * YROW + ((wn * NF) ^ (mrow & 7)) * 32 + q4 * 8;
-    const int xa = mrow * XROW + ((wk * KF + q4) ^ (mrow & 4)) * 32 + (mrow & 3) * 8;
+    const int ya = mrow * YROW + ((wn * NF) ^ (mrow & 7)) * 32 + q4 * 8, xa = mrow * XROW + ((wk * KF) ^ (mrow & 7)) * 32 + q4 * 8;
     auto tr8 = [&](const uint8_t* a, int rows16) {
         const s16x4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a));
         const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a + rows16));
         return __builtin_bit_cast(bf16x8, __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7));
     };
-    auto y_frag = [&](const uint8_t* buf, int pl, int f, int h) { return tr8(buf + (fresh(ya) ^ f << 5) + (pl * YPL + 32 * h * YROW), 16 * YROW); };
-    auto x_frag = [&](const uint8_t* buf, int f, int h) { return tr8(buf + (fresh(xa) ^ ((f & 3) << 3 | (f >> 2) << 7)) + 32 * h * XROW, 16 * XROW); };
-    // One step: GR groups (an x fragment with all y fragments of its 32 rows), x fragments read D groups ahead, y fragments 32 rows
-    // ahead.  The next step's rows that come through registers are stored before group GR - D; those registers are then loaded
-    // for the step after it.  At group GR - D everything of this step is in registers, and what goes straight to LDS has had the
-    // time since the step's start: there the workgroup meets and goes on reading in the next step's buffer.
     f32x4 acc[KF][NF] = {};
-    bf16x8 y[2][NF][NP], x[R];
-    auto read_y = [&](const uint8_t* yb, int h, int o) {
-#pragma unroll
-        for (int f = 0; f < NF; ++f)
-#pragma unroll
-            for (int k = 0; k < NP; ++k) y[o][f][k] = y_frag(yb, k, f, h);
-    };
-    auto products = [&](int i, int o) {
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int f = 0; f < NF; ++f)
-#pragma unroll
-            for (int k = 0; k < NP; ++k)
-                acc[i % KF][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[i % R], y[o][f][k], acc[i % KF][f], 0, 0, 0);
-        __builtin_amdgcn_sched_barrier(0);
-    };
-    // (not __syncthreads: that would also wait for the loads on their way to registers)
-    auto turn = [&]() {
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    bf16x8 y[NF], x[KF];
+    // (not __syncthreads: that would also wait for the loads that are on their way)
+    auto meet = [&]() {
+        asm volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
-    auto landed = [&]() { if constexpr (DMA) asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); };
-    const int64_t mlast = mb + (int64_t)(steps - 1) * MS;                // (behind the last step it is loaded again, unused)
-    // behind a load that goes straight to LDS: rows past the end, made zero where this thread has just put them
-    auto y_cut = [&](uint8_t* buf, int64_t m0) {
-        if constexpr (DMA) {
-            if (m0 + MS > me) {
+    // one step: term PL of step t; ry, rx its places in the rings.  No branches inside: the compiler would move products past them.
+    auto step = [&](auto PL, int t, int ry, int rx) {
+        constexpr int P3 = (PL.value + 3) % NP;
+        constexpr int AHEAD = (PL.value + 3) / NP;                       // row steps that term lies ahead
+        load(Int<P3>(), t + 3, (ry + 3) & 3, (rx + AHEAD) & 3);
 #pragma unroll
-                for (int i = 0; i < YP; ++i)
-                    if (m0 + (i * NT + tid) / (TN / 8) >= me) *(i32x4*)(buf + (i * NT + tid) * 16) = i32x4{0, 0, 0, 0};
-            }
+        for (int f = 0; f < NF; ++f) y[f] = tr8(ys + ry * YB + (fresh(ya) ^ f << 5), 16 * YROW);
+        if constexpr (PL.value == 0) {
+#pragma unroll
+            for (int f = 0; f < KF; ++f) x[f] = tr8(xs + rx * XB + (fresh(xa) ^ f << 5), 16 * XROW);
         }
-    };
-    // (CHECK: the next step may be cut off.  In the others no branches: the compiler would move products past them.)
-    auto step = [&](auto CHECK, auto ODD, uint8_t* yc, uint8_t* xc, uint8_t* yn, uint8_t* xn, int64_t m) {
-        constexpr int H = MS / 32;
-        const int64_t m1 = min(m + MS, mlast), m2 = min(m + 2 * MS, mlast);
-        y_dma(yn, m1);
+        // the next step's loads have come: those of the two behind it are newer
+        constexpr int NEWER = YP * 2 + XP * (((PL.value + 2) % NP == 0) + (P3 == 0));
+        if constexpr (NEWER == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+        else if constexpr (NEWER == 6) asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
+        else { static_assert(NEWER == 4, ""); asm volatile("s_waitcnt vmcnt(4)" ::: "memory"); }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        meet();
 #pragma unroll
-        for (int i = 0; i < GR; ++i) {
-            const int h = i / KF, o = (h + (H & 1) * ODD.value) & 1;
-            constexpr int S = GR - D - 1;                                // the last group before the meeting
-            if (i + D < GR) x[(i + D) % R] = x_frag(xc, (i + D) % KF, (i + D) / KF);
+        for (int i = 0; i < KF; ++i)
 #pragma unroll
-            for (int e = 0; e < XP; ++e) if (i == S - 2 * (XP - 1 - e)) x_store(xn, m1, e);
-            if (i == S) {
-                y_store(yn, m1);
-                landed();
-                if constexpr (CHECK.value) y_cut(yn, m1);
-                x_load(m2);
-                y_load(m2);
-            }
-            if (i == GR - D) {
-                turn();
-                read_y(yn, 0, o ^ 1);
-            }
-            if (i + D >= GR) x[(i + D) % R] = x_frag(xn, i + D - GR, 0);
-            if (i % KF == KF - 4 && h + 1 < H) read_y(yc, h + 1, o ^ 1);
-            products(i, o);
-        }
+            for (int f = 0; f < NF; ++f) acc[i][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[i], y[f], acc[i][f], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (TURNS) meet();
     };
 
-    x_load(mb);
-    y_load(mb);
-    y_dma(y0, mb);
-    y_store(y0, mb);
-#pragma unroll
-    for (int e = 0; e < XP; ++e) x_store(x0, mb, e);
-    landed();
-    y_cut(y0, mb);
-    x_load(min(mb + MS, mlast));
-    y_load(min(mb + MS, mlast));
-    turn();
-    read_y(y0, 0, 0);
-#pragma unroll
-    for (int e = 0; e < D; ++e) x[e] = x_frag(x0, e, 0);
-    int64_t m = mb;
-    int s = 0;
-    for (; s + 3 < steps; s += 2, m += 2 * MS) {
-        step(Flag<false>(), Flag<false>(), y0, x0, y1, x1, m);
-        step(Flag<false>(), Flag<true>(), y1, x1, y0, x0, m + MS);
+    load(Int<0>(), 0, 0, 0);
+    load(Int<1 % NP>(), 1, 1, 1 / NP);
+    load(Int<2 % NP>(), 2, 2, 2 / NP);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    meet();
+    if (TURNS && wave >= NW / 2) meet();
+    for (int t = 0, r = 0; t < steps; t += NP, ++r) {
+        step(Int<0>(), t, t & 3, r & 3);
+        if constexpr (NP > 1) step(Int<1>(), t + 1, (t + 1) & 3, r & 3);
+        if constexpr (NP > 2) step(Int<2>(), t + 2, (t + 2) & 3, r & 3);
     }
-    step(Flag<true>(), Flag<false>(), y0, x0, y1, x1, m);
-    if (s + 1 < steps) step(Flag<true>(), Flag<true>(), y1, x1, y0, x0, m + MS);
-    if (s + 2 < steps) step(Flag<true>(), Flag<false>(), y0, x0, y1, x1, m + 2 * MS);
+    if (TURNS && wave < NW / 2) meet();
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
-    const int kw = k0 + wk * KF * 16 + 16 * g, nw = n0 + wn * NF * 16 + r16;
+    const int kw = k0 + wk * KF * 16 + 4 * g, nw = n0 + wn * NF * 16 + r16;
 #pragma unroll
-    for (int h = 0; h < KF / 4; ++h) {
-        const int k = kw + 64 * h;
-        float ch[16];
+    for (int i = 0; i < KF; ++i) {
+        const int k = kw + 16 * i;
+        float ch[4];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) ch[e] = q.chan && k + e < q.K && q.split == 1 ? q.chan[k + e] : 1.f;
+        for (int e = 0; e < 4; ++e) ch[e] = q.chan && k + e < q.K && q.split == 1 ? q.chan[k + e] : 1.f;
 #pragma unroll
         for (int f = 0; f < NF; ++f) {
             const int n = nw + 16 * f;
-            float v[16];
+            float v[4];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) v[e] = acc[4 * h + e / 4][f][e % 4] * ch[e];
+            for (int e = 0; e < 4; ++e) v[e] = acc[i][f][e] * ch[e];
             if (n < q.N && k < q.K) {
-                if (q.split > 1) {
-                    float* d = q.part + ((int64_t)part * q.N + n) * q.K + k;
-                    wg8_store16(d, q.K - k, v);
-                } else {
+                if (q.split > 1) wg8_store4(q.part + ((int64_t)part * q.N + n) * q.K + k, q.K - k, v);
+                else {
                     const int64_t at = (int64_t)n * q.ldw + k;
-                    if (q.dwtype == IFL_T_F32) wg8_store16((float*)q.dw + at, q.K - k, v);
-                    else if (q.dwtype == IFL_T_BF16) wg8_store16((__bf16*)q.dw + at, q.K - k, v);
-                    else wg8_store16((_Float16*)q.dw + at, q.K - k, v);
+                    if (q.dwtype == IFL_T_F32) wg8_store4((float*)q.dw + at, q.K - k, v);
+                    else if (q.dwtype == IFL_T_BF16) wg8_store4((__bf16*)q.dw + at, q.K - k, v);
+                    else wg8_store4((_Float16*)q.dw + at, q.K - k, v);
                 }
             }
         }
     }
 }
 
-// dw = chan * sum of the parts, in order: four parts' values are on their way at a time
-template <class TW, int V>
+// ------------------------------------------------------------------------------------------------ last launch
+// Workgroups 0 .. join_blocks - 1: dw = chan * sum of the parts, in order, four parts' values on their way at a time, V values a thread.
+// The others: db, 16 columns each, 16 threads of a column every 16th part, joined in LDS in a fixed order.
+template <class TW, class TB, int V>
 __global__ __launch_bounds__(256)
-void wgrad8_join_kernel(WG8 q)
+void wgrad8_finish_kernel(WG8 q, int join_blocks)
 {
-    typedef float FV __attribute__((ext_vector_type(V)));
-    const int64_t nk = (int64_t)q.N * q.K;
-    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V; i < nk; i += (int64_t)gridDim.x * 256 * V) {
-        FV t = 0.f;
-        int s = 0;
-        for (; s + 4 <= q.split; s += 4) {
-            FV u[4];
+    if ((int)blockIdx.x < join_blocks) {
+        typedef float FV __attribute__((ext_vector_type(V)));
+        const int64_t nk = (int64_t)q.N * q.K;
+        for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V; i < nk; i += (int64_t)join_blocks * 256 * V) {
+            FV t = 0.f;
+            int s = 0;
+            for (; s + 4 <= q.split; s += 4) {
+                FV u[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) u[e] = *(const FV*)(q.part + (s + e) * nk + i);
+                for (int e = 0; e < 4; ++e) u[e] = *(const FV*)(q.part + (s + e) * nk + i);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) t += u[e];
+                for (int e = 0; e < 4; ++e) t += u[e];
+            }
+            for (; s < q.split; ++s) t += *(const FV*)(q.part + s * nk + i);
+            const int n = (int)(i / q.K), k = (int)(i - (int64_t)n * q.K);
+            TW* d = (TW*)q.dw + (int64_t)n * q.ldw + k;
+#pragma unroll
+            for (int e = 0; e < V; ++e) d[e] = (TW)(q.chan ? t[e] * q.chan[k + e] : t[e]);
         }
-        for (; s < q.split; ++s) t += *(const FV*)(q.part + s * nk + i);
-        const int n = (int)(i / q.K), k = (int)(i - (int64_t)n * q.K);
-        TW* d = (TW*)q.dw + (int64_t)n * q.ldw + k;
+        return;
+    }
+    __shared__ float red[16][17];
+    const int c = threadIdx.x & 15, r = threadIdx.x >> 4, n = ((int)blockIdx.x - join_blocks) * 16 + c;
+    float t = 0.f;
+    if (n < q.N) {
+#pragma unroll 4
+        for (int s = r; s < q.cs_parts; s += 16) t += q.cs[(int64_t)s * q.N + n];
+    }
+    red[r][c] = t;
+    __syncthreads();
+    if (r == 0 && n < q.N) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) d[e] = (TW)(q.chan ? t[e] * q.chan[k + e] : t[e]);
+        for (int i = 1; i < 16; ++i) t += red[i][c];
+        ((TB*)q.db)[n] = (TB)t;
     }
 }
 
@@ -338,68 +353,38 @@ __global__ void fill_zero_kernel(TW* p, int64_t ld, int rows, int cols)
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < (int64_t)rows * cols; i += (int64_t)gridDim.x * blockDim.x) p[i / cols * ld + i % cols] = (TW)0.f;
 }
 
-// Column sums, first pass: a workgroup takes 64 columns of a range of rows, its four waves every fourth row.  part[blk][N]
-template <class T>
-__global__ __launch_bounds__(256)
-void colsum_kernel(const T* __restrict__ dy, int64_t ldy, float* __restrict__ part, int64_t M, int N, int64_t rows_per)
+// Tiles of 256 x 256 for large layers, else 128 x 128.  The rows are split until about 256 workgroups are at work, each with four
+// steps at least.
+struct WPlan { int tile, split, steps, cs_parts; int64_t cs_rows, kp, np, x_floats, y_floats, part_floats, cs_floats; bool in_place; };
+WPlan wg8_plan(int64_t M, int64_t N, int64_t K, int dytype, bool aligned)
 {
-    __shared__ float red[4][64];
-    const int c = threadIdx.x & 63, r = threadIdx.x >> 6, n = blockIdx.x * 64 + c;
-    const int64_t end = min(M, (int64_t)(blockIdx.y + 1) * rows_per);
-    float t = 0.f;
-    if (n < N) {
-#pragma unroll 8
-        for (int64_t m = (int64_t)blockIdx.y * rows_per + r; m < end; m += 4) t += (float)dy[m * ldy + n];
-    }
-    red[r][c] = t;
-    __syncthreads();
-    if (r == 0 && n < N) part[(int64_t)blockIdx.y * N + n] = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
-}
-// second pass: a workgroup takes 16 columns, 16 threads of each every 16th part, joined in LDS in a fixed order
-template <class TW>
-__global__ __launch_bounds__(256)
-void colsum_join_kernel(const float* __restrict__ part, TW* __restrict__ db, int N, int parts)
-{
-    __shared__ float red[16][17];
-    const int c = threadIdx.x & 15, r = threadIdx.x >> 4, n = blockIdx.x * 16 + c;
-    float t = 0.f;
-    if (n < N) {
-#pragma unroll 4
-        for (int s = r; s < parts; s += 16) t += part[(int64_t)s * N + n];
-    }
-    red[r][c] = t;
-    __syncthreads();
-    if (r == 0 && n < N) {
-#pragma unroll
-        for (int i = 1; i < 16; ++i) t += red[i][c];
-        db[n] = (TW)t;
-    }
-}
-
-// bf16 gradients: tiles of 256 x 256 for large layers if they can go straight to LDS, else 128 x 128; gradients of two or three terms,
-// which take that much more LDS: 128 x 256.  The rows are split until about 256 workgroups are at work, each with two steps at
-// least.
-struct WPlan { int tn, tk, ms, split, steps, cs_parts; int64_t cs_rows; };
-WPlan wg8_plan(int64_t M, int64_t N, int64_t K, int dytype, bool dma)
-{
-    WPlan p = {128, 128, 64, 1, 0, 1, 0};
-    auto tiles = [&](int64_t a, int64_t b) { return ((N + a - 1) / a) * ((K + b - 1) / b); };
-    if (dytype != IFL_T_BF16) { p.tk = 256; p.ms = 32; }
-    else if (dma && tiles(256, 256) >= 32) p.tn = p.tk = 256;
-    const int64_t steps = (M + p.ms - 1) / p.ms, n = tiles(p.tn, p.tk);
+    WPlan p = {};
+    auto tiles = [&](int64_t t) { return ((N + t - 1) / t) * ((K + t - 1) / t); };
+    const int terms = dytype == IFL_T_F32 ? 3 : dytype == IFL_T_F16 ? 2 : 1;
+    p.tile = tiles(256) >= 32 ? 256 : 128;
+    const int64_t steps = (M + MS - 1) / MS, n = K > 0 ? tiles(p.tile) : 1;
     int64_t s = n >= 192 ? 1 : 256 / n;
-    if (s > steps / 2) s = steps / 2;
+    if (s > steps * terms / 4) s = steps * terms / 4;
     if (s > 64) s = 64;
     if (s < 1) s = 1;
     p.steps = (int)((steps + s - 1) / s);
-    p.split = p.steps ? (int)((steps + p.steps - 1) / p.steps) : 1;
-    const int64_t cols = (N + 63) / 64;
-    int64_t c = 512 / cols;
-    if (c > M / 32) c = M / 32;
-    if (c > 256) c = 256;
+    p.split = (int)((steps + p.steps - 1) / p.steps);
+    // column sums (and terms): about 1024 workgroups of 256 columns, 32 rows each at least
+    const int64_t cols = (N + 255) / 256;
+    int64_t c = 1024 / cols;
+    if (c > steps) c = steps;
+    if (c > 512) c = 512;
     if (c < 1) c = 1;
-    p.cs_rows = (M + c - 1) / c;
-    p.cs_parts = p.cs_rows ? (int)((M + p.cs_rows - 1) / p.cs_rows) : 1;
+    p.cs_rows = (steps + c - 1) / c * MS;
+    p.cs_parts = (int)((steps * MS + p.cs_rows - 1) / p.cs_rows);
+    p.in_place = dytype == IFL_T_BF16 && aligned;
+    p.kp = (K + 7) / 8 * 8;
+    p.np = (N + 7) / 8 * 8;
+    auto up = [](int64_t floats) { return (floats + 3) / 4 * 4; };
+    p.x_floats = K > 0 ? up(steps * MS * p.kp / 2) : 0;
+    p.y_floats = K > 0 ? up((p.in_place ? MS : terms * steps * MS) * p.np / 2) : 0;
+    p.part_floats = K > 0 && p.split > 1 ? up(p.split * N * K) : 0;
+    p.cs_floats = up(p.cs_parts * N);
     return p;
 }
 
@@ -407,10 +392,9 @@ WPlan wg8_plan(int64_t M, int64_t N, int64_t K, int dytype, bool dma)
 
 extern "C" int64_t ifl_block8_wgrad_scratch_floats(int64_t M, int64_t N, int64_t K, int dytype)
 {
-    if (M < 1 || N < 1 || K < 0) return 0;
-    const WPlan p = wg8_plan(M, N, K > 0 ? K : 1, dytype, false), d = wg8_plan(M, N, K > 0 ? K : 1, dytype, true);
-    const int64_t s = p.split > d.split ? p.split : d.split;
-    return (K > 0 && s > 1 ? s * N * K : 0) + (int64_t)p.cs_parts * N;
+    if (M < 1 || N < 1 || K < 0 || !b8_type_ok(dytype)) return 0;
+    const WPlan p = wg8_plan(M, N, K, dytype, false);
+    return p.x_floats + p.y_floats + p.part_floats + p.cs_floats;
 }
 
 extern "C" int ifl_block8_wgrad(const void* dy, int dytype, int64_t ldy, const uint8_t* codes, int64_t ldc, const uint8_t* scales,
@@ -419,52 +403,79 @@ extern "C" int ifl_block8_wgrad(const void* dy, int dytype, int64_t ldy, const u
 {
     IFL_CHECK_ARG(b8_fmt_ok(fmt) && b8_type_ok(dytype) && (!dw || b8_type_ok(dwtype)) && (!db || b8_type_ok(dbtype)), IFL_EINVAL, "block8_wgrad: types");
     IFL_CHECK_ARG(M >= 0 && N >= 1 && (K >= 1 || !dw), IFL_EINVAL, "block8_wgrad: %lld x %lld x %lld", (long long)M, (long long)N, (long long)K);
-    IFL_CHECK_ARG(N <= 0x3fffff && K <= 0x3fffff && M < ((int64_t)1 << 40), IFL_ENOTSUP, "block8_wgrad: %lld x %lld x %lld", (long long)M, (long long)N, (long long)K);
+    IFL_CHECK_ARG(N <= 0x3fffff && K <= 0x3fffff && M < ((int64_t)1 << 36), IFL_ENOTSUP, "block8_wgrad: %lld x %lld x %lld", (long long)M, (long long)N, (long long)K);
     IFL_CHECK_ARG((dw || db) && (M == 0 || (dy && scratch)) && (M == 0 || !dw || (codes && scales)), IFL_EINVAL, "block8_wgrad: null pointer");
     IFL_CHECK_ARG((M <= 1 || ldy >= N) && (!dw || ((M <= 1 || (ldc >= K && lds >= ifl_cdiv((int)K, B8_BLK))) && ldw >= K)), IFL_EINVAL, "block8_wgrad: row strides");
     IFL_CHECK_ARG(!dw || M == 0 || ((uintptr_t)codes % 16 == 0 && (M == 1 || ldc % 16 == 0)), IFL_EINVAL, "block8_wgrad: codes in rows of whole, aligned 16 bytes");
-    IFL_CHECK_ARG(ldy < (1 << 23) && ldc < (1 << 23) && lds < (1 << 23), IFL_ENOTSUP, "block8_wgrad: rows of %lld gradients, %lld codes", (long long)ldy, (long long)ldc);
+    IFL_CHECK_ARG(M == 0 || (uintptr_t)scratch % 16 == 0, IFL_EINVAL, "block8_wgrad: scratch");
+    IFL_CHECK_ARG(ldy < (1 << 23), IFL_ENOTSUP, "block8_wgrad: rows of %lld gradients", (long long)ldy);
     hipStream_t st = (hipStream_t)stream;
     if (M == 0) {
         if (dw) { B8_DISPATCH(dwtype, hipLaunchKernelGGL(HIP_KERNEL_NAME(fill_zero_kernel<T>), dim3(256), dim3(256), 0, st, (T*)dw, ldw, (int)N, (int)K)); IFL_LAUNCH_CHECK(); }
         if (db) { B8_DISPATCH(dbtype, hipLaunchKernelGGL(HIP_KERNEL_NAME(fill_zero_kernel<T>), dim3(16), dim3(256), 0, st, (T*)db, N, 1, (int)N)); IFL_LAUNCH_CHECK(); }
         return 0;
     }
-    const bool ywide = (uintptr_t)dy % 16 == 0 && (M == 1 || ldy * b8_size(dytype) % 16 == 0) && N % 8 == 0;
-    const bool dma = dytype == IFL_T_BF16 && ywide;
-    const WPlan p = wg8_plan(M, N, K > 0 ? K : 1, dytype, dma);
+    const int es = b8_size(dytype);
+    const bool wide = (uintptr_t)dy % 16 == 0 && (M == 1 || ldy * es % 16 == 0);
+    const WPlan p = wg8_plan(M, N, dw ? K : 0, dytype, wide && N % 8 == 0);
+    WG8 q = {};
+    q.dy = dy; q.ldy = ldy; q.codes = codes; q.ldc = ldc; q.scales = scales; q.lds = lds; q.chan = chan; q.dw = dw; q.ldw = ldw;
+    q.dwtype = dwtype; q.db = db; q.dbtype = dbtype; q.M = M; q.N = (int)N; q.K = (int)K; q.fmt = fmt; q.want_x = dw != nullptr;
+    q.kp = p.kp; q.np = p.np; q.yplane = (M + MS - 1) / MS * MS * p.np; q.in_place = p.in_place;
+    q.xb = (uint16_t*)scratch;
+    q.yb = (uint16_t*)(scratch + p.x_floats);
+    q.part = scratch + p.x_floats + p.y_floats;
+    q.cs = q.part + p.part_floats;
+    q.split = p.split; q.steps = p.steps; q.cs_parts = p.cs_parts; q.cs_rows = p.cs_rows;
+
+    const int64_t mp = (M + MS - 1) / MS * MS;
     if (dw) {
-        WG8 q = {};
-        q.dy = dy; q.ldy = ldy; q.codes = codes; q.ldc = ldc; q.scales = scales; q.lds = lds; q.chan = chan; q.dw = dw; q.ldw = ldw;
-        q.dwtype = dwtype; q.part = scratch; q.split = p.split; q.steps = p.steps; q.M = M; q.N = (int)N; q.K = (int)K;
-        q.tiles_n = (int)((N + p.tn - 1) / p.tn); q.tiles_k = (int)((K + p.tk - 1) / p.tk);
-        q.per_xcd = (q.tiles_n * q.tiles_k * p.split + 7) / 8;
-        q.ywide = ywide;
-        const dim3 grid(8 * q.per_xcd);
-#define WG8_K(T, NP, TN, TK, WN, WK, MS, F, D) hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_kernel<T, NP, TN, TK, WN, WK, MS, F, D>), grid, dim3(64 * WN * WK), 0, st, q)
-#define WG8_F(F) do { \
-            if (dytype == IFL_T_F32) WG8_K(float, 3, 128, 256, 2, 4, 32, F, false); \
-            else if (dytype == IFL_T_F16) WG8_K(_Float16, 2, 128, 256, 2, 4, 32, F, false); \
-            else if (p.tn == 256) WG8_K(__bf16, 1, 256, 256, 4, 2, 64, F, true); \
-            else { if (dma) WG8_K(__bf16, 1, 128, 128, 2, 2, 64, F, true); else WG8_K(__bf16, 1, 128, 128, 2, 2, 64, F, false); } } while (0)
-        if (fmt == IFL_Q_E4M3) WG8_F(0); else WG8_F(1);
-        IFL_LAUNCH_CHECK();
-        if (p.split > 1) {
-            // four values per thread where the parts are large, else one: the parts' loads are what it waits for
-            const bool v4 = K % 4 == 0 && N * K >= 1 << 18;
-            const int64_t jobs = (v4 ? N * K / 4 : N * K) / 256 + 1;
-            const unsigned jg = (unsigned)(jobs < 4096 ? jobs : 4096);
-            B8_DISPATCH(dwtype, if (v4) hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_join_kernel<T, 4>), dim3(jg), dim3(256), 0, st, q);
-                        else hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_join_kernel<T, 1>), dim3(jg), dim3(256), 0, st, q));
-            IFL_LAUNCH_CHECK();
-        }
+        while (q.x_tpr_log < 8 && (8 << q.x_tpr_log) < p.kp) ++q.x_tpr_log;
+        const int64_t rows = (mp + (256 >> q.x_tpr_log) - 1) / (256 >> q.x_tpr_log);   // in turns of one workgroup
+        const int64_t four = (rows + 3) / 4;
+        q.x_blocks = (int)(four >= 16384 ? 16384 : four >= 512 ? four : rows < 512 ? rows : 512);
     }
-    if (db) {
-        float* part = scratch + (dw && p.split > 1 ? (int64_t)p.split * N * K : 0);
-        const unsigned cols = (unsigned)((N + 63) / 64);
-        B8_DISPATCH(dytype, hipLaunchKernelGGL(HIP_KERNEL_NAME(colsum_kernel<T>), dim3(cols, p.cs_parts), dim3(256), 0, st, (const T*)dy, ldy, part, M, (int)N, p.cs_rows));
+    q.y_cols = (int)((N + 255) / 256);
+    // of gradients that are read in place and whose sums nobody wants only the last rows are looked at, if they do not fill a step
+    int64_t y_blocks = (int64_t)p.cs_parts * q.y_cols;
+    if (p.in_place && !db) {
+        q.y_row0 = M / MS * MS;
+        q.cs_rows = MS;
+        y_blocks = M % MS ? q.y_cols : 0;
+    }
+    const dim3 pg((unsigned)(q.x_blocks + y_blocks));
+#define WG8_P(T, NP) do { \
+        if (wide) hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_prepare_kernel<T, NP, true>), pg, dim3(256), 0, st, q); \
+        else hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_prepare_kernel<T, NP, false>), pg, dim3(256), 0, st, q); \
+    } while (0)
+    if (dytype == IFL_T_F32) WG8_P(float, 3); else if (dytype == IFL_T_F16) WG8_P(_Float16, 2); else WG8_P(__bf16, 1);
+    IFL_LAUNCH_CHECK();
+    if (dw) {
+        q.tiles_n = (int)((N + p.tile - 1) / p.tile);
+        q.tiles_k = (int)((K + p.tile - 1) / p.tile);
+        q.per_xcd = (q.tiles_n * q.tiles_k * p.split + 7) / 8;
+        const dim3 grid(8 * q.per_xcd);
+#define WG8_K(NP) do { \
+        if (p.tile == 256) hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_kernel<NP, 256, 256, 4, 2>), grid, dim3(512), 0, st, q); \
+        else hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_kernel<NP, 128, 128, 2, 2>), grid, dim3(256), 0, st, q); \
+    } while (0)
+        if (dytype == IFL_T_F32) WG8_K(3); else if (dytype == IFL_T_F16) WG8_K(2); else WG8_K(1);
         IFL_LAUNCH_CHECK();
-        B8_DISPATCH(dbtype, hipLaunchKernelGGL(HIP_KERNEL_NAME(colsum_join_kernel<T>), dim3((unsigned)((N + 15) / 16)), dim3(256), 0, st, part, (T*)db, (int)N, p.cs_parts));
+    }
+    int64_t jobs = 0;
+    const bool v4 = K % 4 == 0 && N * K >= 1 << 18;
+    if (dw && p.split > 1) {
+        jobs = (v4 ? N * K / 4 : N * K) / 256 + 1;
+        if (jobs > 4096) jobs = 4096;
+    }
+    if (jobs || db) {
+        const dim3 fg((unsigned)(jobs + (db ? (N + 15) / 16 : 0)));
+#define WG8_E(TW, TB) do { \
+        if (v4) hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_finish_kernel<TW, TB, 4>), fg, dim3(256), 0, st, q, (int)jobs); \
+        else hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_finish_kernel<TW, TB, 1>), fg, dim3(256), 0, st, q, (int)jobs); \
+    } while (0)
+        const int wt = dw ? dwtype : IFL_T_F32, bt = db ? dbtype : wt;
+        B8_DISPATCH(wt, typedef T TW; B8_DISPATCH(bt, WG8_E(TW, T)));
         IFL_LAUNCH_CHECK();
     }
     return 0;
