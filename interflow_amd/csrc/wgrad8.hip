@@ -32,7 +32,7 @@ struct WG8 {
     float* part; int split, steps;       // float32 partial sums [split][N][K], steps of 32 rows per part
     float* cs; int cs_parts; int64_t cs_rows, y_row0;        // partial column sums [cs_parts][N], of cs_rows rows from y_row0 on
     int tiles_n, tiles_k, per_xcd;
-    int x_blocks, x_tpr_log, y_cols;     // first launch: workgroups that restore codes, threads along a row; of 256 columns of dy
+    int x_blocks, x_tpr_log, y_cols, y_tpr_log;      // first launch: workgroups that restore codes, threads along a row; ranges of columns of dy, threads along a row
 };
 
 // One, two or three bf16 terms whose sum is the value, as floats with 16 low zero bits: its leading 8 significant bits, the next 8,
@@ -70,8 +70,8 @@ __device__ __forceinline__ void wg8_store4(TW* d, int left, const float v[4]) {
 constexpr int MS = 32;                                                  // rows per step: the depth of one product
 
 // ------------------------------------------------------------------------------------------------ first launch
-// Workgroups 0 .. x_blocks - 1 restore codes, 8 a thread.  The others take 256 columns (8 a thread) of cs_rows rows of dy: eight
-// threads' rows in turn, column sums on the way, joined in LDS in a fixed order.
+// Workgroups 0 .. x_blocks - 1 restore codes, 8 a thread.  The others take up to 256 columns (8 a thread) of cs_rows rows of dy, with
+// column sums on the way that are joined in LDS in a fixed order.
 template <class T, int NP, bool VEC>
 __global__ __launch_bounds__(256)
 void wgrad8_prepare_kernel(WG8 q)
@@ -101,23 +101,24 @@ void wgrad8_prepare_kernel(WG8 q)
         }
         return;
     }
-    __shared__ float red[8][256 + 8];
+    __shared__ float red[256 * 8 + 256];
     const int b = blockIdx.x - q.x_blocks, part = b / q.y_cols, cb = b - part * q.y_cols;
-    const int c = cb * 256 + (threadIdx.x & 31) * 8, rl = threadIdx.x >> 5;
+    const int tpr = 1 << q.y_tpr_log, rpp = 256 >> q.y_tpr_log, rl = threadIdx.x >> q.y_tpr_log;
+    const int c0 = cb * 8 * tpr, c = c0 + (threadIdx.x & (tpr - 1)) * 8;
     const int64_t first = q.y_row0 + (int64_t)part * q.cs_rows, last = min(mp, first + q.cs_rows);
     const int64_t m32 = q.M / MS * MS;
     const T* dy = (const T*)q.dy;
     float sum[8] = {};
-    for (int64_t r0 = first + rl; r0 < last; r0 += 32) {
+    for (int64_t r0 = first + rl; r0 < last; r0 += 4 * rpp) {
         float v[4][8];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            const int64_t r = r0 + 8 * u;
+            const int64_t r = r0 + u * rpp;
             b8_load8<T, VEC>(dy + (r < q.M ? r : 0) * q.ldy + c, r < q.M && r < last ? q.N - c : 0, v[u]);
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            const int64_t r = r0 + 8 * u;
+            const int64_t r = r0 + u * rpp;
             if (r >= last) break;
 #pragma unroll
             for (int i = 0; i < 8; ++i) sum[i] += v[u][i];
@@ -137,13 +138,15 @@ void wgrad8_prepare_kernel(WG8 q)
         }
     }
     if (!q.db) return;
+    const int pitch = 8 * tpr + 1;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) red[rl][(threadIdx.x & 31) * 8 + i] = sum[i];
+    for (int i = 0; i < 8; ++i) red[rl * pitch + (threadIdx.x & (tpr - 1)) * 8 + i] = sum[i];
     __syncthreads();
-    float t = red[0][threadIdx.x];
-#pragma unroll
-    for (int i = 1; i < 8; ++i) t += red[i][threadIdx.x];
-    if (cb * 256 + (int)threadIdx.x < q.N) q.cs[(int64_t)part * q.N + cb * 256 + threadIdx.x] = t;
+    if ((int)threadIdx.x < 8 * tpr && c0 + (int)threadIdx.x < q.N) {
+        float t = red[threadIdx.x];
+        for (int i = 1; i < rpp; ++i) t += red[i * pitch + threadIdx.x];
+        q.cs[(int64_t)part * q.N + c0 + threadIdx.x] = t;
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ the product
@@ -304,26 +307,43 @@ void wgrad8_kernel(WG8 q)
 }
 
 // ------------------------------------------------------------------------------------------------ last launch
-// Workgroups 0 .. join_blocks - 1: dw = chan * sum of the parts, in order, four parts' values on their way at a time, V values a thread.
-// The others: db, 16 columns each, 16 threads of a column every 16th part, joined in LDS in a fixed order.
-template <class TW, class TB, int V>
+// Workgroups 0 .. join_blocks - 1: dw = chan * sum of the parts, V values a thread, four parts' values on their way at a time.  A small dw
+// has few threads: then 16 of them share a value's parts (ACROSS), each takes every 16th, and the sums meet in LDS.  The
+// others: db, 16 columns each, shared in the same way.  All orders are fixed.
+template <class TW, class TB, int V, bool ACROSS>
 __global__ __launch_bounds__(256)
 void wgrad8_finish_kernel(WG8 q, int join_blocks)
 {
+    typedef float FV __attribute__((ext_vector_type(V)));
+    __shared__ FV red[ACROSS ? 16 * 17 : 1];
+    const int c = threadIdx.x & 15, r = threadIdx.x >> 4;
     if ((int)blockIdx.x < join_blocks) {
-        typedef float FV __attribute__((ext_vector_type(V)));
         const int64_t nk = (int64_t)q.N * q.K;
-        for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V; i < nk; i += (int64_t)join_blocks * 256 * V) {
+        const int first = ACROSS ? r : 0, by = ACROSS ? 16 : 1;
+        const int64_t stride = (int64_t)join_blocks * (ACROSS ? 16 : 256) * V;
+        for (int64_t i0 = (int64_t)blockIdx.x * (ACROSS ? 16 : 256) * V; i0 < nk; i0 += stride) {
+            const int64_t i = i0 + (ACROSS ? c : (int)threadIdx.x) * V;
             FV t = 0.f;
-            int s = 0;
-            for (; s + 4 <= q.split; s += 4) {
-                FV u[4];
+            if (i < nk) {
+                int s = first;
+                for (; s + 3 * by < q.split; s += 4 * by) {
+                    FV u[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) u[e] = *(const FV*)(q.part + (s + e) * nk + i);
+                    for (int e = 0; e < 4; ++e) u[e] = *(const FV*)(q.part + (s + e * by) * nk + i);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) t += u[e];
+                    for (int e = 0; e < 4; ++e) t += u[e];
+                }
+                for (; s < q.split; s += by) t += *(const FV*)(q.part + s * nk + i);
             }
-            for (; s < q.split; ++s) t += *(const FV*)(q.part + s * nk + i);
+            if constexpr (ACROSS) {
+                __syncthreads();
+                red[r * 17 + c] = t;
+                __syncthreads();
+                if (r) continue;
+#pragma unroll
+                for (int e = 1; e < 16; ++e) t += red[e * 17 + c];
+            }
+            if (i >= nk) continue;
             const int n = (int)(i / q.K), k = (int)(i - (int64_t)n * q.K);
             TW* d = (TW*)q.dw + (int64_t)n * q.ldw + k;
 #pragma unroll
@@ -331,18 +351,18 @@ void wgrad8_finish_kernel(WG8 q, int join_blocks)
         }
         return;
     }
-    __shared__ float red[16][17];
-    const int c = threadIdx.x & 15, r = threadIdx.x >> 4, n = ((int)blockIdx.x - join_blocks) * 16 + c;
+    __shared__ float cred[16][17];
+    const int n = ((int)blockIdx.x - join_blocks) * 16 + c;
     float t = 0.f;
     if (n < q.N) {
 #pragma unroll 4
         for (int s = r; s < q.cs_parts; s += 16) t += q.cs[(int64_t)s * q.N + n];
     }
-    red[r][c] = t;
+    cred[r][c] = t;
     __syncthreads();
     if (r == 0 && n < q.N) {
 #pragma unroll
-        for (int i = 1; i < 16; ++i) t += red[i][c];
+        for (int i = 1; i < 16; ++i) t += cred[i][c];
         ((TB*)q.db)[n] = (TB)t;
     }
 }
@@ -353,9 +373,9 @@ __global__ void fill_zero_kernel(TW* p, int64_t ld, int rows, int cols)
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < (int64_t)rows * cols; i += (int64_t)gridDim.x * blockDim.x) p[i / cols * ld + i % cols] = (TW)0.f;
 }
 
-// Tiles of 256 x 256 for large layers, else 128 x 128.  The rows are split until about 256 workgroups are at work, each with four
-// steps at least.
-struct WPlan { int tile, split, steps, cs_parts; int64_t cs_rows, kp, np, x_floats, y_floats, part_floats, cs_floats; bool in_place; };
+// Tiles of 256 x 256 for large layers, else 128 x 128.  The rows are split until the card is full (one workgroup on a CU of the
+// large tiles, two of the small ones), each with four steps at least.
+struct WPlan { int tile, split, steps, cs_parts, y_tpr_log; int64_t cs_rows, kp, np, x_floats, y_floats, part_floats, cs_floats; bool in_place; };
 WPlan wg8_plan(int64_t M, int64_t N, int64_t K, int dytype, bool aligned)
 {
     WPlan p = {};
@@ -363,14 +383,16 @@ WPlan wg8_plan(int64_t M, int64_t N, int64_t K, int dytype, bool aligned)
     const int terms = dytype == IFL_T_F32 ? 3 : dytype == IFL_T_F16 ? 2 : 1;
     p.tile = tiles(256) >= 32 ? 256 : 128;
     const int64_t steps = (M + MS - 1) / MS, n = K > 0 ? tiles(p.tile) : 1;
-    int64_t s = n >= 192 ? 1 : 256 / n;
+    const int64_t full = p.tile == 256 ? 256 : 512;
+    int64_t s = 4 * n >= 3 * full ? 1 : full / n;
     if (s > steps * terms / 4) s = steps * terms / 4;
-    if (s > 64) s = 64;
+    if (s > 256) s = 256;
     if (s < 1) s = 1;
     p.steps = (int)((steps + s - 1) / s);
     p.split = (int)((steps + p.steps - 1) / p.steps);
-    // column sums (and terms): about 1024 workgroups of 256 columns, 32 rows each at least
-    const int64_t cols = (N + 255) / 256;
+    // column sums (and terms): about 1024 workgroups, 32 rows each at least
+    while (p.y_tpr_log < 5 && (8 << p.y_tpr_log) < N) ++p.y_tpr_log;
+    const int64_t cols = (N + (8 << p.y_tpr_log) - 1) / (8 << p.y_tpr_log);
     int64_t c = 1024 / cols;
     if (c > steps) c = steps;
     if (c > 512) c = 512;
@@ -435,7 +457,8 @@ extern "C" int ifl_block8_wgrad(const void* dy, int dytype, int64_t ldy, const u
         const int64_t four = (rows + 3) / 4;
         q.x_blocks = (int)(four >= 16384 ? 16384 : four >= 512 ? four : rows < 512 ? rows : 512);
     }
-    q.y_cols = (int)((N + 255) / 256);
+    q.y_tpr_log = p.y_tpr_log;
+    q.y_cols = (int)((N + (8 << p.y_tpr_log) - 1) / (8 << p.y_tpr_log));
     // of gradients that are read in place and whose sums nobody wants only the last rows are looked at, if they do not fill a step
     int64_t y_blocks = (int64_t)p.cs_parts * q.y_cols;
     if (p.in_place && !db) {
@@ -463,16 +486,17 @@ extern "C" int ifl_block8_wgrad(const void* dy, int dytype, int64_t ldy, const u
         IFL_LAUNCH_CHECK();
     }
     int64_t jobs = 0;
-    const bool v4 = K % 4 == 0 && N * K >= 1 << 18;
+    const bool v4 = K % 4 == 0, across = (v4 ? N * K / 4 : N * K) < 1 << 16;
     if (dw && p.split > 1) {
-        jobs = (v4 ? N * K / 4 : N * K) / 256 + 1;
+        jobs = ((v4 ? N * K / 4 : N * K) + (across ? 15 : 255)) / (across ? 16 : 256);
         if (jobs > 4096) jobs = 4096;
     }
     if (jobs || db) {
         const dim3 fg((unsigned)(jobs + (db ? (N + 15) / 16 : 0)));
+#define WG8_E2(TW, TB, V, A) hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_finish_kernel<TW, TB, V, A>), fg, dim3(256), 0, st, q, (int)jobs)
 #define WG8_E(TW, TB) do { \
-        if (v4) hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_finish_kernel<TW, TB, 4>), fg, dim3(256), 0, st, q, (int)jobs); \
-        else hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_finish_kernel<TW, TB, 1>), fg, dim3(256), 0, st, q, (int)jobs); \
+        if (v4 && across) WG8_E2(TW, TB, 4, true); else if (v4) WG8_E2(TW, TB, 4, false); \
+        else if (across) WG8_E2(TW, TB, 1, true); else WG8_E2(TW, TB, 1, false); \
     } while (0)
         const int wt = dw ? dwtype : IFL_T_F32, bt = db ? dbtype : wt;
         B8_DISPATCH(wt, typedef T TW; B8_DISPATCH(bt, WG8_E(TW, T)));
