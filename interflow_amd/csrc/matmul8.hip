@@ -63,23 +63,54 @@ __device__ __forceinline__ i32x8 mm8_join(i32x4 a, i32x4 b) {
     return r;
 }
 
-// n values of one row of the result from column n on; wide: 16-byte stores fit
-template <class T, int CNT>
-__device__ __forceinline__ void mm8_store(const MM8& q, int64_t m, int64_t n, const float v[CNT], bool wide) {
-    T* p = (T*)q.out + m * q.ldo + n;
-    constexpr int V = 16 / sizeof(T);
-    if (wide && n + CNT <= q.N && CNT % V == 0) {
-        typedef T TV __attribute__((ext_vector_type(V)));
+// A wave's results: m0 the lane's first row, nw its first column, bias its columns' (in LDS).  wide: 16-byte
+// stores fit.
+template <class T, int NF, int MF, int G>
+__device__ __forceinline__ void mm8_results(const MM8& q, const f32x4 (&acc)[NF][MF], int64_t m0, int64_t nw, const float* bias, bool wide) {
+    constexpr int V = 4 * G * sizeof(T) >= 16 ? 16 / sizeof(T) : 4 * G;
+    typedef T TV __attribute__((ext_vector_type(V)));
+    T* p = (T*)q.out + m0 * q.ldo + nw;
+    int rows = (int)(q.M - m0), cols = (int)(q.N - nw);
 #pragma unroll
-        for (int i = 0; i < CNT / V; ++i) {
-            TV t;
+    for (int j = 0; j < MF; ++j) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) t[e] = (T)v[i * V + e];
-            ((TV*)p)[i] = t;
+        for (int h = 0; h < NF / G; ++h) {
+            float v[4 * G];
+#pragma unroll
+            for (int i = 0; i < 4 * G; ++i) v[i] = acc[h * G + i / 4][j][i % 4] + bias[16 * G * h + i];
+            asm volatile("" : "+v"(cols));                               // (compared here: there are no registers for what is made ahead)
+            if (wide && 16 * j < rows && 16 * G * h + 4 * G <= cols) {
+#pragma unroll
+                for (int i = 0; i < 4 * G / V; ++i) {
+                    TV t;
+#pragma unroll
+                    for (int e = 0; e < V; ++e) t[e] = (T)v[i * V + e];
+                    *(TV*)(p + 16 * G * h + V * i) = t;
+                }
+            } else if (16 * j < rows) {
+#pragma unroll
+                for (int i = 0; i < 4 * G; ++i) if (16 * G * h + i < cols) p[16 * G * h + i] = (T)v[i];
+            }
+            __builtin_amdgcn_sched_barrier(0);                           // (one at a time, for the same reason)
         }
-    } else {
+        p += 16 * q.ldo;
+    }
+}
+template <int NF, int MF, int G>
+__device__ __forceinline__ void mm8_part(const MM8& q, const f32x4 (&acc)[NF][MF], int64_t m0, int64_t nw) {
+    float* out = q.part + (int64_t)blockIdx.y * q.M * q.N;
 #pragma unroll
-        for (int i = 0; i < CNT; ++i) if (n + i < q.N) p[i] = (T)v[i];
+    for (int j = 0; j < MF; ++j) {
+        const int64_t m = m0 + 16 * j;
+        if (m < q.M) {
+#pragma unroll
+            for (int i = 0; i < NF; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int64_t n = nw + 16 * G * (i / G) + 4 * (i % G) + e;
+                    if (n < q.N) out[m * q.N + n] = acc[i][j][e];
+                }
+        }
     }
 }
 
@@ -109,7 +140,9 @@ void mm8_tile_kernel(MM8 q)
     __shared__ __attribute__((aligned(16))) uint8_t buf0[(TN + TM) * 128];
     __shared__ __attribute__((aligned(16))) uint8_t buf1[(TN + TM) * 128];
     constexpr int SR = (TN + TM + 64 * NW - 1) / (64 * NW);              // rows of scales per thread
-    __shared__ uint32_t sc[2][SR * 64 * NW];                                  // scale bytes of four steps, per row
+    __shared__ uint32_t sc[2][SR * 64 * NW];                             // scale bytes of four steps, per row
+    __shared__ __attribute__((aligned(16))) float bias[TN];
+    static_assert(TN <= 64 * NW, "");
     const int tiles = q.tiles_m * q.tiles_n;
     const int t = (blockIdx.x & 7) * q.per_xcd + (blockIdx.x >> 3);
     if (t >= tiles) return;
@@ -235,6 +268,7 @@ void mm8_tile_kernel(MM8 q)
 #pragma unroll
         for (int i = 0; i < SR; ++i) sc[grp & 1][i * 64 * NW + threadIdx.x] = snext[i];
     };
+    if (!SPLIT && (int)threadIdx.x < TN) bias[threadIdx.x] = n0 + threadIdx.x < q.N ? mm8_bias(q, n0 + threadIdx.x) : 0.f;      // (the workgroup meets before it is read)
     ask(k_first >> 2);                                                   // (k_first is a multiple of 4)
     put(k_first >> 2);
     int ks = k_first;
@@ -268,43 +302,14 @@ void mm8_tile_kernel(MM8 q)
     }
     __builtin_amdgcn_s_waitcnt(0x0f70);
 
-    const int64_t nw = n0 + wn * NF * 16 + 4 * G * g;
-    if constexpr (SPLIT) {
-        float* out = q.part + (int64_t)blockIdx.y * q.M * q.N;
-#pragma unroll
-        for (int j = 0; j < MF; ++j) {
-            const int64_t m = m0 + wm * MF * 16 + 16 * j + r16;
-            if (m < q.M) {
-#pragma unroll
-                for (int i = 0; i < NF; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int64_t n = nw + 16 * G * (i / G) + 4 * (i % G) + e;
-                        if (n < q.N) out[m * q.N + n] = acc[i][j][e];
-                    }
-            }
-        }
-    } else {
-        const int es = q.otype == IFL_T_F32 ? 4 : 2;
-        const bool wide = ((uintptr_t)q.out | (uint64_t)(q.ldo * es)) % 16 == 0;
-#pragma unroll
-        for (int h = 0; h < NF / G; ++h) {
-            float bias[4 * G];
-#pragma unroll
-            for (int i = 0; i < 4 * G; ++i) bias[i] = nw + 16 * G * h + i < q.N ? mm8_bias(q, nw + 16 * G * h + i) : 0.f;
-#pragma unroll
-            for (int j = 0; j < MF; ++j) {
-                const int64_t m = m0 + wm * MF * 16 + 16 * j + r16;
-                float v[4 * G];
-#pragma unroll
-                for (int i = 0; i < 4 * G; ++i) v[i] = acc[h * G + i / 4][j][i % 4] + bias[i];
-                if (m < q.M) {
-                    if constexpr (EXACT) mm8_store<float, 4 * G>(q, m, nw + 16 * G * h, v, wide);
-                    else if (q.otype == IFL_T_BF16) mm8_store<__bf16, 4 * G>(q, m, nw + 16 * G * h, v, wide);
-                    else mm8_store<_Float16, 4 * G>(q, m, nw + 16 * G * h, v, wide);
-                }
-            }
-        }
+    const int64_t mw = m0 + wm * MF * 16 + r16, nw = n0 + wn * NF * 16 + 4 * G * g;
+    if constexpr (SPLIT) mm8_part<NF, MF, G>(q, acc, mw, nw);
+    else {
+        const float* bs = bias + wn * NF * 16 + 4 * G * g;
+        const bool wide = ((uintptr_t)q.out | (uint64_t)(q.ldo * (EXACT ? 4 : 2))) % 16 == 0;
+        if constexpr (EXACT) mm8_results<float, NF, MF, G>(q, acc, mw, nw, bs, wide);
+        else if (q.otype == IFL_T_BF16) mm8_results<__bf16, NF, MF, G>(q, acc, mw, nw, bs, wide);
+        else mm8_results<_Float16, NF, MF, G>(q, acc, mw, nw, bs, wide);
     }
 }
 
