@@ -66,24 +66,33 @@ __device__ __forceinline__ void b8_store8(T* __restrict__ p, int left, const flo
 
 __device__ __forceinline__ bool b8_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
-// largest finite magnitude of 8 values, as its bits (magnitudes order as unsigned integers)
+// Largest magnitude of 8 values, as its bits (magnitudes order as unsigned integers; what is not finite is B8_INF or more), and
+// the largest finite one.
+constexpr uint32_t B8_INF = 0x7f800000u;
+__device__ __forceinline__ uint32_t b8_max_bits(const float v[8]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+    return m;
+}
 __device__ __forceinline__ uint32_t b8_amax_bits(const float v[8]) {
     uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const uint32_t u = __float_as_uint(v[i]) & 0x7fffffffu;
-        m = max(m, u < 0x7f800000u ? u : 0u);
+        m = max(m, u < B8_INF ? u : 0u);
     }
     return m;
 }
 
-// maximum over groups of LANES neighbouring lanes (4, 8 or 16), in every lane: exchanges inside a row of 16 by DPP
+// maximum over groups of LANES neighbouring lanes (4, 8 or 16; `lanes` where that is not known before), in every lane: exchanges
+// inside a row of 16 by DPP
 template <int LANES>
-__device__ __forceinline__ uint32_t b8_group_max(uint32_t m) {
+__device__ __forceinline__ uint32_t b8_group_max(uint32_t m, int lanes = LANES) {
     m = max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0xB1, 0xf, 0xf, true));                        // lane ^ 1
     m = max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0x4E, 0xf, 0xf, true));                        // lane ^ 2
-    if (LANES >= 8) m = max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0x141, 0xf, 0xf, true));       // mirror within 8
-    if (LANES >= 16) m = max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0x140, 0xf, 0xf, true));      // mirror within 16
+    if (lanes >= 8) m = max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0x141, 0xf, 0xf, true));       // mirror within 8
+    if (lanes >= 16) m = max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0x140, 0xf, 0xf, true));      // mirror within 16
     return m;
 }
 
@@ -99,8 +108,8 @@ __device__ __forceinline__ float b8_scale(int byte) {
     return __uint_as_float(byte == 0 ? 0x00400000u : byte == 255 ? 0x7fc00000u : (uint32_t)byte << 23);
 }
 
-// codes of 8 values already multiplied by 2^-e
-__device__ __forceinline__ i32x2 b8_encode8(const float v[8], int fmt) {
+// codes of 8 values already multiplied by 2^-e; odd: some of them may not be finite
+__device__ __forceinline__ i32x2 b8_encode8(const float v[8], int fmt, bool odd) {
     i32x2 r = {0, 0};
     if (fmt == IFL_Q_E4M3) {
 #pragma unroll
@@ -115,9 +124,6 @@ __device__ __forceinline__ i32x2 b8_encode8(const float v[8], int fmt) {
             r[h] = __builtin_amdgcn_cvt_pk_bf8_f32(v[4 * h + 2], v[4 * h + 3], r[h], true);
         }
     }
-    bool odd = false;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) odd |= !b8_finite(v[i]);
     if (odd) {                                      // (what the conversion makes of infinities depends on a mode bit: set here)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -129,6 +135,22 @@ __device__ __forceinline__ i32x2 b8_encode8(const float v[8], int fmt) {
         }
     }
     return r;
+}
+
+// A block's scale byte and the codes of this lane's 8 values of it (LANES neighbouring lanes have the block).  What is not finite is
+// looked at only where the block's maximum says that there is some (16384 x 2048 bf16: 25.0 us; looked at
+// in every value 26.9).
+template <int LANES>
+__device__ __forceinline__ i32x2 b8_quantize8(const float x[8], int fmt, int& sb, int lanes = LANES) {
+    uint32_t m = b8_group_max<LANES>(b8_max_bits(x), lanes);
+    const bool odd = m >= B8_INF;
+    if (odd) m = b8_group_max<LANES>(b8_amax_bits(x), lanes);                   // (all lanes of a block come here, or none)
+    sb = b8_scale_byte(m, fmt);
+    const float inv = b8_inv_scale(sb);
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = x[i] * inv;
+    return b8_encode8(v, fmt, odd);
 }
 
 __device__ __forceinline__ void b8_decode4(int w, int fmt, float* v) {
@@ -177,3 +199,10 @@ __device__ __forceinline__ bf16x8 b8_bf16x8(int w0, int w1, int byte) {
 
 static inline bool b8_type_ok(int t) { return t == IFL_T_F32 || t == IFL_T_BF16 || t == IFL_T_F16; }
 static inline bool b8_fmt_ok(int f) { return f == IFL_Q_E4M3 || f == IFL_Q_E5M2; }
+
+// ifl_block8_wgrad in two steps for the layer whose other product needs dy in 8-bit blocks: 1 prepares (and quantizes dy, if told
+// where to), 2 multiplies and joins, 3 both.
+struct B8Quant { uint8_t *codes, *scales; int64_t ldc, lds; int fmt; };
+int b8_wgrad(int steps, const B8Quant* quant, const void* dy, int dytype, int64_t ldy, const uint8_t* codes, int64_t ldc, const uint8_t* scales,
+             int64_t lds, int fmt, const float* chan, void* dw, int dwtype, int64_t ldw, void* db, int dbtype, float* scratch, int64_t M,
+             int64_t N, int64_t K, void* stream);

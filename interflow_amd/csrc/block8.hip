@@ -31,11 +31,8 @@ void quantize_kernel(const T* __restrict__ x, int64_t rs, uint8_t* __restrict__ 
             for (int u = 0; u < U; ++u) {
                 const int64_t r = r0 + u * step;
                 if (r >= rows) break;                                   // (the same for all lanes of a group)
-                const int sb = b8_scale_byte(b8_group_max<LANES>(b8_amax_bits(v[u])), fmt);
-                const float inv = b8_inv_scale(sb);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[u][i] *= inv;
-                const i32x2 w = b8_encode8(v[u], fmt);
+                int sb;
+                const i32x2 w = b8_quantize8<LANES>(v[u], fmt, sb);
                 uint8_t* q = codes + r * ldc + c;
                 if (wide && c + 8 <= pad) *(i32x2*)q = w;
                 else {
@@ -65,9 +62,9 @@ void quantize_t_kernel(const T* __restrict__ x, int64_t cs, uint8_t* __restrict_
     float v[32];
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = c0 + i < cols ? (float)x[rc + (int64_t)(c0 + i) * cs] : 0.f;
-    uint32_t m = 0;
+    uint32_t m = 0, any = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) m = max(m, b8_amax_bits(v + 8 * i));
+    for (int i = 0; i < 4; ++i) { m = max(m, b8_amax_bits(v + 8 * i)); any = max(any, b8_max_bits(v + 8 * i)); }
     red[g][lr] = m;
     __syncthreads();
     m = max(max(red[0][lr], red[1][lr]), max(red[2][lr], red[3][lr]));
@@ -83,7 +80,7 @@ void quantize_t_kernel(const T* __restrict__ x, int64_t cs, uint8_t* __restrict_
             float* u = v + 16 * j + 8 * h;
 #pragma unroll
             for (int i = 0; i < 8; ++i) u[i] *= inv;
-            const i32x2 e = b8_encode8(u, fmt);
+            const i32x2 e = b8_encode8(u, fmt, any >= B8_INF);
             w[2 * h] = e[0]; w[2 * h + 1] = e[1];
         }
         if (wide && c0 + 16 * j + 16 <= pad) *(i32x4*)(q + 16 * j) = w;
@@ -167,12 +164,11 @@ void an_relu8_fwd_kernel(const float* __restrict__ x, float* __restrict__ y, uin
             const float t = v[i] + b[i];
             v[i] = here && inside && !(t <= 0.f) ? t : 0.f;              // (NaN stays NaN, as torch's relu leaves it)
         }
-        const int sb = b8_scale_byte(b8_group_max<LANES>(b8_amax_bits(v)), IFL_Q_E4M3);
-        const float inv = b8_inv_scale(sb);
-        float q[8], r[8];
+        int sb;
+        i32x2 w = b8_quantize8<LANES>(v, IFL_Q_E4M3, sb);
+        float r[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) { q[i] = v[i] * inv; r[i] = v[i] == 0.f ? 0.f : v[i] * s[i]; }
-        i32x2 w = b8_encode8(q, IFL_Q_E4M3);
+        for (int i = 0; i < 8; ++i) r[i] = v[i] == 0.f ? 0.f : v[i] * s[i];
 #pragma unroll
         for (int i = 0; i < 8; ++i) if (v[i] > 0.f && ((uint32_t)w[i >> 2] >> 8 * (i & 3) & 0xffu) == 0u) w[i >> 2] |= 1 << 8 * (i & 3);
         if (here) {

@@ -48,14 +48,18 @@ extern "C" int ifl_linear8_bwd(const void* dy, int xtype, int64_t ldy, const uin
     IFL_CHECK_ARG(sizes_ok(M, N, K), IFL_EINVAL, "linear8_bwd: %lld x %lld x %lld", (long long)M, (long long)N, (long long)K);
     IFL_CHECK_ARG(scratch && (uintptr_t)scratch % 16 == 0, IFL_EINVAL, "linear8_bwd: scratch");
     uint8_t* at = (uint8_t*)scratch;
+    const bool sums = dw || db;
+    uint8_t *gc = at, *gs = gc + up16(M * code_ld(N)), *wc = gc + block_bytes(M, N), *ws = wc + up16(K * code_ld(N));
+    float* part = (float*)(wc + block_bytes(K, N));
+    if (dx) at = (uint8_t*)part + up16(4 * ifl_block8_matmul_scratch_floats(M, K, N, xtype));
+    const B8Quant quant = {gc, gs, code_ld(N), scale_ld(N), gfmt};
+    auto gradients = [&](int steps) {
+        return b8_wgrad(steps, dx ? &quant : nullptr, dy, xtype, ldy, codes, code_ld(K), scales, scale_ld(K), IFL_Q_E4M3, nullptr, dw, wtype, K, db, dbtype, (float*)at, M, N, dw ? K : 0, stream);
+    };
     if (dx && M > 0) {
-        uint8_t *gc = at, *gs = gc + up16(M * code_ld(N)), *wc = gc + block_bytes(M, N), *ws = wc + up16(K * code_ld(N));
-        float* part = (float*)(wc + block_bytes(K, N));
-        at = (uint8_t*)part + up16(4 * ifl_block8_matmul_scratch_floats(M, K, N, xtype));
-        if (int rc = ifl_block8_quantize(dy, xtype, ldy, 1, gc, code_ld(N), gs, scale_ld(N), M, N, gfmt, stream)) return rc;
+        if (int rc = sums ? gradients(1) : ifl_block8_quantize(dy, xtype, ldy, 1, gc, code_ld(N), gs, scale_ld(N), M, N, gfmt, stream)) return rc;
         if (int rc = ifl_block8_quantize(w, wtype, w_cs, w_rs, wc, code_ld(N), ws, scale_ld(N), K, N, IFL_Q_E4M3, stream)) return rc;
         if (int rc = ifl_block8_matmul(gc, code_ld(N), gs, scale_ld(N), gfmt, wc, code_ld(N), ws, scale_ld(N), IFL_Q_E4M3, nullptr, 0, dx, xtype, K, part, M, K, N, stream)) return rc;
     }
-    if (dw || db) return ifl_block8_wgrad(dy, xtype, ldy, codes, code_ld(K), scales, scale_ld(K), IFL_Q_E4M3, nullptr, dw, wtype, K, db, dbtype, (float*)at, M, N, dw ? K : 0, stream);
-    return 0;
+    return sums ? gradients(dx ? 2 : 3) : 0;
 }

@@ -364,11 +364,8 @@ void mm8_skinny_kernel(MM8 q)
             const int m = i / KB, kb = i - m * KB, c = kb * B8_BLK + l16 * 8;
             float v[8];
             b8_load8<TX, false>((const TX*)q.x + m * q.ldx + c, q.K - c, v);
-            const int s = b8_scale_byte(b8_group_max<16>(b8_amax_bits(v)), IFL_Q_E4M3);
-            const float inv = b8_inv_scale(s);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] *= inv;
-            *(i32x2*)(own + m * KP + c) = b8_encode8(v, IFL_Q_E4M3);
+            int s;
+            *(i32x2*)(own + m * KP + c) = b8_quantize8<16>(v, IFL_Q_E4M3, s);
             if (l16 == 0) own[(int)q.M * KP + i] = (uint8_t)s;
         }
         __syncthreads();
