@@ -27,8 +27,8 @@ struct WG8 {
     int want_x;                          // 0: column sums alone
     uint8_t *gc, *gs; int64_t ldgc, ldgs; int gfmt;  // where dy's own 8-bit blocks go, if they are wanted
     // scratch
-    uint16_t* xb; int64_t kp;            // restored codes [rows up to a multiple of 32][kp], zeros behind row M
-    uint16_t* yb; int64_t np, yplane;    // terms of dy [NP][rows up to a multiple of 32][np]; of bf16 read in place: its last M % 32 rows
+    uint16_t* xb;                        // restored codes, rows up to a multiple of 64 (zeros)
+    uint16_t* yb; int64_t yplane;        // terms of dy in the same way, yplane apart; or of bf16 read in place the last M % 64 rows
     int in_place;
     float* part; int split, steps;       // float32 partial sums [split][N][K], steps of 32 rows per part
     float* cs; int cs_parts; int64_t cs_rows, y_row0;        // partial column sums [cs_parts][N], of cs_rows rows from y_row0 on
@@ -36,22 +36,16 @@ struct WG8 {
     int x_blocks, x_tpr_log, y_cols, y_tpr_log;      // first launch: workgroups that restore codes, threads along a row; ranges of columns of dy, threads along a row
 };
 
-// One, two or three bf16 terms whose sum is the value, as floats with 16 low zero bits: its leading 8 significant bits, the next 8,
-// the rest.  What is not finite is the first term alone.
-template <int NP>
-__device__ __forceinline__ void wg8_terms(float x, float t[NP]) {
-    if constexpr (NP == 1) t[0] = x;                                     // (from bf16)
-    else {
-        x = __builtin_canonicalizef(x);                                  // (a NaN has a high bit set)
-        t[0] = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
-        float r = x - t[0];
-        r = r == r ? r : 0.f;
-#pragma unroll
-        for (int i = 1; i < NP; ++i) {
-            t[i] = __uint_as_float(__float_as_uint(r) & 0xffff0000u);
-            r -= t[i];
-        }
-    }
+// The next of the bf16 terms whose sum is a value, as a float with 16 low zero bits: its leading 8 significant bits; x becomes what is
+// left.  What is not finite is the first term alone.  (FIRST; of bf16 the first term is the value.)
+template <bool FIRST, class T>
+__device__ __forceinline__ uint32_t wg8_term(float& x) {
+    if constexpr (sizeof(T) == 2 && !__is_same(T, _Float16)) return __float_as_uint(x);
+    if (FIRST) x = __builtin_canonicalizef(x);                           // (a NaN has a high bit set)
+    const uint32_t t = __float_as_uint(x) & 0xffff0000u;
+    x -= __uint_as_float(t);
+    if (FIRST) x = x == x ? x : 0.f;
+    return t;
 }
 
 template <class TW>
@@ -69,37 +63,68 @@ __device__ __forceinline__ void wg8_store4(TW* d, int left, const float v[4]) {
 }
 
 constexpr int MS = 32;                                                  // rows per step: the depth of one product
+constexpr int MP = 2 * MS;                                              // what rows are padded to with zeros
+__host__ __device__ inline int64_t wg8_rows(int64_t M) { return (M + MP - 1) / MP * MP; }
 
 // ------------------------------------------------------------------------------------------------ first launch
-// Workgroups 0 .. x_blocks - 1 restore codes, 8 a thread.  The others take up to 256 columns (8 a thread) of cs_rows rows of dy, with
-// column sums on the way that are joined in LDS in a fixed order.  QUANT: they also put dy into 8-bit blocks (for the layer's
-// other product), which saves a pass over it (16384 x 2048, both operands, bf16: 46 us instead of 25 + 33).
+// The product's fragments are 8 rows of a column; of 32 rows lane group g = 0 .. 3 has 4 g .. 4 g + 3 and 16 + 4 g .. 16 + 4 g + 3
+// (what two transposing reads give it).  So that they can be read from LDS 16 bytes at a time, what this launch writes is ordered
+// [32 rows][g][column][8 rows].
+//
+// A thread has the 8 rows of one g and 8 columns; 16 bytes per column.  They meet in LDS so that the stores are whole lines (slot
+// i of the workgroup's at i ^ (i / 16 & 7): no bank conflicts on either side).
+__device__ __forceinline__ void wg8_put(i32x4* lds, const i32x4 w[8], uint16_t* out, int64_t row0, int64_t rows, int64_t cols, int c0, int tpr_log) {
+    int j = threadIdx.x;
+    asm volatile("" : "+v"(j));                                          // (places are made here, not kept)
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { const int at = j * 8 + i; lds[at ^ (at >> 4 & 7)] = w[i]; }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+        const int at = n * 256 + j, gg = at >> (3 + tpr_log), c = c0 + (at & ((8 << tpr_log) - 1));
+        const int64_t r = row0 + 8 * gg;                                 // (counted in groups of 8 rows that follow one another)
+        if (c < cols && r < rows) *(i32x4*)(out + (r / 8 * cols + c) * 8) = lds[at ^ (at >> 4 & 7)];
+    }
+}
+// row e of group gg (from a multiple of 32 on)
+__device__ __forceinline__ int wg8_row(int gg, int e) { return (gg >> 2) * 32 + 4 * (gg & 3) + (e & 3) + 16 * (e >> 2); }
+
+// Workgroups 0 .. x_blocks - 1 restore codes.  The others take up to 256 columns of cs_rows rows of dy, with column sums on the
+// way that are joined in LDS in a fixed order, and dy's terms, if the product does not read it in place.  QUANT: they also put dy
+// into 8-bit blocks (for the layer's other product), which saves a pass over it (16384 x 2048, both operands, bf16: @@ us
+// instead of 25 + 33).
 template <class T, int NP, bool VEC, bool QUANT>
-__global__ __launch_bounds__(256)
+__global__ __launch_bounds__(256, NP > 1 ? 2 : 3)
 void wgrad8_prepare_kernel(WG8 q)
 {
-    const int64_t mp = (q.M + MS - 1) / MS * MS;
+    __shared__ __attribute__((aligned(16))) i32x4 stage[2048];
+    const int64_t mp = wg8_rows(q.M);
     if ((int)blockIdx.x < q.x_blocks) {
-        const int rpb = 256 >> q.x_tpr_log;
-        const int64_t step = (int64_t)q.x_blocks * rpb;
-        constexpr int U = 4;
-        for (int64_t r0 = (int64_t)blockIdx.x * rpb + (threadIdx.x >> q.x_tpr_log); r0 < mp; r0 += U * step) {
-            for (int c = (threadIdx.x & ((1 << q.x_tpr_log) - 1)) * 8; c < q.kp; c += 8 << q.x_tpr_log) {
-                i32x2 w[U];
-                int sb[U];
+        const int tpr = 1 << q.x_tpr_log, gg = threadIdx.x >> q.x_tpr_log, rpp = 8 * (256 >> q.x_tpr_log);
+        const int cols = (q.K + 8 * tpr - 1) / (8 * tpr);
+        const int64_t jobs = (mp + rpp - 1) / rpp * cols;
+        for (int64_t job = blockIdx.x; job < jobs; job += q.x_blocks) {
+            const int64_t row0 = job / cols * rpp;
+            const int c0 = (int)(job % cols) * 8 * tpr, c = c0 + (threadIdx.x & (tpr - 1)) * 8;
+            i32x2 w[8];
+            int sb[8];
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int64_t r = r0 + u * step;
-                    const bool in = r < q.M && c < q.K;                  // (rows are whole 16 bytes)
-                    w[u] = in ? *(const i32x2*)(q.codes + r * q.ldc + c) : i32x2{0, 0};
-                    sb[u] = in ? q.scales[r * q.lds + c / B8_BLK] : 127;
-                }
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int64_t r = r0 + u * step;
-                    if (r < mp) *(bf16x8*)(q.xb + r * q.kp + c) = q.fmt == IFL_Q_E4M3 ? b8_bf16x8<IFL_Q_E4M3>(w[u][0], w[u][1], sb[u]) : b8_bf16x8<IFL_Q_E5M2>(w[u][0], w[u][1], sb[u]);
-                }
+            for (int e = 0; e < 8; ++e) {
+                const int64_t r = row0 + wg8_row(gg, e);
+                const bool in = r < q.M && c < q.K;                      // (rows are whole 16 bytes)
+                w[e] = in ? *(const i32x2*)(q.codes + r * q.ldc + c) : i32x2{0, 0};
+                sb[e] = in ? q.scales[r * q.lds + c / B8_BLK] : 127;
             }
+            i32x4 v[8], t[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = __builtin_bit_cast(i32x4, q.fmt == IFL_Q_E4M3 ? b8_bf16x8<IFL_Q_E4M3>(w[e][0], w[e][1], sb[e]) : b8_bf16x8<IFL_Q_E5M2>(w[e][0], w[e][1], sb[e]));
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    t[i][e] = (int)__builtin_amdgcn_perm((uint32_t)v[2 * e + 1][i / 2], (uint32_t)v[2 * e][i / 2], i & 1 ? 0x07060302u : 0x05040100u);
+            wg8_put(stage, t, q.xb, row0, mp, q.K, c0, q.x_tpr_log);
         }
         return;
     }
@@ -108,42 +133,70 @@ void wgrad8_prepare_kernel(WG8 q)
     const int tpr = 1 << q.y_tpr_log, rpp = 256 >> q.y_tpr_log, rl = threadIdx.x >> q.y_tpr_log;
     const int c0 = cb * 8 * tpr, c = c0 + (threadIdx.x & (tpr - 1)) * 8;
     const int64_t first = q.y_row0 + (int64_t)part * q.cs_rows, last = min(mp, first + q.cs_rows);
-    const int64_t m32 = q.M / MS * MS;
+    const int64_t whole = q.M / MP * MP;
     const T* dy = (const T*)q.dy;
     float sum[8] = {};
-    for (int64_t r0 = first + rl; r0 < last; r0 += 4 * rpp) {
-        float v[4][8];
+    for (int64_t row0 = first; row0 < last; row0 += 8 * rpp) {
+        // rows and columns past the end: the last one's values, then zeros
+        float v[8][8];
+        const T* rows = dy + row0 * q.ldy;
+        const int left = (int)(min(q.M, last) - row0);                   // (negative: all of them are zeros, read from row M - 1)
+        int row = wg8_row(rl, 0), cc = c;
+        asm volatile("" : "+v"(row), "+v"(cc));                          // (addresses are made here, not kept)
+        auto at = [&](int e) { return rows + (int64_t)min(row + (e & 3) + 16 * (e >> 2), left > 0 ? left - 1 : (int)(q.M - 1 - row0)) * q.ldy; };
+        if (VEC && cc + 8 <= q.N) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int64_t r = r0 + u * rpp;
-            b8_load8<T, VEC>(dy + (r < q.M ? r : 0) * q.ldy + c, r < q.M && r < last ? q.N - c : 0, v[u]);
+            for (int e = 0; e < 8; ++e) b8_load8<T, true>(at(e) + cc, 8, v[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) { const float t = (float)at(e)[min(cc + i, q.N - 1)]; v[e][i] = cc + i < q.N ? t : 0.f; }
         }
+        if (left < 8 * rpp) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int64_t r = r0 + u * rpp;
-            if (r >= last) break;
+            for (int e = 0; e < 8; ++e)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum[i] += v[u][i];
+                for (int i = 0; i < 8; ++i) v[e][i] = row + (e & 3) + 16 * (e >> 2) < left ? v[e][i] : 0.f;
+        }
+        __builtin_amdgcn_sched_barrier(0);                               // (here and below: the compiler would otherwise do it all side by side, in 300 registers)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int r = row + (e & 3) + 16 * (e >> 2);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[i] += v[e][i];
             if constexpr (QUANT) {
                 int sb;                                                  // (of a block: 16 threads, or the 4 or 8 of a short row)
-                const i32x2 w = b8_quantize8<16>(v[u], q.gfmt, sb, tpr);
-                if (r < q.M) {
-                    if (c < q.ldgc) *(i32x2*)(q.gc + r * q.ldgc + c) = w;
-                    if (c < q.N && (c & (B8_BLK - 1)) == 0) q.gs[r * q.ldgs + c / B8_BLK] = (uint8_t)sb;
+                const i32x2 w = b8_quantize8<16>(v[e], q.gfmt, sb, tpr);
+                if (r < left) {
+                    if (cc < q.ldgc) *(i32x2*)(q.gc + (row0 + r) * q.ldgc + cc) = w;
+                    if (cc < q.N && (cc & (B8_BLK - 1)) == 0) q.gs[(row0 + r) * q.ldgs + cc / B8_BLK] = (uint8_t)sb;
                 }
             }
-            // terms of what is not read in place: everything, or the rows behind the last 32 whole ones
-            if (q.want_x && c < q.np && (!q.in_place || r >= m32)) {
-                float t[8][NP];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) wg8_terms<NP>(v[u][i], t[i]);
-#pragma unroll
-                for (int k = 0; k < NP; ++k) {
+            if constexpr (NP == 1) {
+                if (q.want_x && q.in_place && cc < q.N && row0 + r >= whole && row0 + r < last) {        // the last rows, as they are
                     i32x4 w;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) w[e] = (int)__builtin_amdgcn_perm(__float_as_uint(t[2 * e + 1][k]), __float_as_uint(t[2 * e][k]), 0x07060302u);   // the high halves
-                    *(i32x4*)(q.yb + k * q.yplane + (q.in_place ? r - m32 : r) * q.np + c) = w;
+                    for (int i = 0; i < 4; ++i) w[i] = (int)__builtin_amdgcn_perm(__float_as_uint(v[e][2 * i + 1]), __float_as_uint(v[e][2 * i]), 0x07060302u);    // the high halves
+                    *(i32x4*)(q.yb + (row0 + r - whole) * q.N + cc) = w;
                 }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (q.want_x && !q.in_place) {
+#pragma unroll
+            for (int k = 0; k < NP; ++k) {
+                i32x4 t[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t lo = k ? wg8_term<false, T>(v[2 * e][i]) : wg8_term<true, T>(v[2 * e][i]);
+                        const uint32_t hi = k ? wg8_term<false, T>(v[2 * e + 1][i]) : wg8_term<true, T>(v[2 * e + 1][i]);
+                        t[i][e] = (int)__builtin_amdgcn_perm(hi, lo, 0x07060302u);       // the high halves
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                wg8_put(stage, t, q.yb + k * q.yplane, row0, last, q.N, c0, q.y_tpr_log);
             }
         }
     }
@@ -160,12 +213,14 @@ void wgrad8_prepare_kernel(WG8 q)
 }
 
 // ------------------------------------------------------------------------------------------------ the product
-// Workgroup = TN x TK of dw over a range of rows, 32 at a time.  Rows of both operands lie in LDS as they do in memory; the fragments,
-// which run along m, come out of LDS transposed (ds_read_b64_tr_b16: 16 lanes read 4 rows of 16 values and get columns).  The
-// instruction's first operand is the k side: a lane ends up with 4 neighbouring k of one n.
+// Workgroup = TN x TK of dw over a range of rows, 32 at a time.  The instruction's first operand is the k side: a lane ends up with 4
+// neighbouring k of one n.
 //
-// A fragment read touches, per group of 16 lanes, 4 rows and 4 pieces of 8 bytes of each: one granule of 32 bytes, granule i of row m at
-// place i ^ (m & 7), which leaves no bank conflicts.  Loads go straight to LDS in lane order, so it is the source that is permuted.
+// The k side, and dy's terms, lie in LDS as they do in memory, [g][column][8 rows]: a fragment is 16 bytes a lane, 16 lanes 256 bytes in a
+// row.  bf16 gradients are read in place (TR): their rows lie in LDS as in memory, and fragments come out transposed
+// (ds_read_b64_tr_b16: 16 lanes read 4 rows of 16 values and get columns), at half the rate.  Such a read touches, per group of 16
+// lanes, 4 rows and 4 pieces of 8 bytes of each: one granule of 32 bytes, granule i of row m at place i ^ (m & 7), which leaves no
+// bank conflicts.  Loads go straight to LDS in lane order, so it is the source that is permuted.
 //
 // A step is a term of dy with 32 rows (the terms of the same rows follow one another and share the k side's fragments).  It has two
 // phases.  MEM: the loads of the step three ahead are issued (rings of four), this step's fragments are read.  COMPUTE: its
@@ -174,13 +229,13 @@ void wgrad8_prepare_kernel(WG8 q)
 // all workgroups ask for at the same time take to come from memory.
 template <int V> struct Int { static constexpr int value = V; };
 
-template <int NP, int TN, int TK, int WN, int WK>
+template <int NP, bool TR, int TN, int TK, int WN, int WK>
 __global__ __launch_bounds__(64 * WN * WK)
 void wgrad8_kernel(WG8 q)
 {
     constexpr int NW = WN * WK, NT = 64 * NW, NF = TN / WN / 16, KF = TK / WK / 16;
     constexpr bool TURNS = NW == 8;
-    constexpr int YROW = TN * 2, XROW = TK * 2, YB = MS * YROW, XB = MS * XROW;          // bytes
+    constexpr int YROW = TN * 2, YB = MS * YROW, XB = MS * TK * 2;         // bytes
     constexpr int YP = YB / 16 / NT, XP = XB / 16 / NT;                  // 16-byte pieces per thread
     static_assert(YP == 2 && XP == 2 && NF == 4 && (KF == 4 || KF == 8), "");
     __shared__ __attribute__((aligned(16))) uint8_t ys[4 * YB], xs[4 * XB];
@@ -193,7 +248,7 @@ void wgrad8_kernel(WG8 q)
     const uint32_t tid = threadIdx.x;
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, g = lane >> 4;
     const int wk = wave % WK, wn = wave / WK;
-    const int s0 = part * q.steps, rows_steps = (int)((q.M + MS - 1) / MS), steps = (min(rows_steps, s0 + q.steps) - s0) * NP;
+    const int s0 = part * q.steps, rows_steps = (int)(wg8_rows(q.M) / MS), steps = (min(rows_steps, s0 + q.steps) - s0) * NP;
     // (fresh: an address or offset that is made again at its use instead of being held in registers of its own)
     auto fresh = [](auto x) { asm volatile("" : "+v"(x)); return x; };
 
@@ -203,39 +258,41 @@ void wgrad8_kernel(WG8 q)
         const uint32_t at = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)to;
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(at), "v"(o), "s"(base) : "memory", "m0");
     };
-    // a thread's pieces: a column (past the end: any, its results are not stored), rows that lie a multiple of 8 apart
-    constexpr int YSTEP = NT / (TN / 8), XSTEP = NT / (TK / 8);
-    static_assert(YSTEP % 8 == 0 && XSTEP % 8 == 0, "");
-    const int64_t ldy = q.in_place ? q.ldy : q.np;
-    uint32_t yo, xo;
-    {
-        const int r = tid / (TN / 8), c = ((tid % (TN / 8) >> 1) ^ (r & 7)) * 2 + (tid & 1);
-        yo = (n0 + c * 8 < q.np ? n0 * 2 + c * 16 : 0) + (uint32_t)(r * 2 * (int)ldy);
-        const int rx = tid / (TK / 8), cx = ((tid % (TK / 8) >> 1) ^ (rx & 7)) * 2 + (tid & 1);
-        xo = (k0 + cx * 8 < q.kp ? k0 * 2 + cx * 16 : 0) + (uint32_t)(rx * 2 * (int)q.kp);
-    }
-    const int m32 = (int)(q.M / MS);
+    // a thread's pieces: a column (past the end: any, its results are not stored), and rows (TR) or groups of 8 that lie apart
+    constexpr int YSTEP = TR ? NT / (TN / 8) : NT / TN, XSTEP = NT / TK;
+    static_assert(YSTEP >= 1 && XSTEP >= 1 && (!TR || YSTEP % 8 == 0), "");
+    const int yr = TR ? tid / (TN / 8) : tid / TN, xr = tid / TK;
+    const int yn = n0 + (TR ? (((tid % (TN / 8) >> 1) ^ (yr & 7)) * 2 + (tid & 1)) * 8 : tid % TN), xk = k0 + tid % TK;
+    const uint32_t yc = yn < q.N ? (uint32_t)yn * (TR ? 2 : 16) : 0, xc = xk < q.K ? (uint32_t)xk * 16 : 0;
+    const int whole = TR ? (int)(q.M / MP) * 2 : 0;                      // steps read in place
     // step t: term PL of rows 32 (s0 + t / NP) on; behind the last step it is loaded again, unused
-    auto load = [&](auto PL, int t, int ry, int rx) {
+    auto load = [&](auto PL, int t, int ry, int rx) __attribute__((always_inline)) {
         const int s = s0 + min(t, steps - 1) / NP;
-        // of rows read in place the last ones, which do not fill a step, were copied to a place with zeros behind them: np apart there
-        const uint16_t* y = q.in_place ? (const uint16_t*)q.dy + (int64_t)s * MS * ldy : q.yb + PL.value * q.yplane + (int64_t)s * MS * ldy;
-        const bool cut = q.in_place && s >= m32;
-        y = cut ? q.yb : y;
-        const int dl = cut ? (int)(q.np - ldy) * 2 : 0;                  // (rows of the copy are closer together)
+        const uint8_t* y;
+        uint32_t yl;                                                     // bytes from row to row, or group to group
+        if constexpr (TR) {                                              // the last rows were copied to a place with zeros behind them
+            const bool cut = s >= whole;
+            y = cut ? (const uint8_t*)q.yb : (const uint8_t*)q.dy;
+            yl = (uint32_t)(cut ? q.N : (int)q.ldy) * 2;
+            y += (int64_t)(cut ? s - whole : s) * (MS * yl);
+        } else {
+            yl = (uint32_t)q.N * 16;
+            y = (const uint8_t*)(q.yb + PL.value * q.yplane) + (int64_t)s * 4 * yl;
+        }
+        const uint32_t xl = (uint32_t)q.K * 16;
 #pragma unroll
-        for (int i = 0; i < YP; ++i)
-            to_lds(y, fresh(yo) + (uint32_t)(((int)(fresh(tid) / (TN / 8)) + i * YSTEP) * dl + i * YSTEP * 2 * (int)ldy), ys + ry * YB + (i * NT + wave * 64) * 16);
+        for (int i = 0; i < YP; ++i) to_lds(y, (uint32_t)(fresh(yr) + i * YSTEP) * yl + yc, ys + ry * YB + (i * NT + wave * 64) * 16);
         if constexpr (PL.value == 0) {
-            const uint16_t* x = q.xb + (int64_t)s * MS * q.kp;
+            const uint8_t* x = (const uint8_t*)q.xb + (int64_t)s * 4 * xl;
 #pragma unroll
-            for (int i = 0; i < XP; ++i) to_lds(x, fresh(xo) + (uint32_t)(i * XSTEP * 2 * (int)q.kp), xs + rx * XB + (i * NT + wave * 64) * 16);
+            for (int i = 0; i < XP; ++i) to_lds(x, (uint32_t)(fresh(xr) + i * XSTEP) * xl + xc, xs + rx * XB + (i * NT + wave * 64) * 16);
         }
     };
 
-    // ---- fragments (places are XORs of a lane's own and of a fragment's constants)
+    // ---- fragments (TR: places are XORs of a lane's own and of a fragment's constants)
     const int mrow = 4 * g + (r16 >> 2), q4 = r16 & 3;
-    const int ya = mrow * YROW + ((wn * NF) ^ (mrow & 7)) * 32 + q4 * 8, xa = mrow * XROW + ((wk * KF) ^ (mrow & 7)) * 32 + q4 * 8;
+    const int ya = TR ? mrow * YROW + ((wn * NF) ^ (mrow & 7)) * 32 + q4 * 8 : (g * TN + wn * NF * 16 + r16) * 16;
+    const int xa = (g * TK + wk * KF * 16 + r16) * 16;
     auto tr8 = [&](const uint8_t* a, int rows16) {
         const s16x4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a));
         const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a + rows16));
@@ -250,15 +307,18 @@ void wgrad8_kernel(WG8 q)
         asm volatile("" ::: "memory");
     };
     // one step: term PL of step t; ry, rx its places in the rings.  No branches inside: the compiler would move products past them.
-    auto step = [&](auto PL, int t, int ry, int rx) {
+    auto step = [&](auto PL, int t, int ry, int rx) __attribute__((always_inline)) {
         constexpr int P3 = (PL.value + 3) % NP;
         constexpr int AHEAD = (PL.value + 3) / NP;                       // row steps that term lies ahead
         load(Int<P3>(), t + 3, (ry + 3) & 3, (rx + AHEAD) & 3);
 #pragma unroll
-        for (int f = 0; f < NF; ++f) y[f] = tr8(ys + ry * YB + (fresh(ya) ^ f << 5), 16 * YROW);
+        for (int f = 0; f < NF; ++f) {
+            if constexpr (TR) y[f] = tr8(ys + ry * YB + (fresh(ya) ^ f << 5), 16 * YROW);
+            else y[f] = *(const bf16x8*)(ys + ry * YB + ya + f * 256);
+        }
         if constexpr (PL.value == 0) {
 #pragma unroll
-            for (int f = 0; f < KF; ++f) x[f] = tr8(xs + rx * XB + (fresh(xa) ^ f << 5), 16 * XROW);
+            for (int f = 0; f < KF; ++f) x[f] = *(const bf16x8*)(xs + rx * XB + xa + f * 256);
         }
         // the next step's loads have come: those of the two behind it are newer
         constexpr int NEWER = YP * 2 + XP * (((PL.value + 2) % NP == 0) + (P3 == 0));
@@ -385,14 +445,14 @@ __global__ void fill_zero_kernel(TW* p, int64_t ld, int rows, int cols)
 
 // Tiles of 256 x 256 for large layers, else 128 x 128.  The rows are split until the card is full (one workgroup on a CU of the
 // large tiles, two of the small ones), each with four steps at least.
-struct WPlan { int tile, split, steps, cs_parts, y_tpr_log; int64_t cs_rows, kp, np, x_floats, y_floats, part_floats, cs_floats; bool in_place; };
+struct WPlan { int tile, split, steps, cs_parts, y_tpr_log; int64_t cs_rows, x_floats, y_floats, part_floats, cs_floats; bool in_place; };
 WPlan wg8_plan(int64_t M, int64_t N, int64_t K, int dytype, bool aligned)
 {
     WPlan p = {};
     auto tiles = [&](int64_t t) { return ((N + t - 1) / t) * ((K + t - 1) / t); };
     const int terms = dytype == IFL_T_F32 ? 3 : dytype == IFL_T_F16 ? 2 : 1;
     p.tile = tiles(256) >= 32 ? 256 : 128;
-    const int64_t steps = (M + MS - 1) / MS, n = K > 0 ? tiles(p.tile) : 1;
+    const int64_t steps = wg8_rows(M) / MS, n = K > 0 ? tiles(p.tile) : 1;
     const int64_t full = p.tile == 256 ? 256 : 512;
     int64_t s = 4 * n >= 3 * full ? 1 : full / n;
     if (s > steps * terms / 4) s = steps * terms / 4;
@@ -400,22 +460,20 @@ WPlan wg8_plan(int64_t M, int64_t N, int64_t K, int dytype, bool aligned)
     if (s < 1) s = 1;
     p.steps = (int)((steps + s - 1) / s);
     p.split = (int)((steps + p.steps - 1) / p.steps);
-    // column sums (and terms): about 1024 workgroups, 32 rows each at least
+    // column sums (and terms): about as many workgroups as run at a time (bf16: 3 on a CU) or two such rounds (the terms' kernels: 512
+    // instead of 1024 took 87 us instead of 80 at 16384 x 2048), each with the rows of one pass at least
     p.y_tpr_log = 2;
     while (p.y_tpr_log < 5 && (8 << p.y_tpr_log) < N) ++p.y_tpr_log;
-    const int64_t cols = (N + (8 << p.y_tpr_log) - 1) / (8 << p.y_tpr_log);
-    int64_t c = 1024 / cols;
-    if (c > steps) c = steps;
-    if (c > 512) c = 512;
+    const int64_t cols = (N + (8 << p.y_tpr_log) - 1) / (8 << p.y_tpr_log), pass = 8 * (256 >> p.y_tpr_log);
+    int64_t c = (terms > 1 ? 1024 : 768) / cols;
+    if (c > (M + pass - 1) / pass) c = (M + pass - 1) / pass;
     if (c < 1) c = 1;
-    p.cs_rows = (steps + c - 1) / c * MS;
+    p.cs_rows = ((steps + c - 1) / c + 1) / 2 * MP;
     p.cs_parts = (int)((steps * MS + p.cs_rows - 1) / p.cs_rows);
     p.in_place = dytype == IFL_T_BF16 && aligned;
-    p.kp = (K + 7) / 8 * 8;
-    p.np = (N + 7) / 8 * 8;
     auto up = [](int64_t floats) { return (floats + 3) / 4 * 4; };
-    p.x_floats = K > 0 ? up(steps * MS * p.kp / 2) : 0;
-    p.y_floats = K > 0 ? up((p.in_place ? MS : terms * steps * MS) * p.np / 2) : 0;
+    p.x_floats = K > 0 ? up(steps * MS * K / 2) : 0;
+    p.y_floats = K > 0 ? up((p.in_place ? MP : terms * steps * MS) * N / 2) : 0;
     p.part_floats = K > 0 && p.split > 1 ? up(p.split * N * K) : 0;
     p.cs_floats = up(p.cs_parts * N);
     return p;
@@ -462,20 +520,18 @@ int b8_wgrad(int todo, const B8Quant* quant, const void* dy, int dytype, int64_t
     WG8 q = {};
     q.dy = dy; q.ldy = ldy; q.codes = codes; q.ldc = ldc; q.scales = scales; q.lds = lds; q.chan = chan; q.dw = dw; q.ldw = ldw;
     q.dwtype = dwtype; q.db = db; q.dbtype = dbtype; q.M = M; q.N = (int)N; q.K = (int)K; q.fmt = fmt; q.want_x = dw != nullptr;
-    q.kp = p.kp; q.np = p.np; q.yplane = (M + MS - 1) / MS * MS * p.np; q.in_place = p.in_place;
+    q.yplane = wg8_rows(M) * N; q.in_place = p.in_place;
     q.xb = (uint16_t*)scratch;
     q.yb = (uint16_t*)(scratch + p.x_floats);
     q.part = scratch + p.x_floats + p.y_floats;
     q.cs = q.part + p.part_floats;
     q.split = p.split; q.steps = p.steps; q.cs_parts = p.cs_parts; q.cs_rows = p.cs_rows;
 
-    const int64_t mp = (M + MS - 1) / MS * MS;
     if (todo & 1) {
         if (dw) {
-            while (q.x_tpr_log < 8 && (8 << q.x_tpr_log) < p.kp) ++q.x_tpr_log;
-            const int64_t rows = (mp + (256 >> q.x_tpr_log) - 1) / (256 >> q.x_tpr_log);           // in turns of one workgroup
-            const int64_t four = (rows + 3) / 4;
-            q.x_blocks = (int)(four >= 16384 ? 16384 : four >= 512 ? four : rows < 512 ? rows : 512);
+            while (q.x_tpr_log < 5 && (8 << q.x_tpr_log) < K) ++q.x_tpr_log;
+            const int64_t rpp = 8 * (256 >> q.x_tpr_log), jobs = (wg8_rows(M) + rpp - 1) / rpp * ((K + (8 << q.x_tpr_log) - 1) / (8 << q.x_tpr_log));
+            q.x_blocks = (int)(jobs < 16384 ? jobs : 16384);
         }
         q.y_tpr_log = p.y_tpr_log;
         q.y_cols = (int)((N + (8 << p.y_tpr_log) - 1) / (8 << p.y_tpr_log));
@@ -483,9 +539,9 @@ int b8_wgrad(int todo, const B8Quant* quant, const void* dy, int dytype, int64_t
         // fill a step
         int64_t y_blocks = (int64_t)p.cs_parts * q.y_cols;
         if (p.in_place && !db && !quant) {
-            q.y_row0 = M / MS * MS;
-            q.cs_rows = MS;
-            y_blocks = M % MS ? q.y_cols : 0;
+            q.y_row0 = M / MP * MP;
+            q.cs_rows = MP;
+            y_blocks = M % MP ? q.y_cols : 0;
         }
         if (quant) { q.gc = quant->codes; q.gs = quant->scales; q.ldgc = quant->ldc; q.ldgs = quant->lds; q.gfmt = quant->fmt; }
         const dim3 pg((unsigned)(q.x_blocks + y_blocks));
@@ -503,11 +559,12 @@ int b8_wgrad(int todo, const B8Quant* quant, const void* dy, int dytype, int64_t
         q.tiles_k = (int)((K + p.tile - 1) / p.tile);
         q.per_xcd = (q.tiles_n * q.tiles_k * p.split + 7) / 8;
         const dim3 grid(8 * q.per_xcd);
-#define WG8_K(NP) do { \
-        if (p.tile == 256) hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_kernel<NP, 256, 256, 4, 2>), grid, dim3(512), 0, st, q); \
-        else hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_kernel<NP, 128, 128, 2, 2>), grid, dim3(256), 0, st, q); \
+#define WG8_K(NP, TR) do { \
+        if (p.tile == 256) hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_kernel<NP, TR, 256, 256, 4, 2>), grid, dim3(512), 0, st, q); \
+        else hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_kernel<NP, TR, 128, 128, 2, 2>), grid, dim3(256), 0, st, q); \
     } while (0)
-        if (dytype == IFL_T_F32) WG8_K(3); else if (dytype == IFL_T_F16) WG8_K(2); else WG8_K(1);
+        if (dytype == IFL_T_F32) WG8_K(3, false); else if (dytype == IFL_T_F16) WG8_K(2, false);
+        else if (p.in_place) WG8_K(1, true); else WG8_K(1, false);
         IFL_LAUNCH_CHECK();
     }
     int64_t jobs = 0;
