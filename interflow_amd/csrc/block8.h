@@ -24,19 +24,21 @@ template <> struct B8Type<IFL_T_BF16> { typedef __bf16 type; };
 template <> struct B8Type<IFL_T_F16> { typedef _Float16 type; };
 static inline int b8_size(int t) { return t == IFL_T_F32 ? 4 : 2; }
 
-// 8 consecutive elements as floats; `left` of them exist.  VEC: 16-byte aligned.
-template <class T, bool VEC>
+// N consecutive elements that need no alignment but their own: global loads and stores of 8 and 16 bytes take any address here, at
+// full speed where it is aligned
+template <class T, int N>
+struct B8Vec { typedef T Aligned __attribute__((ext_vector_type(N))); typedef Aligned type __attribute__((aligned(alignof(T)))); };
+
+// 8 consecutive elements as floats; `left` of them exist (the others are zeros)
+template <class T>
 __device__ __forceinline__ void b8_load8(const T* __restrict__ p, int left, float v[8]) {
-    if (VEC && left >= 8) {
-        if constexpr (sizeof(T) == 4) {
-            const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
+    if (left >= 8) {
+        constexpr int V = 16 / sizeof(T);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
-        } else {
-            typedef T T8 __attribute__((ext_vector_type(8)));
-            const T8 a = *(const T8*)p;
+        for (int h = 0; h < 8 / V; ++h) {
+            const typename B8Vec<T, V>::type a = ((const typename B8Vec<T, V>::type*)p)[h];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = (float)a[i];
+            for (int i = 0; i < V; ++i) v[h * V + i] = (float)a[i];
         }
     } else {
 #pragma unroll
@@ -44,19 +46,16 @@ __device__ __forceinline__ void b8_load8(const T* __restrict__ p, int left, floa
     }
 }
 
-template <class T, bool VEC>
+template <class T>
 __device__ __forceinline__ void b8_store8(T* __restrict__ p, int left, const float v[8]) {
-    if (VEC && left >= 8) {
-        if constexpr (sizeof(T) == 4) {
-            const f32x4 a = {v[0], v[1], v[2], v[3]}, b = {v[4], v[5], v[6], v[7]};
-            *(f32x4*)p = a;
-            *(f32x4*)(p + 4) = b;
-        } else {
-            typedef T T8 __attribute__((ext_vector_type(8)));
-            T8 a;
+    if (left >= 8) {
+        constexpr int V = 16 / sizeof(T);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) a[i] = (T)v[i];
-            *(T8*)p = a;
+        for (int h = 0; h < 8 / V; ++h) {
+            typename B8Vec<T, V>::Aligned a;
+#pragma unroll
+            for (int i = 0; i < V; ++i) a[i] = (T)v[h * V + i];
+            ((typename B8Vec<T, V>::type*)p)[h] = a;
         }
     } else {
 #pragma unroll
@@ -159,14 +158,19 @@ __device__ __forceinline__ void b8_decode4(int w, int fmt, float* v) {
     v[0] = a[0]; v[1] = a[1]; v[2] = b[0]; v[3] = b[1];
 }
 
-// 8 codes of a row from column c on, `left` of them exist; VEC: 8-byte aligned
-template <bool VEC>
+// 8 codes, `left` of them exist (the others are zeros)
+typedef i32x2 i32x2_any __attribute__((aligned(1)));
 __device__ __forceinline__ i32x2 b8_load_codes(const uint8_t* __restrict__ p, int left) {
-    if (VEC && left >= 8) return *(const i32x2*)p;
+    if (left >= 8) return *(const i32x2_any*)p;
     i32x2 r = {0, 0};
 #pragma unroll
     for (int i = 0; i < 8; ++i) if (i < left) r[i >> 2] |= (int)((uint32_t)p[i] << 8 * (i & 3));
     return r;
+}
+__device__ __forceinline__ void b8_store_codes(uint8_t* __restrict__ p, int left, i32x2 w) {
+    if (left >= 8) { *(i32x2_any*)p = w; return; }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) if (i < left) p[i] = (uint8_t)((uint32_t)w[i >> 2] >> 8 * (i & 3));
 }
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));

@@ -7,11 +7,12 @@ namespace {
 
 // ------------------------------------------------------------------------------------------------ quantize, rows contiguous
 // Group of LANES lanes = one block of a row; kg (a power of two) groups side by side along a row, the rest along rows.  Four
-// rows per group are in flight at once: their loads are issued before the first is used.
-template <class T, int LANES, bool VEC>
+// rows per group are in flight at once: their loads are issued before the first is used.  Few, long rows: gridDim.y workgroups share
+// one (4 x 1000000: 500 us with one each, 7.6 so).  16384 x 2048: bf16 19.4 us, 5.2 TB/s, float32 27.0 us, 6.2 TB/s.
+template <class T, int LANES>
 __global__ __launch_bounds__(256)
 void quantize_kernel(const T* __restrict__ x, int64_t rs, uint8_t* __restrict__ codes, int64_t ldc, uint8_t* __restrict__ scales,
-                     int64_t lds, int64_t rows, int cols, int pad, int wide, int kg_log, int fmt)
+                     int64_t lds, int64_t rows, int cols, int pad, int kg_log, int fmt)
 {
     constexpr int U = 4, GPB = 256 / LANES;
     const int lane = threadIdx.x % LANES, grp = threadIdx.x / LANES;
@@ -19,13 +20,13 @@ void quantize_kernel(const T* __restrict__ x, int64_t rs, uint8_t* __restrict__ 
     const int KB = (cols + B8_BLK - 1) / B8_BLK;
     const int64_t step = (int64_t)gridDim.x * rpb;
     for (int64_t r0 = (int64_t)blockIdx.x * rpb + gr; r0 < rows; r0 += U * step) {
-        for (int kb = gk; kb < KB; kb += 1 << kg_log) {
+        for (int kb = gk + (blockIdx.y << kg_log); kb < KB; kb += gridDim.y << kg_log) {
             const int c = kb * B8_BLK + lane * 8;
             float v[U][8];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int64_t r = r0 + u * step;
-                b8_load8<T, VEC>(x + r * rs + c, r < rows ? cols - c : 0, v[u]);
+                b8_load8<T>(x + r * rs + c, r < rows ? cols - c : 0, v[u]);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -33,12 +34,7 @@ void quantize_kernel(const T* __restrict__ x, int64_t rs, uint8_t* __restrict__ 
                 if (r >= rows) break;                                   // (the same for all lanes of a group)
                 int sb;
                 const i32x2 w = b8_quantize8<LANES>(v[u], fmt, sb);
-                uint8_t* q = codes + r * ldc + c;
-                if (wide && c + 8 <= pad) *(i32x2*)q = w;
-                else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) if (c + i < pad) q[i] = (uint8_t)((uint32_t)w[i >> 2] >> 8 * (i & 3));
-                }
+                b8_store_codes(codes + r * ldc + c, pad - c, w);
                 if (lane == 0) scales[r * lds + kb] = (uint8_t)sb;
             }
         }
@@ -48,20 +44,45 @@ void quantize_kernel(const T* __restrict__ x, int64_t rs, uint8_t* __restrict__ 
 // ------------------------------------------------------------------------------------------------ quantize, columns contiguous
 // x[r][c] at x + r + c * cs (a transposed view).  Workgroup = 64 rows x one block of 128 columns: lanes run along the rows
 // (contiguous in memory), a thread holds 32 columns of its row, the four threads of a row meet in LDS for the maximum and
-// write 32 code bytes each.
+// write 32 code bytes each.  Values of 16 bits come through LDS, 8 rows of a column in one load (16384 x 2048 bf16: 55 us with a
+// load for each, 22.6 so; float32 28.0, without).
 template <class T>
 __global__ __launch_bounds__(256)
 void quantize_t_kernel(const T* __restrict__ x, int64_t cs, uint8_t* __restrict__ codes, int64_t ldc, uint8_t* __restrict__ scales,
-                       int64_t lds, int64_t rows, int cols, int pad, int wide, int fmt)
+                       int64_t lds, int64_t rows, int cols, int pad, int fmt)
 {
+    constexpr bool STAGE = sizeof(T) == 2;
+    constexpr int PITCH = 72;                                            // rows of a column in LDS: 16-byte aligned, neighbours 36 banks apart
     __shared__ uint32_t red[4][64];
+    __shared__ __attribute__((aligned(16))) T tile[STAGE ? 128 * PITCH : 1];
     const int lr = threadIdx.x & 63, g = threadIdx.x >> 6;
-    const int64_t r = (int64_t)blockIdx.x * 64 + lr;
+    const int64_t first = (int64_t)blockIdx.x * 64, r = first + lr;
     const int kb = blockIdx.y, c0 = kb * B8_BLK + g * 32;
     const int64_t rc = r < rows ? r : rows - 1;
     float v[32];
+    if constexpr (STAGE) {
+        const int p = (threadIdx.x & 7) * 8, left = (int)min((int64_t)64, rows - first) - p;
+        typedef typename B8Vec<T, 8>::type T8;
+        T8 w[4];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = c0 + i < cols ? (float)x[rc + (int64_t)(c0 + i) * cs] : 0.f;
+        for (int i = 0; i < 4; ++i) {
+            const int c = min(kb * B8_BLK + (int)(threadIdx.x >> 3) + 32 * i, cols - 1);
+            const T* s = x + first + p + (int64_t)c * cs;
+            if (left >= 8) w[i] = *(const T8*)s;
+            else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[i][e] = e < left ? s[e] : (T)0.f;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *(typename B8Vec<T, 8>::Aligned*)(tile + ((threadIdx.x >> 3) + 32 * i) * PITCH + p) = w[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = c0 + i < cols ? (float)tile[(g * 32 + i) * PITCH + lr] : 0.f;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = c0 + i < cols ? (float)x[rc + (int64_t)(c0 + i) * cs] : 0.f;
+    }
     uint32_t m = 0, any = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) { m = max(m, b8_amax_bits(v + 8 * i)); any = max(any, b8_max_bits(v + 8 * i)); }
@@ -71,30 +92,28 @@ void quantize_t_kernel(const T* __restrict__ x, int64_t cs, uint8_t* __restrict_
     if (r >= rows) return;
     const int sb = b8_scale_byte(m, fmt);
     const float inv = b8_inv_scale(sb);
+    typedef i32x4 i32x4_any __attribute__((aligned(1)));
     uint8_t* q = codes + r * ldc + c0;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-        i32x4 w;
+        i32x2 w[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             float* u = v + 16 * j + 8 * h;
 #pragma unroll
             for (int i = 0; i < 8; ++i) u[i] *= inv;
-            const i32x2 e = b8_encode8(u, fmt, any >= B8_INF);
-            w[2 * h] = e[0]; w[2 * h + 1] = e[1];
+            w[h] = b8_encode8(u, fmt, any >= B8_INF);
         }
-        if (wide && c0 + 16 * j + 16 <= pad) *(i32x4*)(q + 16 * j) = w;
-        else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) if (c0 + 16 * j + i < pad) q[16 * j + i] = (uint8_t)((uint32_t)w[i >> 2] >> 8 * (i & 3));
-        }
+        if (c0 + 16 * j + 16 <= pad) *(i32x4_any*)(q + 16 * j) = i32x4{w[0][0], w[0][1], w[1][0], w[1][1]};
+        else { b8_store_codes(q + 16 * j, pad - (c0 + 16 * j), w[0]); b8_store_codes(q + 16 * j + 8, pad - (c0 + 16 * j + 8), w[1]); }
     }
     if (g == 0) scales[r * lds + kb] = (uint8_t)sb;
 }
 
 // ------------------------------------------------------------------------------------------------ restore
-// out = code * 2^e (* chan[c]): a thread takes 8 columns, tpr (a power of two) threads along a row; four rows in flight.
-template <class T, bool VEC>
+// out = code * 2^e (* chan[c]): a thread takes 8 columns, tpr (a power of two) threads along a row; four rows in flight; few, long
+// rows are shared as above.  16384 x 2048: bf16 17.7 us, 5.7 TB/s, float32 29.9 us, 5.6 TB/s.
+template <class T>
 __global__ __launch_bounds__(256)
 void dequantize_kernel(const uint8_t* __restrict__ codes, int64_t ldc, const uint8_t* __restrict__ scales, int64_t lds, int fmt,
                        const float* __restrict__ chan, T* __restrict__ out, int64_t ldo, int64_t rows, int cols, int tpr_log)
@@ -103,13 +122,13 @@ void dequantize_kernel(const uint8_t* __restrict__ codes, int64_t ldc, const uin
     const int rpb = 256 >> tpr_log;
     const int64_t step = (int64_t)gridDim.x * rpb;
     for (int64_t r0 = (int64_t)blockIdx.x * rpb + (threadIdx.x >> tpr_log); r0 < rows; r0 += U * step) {
-        for (int c = (threadIdx.x & ((1 << tpr_log) - 1)) * 8; c < cols; c += 8 << tpr_log) {
+        for (int c = ((threadIdx.x & ((1 << tpr_log) - 1)) + (blockIdx.y << tpr_log)) * 8; c < cols; c += 8 * gridDim.y << tpr_log) {
             i32x2 w[U];
             int sb[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int64_t r = r0 + u * step;
-                w[u] = b8_load_codes<VEC>(codes + r * ldc + c, r < rows ? cols - c : 0);
+                w[u] = b8_load_codes(codes + r * ldc + c, r < rows ? cols - c : 0);
                 sb[u] = r < rows ? scales[r * lds + c / B8_BLK] : 0;
             }
             float f[8];
@@ -125,7 +144,7 @@ void dequantize_kernel(const uint8_t* __restrict__ codes, int64_t ldc, const uin
                 const float s = b8_scale(sb[u]);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) { v[i] *= s; if (chan) v[i] *= f[i]; }
-                b8_store8<T, VEC>(out + r * ldo + c, cols - c, v);
+                b8_store8<T>(out + r * ldo + c, cols - c, v);
             }
         }
     }
@@ -149,8 +168,8 @@ void an_relu8_fwd_kernel(const float* __restrict__ x, float* __restrict__ y, uin
     const int c = gk * B8_BLK + lane * 8;
     const bool here = c < C;                                             // (C is a multiple of 8)
     float b[8], s[8];
-    b8_load8<float, false>(bias + (here ? c : 0), 8, b);
-    b8_load8<float, false>(logs + (here ? c : 0), 8, s);
+    b8_load8<float>(bias + (here ? c : 0), 8, b);
+    b8_load8<float>(logs + (here ? c : 0), 8, s);
 #pragma unroll
     for (int i = 0; i < 8; ++i) s[i] = expf(s[i]);
     for (uint32_t p = blockIdx.x * ppb + gr; p < npx; p += gridDim.x * ppb) {
@@ -158,7 +177,7 @@ void an_relu8_fwd_kernel(const float* __restrict__ x, float* __restrict__ y, uin
         const bool inside = px > 0 && px < (uint32_t)w2 - 1 && py > 0 && py < (uint32_t)h2 - 1;
         const int64_t o = (int64_t)p * C + c;
         float v[8];
-        b8_load8<float, true>(x + o, here && inside ? 8 : 0, v);
+        b8_load8<float>(x + o, here && inside ? 8 : 0, v);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float t = v[i] + b[i];
@@ -172,7 +191,7 @@ void an_relu8_fwd_kernel(const float* __restrict__ x, float* __restrict__ y, uin
 #pragma unroll
         for (int i = 0; i < 8; ++i) if (v[i] > 0.f && ((uint32_t)w[i >> 2] >> 8 * (i & 3) & 0xffu) == 0u) w[i >> 2] |= 1 << 8 * (i & 3);
         if (here) {
-            b8_store8<float, true>(y + o, 8, r);
+            b8_store8<float>(y + o, 8, r);
             *(i32x2*)(codes + o) = w;
             if (lane == 0) scales[(int64_t)p * KB + gk] = (uint8_t)sb;
         }
@@ -199,7 +218,7 @@ void an_relu8_bwd_kernel(const float* __restrict__ g, const uint8_t* __restrict_
             const bool inside = px > 0 && px < (uint32_t)w2 - 1 && py > 0 && py < (uint32_t)h2 - 1;
             const int64_t o = (int64_t)p * C + c;
             float d[8], v[8], r[8];
-            b8_load8<float, true>(g + o, inside ? 8 : 0, d);
+            b8_load8<float>(g + o, inside ? 8 : 0, d);
             const i32x2 w = *(const i32x2*)(codes + o);
             const float sc = b8_scale(scales[(int64_t)p * KB + c / B8_BLK]);
             b8_decode4(w[0], IFL_Q_E4M3, v);
@@ -211,7 +230,7 @@ void an_relu8_bwd_kernel(const float* __restrict__ g, const uint8_t* __restrict_
                 sg[i] += e;
                 sv[i] = fmaf(e, v[i] * sc, sv[i]);
             }
-            b8_store8<float, true>(dx + o, 8, r);
+            b8_store8<float>(dx + o, 8, r);
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) { sm[(pl * 2) * C + c + i] = sg[i]; sm[(pl * 2 + 1) * C + c + i] = sv[i]; }
@@ -242,6 +261,12 @@ void an_relu8_reduce_kernel(const float* __restrict__ part, int nblk, const floa
 int log2_up(int64_t n, int most) { int l = 0; while (l < most && (1 << l) < n) ++l; return l; }
 bool aligned(const void* p, int64_t stride_bytes, int a) { return (uintptr_t)p % a == 0 && stride_bytes % a == 0; }
 
+// how many workgroups share rows that are `passes` passes of a workgroup long: until there are 4096 of them
+unsigned share_rows(int64_t grid, int64_t passes) {
+    const int64_t n = grid >= 4096 ? 1 : 4096 / grid;
+    return (unsigned)(n < passes ? n : passes);
+}
+
 constexpr int AN8_BLOCKS = 1024;                                         // most blocks (partial sums) of the backward pass
 
 }  // namespace
@@ -259,18 +284,15 @@ extern "C" int ifl_block8_quantize(const void* x, int xtype, int64_t row_stride,
     IFL_CHECK_ARG(col_stride == 1 || row_stride == 1 || rows == 1, IFL_EINVAL, "block8_quantize: strides %lld, %lld: one of them has to be 1", (long long)row_stride, (long long)col_stride);
     const int64_t pad64 = (cols + 15) / 16 * 16;
     const int pad = (int)(pad64 < ldc ? pad64 : ldc);
-    const int es = b8_size(xtype);
     hipStream_t st = (hipStream_t)stream;
     if (col_stride != 1) {
         const int64_t gx = (rows + 63) / 64;
         IFL_CHECK_ARG(gx <= 0x7fffffff && KB <= 65535, IFL_ENOTSUP, "block8_quantize: transposed %lld x %lld", (long long)rows, (long long)cols);
         B8_DISPATCH(xtype, hipLaunchKernelGGL(HIP_KERNEL_NAME(quantize_t_kernel<T>), dim3((unsigned)gx, KB), dim3(256), 0, st, (const T*)x, col_stride, codes, ldc, scales,
-                                              lds, rows, (int)cols, pad, (int)aligned(codes, ldc, 16), fmt));
+                                              lds, rows, (int)cols, pad, fmt));
         IFL_LAUNCH_CHECK();
         return 0;
     }
-    const bool vec = aligned(x, row_stride * es, 16);
-    const int wide = aligned(codes, ldc, 8);
     const int lanes = cols <= 32 ? 4 : cols <= 64 ? 8 : 16;
     const int gpb_log = lanes == 4 ? 6 : lanes == 8 ? 5 : 4;
     const int kgl = log2_up(KB, gpb_log);
@@ -278,9 +300,9 @@ extern "C" int ifl_block8_quantize(const void* x, int xtype, int64_t row_stride,
     int64_t grid = (rows + 4 * rpb - 1) / (4 * rpb);
     if (grid < 1024) grid = (rows + rpb - 1) / rpb < 1024 ? (rows + rpb - 1) / rpb : 1024;      // few rows: spread them before stacking them
     if (grid > 65536) grid = 65536;
-#define Q8_GO(L, V) hipLaunchKernelGGL(HIP_KERNEL_NAME(quantize_kernel<T, L, V>), dim3((unsigned)grid), dim3(256), 0, st, (const T*)x, row_stride, codes, ldc, scales, lds, rows, (int)cols, pad, wide, kgl, fmt)
-#define Q8_LANES(V) do { if (lanes == 4) Q8_GO(4, V); else if (lanes == 8) Q8_GO(8, V); else Q8_GO(16, V); } while (0)
-    B8_DISPATCH(xtype, if (vec) Q8_LANES(true); else Q8_LANES(false));
+    const dim3 g2((unsigned)grid, share_rows(grid, (KB + (1 << kgl) - 1) >> kgl));
+#define Q8_GO(L) hipLaunchKernelGGL(HIP_KERNEL_NAME(quantize_kernel<T, L>), g2, dim3(256), 0, st, (const T*)x, row_stride, codes, ldc, scales, lds, rows, (int)cols, pad, kgl, fmt)
+    B8_DISPATCH(xtype, if (lanes == 4) Q8_GO(4); else if (lanes == 8) Q8_GO(8); else Q8_GO(16));
     IFL_LAUNCH_CHECK();
     return 0;
 }
@@ -294,14 +316,13 @@ extern "C" int ifl_block8_dequantize(const uint8_t* codes, int64_t ldc, const ui
     if (rows == 0) return 0;
     IFL_CHECK_ARG(codes && scales && out, IFL_EINVAL, "block8_dequantize: null pointer");
     IFL_CHECK_ARG(ldc >= cols && ldo >= cols && lds >= ifl_cdiv((int)cols, B8_BLK), IFL_EINVAL, "block8_dequantize: row strides");
-    const bool vec = aligned(codes, ldc, 8) && aligned(out, ldo * b8_size(otype), 16);
     const int tl = log2_up((cols + 7) / 8, 8);
     const int64_t rpb = 256 >> tl;
     int64_t grid = (rows + 4 * rpb - 1) / (4 * rpb);
     if (grid < 1024) grid = (rows + rpb - 1) / rpb < 1024 ? (rows + rpb - 1) / rpb : 1024;
     if (grid > 65536) grid = 65536;
-#define D8_GO(V) hipLaunchKernelGGL(HIP_KERNEL_NAME(dequantize_kernel<T, V>), dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, codes, ldc, scales, lds, fmt, chan, (T*)out, ldo, rows, (int)cols, tl)
-    B8_DISPATCH(otype, if (vec) D8_GO(true); else D8_GO(false));
+    const dim3 g2((unsigned)grid, share_rows(grid, (cols + (8 << tl) - 1) >> (3 + tl)));
+    B8_DISPATCH(otype, hipLaunchKernelGGL(HIP_KERNEL_NAME(dequantize_kernel<T>), g2, dim3(256), 0, (hipStream_t)stream, codes, ldc, scales, lds, fmt, chan, (T*)out, ldo, rows, (int)cols, tl));
     IFL_LAUNCH_CHECK();
     return 0;
 }

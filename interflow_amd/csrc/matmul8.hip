@@ -63,12 +63,10 @@ __device__ __forceinline__ i32x8 mm8_join(i32x4 a, i32x4 b) {
     return r;
 }
 
-// A wave's results: m0 the lane's first row, nw its first column, bias its columns' (in LDS).  wide: 16-byte
-// stores fit.
+// A wave's results: m0 the lane's first row, nw its first column, bias its columns' (in LDS).
 template <class T, int NF, int MF, int G>
-__device__ __forceinline__ void mm8_results(const MM8& q, const f32x4 (&acc)[NF][MF], int64_t m0, int64_t nw, const float* bias, bool wide) {
+__device__ __forceinline__ void mm8_results(const MM8& q, const f32x4 (&acc)[NF][MF], int64_t m0, int64_t nw, const float* bias) {
     constexpr int V = 4 * G * sizeof(T) >= 16 ? 16 / sizeof(T) : 4 * G;
-    typedef T TV __attribute__((ext_vector_type(V)));
     T* p = (T*)q.out + m0 * q.ldo + nw;
     int rows = (int)(q.M - m0), cols = (int)(q.N - nw);
 #pragma unroll
@@ -79,13 +77,13 @@ __device__ __forceinline__ void mm8_results(const MM8& q, const f32x4 (&acc)[NF]
 #pragma unroll
             for (int i = 0; i < 4 * G; ++i) v[i] = acc[h * G + i / 4][j][i % 4] + bias[16 * G * h + i];
             asm volatile("" : "+v"(cols));                               // (compared here: there are no registers for what is made ahead)
-            if (wide && 16 * j < rows && 16 * G * h + 4 * G <= cols) {
+            if (16 * j < rows && 16 * G * h + 4 * G <= cols) {
 #pragma unroll
                 for (int i = 0; i < 4 * G / V; ++i) {
-                    TV t;
+                    typename B8Vec<T, V>::Aligned t;
 #pragma unroll
                     for (int e = 0; e < V; ++e) t[e] = (T)v[i * V + e];
-                    *(TV*)(p + 16 * G * h + V * i) = t;
+                    *(typename B8Vec<T, V>::type*)(p + 16 * G * h + V * i) = t;
                 }
             } else if (16 * j < rows) {
 #pragma unroll
@@ -306,10 +304,9 @@ void mm8_tile_kernel(MM8 q)
     if constexpr (SPLIT) mm8_part<NF, MF, G>(q, acc, mw, nw);
     else {
         const float* bs = bias + wn * NF * 16 + 4 * G * g;
-        const bool wide = ((uintptr_t)q.out | (uint64_t)(q.ldo * (EXACT ? 4 : 2))) % 16 == 0;
-        if constexpr (EXACT) mm8_results<float, NF, MF, G>(q, acc, mw, nw, bs, wide);
-        else if (q.otype == IFL_T_BF16) mm8_results<__bf16, NF, MF, G>(q, acc, mw, nw, bs, wide);
-        else mm8_results<_Float16, NF, MF, G>(q, acc, mw, nw, bs, wide);
+        if constexpr (EXACT) mm8_results<float, NF, MF, G>(q, acc, mw, nw, bs);
+        else if (q.otype == IFL_T_BF16) mm8_results<__bf16, NF, MF, G>(q, acc, mw, nw, bs);
+        else mm8_results<_Float16, NF, MF, G>(q, acc, mw, nw, bs);
     }
 }
 
@@ -363,7 +360,7 @@ void mm8_skinny_kernel(MM8 q)
         for (int i = threadIdx.x >> 4; i < (int)q.M * KB; i += 64 * SK_WAVES / 16) {
             const int m = i / KB, kb = i - m * KB, c = kb * B8_BLK + l16 * 8;
             float v[8];
-            b8_load8<TX, false>((const TX*)q.x + m * q.ldx + c, q.K - c, v);
+            b8_load8<TX>((const TX*)q.x + m * q.ldx + c, q.K - c, v);
             int s;
             *(i32x2*)(own + m * KP + c) = b8_quantize8<16>(v, IFL_Q_E4M3, s);
             if (l16 == 0) own[(int)q.M * KP + i] = (uint8_t)s;

@@ -50,12 +50,11 @@ __device__ __forceinline__ uint32_t wg8_term(float& x) {
 
 template <class TW>
 __device__ __forceinline__ void wg8_store4(TW* d, int left, const float v[4]) {
-    typedef TW TW4 __attribute__((ext_vector_type(4)));
-    if (left >= 4 && (uintptr_t)d % sizeof(TW4) == 0) {
-        TW4 w;
+    if (left >= 4) {
+        typename B8Vec<TW, 4>::Aligned w;
 #pragma unroll
         for (int e = 0; e < 4; ++e) w[e] = (TW)v[e];
-        *(TW4*)d = w;
+        *(typename B8Vec<TW, 4>::type*)d = w;
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e) if (e < left) d[e] = (TW)v[e];
@@ -92,9 +91,9 @@ __device__ __forceinline__ int wg8_row(int gg, int e) { return (gg >> 2) * 32 + 
 
 // Workgroups 0 .. x_blocks - 1 restore codes.  The others take up to 256 columns of cs_rows rows of dy, with column sums on the
 // way that are joined in LDS in a fixed order, and dy's terms, if the product does not read it in place.  QUANT: they also put dy
-// into 8-bit blocks (for the layer's other product), which saves a pass over it (16384 x 2048, both operands, bf16: @@ us
+// into 8-bit blocks (for the layer's other product), which saves a pass over it (16384 x 2048, both operands, bf16: 43 us
 // instead of 25 + 33).
-template <class T, int NP, bool VEC, bool QUANT>
+template <class T, int NP, bool QUANT>
 __global__ __launch_bounds__(256, NP > 1 ? 2 : 3)
 void wgrad8_prepare_kernel(WG8 q)
 {
@@ -144,9 +143,9 @@ void wgrad8_prepare_kernel(WG8 q)
         int row = wg8_row(rl, 0), cc = c;
         asm volatile("" : "+v"(row), "+v"(cc));                          // (addresses are made here, not kept)
         auto at = [&](int e) { return rows + (int64_t)min(row + (e & 3) + 16 * (e >> 2), left > 0 ? left - 1 : (int)(q.M - 1 - row0)) * q.ldy; };
-        if (VEC && cc + 8 <= q.N) {
+        if (cc + 8 <= q.N) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) b8_load8<T, true>(at(e) + cc, 8, v[e]);
+            for (int e = 0; e < 8; ++e) b8_load8<T>(at(e) + cc, 8, v[e]);
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
@@ -545,10 +544,9 @@ int b8_wgrad(int todo, const B8Quant* quant, const void* dy, int dytype, int64_t
         }
         if (quant) { q.gc = quant->codes; q.gs = quant->scales; q.ldgc = quant->ldc; q.ldgs = quant->lds; q.gfmt = quant->fmt; }
         const dim3 pg((unsigned)(q.x_blocks + y_blocks));
-#define WG8_P2(T, NP, V, Q) hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_prepare_kernel<T, NP, V, Q>), pg, dim3(256), 0, st, q)
 #define WG8_P(T, NP) do { \
-            if (wide && quant) WG8_P2(T, NP, true, true); else if (wide) WG8_P2(T, NP, true, false); \
-            else if (quant) WG8_P2(T, NP, false, true); else WG8_P2(T, NP, false, false); \
+            if (quant) hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_prepare_kernel<T, NP, true>), pg, dim3(256), 0, st, q); \
+            else hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_prepare_kernel<T, NP, false>), pg, dim3(256), 0, st, q); \
         } while (0)
         if (dytype == IFL_T_F32) WG8_P(float, 3); else if (dytype == IFL_T_F16) WG8_P(_Float16, 2); else WG8_P(__bf16, 1);
         IFL_LAUNCH_CHECK();

@@ -330,8 +330,9 @@ class _AnRelu8(torch.autograd.Function):
         B, hp, wp_, C = shape
         gy = _aligned(hip._dev_f32(gy, "an_relu8 gradient"))
         dx = torch.empty_like(gy)
-        db, dl = torch.empty(bshape, dtype=torch.float32, device=gy.device), torch.empty(lshape, dtype=torch.float32, device=gy.device)
-        part = torch.empty((block8._size("ifl_an_relu8_blocks", B, hp - 2, wp_ - 2, C) * 2 * C,), dtype=torch.float32, device=gy.device)
+        dl = torch.empty_like(l)                                         # (float32, contiguous, of logs' shape)
+        db = torch.empty_like(l) if bshape == lshape else gy.new_empty(bshape)
+        part = gy.new_empty((block8._size("ifl_an_relu8_blocks", B, hp - 2, wp_ - 2, C) * 2 * C,))
         p = raw.data_ptr()
         block8._call("ifl_an_relu8_bwd", gy.get_device(), gy.data_ptr(), p, p + gy.numel(), l.data_ptr(), dx.data_ptr(), db.data_ptr(), dl.data_ptr(),
                      part.data_ptr(), B, hp - 2, wp_ - 2, C)
