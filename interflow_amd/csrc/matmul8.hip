@@ -31,15 +31,13 @@ __device__ __forceinline__ float mm8_bias(const MM8& q, int64_t n) {
     return !q.bias ? 0.f : q.btype == IFL_T_F32 ? ((const float*)q.bias)[n] : q.btype == IFL_T_BF16 ? (float)((const __bf16*)q.bias)[n] : (float)((const _Float16*)q.bias)[n];
 }
 
-// 16 bytes of a row from k on, zero where k >= K (rows are whole 16 bytes in memory)
-__device__ __forceinline__ i32x4 mm8_load16(const uint8_t* __restrict__ row, int k, int K) {
-    i32x4 r = *(const i32x4*)(row + (k < K ? k : 0));
-    if (k + 16 > K) {
+// 16 bytes of a row from k on (rows are whole 16 bytes in memory), and zeros in them where k >= K
+__device__ __forceinline__ i32x4 mm8_load16(const uint8_t* __restrict__ row, int k, int K) { return *(const i32x4*)(row + (k < K ? k : 0)); }
+__device__ __forceinline__ i32x4 mm8_cut16(i32x4 r, int k, int K) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int left = K - k - 4 * i;
-            r[i] = left >= 4 ? r[i] : left <= 0 ? 0 : (int)((uint32_t)r[i] & ((1u << 8 * left) - 1));
-        }
+    for (int i = 0; i < 4; ++i) {
+        const int left = K - k - 4 * i;
+        r[i] = left >= 4 ? r[i] : left <= 0 ? 0 : (int)((uint32_t)r[i] & ((1u << 8 * left) - 1));
     }
     return r;
 }
@@ -192,7 +190,8 @@ void mm8_tile_kernel(MM8 q)
             const bool nside = (i * NW * 64) >> 3 < TN;
             int ch;
             const uint32_t o = piece(i, nside, ch);
-            *(i32x4*)(buf + ((i * NW + wave) * 64 + lane) * 16) = mm8_load16((nside ? bb : ab) + o, ks * B8_BLK + ch * 16, q.K);
+            const int k = ks * B8_BLK + ch * 16;
+            *(i32x4*)(buf + ((i * NW + wave) * 64 + lane) * 16) = mm8_cut16(mm8_load16((nside ? bb : ab) + o, k, q.K), k, q.K);
         }
     };
 
@@ -324,10 +323,10 @@ void mm8_join_kernel(MM8 q)
 }
 
 // ------------------------------------------------------------------------------------------------ few rows
-// M <= 16 MF: bound by reading B once, so nothing is staged.  Workgroup = 16 n; its 8 waves take every eighth step of K, four of
-// their steps' loads in flight at a time, and meet in LDS.  OWN: the m side is not quantized yet: each workgroup quantizes all of
-// it (M K values, 32 a thread at most) into LDS, which saves a launch.
-constexpr int SK_WAVES = 8, SK_OWN = 16384;                              // OWN: most bytes of codes in LDS
+// M <= 16 MF: bound by reading B once, so nothing is staged.  Workgroup = 16 n; its 16 waves take every sixteenth step of K (8 waves were
+// 5 to 10% slower), four (M > 16: two) of their steps' loads in flight at a time, and meet in LDS.  OWN: the m side is not quantized yet: each
+// workgroup quantizes all of it (M K values) into LDS, which saves a launch.
+constexpr int SK_WAVES = 16;
 
 template <int MF, int FA, int FB, bool EXACT, bool OWN, class TX>
 __global__ __launch_bounds__(64 * SK_WAVES)
@@ -335,22 +334,40 @@ void mm8_skinny_kernel(MM8 q)
 {
     __shared__ float red[SK_WAVES][16 * 16 * MF];
     extern __shared__ __attribute__((aligned(16))) uint8_t own[];        // [M][KP] codes, then [M][KB] scale bytes
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, g = lane >> 4;
     const int KB = (q.K + B8_BLK - 1) / B8_BLK, KP = KB * B8_BLK;
     const int64_t n0 = (int64_t)blockIdx.x * 16;
     const int64_t n = min(n0 + r16, q.N - 1);
     const uint8_t *pb = q.b + n * q.ldb, *psb = q.sb + n * q.lsb;
-    constexpr int U = 4;
-    i32x8 b[U];
-    int cb[U];
+    // what this lane multiplies of the m side (OWN: of its copy in LDS)
+    const uint8_t *pa[MF], *psa[MF];
+#pragma unroll
+    for (int j = 0; j < MF; ++j) {
+        const int m = min(16 * j + r16, (int)q.M - 1);
+        pa[j] = OWN ? own + m * KP : q.a + m * q.lda;
+        psa[j] = OWN ? own + (int)q.M * KP + m * KB : q.sa + m * q.lsa;
+    }
+    constexpr int U = OWN || MF == 1 ? 4 : 2;
+    // Of a step's 128 bytes a lane takes 16 from 16 g and 16 from 64 + 16 g; in odd rows the second ones first.  With the same half of
+    // every row in one load they kept each other waiting (1 x 8192 x 2048: 8.2 us, so 6.8; 32 x 4096 x 4096: 10.5 and 7.9).
+    const int odd = (r16 & 1) * 64;
+    i32x4 b[U][2], a[U][MF][2];
+    int cb[U], ca[U][MF];
     auto load = [&](int ks0) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int ks = ks0 + u * SK_WAVES;
-            if (ks < KB) {
-                const int k = ks * B8_BLK + 16 * g;
-                b[u] = mm8_join(mm8_load16(pb, k, q.K), mm8_load16(pb, k + 64, q.K));
-                cb[u] = psb[ks];
+            const int ks = ks0 + u * SK_WAVES, k = ks * B8_BLK + 16 * g;
+            if (ks >= KB) break;
+            b[u][0] = mm8_load16(pb, k + odd, q.K);
+            b[u][1] = mm8_load16(pb, k + (odd ^ 64), q.K);
+            cb[u] = psb[ks];
+            if constexpr (!OWN) {
+#pragma unroll
+                for (int j = 0; j < MF; ++j) {
+                    a[u][j][0] = mm8_load16(pa[j], k + odd, q.K);
+                    a[u][j][1] = mm8_load16(pa[j], k + (odd ^ 64), q.K);
+                    ca[u][j] = psa[j][ks];
+                }
             }
         }
     };
@@ -372,23 +389,21 @@ void mm8_skinny_kernel(MM8 q)
         if (ks0 != wave) load(ks0);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int ks = ks0 + u * SK_WAVES;
+            const int ks = ks0 + u * SK_WAVES, k = ks * B8_BLK + 16 * g;
             if (ks >= KB) break;
-            const int k = ks * B8_BLK + 16 * g;
+            const bool cut = (ks + 1) * B8_BLK > q.K;                    // a step that K does not fill
+            auto order = [&](i32x4 (&w)[2]) { const i32x4 t = odd ? w[1] : w[0]; w[1] = odd ? w[0] : w[1]; w[0] = t; };
+            order(b[u]);
+            if (cut) { b[u][0] = mm8_cut16(b[u][0], k, q.K); b[u][1] = mm8_cut16(b[u][1], k + 64, q.K); }
 #pragma unroll
             for (int j = 0; j < MF; ++j) {
-                const int m = min(16 * j + r16, (int)q.M - 1);
-                i32x8 a;
-                int ca;
                 if constexpr (OWN) {
-                    a = mm8_join(*(const i32x4*)(own + m * KP + k), *(const i32x4*)(own + m * KP + k + 64));
-                    ca = own[(int)q.M * KP + m * KB + ks];
-                } else {
-                    const uint8_t* pa = q.a + m * q.lda;
-                    a = mm8_join(mm8_load16(pa, k, q.K), mm8_load16(pa, k + 64, q.K));
-                    ca = q.sa[m * q.lsa + ks];
-                }
-                acc[j] = mm8_mfma<FA, FB, EXACT>(b[u], a, acc[j], cb[u], ca);
+                    a[u][j][0] = *(const i32x4*)(pa[j] + k);
+                    a[u][j][1] = *(const i32x4*)(pa[j] + k + 64);
+                    ca[u][j] = psa[j][ks];
+                } else order(a[u][j]);
+                if (!OWN && cut) { a[u][j][0] = mm8_cut16(a[u][j][0], k, q.K); a[u][j][1] = mm8_cut16(a[u][j][1], k + 64, q.K); }
+                acc[j] = mm8_mfma<FA, FB, EXACT>(mm8_join(b[u][0], b[u][1]), mm8_join(a[u][j][0], a[u][j][1]), acc[j], cb[u], ca[u][j]);
             }
         }
     }
@@ -415,6 +430,9 @@ void mm8_skinny_kernel(MM8 q)
 // ------------------------------------------------------------------------------------------------ which of them
 // Few rows: the skinny kernel.  Else the largest tile that still gives the 256 CUs work (measured: DESIGN), float32 results at most
 // 128 (their fragments are held as bf16); a product of few tiles and a long K is split along K.
+// The skinny kernel quantizes the m side itself where that is at most 32768 values: then it is the faster way, in a graph (1 x 2048 x
+// 2048: 3.5 us, 6.9 with a launch for it; 16 x 2048 x 2048: 6.2 and 7.3) and out of one (9 and 13.6).
+bool mm8_own(int64_t M, int64_t K) { return M <= 16 && M * K <= 32768; }
 struct Plan { int kind, tile, split, ksteps; };
 Plan mm8_plan(int64_t M, int64_t N, int64_t K, int otype)
 {
@@ -518,7 +536,7 @@ extern "C" int ifl_block8_matmul(const uint8_t* a, int64_t lda, const uint8_t* s
 extern "C" int64_t ifl_block8_linear_scratch_bytes(int64_t M, int64_t N, int64_t K, int otype)
 {
     if (M < 1 || N < 1 || K < 1) return 0;
-    if (M * K <= SK_OWN / 2 && M <= 16) return 0;
+    if (mm8_own(M, K)) return 0;
     return M * ((K + 15) / 16 * 16) + M * ((K + 511) / 512 * 4) + 4 * ifl_block8_matmul_scratch_floats(M, N, K, otype) + 16;
 }
 
@@ -531,7 +549,7 @@ extern "C" int ifl_block8_linear(const void* x, int xtype, int64_t ldx, const ui
     if (M == 0) return 0;
     IFL_CHECK_ARG(x && (M == 1 || ldx >= K), IFL_EINVAL, "block8_linear: x");
     hipStream_t st = (hipStream_t)stream;
-    if (M * K <= SK_OWN / 2 && M <= 16) {
+    if (mm8_own(M, K)) {
         MM8 q = {};
         q.b = b; q.sb = sb; q.ldb = ldb; q.lsb = lsb; q.bias = bias; q.btype = btype; q.out = out; q.otype = xtype; q.ldo = ldo;
         q.M = M; q.N = N; q.K = (int)K; q.x = x; q.ldx = ldx;
