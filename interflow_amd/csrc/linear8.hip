@@ -23,8 +23,11 @@ extern "C" int ifl_linear8_fwd(const void* x, int xtype, int64_t x_rs, int64_t x
                                int64_t K, void* stream)
 {
     IFL_CHECK_ARG(sizes_ok(M, N, K), IFL_EINVAL, "linear8_fwd: %lld x %lld x %lld", (long long)M, (long long)N, (long long)K);
+    IFL_CHECK_ARG(b8_type_ok(xtype) && b8_type_ok(wtype) && (!bias || b8_type_ok(btype)), IFL_EINVAL, "linear8_fwd: element types");
     if (M == 0) return 0;
-    IFL_CHECK_ARG(scratch && (uintptr_t)scratch % 16 == 0, IFL_EINVAL, "linear8_fwd: scratch");
+    IFL_CHECK_ARG(x && w && codes && scales && y, IFL_EINVAL, "linear8_fwd: null pointer");
+    IFL_CHECK_ARG(w_rs == 1 || w_cs == 1 || N == 1, IFL_EINVAL, "linear8_fwd: strides of w");
+    IFL_CHECK_ARG(scratch && (uintptr_t)scratch % 16 == 0 && (uintptr_t)codes % 16 == 0 && (uintptr_t)scales % 4 == 0, IFL_EINVAL, "linear8_fwd: alignment of scratch, codes or scales");
     uint8_t* wc = (uint8_t*)scratch;
     uint8_t* ws = wc + up16(N * code_ld(K));
     float* part = (float*)(wc + block_bytes(N, K));
@@ -46,6 +49,10 @@ extern "C" int ifl_linear8_bwd(const void* dy, int xtype, int64_t ldy, const uin
                                int64_t N, int64_t K, void* stream)
 {
     IFL_CHECK_ARG(sizes_ok(M, N, K), IFL_EINVAL, "linear8_bwd: %lld x %lld x %lld", (long long)M, (long long)N, (long long)K);
+    IFL_CHECK_ARG(b8_type_ok(xtype) && b8_type_ok(wtype) && b8_fmt_ok(gfmt) && (!db || b8_type_ok(dbtype)), IFL_EINVAL, "linear8_bwd: types");
+    IFL_CHECK_ARG(M == 0 || (dy && (w || !dx) && ((codes && scales) || !dw)), IFL_EINVAL, "linear8_bwd: null pointer");
+    IFL_CHECK_ARG(M <= 1 || ldy >= N, IFL_EINVAL, "linear8_bwd: rows of dy %lld apart", (long long)ldy);
+    IFL_CHECK_ARG(!dx || w_rs == 1 || w_cs == 1 || K == 1, IFL_EINVAL, "linear8_bwd: strides of w");
     IFL_CHECK_ARG(scratch && (uintptr_t)scratch % 16 == 0, IFL_EINVAL, "linear8_bwd: scratch");
     uint8_t* at = (uint8_t*)scratch;
     const bool sums = dw || db;

@@ -94,6 +94,24 @@ def test_checkpoint_switch():
     ("ifl_block8_wgrad", (16, 0, 8, 16, 64, 16, 1, 0, None, 16, 0, 64, None, 0, None, 4, 8, 64, None)),
     ("ifl_block8_wgrad", (16, 0, 8, 8, 64, 16, 1, 0, None, 16, 0, 64, None, 0, 16, 4, 8, 64, None)),
     ("ifl_block8_wgrad", (16, 0, 8, 16, 72, 16, 1, 0, None, 16, 0, 64, None, 0, 16, 4, 8, 64, None)),
+    ("ifl_block8_linear", (16, 3, 64, 16, 64, 16, 4, 0, None, 0, 16, 8, 16, 1, 8, 64, None)),
+    ("ifl_block8_linear", (16, 0, 64, 16, 64, 16, 4, 2, None, 0, 16, 8, 16, 1, 8, 64, None)),
+    ("ifl_block8_linear", (None, 0, 64, 16, 64, 16, 4, 0, None, 0, 16, 8, 16, 1, 8, 64, None)),
+    ("ifl_block8_linear", (16, 0, 63, 16, 64, 16, 4, 0, None, 0, 16, 8, 16, 2, 8, 64, None)),
+    ("ifl_block8_linear", (16, 0, 64, 16, 64, 16, 4, 0, None, 0, 16, 7, 16, 1, 8, 64, None)),
+    ("ifl_block8_linear", (16, 0, 64, 16, 64, 16, 4, 0, None, 0, 16, 8, None, 17, 8, 64, None)),
+    ("ifl_block8_linear", (16, 0, 64, 8, 64, 16, 4, 0, None, 0, 16, 8, 16, 1, 8, 64, None)),
+    ("ifl_linear8_fwd", (16, 0, 64, 1, 16, 0, 64, 1, None, 0, 16, 16, 16, None, 4, 8, 64, None)),
+    ("ifl_linear8_fwd", (16, 0, 64, 1, 16, 0, 64, 1, None, 0, 16, 16, 16, 8, 4, 8, 64, None)),
+    ("ifl_linear8_fwd", (16, 0, 64, 1, 16, 0, 64, 1, None, 0, 16, 16, 16, 16, 4, 0, 64, None)),
+    ("ifl_linear8_fwd", (16, 3, 64, 1, 16, 0, 64, 1, None, 0, 16, 16, 16, 16, 4, 8, 64, None)),
+    ("ifl_linear8_fwd", (None, 0, 64, 1, 16, 0, 64, 1, None, 0, 16, 16, 16, 16, 4, 8, 64, None)),
+    ("ifl_linear8_bwd", (16, 0, 8, 16, 16, 16, 0, 64, 1, 0, None, 16, None, 0, None, 4, 8, 64, None)),
+    ("ifl_linear8_bwd", (16, 0, 8, 16, 16, 16, 0, 64, 1, 0, None, 16, None, 0, 16, 4, 8, 0, None)),
+    ("ifl_linear8_bwd", (16, 3, 8, 16, 16, 16, 0, 64, 1, 0, None, 16, None, 0, 16, 4, 8, 64, None)),
+    ("ifl_linear8_bwd", (16, 0, 7, 16, 16, 16, 0, 64, 1, 0, None, 16, None, 0, 16, 4, 8, 64, None)),
+    ("ifl_linear8_bwd", (16, 0, 8, 16, 16, 16, 0, 64, 1, 2, 16, None, None, 0, 16, 4, 8, 64, None)),
+    ("ifl_linear8_bwd", (None, 0, 8, 16, 16, 16, 0, 64, 1, 0, None, 16, None, 0, 16, 4, 8, 64, None)),
     ("ifl_an_relu8_fwd", (16, 16, 16, 16, 16, 16, 0, 4, 4, 64, None)),
     ("ifl_an_relu8_fwd", (4, 16, 16, 16, 16, 16, 1, 4, 4, 64, None)),
     ("ifl_an_relu8_bwd", (16, 16, 16, 16, 16, None, 16, 16, 1, 4, 4, 64, None)),

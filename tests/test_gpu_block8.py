@@ -62,6 +62,33 @@ def test_quantize_and_restore_bit_for_bit(rows, cols, fmt, dtype):
 
 
 @pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("rows, cols", [(3, 70001), (1, 300000), (17, 20000)])
+def test_few_long_rows(rows, cols, dtype):
+    """Rows that several workgroups share, as they are and as columns of a transposed matrix."""
+    x = rand(gen(rows), rows, cols, spread=2.0, dtype=DT[dtype])
+    codes, e = R.split(x, "e4m3")
+    for y in (x, x.t().contiguous().t()):
+        q = block8.quantize(y)
+        assert same(q.codes.float().double(), codes) and torch.equal(q.scales.view(torch.uint8).int(), (e + 127).int())
+        assert same(block8.dequantize(q, DT[dtype]), R.of(q).to(DT[dtype]))
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("rows, cols", [(1, 130), (7, 9), (8, 128), (63, 129), (65, 127), (129, 200), (200, 1)])
+def test_quantize_transposed(rows, cols, dtype):
+    """Columns contiguous, columns an odd distance apart, an odd start: values behind the last row and column are NaN."""
+    g = gen(rows + cols)
+    for start, apart in ((0, rows + rows % 2), (1, rows + 3), (5, rows + 8)):
+        store = torch.full((start + cols * apart + 300,), math.nan, dtype=DT[dtype], device="cuda")
+        x = torch.as_strided(store, (rows, cols), (1, apart), start)
+        x.copy_(rand(g, rows, cols, spread=2.0, dtype=DT[dtype]))
+        for fmt in ("e4m3", "e5m2"):
+            q = block8.quantize(x, fmt)
+            codes, e = R.split(x.contiguous(), fmt)
+            assert same(q.codes.float().double(), codes) and torch.equal(q.scales.view(torch.uint8).int(), (e + 127).int()), (start, apart, fmt)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
 def test_quantize_strides(dtype):
     base = rand(gen(3), 300, 417, spread=2.0, dtype=DT[dtype])
     views = {"transposed": base.t(), "columns 1..": base[:, 1:], "every second row": base[::2], "every second column": base[:, ::2],
@@ -245,6 +272,45 @@ def test_weight_grad_strides_and_parts():
     close(block8.weight_grad(ones, q)[0], ones.double().t() @ R.of(q), 121, ones.double().t() @ R.of(q).abs())
 
 
+@pytest.mark.parametrize("M", [1, 2, 31, 32, 33, 63, 64, 65, 95, 96, 127, 129, 192, 1000])
+@pytest.mark.parametrize("dtype", list(DT))
+def test_weight_grad_row_counts(M, dtype):
+    """Rows that fill the product's steps and rows that do not, with NaN behind the last one of both operands and beside the columns;
+    and each of the two gradients alone."""
+    g = gen(50 + M)
+    N, K = 72, 136
+    big = torch.full((M + 70, 96), math.nan, dtype=DT[dtype], device="cuda")
+    big[:M, 16:16 + N] = rand(g, M, N, dtype=DT[dtype])
+    dy = big[:M, 16:16 + N]
+    x = torch.full((M + 70, K), math.nan, device="cuda")
+    x[:M] = rand(g, M, K, spread=1.0)
+    all_rows = block8.quantize(x)
+    q = block8.Block8(all_rows.codes[:M], all_rows.scales[:M])
+    v = R.of(q)
+    dw, db = block8.weight_grad(dy, q, bias_dtype=torch.float32)
+    close(dw, dy.double().t() @ v, M + 1, dy.double().abs().t() @ v.abs(), M)
+    close(db, dy.double().sum(0), M, dy.double().abs().sum(0), M)
+    assert torch.equal(block8.weight_grad(dy, q)[0], dw)
+    assert torch.equal(block8.weight_grad(dy, q, bias_dtype=torch.float32, weight=False)[1], db)
+    packed = dy.contiguous()                                                  # (rows 144 bytes apart instead of 192)
+    assert torch.equal(block8.weight_grad(packed, q)[0], dw)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+def test_weight_grad_of_tiny_values(dtype):
+    """Operands become bf16 terms, whose smallest step is 2^-133: a checkpoint's value, rounded to one, is off by at most half a step,
+    a float32 gradient, cut off after its third, by less than a whole one."""
+    g = gen(51)
+    M, N, K = 200, 40, 70
+    for sy, sx in ((-10 if dtype == "f16" else -120, 60), (5 if dtype == "f16" else 60, -128)):
+        dy, q = (rand(g, M, N) * 2.0 ** sy).to(DT[dtype]), block8.quantize(rand(g, M, K) * 2.0 ** sx)
+        v, d = R.of(q), dy.double()
+        got = block8.weight_grad(dy, q)[0].double()
+        mag = d.abs().t() @ v.abs()
+        step = 2.0 ** -134 * d.abs().sum(0)[:, None] + 2.0 ** -133 * v.abs().sum(0)[None, :]
+        assert bool(((got - d.t() @ v).abs() <= (M + 2) * 2.0 ** -23 * mag + step + 2.0 ** -149).all()), (sy, sx)
+
+
 # ------------------------------------------------------------------------------------------------ the linear layer
 @pytest.mark.parametrize("shape, N", [((1, 512), 256), ((3, 40), 7), ((2, 5, 200), 64), ((40, 1000), 130), ((300,), 20), ((260, 384), 300)])
 @pytest.mark.parametrize("dtype", list(DT))
@@ -264,6 +330,18 @@ def test_linear_is_quantize_and_matmul(rows):
     g = gen(rows)
     x, w = rand(g, rows, 1000, spread=1.0, dtype=torch.bfloat16), block8.quantize(rand(g, 333, 1000))
     assert torch.equal(block8.linear(x, w), block8.matmul(block8.quantize(x), w, dtype=torch.bfloat16))
+
+
+@pytest.mark.parametrize("rows, K, N", [(16, 2048, 100), (16, 2049, 100), (1, 32768, 40), (1, 32769, 40), (5, 6553, 33), (3, 16, 1), (16, 8, 17)])
+@pytest.mark.parametrize("dtype", list(DT))
+def test_linear_of_few_rows(rows, K, N, dtype):
+    """On both sides of the size up to which one launch does it all: the same result as quantizing and multiplying."""
+    g = gen(rows + K)
+    x, w, bias = rand(g, rows, K, spread=1.0, dtype=DT[dtype]), block8.quantize(rand(g, N, K)), rand(g, N)
+    y = block8.linear(x, w, bias)
+    assert same(y, block8.matmul(block8.quantize(x), w, bias, dtype=DT[dtype]))
+    v, u = R.values(x), R.of(w)
+    close(y, v @ u.t() + bias.double(), K + 1, v.abs() @ u.abs().t() + bias.double().abs(), (rows, K, N), product8=True)
 
 
 @pytest.mark.parametrize("shape, N, bias", [((1, 64), 16, True), ((17, 33), 9, False), ((3, 50, 320), 64, True), ((300, 256), 200, True), ((1030, 130), 70, False)])
@@ -487,6 +565,18 @@ def test_convolution_from_a_checkpoint(k, cin, cout):
     assert float((kept[4] - restored[4]).abs().max()) <= 4 * n * 2.0 ** -23 * float(x.abs().max() * 4) * float(gy.abs().max()) * n
     rel = float((kept[4] - plain[4]).norm() / plain[4].norm())
     assert 0 < rel < 2.0 ** -4, rel
+
+
+def test_a_checkpoints_logs_may_not_change_before_they_are_used():
+    g = gen(23)
+    x, bias, logs = ring(rand(g, 1, 4, 5, 64)), rand(g, 64), 0.3 * rand(g, 64)
+    _, used = train_ops.an_relu8_ring(x, bias, logs)
+    want = used.restore()
+    _, late = train_ops.an_relu8_ring(x, bias, logs)
+    logs += 1
+    assert torch.equal(used.restore(), want)
+    with pytest.raises(RuntimeError):
+        late.restore()
 
 
 # ------------------------------------------------------------------------------------------------ streams, graphs, two at once
