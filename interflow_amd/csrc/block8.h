@@ -195,6 +195,113 @@ __device__ __forceinline__ bf16x8 b8_bf16x8(int w0, int w1, int byte) {
     return r;
 }
 
+// ------------------------------------------------------------------------------------------------ quantize, rows contiguous
+// Group of LANES lanes = one block of a row; kg (a power of two) groups side by side along a row, the rest along rows.  Four
+// rows per group are in flight at once: their loads are issued before the first is used.  Few, long rows: gy workgroups share
+// one (4 x 1000000: 500 us with one each, 7.6 so).  16384 x 2048: bf16 19.4 us, 5.2 TB/s, float32 27.0 us, 6.2 TB/s.
+struct B8Rows { const void* x; int64_t rs; uint8_t* codes; int64_t ldc; uint8_t* scales; int64_t lds; int64_t rows; int cols, pad, kg_log, fmt, gx, gy; };
+template <class T, int LANES>
+__device__ __forceinline__ void b8_quantize_rows(const B8Rows& q, int block) {
+    constexpr int U = 4, GPB = 256 / LANES;
+    const T* __restrict__ x = (const T*)q.x;
+    const int by = block / q.gx, bx = block - by * q.gx;
+    const int lane = threadIdx.x % LANES, grp = threadIdx.x / LANES;
+    const int gk = grp & ((1 << q.kg_log) - 1), gr = grp >> q.kg_log, rpb = GPB >> q.kg_log;
+    const int KB = (q.cols + B8_BLK - 1) / B8_BLK;
+    const int64_t step = (int64_t)q.gx * rpb;
+    for (int64_t r0 = (int64_t)bx * rpb + gr; r0 < q.rows; r0 += U * step) {
+        for (int kb = gk + (by << q.kg_log); kb < KB; kb += q.gy << q.kg_log) {
+            const int c = kb * B8_BLK + lane * 8;
+            float v[U][8];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t r = r0 + u * step;
+                b8_load8<T>(x + r * q.rs + c, r < q.rows ? q.cols - c : 0, v[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t r = r0 + u * step;
+                if (r >= q.rows) break;                                  // (the same for all lanes of a group)
+                int sb;
+                const i32x2 w = b8_quantize8<LANES>(v[u], q.fmt, sb);
+                b8_store_codes(q.codes + r * q.ldc + c, q.pad - c, w);
+                if (lane == 0) q.scales[r * q.lds + kb] = (uint8_t)sb;
+            }
+        }
+    }
+}
+// columns that rows of codes are filled up to (with zeros): whole 16 bytes, if the rows have them
+static inline int b8_pad(int64_t cols, int64_t ldc) { const int64_t p = (cols + 15) / 16 * 16; return (int)(p < ldc ? p : ldc); }
+
+// ------------------------------------------------------------------------------------------------ quantize, columns contiguous
+// x[r][c] at x + r + c * cs (a transposed view).  Workgroup = 64 rows x one block of 128 columns: lanes run along the rows
+// (contiguous in memory), a thread holds 32 columns of its row, the four threads of a row meet in LDS for the maximum and
+// write 32 code bytes each.  Values of 16 bits come through LDS, 8 rows of a column in one load (16384 x 2048 bf16: 55 us with a
+// load for each, 22.6 so; float32 28.0, without).
+struct B8Cols { const void* x; int64_t cs; uint8_t* codes; int64_t ldc; uint8_t* scales; int64_t lds; int64_t rows; int cols, pad, fmt; };
+constexpr int B8_PITCH = 72;                                             // rows of a column in LDS: 16-byte aligned, neighbours 36 banks apart
+constexpr int B8_COLS_LDS = 4 * 64 * 4 + 128 * B8_PITCH * 2;             // bytes that a workgroup needs, 16-byte aligned
+template <class T>
+__device__ __forceinline__ void b8_quantize_cols(const B8Cols& q, void* sm, int64_t bx, int kb) {
+    constexpr bool STAGE = sizeof(T) == 2;
+    const T* __restrict__ x = (const T*)q.x;
+    uint32_t (*red)[64] = (uint32_t(*)[64])sm;
+    T* tile = (T*)((uint8_t*)sm + 4 * 64 * 4);
+    const int lr = threadIdx.x & 63, g = threadIdx.x >> 6;
+    const int64_t first = bx * 64, r = first + lr;
+    const int c0 = kb * B8_BLK + g * 32;
+    const int64_t rc = r < q.rows ? r : q.rows - 1;
+    float v[32];
+    if constexpr (STAGE) {
+        const int p = (threadIdx.x & 7) * 8, left = (int)min((int64_t)64, q.rows - first) - p;
+        typedef typename B8Vec<T, 8>::type T8;
+        T8 w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int c = min(kb * B8_BLK + (int)(threadIdx.x >> 3) + 32 * i, q.cols - 1);
+            const T* s = x + first + p + (int64_t)c * q.cs;
+            if (left >= 8) w[i] = *(const T8*)s;
+            else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[i][e] = e < left ? s[e] : (T)0.f;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *(typename B8Vec<T, 8>::Aligned*)(tile + ((threadIdx.x >> 3) + 32 * i) * B8_PITCH + p) = w[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = c0 + i < q.cols ? (float)tile[(g * 32 + i) * B8_PITCH + lr] : 0.f;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = c0 + i < q.cols ? (float)x[rc + (int64_t)(c0 + i) * q.cs] : 0.f;
+    }
+    uint32_t m = 0, any = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { m = max(m, b8_amax_bits(v + 8 * i)); any = max(any, b8_max_bits(v + 8 * i)); }
+    red[g][lr] = m;
+    __syncthreads();
+    m = max(max(red[0][lr], red[1][lr]), max(red[2][lr], red[3][lr]));
+    if (r >= q.rows) return;
+    const int sb = b8_scale_byte(m, q.fmt);
+    const float inv = b8_inv_scale(sb);
+    typedef i32x4 i32x4_any __attribute__((aligned(1)));
+    uint8_t* d = q.codes + r * q.ldc + c0;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        i32x2 w[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float* u = v + 16 * j + 8 * h;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) u[i] *= inv;
+            w[h] = b8_encode8(u, q.fmt, any >= B8_INF);
+        }
+        if (c0 + 16 * j + 16 <= q.pad) *(i32x4_any*)(d + 16 * j) = i32x4{w[0][0], w[0][1], w[1][0], w[1][1]};
+        else { b8_store_codes(d + 16 * j, q.pad - (c0 + 16 * j), w[0]); b8_store_codes(d + 16 * j + 8, q.pad - (c0 + 16 * j + 8), w[1]); }
+    }
+    if (g == 0) q.scales[r * q.lds + kb] = (uint8_t)sb;
+}
+
 // dispatch on an element type: body sees `T`
 #define B8_DISPATCH(type, ...) \
     do { if ((type) == IFL_T_F32) { typedef float T; __VA_ARGS__; } \
@@ -204,9 +311,13 @@ __device__ __forceinline__ bf16x8 b8_bf16x8(int w0, int w1, int byte) {
 static inline bool b8_type_ok(int t) { return t == IFL_T_F32 || t == IFL_T_BF16 || t == IFL_T_F16; }
 static inline bool b8_fmt_ok(int f) { return f == IFL_Q_E4M3 || f == IFL_Q_E5M2; }
 
-// ifl_block8_wgrad in two steps for the layer whose other product needs dy in 8-bit blocks: 1 prepares (and quantizes dy, if told
-// where to), 2 multiplies and joins, 3 both.
-struct B8Quant { uint8_t *codes, *scales; int64_t ldc, lds; int fmt; };
+// two matrices of K columns in e4m3, rows of codes and scales alike, in one launch; everything checked by the caller, M and N at least 1
+int b8_quantize2(const void* x, int xtype, int64_t x_rs, const void* w, int wtype, int64_t w_rs, uint8_t* xc, uint8_t* xs, uint8_t* wc, uint8_t* ws,
+                 int64_t ldc, int64_t lds, int64_t M, int64_t N, int64_t K, void* stream);
+
+// ifl_block8_wgrad in two steps for the layer whose other product needs dy in 8-bit blocks, and its weights along their columns: 1
+// prepares (and quantizes dy, if told where to, and w, if there is one), 2 multiplies and joins, 3 both.
+struct B8Quant { uint8_t *codes, *scales; int64_t ldc, lds; int fmt; B8Cols w; int wtype; };
 int b8_wgrad(int steps, const B8Quant* quant, const void* dy, int dytype, int64_t ldy, const uint8_t* codes, int64_t ldc, const uint8_t* scales,
              int64_t lds, int fmt, const float* chan, void* dw, int dwtype, int64_t ldw, void* db, int dbtype, float* scratch, int64_t M,
              int64_t N, int64_t K, void* stream);

@@ -5,109 +5,26 @@
 
 namespace {
 
-// ------------------------------------------------------------------------------------------------ quantize, rows contiguous
-// Group of LANES lanes = one block of a row; kg (a power of two) groups side by side along a row, the rest along rows.  Four
-// rows per group are in flight at once: their loads are issued before the first is used.  Few, long rows: gridDim.y workgroups share
-// one (4 x 1000000: 500 us with one each, 7.6 so).  16384 x 2048: bf16 19.4 us, 5.2 TB/s, float32 27.0 us, 6.2 TB/s.
+// ------------------------------------------------------------------------------------------------ quantize
 template <class T, int LANES>
 __global__ __launch_bounds__(256)
-void quantize_kernel(const T* __restrict__ x, int64_t rs, uint8_t* __restrict__ codes, int64_t ldc, uint8_t* __restrict__ scales,
-                     int64_t lds, int64_t rows, int cols, int pad, int kg_log, int fmt)
-{
-    constexpr int U = 4, GPB = 256 / LANES;
-    const int lane = threadIdx.x % LANES, grp = threadIdx.x / LANES;
-    const int gk = grp & ((1 << kg_log) - 1), gr = grp >> kg_log, rpb = GPB >> kg_log;
-    const int KB = (cols + B8_BLK - 1) / B8_BLK;
-    const int64_t step = (int64_t)gridDim.x * rpb;
-    for (int64_t r0 = (int64_t)blockIdx.x * rpb + gr; r0 < rows; r0 += U * step) {
-        for (int kb = gk + (blockIdx.y << kg_log); kb < KB; kb += gridDim.y << kg_log) {
-            const int c = kb * B8_BLK + lane * 8;
-            float v[U][8];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int64_t r = r0 + u * step;
-                b8_load8<T>(x + r * rs + c, r < rows ? cols - c : 0, v[u]);
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int64_t r = r0 + u * step;
-                if (r >= rows) break;                                   // (the same for all lanes of a group)
-                int sb;
-                const i32x2 w = b8_quantize8<LANES>(v[u], fmt, sb);
-                b8_store_codes(codes + r * ldc + c, pad - c, w);
-                if (lane == 0) scales[r * lds + kb] = (uint8_t)sb;
-            }
-        }
-    }
+void quantize_kernel(B8Rows q) { b8_quantize_rows<T, LANES>(q, blockIdx.x); }
+
+// two matrices with as many columns in one launch: a layer's input and its weights (16384 and 2048 rows of 2048 bf16: 30 us, 28 + 6
+// one after the other)
+template <class T, class T2, int LANES>
+__global__ __launch_bounds__(256)
+void quantize2_kernel(B8Rows q, B8Rows q2) {
+    const int n = q.gx * q.gy;
+    if ((int)blockIdx.x < n) b8_quantize_rows<T, LANES>(q, blockIdx.x);
+    else b8_quantize_rows<T2, LANES>(q2, blockIdx.x - n);
 }
 
-// ------------------------------------------------------------------------------------------------ quantize, columns contiguous
-// x[r][c] at x + r + c * cs (a transposed view).  Workgroup = 64 rows x one block of 128 columns: lanes run along the rows
-// (contiguous in memory), a thread holds 32 columns of its row, the four threads of a row meet in LDS for the maximum and
-// write 32 code bytes each.  Values of 16 bits come through LDS, 8 rows of a column in one load (16384 x 2048 bf16: 55 us with a
-// load for each, 22.6 so; float32 28.0, without).
 template <class T>
 __global__ __launch_bounds__(256)
-void quantize_t_kernel(const T* __restrict__ x, int64_t cs, uint8_t* __restrict__ codes, int64_t ldc, uint8_t* __restrict__ scales,
-                       int64_t lds, int64_t rows, int cols, int pad, int fmt)
-{
-    constexpr bool STAGE = sizeof(T) == 2;
-    constexpr int PITCH = 72;                                            // rows of a column in LDS: 16-byte aligned, neighbours 36 banks apart
-    __shared__ uint32_t red[4][64];
-    __shared__ __attribute__((aligned(16))) T tile[STAGE ? 128 * PITCH : 1];
-    const int lr = threadIdx.x & 63, g = threadIdx.x >> 6;
-    const int64_t first = (int64_t)blockIdx.x * 64, r = first + lr;
-    const int kb = blockIdx.y, c0 = kb * B8_BLK + g * 32;
-    const int64_t rc = r < rows ? r : rows - 1;
-    float v[32];
-    if constexpr (STAGE) {
-        const int p = (threadIdx.x & 7) * 8, left = (int)min((int64_t)64, rows - first) - p;
-        typedef typename B8Vec<T, 8>::type T8;
-        T8 w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int c = min(kb * B8_BLK + (int)(threadIdx.x >> 3) + 32 * i, cols - 1);
-            const T* s = x + first + p + (int64_t)c * cs;
-            if (left >= 8) w[i] = *(const T8*)s;
-            else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) w[i][e] = e < left ? s[e] : (T)0.f;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) *(typename B8Vec<T, 8>::Aligned*)(tile + ((threadIdx.x >> 3) + 32 * i) * PITCH + p) = w[i];
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = c0 + i < cols ? (float)tile[(g * 32 + i) * PITCH + lr] : 0.f;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = c0 + i < cols ? (float)x[rc + (int64_t)(c0 + i) * cs] : 0.f;
-    }
-    uint32_t m = 0, any = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { m = max(m, b8_amax_bits(v + 8 * i)); any = max(any, b8_max_bits(v + 8 * i)); }
-    red[g][lr] = m;
-    __syncthreads();
-    m = max(max(red[0][lr], red[1][lr]), max(red[2][lr], red[3][lr]));
-    if (r >= rows) return;
-    const int sb = b8_scale_byte(m, fmt);
-    const float inv = b8_inv_scale(sb);
-    typedef i32x4 i32x4_any __attribute__((aligned(1)));
-    uint8_t* q = codes + r * ldc + c0;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        i32x2 w[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            float* u = v + 16 * j + 8 * h;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) u[i] *= inv;
-            w[h] = b8_encode8(u, fmt, any >= B8_INF);
-        }
-        if (c0 + 16 * j + 16 <= pad) *(i32x4_any*)(q + 16 * j) = i32x4{w[0][0], w[0][1], w[1][0], w[1][1]};
-        else { b8_store_codes(q + 16 * j, pad - (c0 + 16 * j), w[0]); b8_store_codes(q + 16 * j + 8, pad - (c0 + 16 * j + 8), w[1]); }
-    }
-    if (g == 0) scales[r * lds + kb] = (uint8_t)sb;
+void quantize_t_kernel(B8Cols q) {
+    __shared__ __attribute__((aligned(16))) uint8_t sm[B8_COLS_LDS];
+    b8_quantize_cols<T>(q, sm, blockIdx.x, blockIdx.y);
 }
 
 // ------------------------------------------------------------------------------------------------ restore
@@ -267,6 +184,18 @@ unsigned share_rows(int64_t grid, int64_t passes) {
     return (unsigned)(n < passes ? n : passes);
 }
 
+int rows_lanes(int64_t cols) { return cols <= 32 ? 4 : cols <= 64 ? 8 : 16; }
+B8Rows rows_job(const void* x, int64_t rs, uint8_t* codes, int64_t ldc, uint8_t* scales, int64_t lds, int64_t rows, int64_t cols, int fmt) {
+    const int lanes = rows_lanes(cols), gpb_log = lanes == 4 ? 6 : lanes == 8 ? 5 : 4;
+    const int64_t KB = (cols + B8_BLK - 1) / B8_BLK;
+    const int kgl = log2_up(KB, gpb_log);
+    const int64_t rpb = 1 << (gpb_log - kgl);
+    int64_t grid = (rows + 4 * rpb - 1) / (4 * rpb);
+    if (grid < 1024) grid = (rows + rpb - 1) / rpb < 1024 ? (rows + rpb - 1) / rpb : 1024;      // few rows: spread them before stacking them
+    if (grid > 65536) grid = 65536;
+    return {x, rs, codes, ldc, scales, lds, rows, (int)cols, b8_pad(cols, ldc), kgl, fmt, (int)grid, (int)share_rows(grid, (KB + (1 << kgl) - 1) >> kgl)};
+}
+
 constexpr int AN8_BLOCKS = 1024;                                         // most blocks (partial sums) of the backward pass
 
 }  // namespace
@@ -282,27 +211,30 @@ extern "C" int ifl_block8_quantize(const void* x, int xtype, int64_t row_stride,
     IFL_CHECK_ARG(x && codes && scales, IFL_EINVAL, "block8_quantize: null pointer");
     IFL_CHECK_ARG(ldc >= cols && lds >= KB, IFL_EINVAL, "block8_quantize: row strides %lld, %lld for %lld columns", (long long)ldc, (long long)lds, (long long)cols);
     IFL_CHECK_ARG(col_stride == 1 || row_stride == 1 || rows == 1, IFL_EINVAL, "block8_quantize: strides %lld, %lld: one of them has to be 1", (long long)row_stride, (long long)col_stride);
-    const int64_t pad64 = (cols + 15) / 16 * 16;
-    const int pad = (int)(pad64 < ldc ? pad64 : ldc);
     hipStream_t st = (hipStream_t)stream;
     if (col_stride != 1) {
         const int64_t gx = (rows + 63) / 64;
         IFL_CHECK_ARG(gx <= 0x7fffffff && KB <= 65535, IFL_ENOTSUP, "block8_quantize: transposed %lld x %lld", (long long)rows, (long long)cols);
-        B8_DISPATCH(xtype, hipLaunchKernelGGL(HIP_KERNEL_NAME(quantize_t_kernel<T>), dim3((unsigned)gx, KB), dim3(256), 0, st, (const T*)x, col_stride, codes, ldc, scales,
-                                              lds, rows, (int)cols, pad, fmt));
+        const B8Cols q = {x, col_stride, codes, ldc, scales, lds, rows, (int)cols, b8_pad(cols, ldc), fmt};
+        B8_DISPATCH(xtype, hipLaunchKernelGGL(HIP_KERNEL_NAME(quantize_t_kernel<T>), dim3((unsigned)gx, KB), dim3(256), 0, st, q));
         IFL_LAUNCH_CHECK();
         return 0;
     }
-    const int lanes = cols <= 32 ? 4 : cols <= 64 ? 8 : 16;
-    const int gpb_log = lanes == 4 ? 6 : lanes == 8 ? 5 : 4;
-    const int kgl = log2_up(KB, gpb_log);
-    const int64_t rpb = 1 << (gpb_log - kgl);
-    int64_t grid = (rows + 4 * rpb - 1) / (4 * rpb);
-    if (grid < 1024) grid = (rows + rpb - 1) / rpb < 1024 ? (rows + rpb - 1) / rpb : 1024;      // few rows: spread them before stacking them
-    if (grid > 65536) grid = 65536;
-    const dim3 g2((unsigned)grid, share_rows(grid, (KB + (1 << kgl) - 1) >> kgl));
-#define Q8_GO(L) hipLaunchKernelGGL(HIP_KERNEL_NAME(quantize_kernel<T, L>), g2, dim3(256), 0, st, (const T*)x, row_stride, codes, ldc, scales, lds, rows, (int)cols, pad, kgl, fmt)
+    const B8Rows q = rows_job(x, row_stride, codes, ldc, scales, lds, rows, cols, fmt);
+    const int lanes = rows_lanes(cols);
+#define Q8_GO(L) hipLaunchKernelGGL(HIP_KERNEL_NAME(quantize_kernel<T, L>), dim3(q.gx * q.gy), dim3(256), 0, st, q)
     B8_DISPATCH(xtype, if (lanes == 4) Q8_GO(4); else if (lanes == 8) Q8_GO(8); else Q8_GO(16));
+    IFL_LAUNCH_CHECK();
+    return 0;
+}
+
+int b8_quantize2(const void* x, int xtype, int64_t x_rs, const void* w, int wtype, int64_t w_rs, uint8_t* xc, uint8_t* xs, uint8_t* wc, uint8_t* ws,
+                 int64_t ldc, int64_t lds, int64_t M, int64_t N, int64_t K, void* stream)
+{
+    const B8Rows a = rows_job(x, x_rs, xc, ldc, xs, lds, M, K, IFL_Q_E4M3), b = rows_job(w, w_rs, wc, ldc, ws, lds, N, K, IFL_Q_E4M3);
+    const int lanes = rows_lanes(K);
+#define Q8_GO2(L) hipLaunchKernelGGL(HIP_KERNEL_NAME(quantize2_kernel<TX, T, L>), dim3(a.gx * a.gy + b.gx * b.gy), dim3(256), 0, (hipStream_t)stream, a, b)
+    B8_DISPATCH(xtype, typedef T TX; B8_DISPATCH(wtype, if (lanes == 4) Q8_GO2(4); else if (lanes == 8) Q8_GO2(8); else Q8_GO2(16)));
     IFL_LAUNCH_CHECK();
     return 0;
 }

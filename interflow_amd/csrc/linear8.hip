@@ -31,8 +31,12 @@ extern "C" int ifl_linear8_fwd(const void* x, int xtype, int64_t x_rs, int64_t x
     uint8_t* wc = (uint8_t*)scratch;
     uint8_t* ws = wc + up16(N * code_ld(K));
     float* part = (float*)(wc + block_bytes(N, K));
-    if (int rc = ifl_block8_quantize(x, xtype, x_rs, x_cs, codes, code_ld(K), scales, scale_ld(K), M, K, IFL_Q_E4M3, stream)) return rc;
-    if (int rc = ifl_block8_quantize(w, wtype, w_rs, w_cs, wc, code_ld(K), ws, scale_ld(K), N, K, IFL_Q_E4M3, stream)) return rc;
+    if (x_cs == 1 && w_cs == 1) {
+        if (int rc = b8_quantize2(x, xtype, x_rs, w, wtype, w_rs, codes, scales, wc, ws, code_ld(K), scale_ld(K), M, N, K, stream)) return rc;
+    } else {
+        if (int rc = ifl_block8_quantize(x, xtype, x_rs, x_cs, codes, code_ld(K), scales, scale_ld(K), M, K, IFL_Q_E4M3, stream)) return rc;
+        if (int rc = ifl_block8_quantize(w, wtype, w_rs, w_cs, wc, code_ld(K), ws, scale_ld(K), N, K, IFL_Q_E4M3, stream)) return rc;
+    }
     return ifl_block8_matmul(codes, code_ld(K), scales, scale_ld(K), IFL_Q_E4M3, wc, code_ld(K), ws, scale_ld(K), IFL_Q_E4M3, bias, btype, y, xtype, N, part,
                              M, N, K, stream);
 }
@@ -59,13 +63,17 @@ extern "C" int ifl_linear8_bwd(const void* dy, int xtype, int64_t ldy, const uin
     uint8_t *gc = at, *gs = gc + up16(M * code_ld(N)), *wc = gc + block_bytes(M, N), *ws = wc + up16(K * code_ld(N));
     float* part = (float*)(wc + block_bytes(K, N));
     if (dx) at = (uint8_t*)part + up16(4 * ifl_block8_matmul_scratch_floats(M, K, N, xtype));
-    const B8Quant quant = {gc, gs, code_ld(N), scale_ld(N), gfmt};
+    // (w^T has rows of w's columns: next to each other in memory as a rule)
+    const bool together = dx && sums && w_cs == 1;
+    const B8Quant quant = {gc, gs, code_ld(N), scale_ld(N), gfmt,
+                           {together ? w : nullptr, w_rs, wc, code_ld(N), ws, scale_ld(N), K, (int)N, b8_pad(N, code_ld(N)), IFL_Q_E4M3}, wtype};
     auto gradients = [&](int steps) {
         return b8_wgrad(steps, dx ? &quant : nullptr, dy, xtype, ldy, codes, code_ld(K), scales, scale_ld(K), IFL_Q_E4M3, nullptr, dw, wtype, K, db, dbtype, (float*)at, M, N, dw ? K : 0, stream);
     };
     if (dx && M > 0) {
         if (int rc = sums ? gradients(1) : ifl_block8_quantize(dy, xtype, ldy, 1, gc, code_ld(N), gs, scale_ld(N), M, N, gfmt, stream)) return rc;
-        if (int rc = ifl_block8_quantize(w, wtype, w_cs, w_rs, wc, code_ld(N), ws, scale_ld(N), K, N, IFL_Q_E4M3, stream)) return rc;
+        if (!together)
+            if (int rc = ifl_block8_quantize(w, wtype, w_cs, w_rs, wc, code_ld(N), ws, scale_ld(N), K, N, IFL_Q_E4M3, stream)) return rc;
         if (int rc = ifl_block8_matmul(gc, code_ld(N), gs, scale_ld(N), gfmt, wc, code_ld(N), ws, scale_ld(N), IFL_Q_E4M3, nullptr, 0, dx, xtype, K, part, M, K, N, stream)) return rc;
     }
     return sums ? gradients(dx ? 2 : 3) : 0;

@@ -26,6 +26,7 @@ struct WG8 {
     int64_t M; int N, K, fmt;
     int want_x;                          // 0: column sums alone
     uint8_t *gc, *gs; int64_t ldgc, ldgs; int gfmt;  // where dy's own 8-bit blocks go, if they are wanted
+    B8Cols w; int w_blocks, w_tiles;                 // and the layer's weights, to be quantized along their columns: workgroups, those of a block of columns
     // scratch
     uint16_t* xb;                        // restored codes, rows up to a multiple of 64 (zeros)
     uint16_t* yb; int64_t yplane;        // terms of dy in the same way, yplane apart; or of bf16 read in place the last M % 64 rows
@@ -89,21 +90,28 @@ __device__ __forceinline__ void wg8_put(i32x4* lds, const i32x4 w[8], uint16_t* 
 // row e of group gg (from a multiple of 32 on)
 __device__ __forceinline__ int wg8_row(int gg, int e) { return (gg >> 2) * 32 + 4 * (gg & 3) + (e & 3) + 16 * (e >> 2); }
 
-// Workgroups 0 .. x_blocks - 1 restore codes.  The others take up to 256 columns of cs_rows rows of dy, with column sums on the
-// way that are joined in LDS in a fixed order, and dy's terms, if the product does not read it in place.  QUANT: they also put dy
-// into 8-bit blocks (for the layer's other product), which saves a pass over it (16384 x 2048, both operands, bf16: 43 us
-// instead of 25 + 33).
-template <class T, int NP, bool QUANT>
+// QUANT, for a layer's other product: the first w_blocks workgroups quantize its weights, tiles of 64 x 128, and those of dy put it into
+// 8-bit blocks as well.  The next x_blocks restore codes.  The others take up to 256 columns of cs_rows rows of dy, with column
+// sums on the way that are joined in LDS in a fixed order, and dy's terms, if the product does not read it in place.  (16384 x 2048,
+// both operands, bf16: 30 us; with dy's blocks 43, 25 more on its own; with 2048 x 2048 weights 47, 19 more on their own.)
+template <class T, int NP, bool QUANT, class TW>
 __global__ __launch_bounds__(256, NP > 1 ? 2 : 3)
 void wgrad8_prepare_kernel(WG8 q)
 {
     __shared__ __attribute__((aligned(16))) i32x4 stage[2048];
+    static_assert(sizeof(stage) >= B8_COLS_LDS, "");
+    if (QUANT && (int)blockIdx.x < q.w_blocks) {
+        const int kb = blockIdx.x / q.w_tiles;
+        b8_quantize_cols<TW>(q.w, stage, blockIdx.x - kb * q.w_tiles, kb);
+        return;
+    }
     const int64_t mp = wg8_rows(q.M);
-    if ((int)blockIdx.x < q.x_blocks) {
+    const int bid = blockIdx.x - (QUANT ? q.w_blocks : 0);
+    if (bid < q.x_blocks) {
         const int tpr = 1 << q.x_tpr_log, gg = threadIdx.x >> q.x_tpr_log, rpp = 8 * (256 >> q.x_tpr_log);
         const int cols = (q.K + 8 * tpr - 1) / (8 * tpr);
         const int64_t jobs = (mp + rpp - 1) / rpp * cols;
-        for (int64_t job = blockIdx.x; job < jobs; job += q.x_blocks) {
+        for (int64_t job = bid; job < jobs; job += q.x_blocks) {
             const int64_t row0 = job / cols * rpp;
             const int c0 = (int)(job % cols) * 8 * tpr, c = c0 + (threadIdx.x & (tpr - 1)) * 8;
             i32x2 w[8];
@@ -128,7 +136,7 @@ void wgrad8_prepare_kernel(WG8 q)
         return;
     }
     __shared__ float red[256 * 8 + 256];
-    const int b = blockIdx.x - q.x_blocks, part = b / q.y_cols, cb = b - part * q.y_cols;
+    const int b = bid - q.x_blocks, part = b / q.y_cols, cb = b - part * q.y_cols;
     const int tpr = 1 << q.y_tpr_log, rpp = 256 >> q.y_tpr_log, rl = threadIdx.x >> q.y_tpr_log;
     const int c0 = cb * 8 * tpr, c = c0 + (threadIdx.x & (tpr - 1)) * 8;
     const int64_t first = q.y_row0 + (int64_t)part * q.cs_rows, last = min(mp, first + q.cs_rows);
@@ -542,11 +550,18 @@ int b8_wgrad(int todo, const B8Quant* quant, const void* dy, int dytype, int64_t
             q.cs_rows = MP;
             y_blocks = M % MP ? q.y_cols : 0;
         }
-        if (quant) { q.gc = quant->codes; q.gs = quant->scales; q.ldgc = quant->ldc; q.ldgs = quant->lds; q.gfmt = quant->fmt; }
-        const dim3 pg((unsigned)(q.x_blocks + y_blocks));
-#define WG8_P(T, NP) do { \
-            if (quant) hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_prepare_kernel<T, NP, true>), pg, dim3(256), 0, st, q); \
-            else hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_prepare_kernel<T, NP, false>), pg, dim3(256), 0, st, q); \
+        if (quant) {
+            q.gc = quant->codes; q.gs = quant->scales; q.ldgc = quant->ldc; q.ldgs = quant->lds; q.gfmt = quant->fmt;
+            if (quant->w.x) {
+                q.w = quant->w;
+                q.w_tiles = (int)((q.w.rows + 63) / 64);
+                q.w_blocks = q.w_tiles * ((q.w.cols + B8_BLK - 1) / B8_BLK);
+            }
+        }
+        const dim3 pg((unsigned)(q.w_blocks + q.x_blocks + y_blocks));
+#define WG8_P(TY, NP) do { \
+            if (!quant) hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_prepare_kernel<TY, NP, false, float>), pg, dim3(256), 0, st, q); \
+            else B8_DISPATCH(quant->wtype, hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_prepare_kernel<TY, NP, true, T>), pg, dim3(256), 0, st, q)); \
         } while (0)
         if (dytype == IFL_T_F32) WG8_P(float, 3); else if (dytype == IFL_T_F16) WG8_P(_Float16, 2); else WG8_P(__bf16, 1);
         IFL_LAUNCH_CHECK();
