@@ -254,9 +254,9 @@ class Checkpoint8:
                 self._chan = torch.exp(logs.reshape(-1).float())
 
     @staticmethod
-    def room(shape, dev):
+    def room(shape, like):
         px, C = shape[0] * shape[1] * shape[2], shape[3]
-        return torch.empty((px * (C + -(-C // block8.BLOCK)),), dtype=torch.uint8, device=dev)
+        return like.new_empty((px * (C + -(-C // block8.BLOCK)),), dtype=torch.uint8)
 
     @property
     def codes(self):
@@ -299,44 +299,42 @@ def _plain_f32(t):
     return t.detach().float().contiguous()
 
 
+def _once(backward):
+    """`once_differentiable`, whose context manager a backward pass that nobody differentiates (gradients are off in it) goes without."""
+    checked = once_differentiable(backward)
+    return lambda ctx, *grads: (checked if torch.is_grad_enabled() else backward)(ctx, *grads)
+
+
 class _AnRelu8(torch.autograd.Function):
-    """y = relu((x + bias) * exp(logs)) on a ringed tensor; the backward reads an 8-bit checkpoint (ifl_an_relu8_fwd / _bwd)."""
+    """y = relu((x + bias) * exp(logs)) on a ringed tensor; writes the 8-bit checkpoint `raw`, which the backward reads
+    (ifl_an_relu8_fwd / _bwd)."""
 
     @staticmethod
-    def forward(ctx, x, bias, logs):
-        x = _aligned(hip._dev_f32(x, "an_relu8 input"))
-        B, hp, wp_, C = x.shape
+    def forward(ctx, x, bias, logs, raw):
+        B, hp, wp_, C = ctx.shape = x.shape
         b, l = _plain_f32(bias), _plain_f32(logs)
-        assert b.numel() == C and l.numel() == C, (tuple(bias.shape), tuple(logs.shape), C)
-        dev = x.get_device()
-        block8._same_device(dev, b, l)
         y = torch.empty_like(x)
-        raw = Checkpoint8.room(x.shape, x.device)
         p = raw.data_ptr()
-        block8._call("ifl_an_relu8_fwd", dev, x.data_ptr(), y.data_ptr(), p, p + x.numel(), b.data_ptr(), l.data_ptr(), B, hp - 2, wp_ - 2, C)
+        block8._call("ifl_an_relu8_fwd", x.get_device(), x.data_ptr(), y.data_ptr(), p, p + x.numel(), b.data_ptr(), l.data_ptr(), B, hp - 2, wp_ - 2, C)
         ctx.save_for_backward(raw, l)
-        ctx.shapes = (x.shape, bias.shape, logs.shape)
-        ctx.mark_non_differentiable(raw)
-        ctx.set_materialize_grads(False)
-        return y, raw
+        ctx.bias_shape = bias.shape
+        ctx.logs_shape = logs.shape
+        return y
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, gy, _raw):
-        if gy is None:
-            return None, None, None
+    @_once
+    def backward(ctx, gy):
         raw, l = ctx.saved_tensors
-        shape, bshape, lshape = ctx.shapes
-        B, hp, wp_, C = shape
+        B, hp, wp_, C = ctx.shape
         gy = _aligned(hip._dev_f32(gy, "an_relu8 gradient"))
         dx = torch.empty_like(gy)
         dl = torch.empty_like(l)                                         # (float32, contiguous, of logs' shape)
-        db = torch.empty_like(l) if bshape == lshape else gy.new_empty(bshape)
+        db = torch.empty_like(l) if ctx.bias_shape == ctx.logs_shape else gy.new_empty(ctx.bias_shape)
         part = gy.new_empty((block8._size("ifl_an_relu8_blocks", B, hp - 2, wp_ - 2, C) * 2 * C,))
         p = raw.data_ptr()
         block8._call("ifl_an_relu8_bwd", gy.get_device(), gy.data_ptr(), p, p + gy.numel(), l.data_ptr(), dx.data_ptr(), db.data_ptr(), dl.data_ptr(),
                      part.data_ptr(), B, hp - 2, wp_ - 2, C)
-        return dx, db, dl
+        return dx, db, dl, None
 
 
 def an_relu8_ring(x_ring, bias, logs):
@@ -344,9 +342,13 @@ def an_relu8_ring(x_ring, bias, logs):
     per 128 channels) of a pixel instead of x's 4 C: dx is exact (the checkpoint's zeros are the ReLU's mask), the gradient of
     logs is that of the checkpoint's values.  Ringed tensors, channels a multiple of 32, at most 1024.  Hand the checkpoint to the
     convolution that reads y (`conv2d_ring(checkpoints=...)`) and y itself is not kept either."""
-    assert x_ring.dim() == 4 and x_ring.shape[1] >= 3 and x_ring.shape[2] >= 3, tuple(x_ring.shape)
-    y, raw = _AnRelu8.apply(x_ring, bias, logs)
-    return y, Checkpoint8(raw, x_ring.shape, logs=logs)
+    x = _aligned(hip._dev_f32(x_ring, "an_relu8 input"))
+    shape = x.shape
+    assert len(shape) == 4 and shape[1] >= 3 and shape[2] >= 3, tuple(shape)
+    assert bias.numel() == shape[3] and logs.numel() == shape[3], (tuple(bias.shape), tuple(logs.shape), shape[3])
+    block8._same_device(x.get_device(), bias, logs)
+    raw = Checkpoint8.room(shape, x)
+    return _AnRelu8.apply(x, bias, logs, raw), Checkpoint8(raw, shape, logs=logs)
 
 
 class _Linear8(torch.autograd.Function):
@@ -361,7 +363,7 @@ class _Linear8(torch.autograd.Function):
         return y if len(shape) == 2 else y.view(*shape[:-1], w.shape[0])
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, g):
         raw, w = ctx.saved_tensors
         shape, bias_dtype, f = ctx.meta
