@@ -318,8 +318,10 @@ int ifl_coupling_bwd(const float* z, const float* dzout, const float* dld, const
  * ifl_block8_linear: the same with the m side x [M][K] (IFL_T_*, columns contiguous) quantized to e4m3 on the way; out has x's
  * type.  scratch: ifl_block8_linear_scratch_bytes bytes, 16-byte aligned (NULL if 0).
  * ifl_block8_wgrad: dw[n * ldw + k] = chan[k] sum_m dy[m * ldy + n] A[m][k] (chan may be NULL) and db[n] = sum_m dy[m * ldy + n]; dw or
- * db may be NULL.  Code rows 16-byte aligned.  Sums of exact products in float32, in an order that depends on the sizes only.  scratch:
- * ifl_block8_wgrad_scratch_floats floats (K = 0 for db alone).  M = 0 gives zeros.                                              */
+ * db may be NULL.  Code rows 16-byte aligned.  Sums of products in float32, in an order that depends on the sizes only; the products
+ * are exact unless an operand has bits below 2^-133, bf16's smallest step.  scratch: ifl_block8_wgrad_scratch_floats floats, 16-byte
+ * aligned (K = 0 for db alone): about 2 bytes per code and 2, 4 or 6 per gradient (bf16 -- 0 where dy is aligned -- float16,
+ * float32), and partial sums.  M = 0 gives zeros.                                                                            */
 enum { IFL_T_F32 = 0, IFL_T_BF16 = 1, IFL_T_F16 = 2 };
 enum { IFL_Q_E4M3 = 0, IFL_Q_E5M2 = 1 };
 int ifl_block8_quantize(const void* x, int xtype, int64_t row_stride, int64_t col_stride, uint8_t* codes, int64_t ldc, uint8_t* scales,

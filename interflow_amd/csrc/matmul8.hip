@@ -9,8 +9,10 @@
 // What the 8-bit instructions keep: within 8 products they drop what is below 2^-13 of the largest (measured), so a result is off
 // by about 1.5e-5 of itself (2-norm; 1.7e-5 of sum |a b| at most in random data, 7 2^-13 of it at worst) -- a thirtieth of what
 // rounding it to float16 costs and a hundredth of bfloat16's.  A float32 result would show it: for that the codes times their
-// scales, exact in bf16, go through v_mfma_f32_16x16x32_bf16, which keeps 24 bits, at half the rate.
-//  Lane l gives row l % 16 and 32 of the 128 values; which 32 is free as long
+// scales, exact in bf16 (what is below its smallest step, 2^-133, aside), go through v_mfma_f32_16x16x32_bf16, which keeps 24 bits, at half
+// the rate.
+//
+// Lane l gives row l % 16 and 32 of the 128 values; which 32 is free as long
 // as both operands agree (all of a block share a scale): 16 bytes from 16 (l / 16) and 16 from 64 + 16 (l / 16).
 #include "block8.h"
 
@@ -428,8 +430,10 @@ void mm8_skinny_kernel(MM8 q)
 }
 
 // ------------------------------------------------------------------------------------------------ which of them
-// Few rows: the skinny kernel.  Else the largest tile that still gives the 256 CUs work (measured: DESIGN), float32 results at most
-// 128 (their fragments are held as bf16); a product of few tiles and a long K is split along K.
+// Few rows: the skinny kernel.  Else the tile that costs least, from the number n of tiles that the busiest of 256 CUs gets: in us at
+// K = 2048 about 4 + 4 n for 64 x 64, 7 + 11 n for 128 x 128, 38 n for 256 x 256 (float32 results 1.6 times that, and at most 128: their
+// fragments are held as bf16).  Measured, 64 / 128 / 256: 1024 x 2048 10.7 / 16.2 / 30.7, 2048 x 2048 18.5 / 18.4 / 33, 16384 x 512
+// 35.6 / 25.5 / 33.8, 3584 x 3584 52.8 / 43.4 / 36.3, 8192 x 2048 69.2 / 47.7 / 39.0.  A product of few tiles and a long K is split along K.
 // The skinny kernel quantizes the m side itself where that is at most 32768 values: then it is the faster way, in a graph (1 x 2048 x
 // 2048: 3.5 us, 6.9 with a launch for it; 16 x 2048 x 2048: 6.2 and 7.3) and out of one (9 and 13.6).
 bool mm8_own(int64_t M, int64_t K) { return M <= 16 && M * K <= 32768; }
@@ -439,9 +443,10 @@ Plan mm8_plan(int64_t M, int64_t N, int64_t K, int otype)
     Plan p = {0, 0, 1, 0};
     if (M <= 32) { p.kind = M <= 16 ? 1 : 2; return p; }
     auto tiles = [&](int t) { return ((M + t - 1) / t) * ((N + t - 1) / t); };
-    p.tile = 64;
-    if (otype != IFL_T_F32 && tiles(256) >= 192) p.tile = 256;
-    else if (tiles(128) >= 192) p.tile = 128;
+    auto busiest = [&](int t) { return (tiles(t) + 255) / 256; };
+    const int64_t c64 = 4 + 4 * busiest(64), c128 = 7 + 11 * busiest(128), c256 = 38 * busiest(256);
+    p.tile = c64 <= c128 ? 64 : 128;
+    if (otype != IFL_T_F32 && c256 < (c64 < c128 ? c64 : c128)) p.tile = 256;
     const int64_t n = tiles(p.tile), steps = (K + B8_BLK - 1) / B8_BLK;
     if (p.tile == 64 && n <= 128 && steps >= 8) {
         int64_t s = 256 / n;

@@ -3,10 +3,12 @@
 // The sum runs over the rows of both operands, whose scales change from row to row, so the 8-bit instructions cannot apply them.
 // A code times its scale is exact in bf16, and so is a bf16 gradient; a float16 gradient is the sum of two bf16 terms and a
 // float32 one of three (its 24 significant bits in pieces of 8).  So every product goes exactly through
-// v_mfma_f32_16x16x32_bf16 (one, two or three of them), which keeps 24 bits of the sums.
+// v_mfma_f32_16x16x32_bf16 (one, two or three of them), which keeps 24 bits of the sums.  (Below 2^-109 a float32's last piece, and in a block
+// of values that small a code, falls under bf16's smallest step, 2^-133, and is lost.)
 //
-// Three launches: codes restored to bf16 and gradients split into their terms, with dy's column sums (memory-bound, one pass); the
-// product; the parts of a split sum joined.  Restoring and splitting inside the product, where every workgroup of a row of
+// Three launches: codes restored to bf16 and gradients split into their terms, with dy's column sums (memory-bound, one pass, 4.9 TB/s); the
+// product (2048 x 2048 over 65536 rows: bf16 1.25 PFLOP/s, the three terms of float32 together 1.6; a large library product in bf16 1.34);
+// the parts of a split sum joined.  Restoring and splitting inside the product, where every workgroup of a row of
 // tiles repeats it, was the slower way: its arithmetic does not fit beside the matrix instructions (2048 x 2048 over 65536 rows,
 // bf16: 615 us with it, 390 without; float32: 1644 and 841).
 #include "block8.h"
@@ -450,16 +452,19 @@ __global__ void fill_zero_kernel(TW* p, int64_t ld, int rows, int cols)
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < (int64_t)rows * cols; i += (int64_t)gridDim.x * blockDim.x) p[i / cols * ld + i % cols] = (TW)0.f;
 }
 
-// Tiles of 256 x 256 for large layers, else 128 x 128.  The rows are split until the card is full (one workgroup on a CU of the
-// large tiles, two of the small ones), each with four steps at least.
+// Tiles of 128 x 128, or 256 x 256 where there are 32 of them, an eighth of them at most lies past the edge, and a workgroup gets 48 steps.
+// Measured (bf16; 128 / 256): 1024 x 2048 x 2048 33.0 / 40.3 us, 4096 x 2048 x 2048 56.7 / 59.5, 16384 x 2048 x 2048 156 / 141, 2048 x
+// 4096 x 4096 90.2 / 71.9, 16384 x 1024 x 1024 60.8 / 64.0, 16384 x 64 x 2048 42.5 / 50.0.  The rows are split until the card is full
+// (one workgroup on a CU of the large tiles, two of the small ones), each with four steps at least.
 struct WPlan { int tile, split, steps, cs_parts, y_tpr_log; int64_t cs_rows, x_floats, y_floats, part_floats, cs_floats; bool in_place; };
 WPlan wg8_plan(int64_t M, int64_t N, int64_t K, int dytype, bool aligned)
 {
     WPlan p = {};
     auto tiles = [&](int64_t t) { return ((N + t - 1) / t) * ((K + t - 1) / t); };
     const int terms = dytype == IFL_T_F32 ? 3 : dytype == IFL_T_F16 ? 2 : 1;
-    p.tile = tiles(256) >= 32 ? 256 : 128;
-    const int64_t steps = wg8_rows(M) / MS, n = K > 0 ? tiles(p.tile) : 1;
+    const int64_t steps = wg8_rows(M) / MS;
+    p.tile = tiles(256) >= 32 && 32 * tiles(256) <= 9 * tiles(128) && steps * terms * tiles(256) >= 48 * 256 ? 256 : 128;
+    const int64_t n = K > 0 ? tiles(p.tile) : 1;
     const int64_t full = p.tile == 256 ? 256 : 512;
     int64_t s = 4 * n >= 3 * full ? 1 : full / n;
     if (s > steps * terms / 4) s = steps * terms / 4;
