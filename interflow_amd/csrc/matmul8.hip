@@ -102,12 +102,14 @@ __device__ __forceinline__ void mm8_part(const MM8& q, const f32x4 (&acc)[NF][MF
         const int64_t m = m0 + 16 * j;
         if (m < q.M) {
 #pragma unroll
-            for (int i = 0; i < NF; ++i)
+            for (int i = 0; i < NF; ++i) {
+                const int64_t n = nw + 16 * G * (i / G) + 4 * (i % G);
+                if (n + 4 <= q.N) *(B8Vec<float, 4>::type*)(out + m * q.N + n) = acc[i][j];
+                else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int64_t n = nw + 16 * G * (i / G) + 4 * (i % G) + e;
-                    if (n < q.N) out[m * q.N + n] = acc[i][j][e];
+                    for (int e = 0; e < 4; ++e) if (n + e < q.N) out[m * q.N + n + e] = acc[i][j][e];
                 }
+            }
         }
     }
 }
@@ -121,9 +123,9 @@ __device__ __forceinline__ void mm8_part(const MM8& q, const f32x4 (&acc)[NF][MF
 // stored); a last step that K does not fill goes through registers with zeros behind K.
 //
 // Waves WN x WM; a wave has NF x MF fragments of 16 x 16.  Row r of n-fragment f is row 16 G (f / G) + 4 G (r / 4) + 4 (f % G) +
-// r % 4 of the wave's: so the four values a lane gets from each of G fragments are 4 G neighbours of one output row, 32 bytes
-// of 16-bit results (G = 4, or NF if less), 16 of float32 (G = 1: four lanes' 16-byte stores then fill 64 bytes of a row; with
-// G = 4 each store left gaps for the next: 169 us instead of 144 at 16384 x 2048 x 2048).
+// r % 4 of the wave's: so the four values a lane gets from each of G fragments are 4 G neighbours of one output row, and 16 bytes
+// (G = 2 for 16-bit results, 1 for float32): four lanes' stores fill 64 bytes of a row.  With twice as many neighbours to a lane each
+// store left gaps for the next (16384 x 2048 x 2048: 69.3 us instead of 67.3, float32 169 instead of 144).
 //
 // Workgroups go to the 8 XCDs in turn; an XCD takes a contiguous run of tiles, in groups of 8 along m, so that the 32 tiles
 // it works on at a time share rows of both operands in its own L2.
@@ -131,7 +133,7 @@ template <int TN, int TM, int WN, int WM, int FA, int FB, bool EXACT, bool SPLIT
 __global__ __launch_bounds__(64 * WN * WM, 1)
 void mm8_tile_kernel(MM8 q)
 {
-    constexpr int NW = WN * WM, NF = TN / WN / 16, MF = TM / WM / 16, G = EXACT ? 1 : NF < 4 ? NF : 4;
+    constexpr int NW = WN * WM, NF = TN / WN / 16, MF = TM / WM / 16, G = EXACT ? 1 : 2;
     constexpr int CH = (TN + TM) * 8, PER = CH / (64 * NW);              // 16-byte pieces of a step, per thread
     constexpr int D = 1, R = 2 * D;                                          // n-fragments read ahead, and the registers they rotate through
     static_assert(NF % R == 0 && D < R, "");
@@ -430,10 +432,11 @@ void mm8_skinny_kernel(MM8 q)
 }
 
 // ------------------------------------------------------------------------------------------------ which of them
-// Few rows: the skinny kernel.  Else the tile that costs least, from the number n of tiles that the busiest of 256 CUs gets: in us at
-// K = 2048 about 4 + 4 n for 64 x 64, 7 + 11 n for 128 x 128, 38 n for 256 x 256 (float32 results 1.6 times that, and at most 128: their
-// fragments are held as bf16).  Measured, 64 / 128 / 256: 1024 x 2048 10.7 / 16.2 / 30.7, 2048 x 2048 18.5 / 18.4 / 33, 16384 x 512
-// 35.6 / 25.5 / 33.8, 3584 x 3584 52.8 / 43.4 / 36.3, 8192 x 2048 69.2 / 47.7 / 39.0.  A product of few tiles and a long K is split along K.
+// Few rows: the skinny kernel.  Else the tile that costs least.  With n tiles on a CU, halfway between the busiest one's and the mean, a
+// product takes in us at K = 2048 about 2 + 4.4 n in tiles of 64 x 64, 7 + 10.5 n of 128 x 128, 4 + 34 n of 256 x 256; the second terms grow with
+// K (float32 results 1.6 times that, and at most 128: their fragments are held as bf16).  Measured, 64 / 128 / 256: 1024 x 2048 10.7 / 16.2 /
+// 30.7, 2048 x 2048 18.5 / 18.4 / 33, 16384 x 512 35.6 / 25.5 / 33.8, 3584 x 3584 52.8 / 43.4 / 36.3, 8192 x 2048 69.2 / 47.7 / 39.0, 5000 x 1000
+// 24.9 / 22.6, and at K = 4096 48.1 / 37.7.  A product of few tiles and a long K is split along K.
 // The skinny kernel quantizes the m side itself where that is at most 32768 values: then it is the faster way, in a graph (1 x 2048 x
 // 2048: 3.5 us, 6.9 with a launch for it; 16 x 2048 x 2048: 6.2 and 7.3) and out of one (9 and 13.6).
 bool mm8_own(int64_t M, int64_t K) { return M <= 16 && M * K <= 32768; }
@@ -443,10 +446,13 @@ Plan mm8_plan(int64_t M, int64_t N, int64_t K, int otype)
     Plan p = {0, 0, 1, 0};
     if (M <= 32) { p.kind = M <= 16 ? 1 : 2; return p; }
     auto tiles = [&](int t) { return ((M + t - 1) / t) * ((N + t - 1) / t); };
-    auto busiest = [&](int t) { return (tiles(t) + 255) / 256; };
-    const int64_t c64 = 4 + 4 * busiest(64), c128 = 7 + 11 * busiest(128), c256 = 38 * busiest(256);
+    auto cost = [&](int t, double fixed, double each) {
+        const double mean = tiles(t) / 256.0, busiest = (double)((tiles(t) + 255) / 256);
+        return fixed + each * (busiest <= 1 ? 1 : (mean + busiest) / 2) * (double)K / 2048;
+    };
+    const double c64 = cost(64, 2, 4.4), c128 = cost(128, 7, 10.5), c256 = cost(256, 4, 34);
     p.tile = c64 <= c128 ? 64 : 128;
-    if (otype != IFL_T_F32 && c256 < (c64 < c128 ? c64 : c128)) p.tile = 256;
+    if (otype != IFL_T_F32 && c256 < c64 && c256 < c128) p.tile = 256;
     const int64_t n = tiles(p.tile), steps = (K + B8_BLK - 1) / B8_BLK;
     if (p.tile == 64 && n <= 128 && steps >= 8) {
         int64_t s = 256 / n;
