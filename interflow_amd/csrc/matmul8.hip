@@ -182,10 +182,10 @@ void mm8_tile_kernel(MM8 q)
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const uint8_t* src = (i * NW * 64) >> 3 < TN ? bk : ak;      // (a piece's side is the same for all waves)
-            uint32_t o = off[i];
-            asm volatile("" : "+v"(o));                                  // (a 32-bit offset at the load, not a 64-bit one kept for it)
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + o),
-                                             (__attribute__((address_space(3))) void*)(buf + (i * NW + wave) * 1024), 16, 0, 0);
+            const uint32_t at = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)(buf + (i * NW + wave) * 1024);
+            // By hand: the compiler waits for all loads wherever it thinks that one might have written what is read, here once in two steps
+            // (8192 x 8192 x 4096 behind the quantization of its input: 285 us, so 252).  M0 is read one wait state after it is written.
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(at), "v"(off[i]), "s"(src) : "memory", "m0");
         }
     };
     auto fill_last = [&](uint8_t* buf, int ks) {
@@ -234,8 +234,9 @@ void mm8_tile_kernel(MM8 q)
         cb[i % R] = s[4 * (nrow0 + nrow(i))];
     };
     auto turn = [&]() {
-        __builtin_amdgcn_s_waitcnt(0x0070);                              // vmcnt(0), lgkmcnt(0)
-        __syncthreads();
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
     };
     // One step: NF groups of MF products.  Fragments of the n side are read D groups ahead.  Before the last D groups everything
     // this step needs is in registers, and the next step's bytes have had the time of NF - D groups to arrive: there the
@@ -243,12 +244,22 @@ void mm8_tile_kernel(MM8 q)
     // while the last D groups run.
     // (No branches inside, the compiler would move products past them: behind the last steps it is the last whole step that is
     // loaded again, unused.)
-    auto step = [&](uint8_t* cur, const uint8_t* nxt, int ks, int o) {
+    const int last = (k_end - 1) >> 2;
+    auto ask = [&](int grp) {
+#pragma unroll
+        for (int i = 0; i < SR; ++i) snext[i] = ((const uint32_t*)sp[i])[min(grp, last)];
+    };
+    auto put = [&](int grp) {
+#pragma unroll
+        for (int i = 0; i < SR; ++i) sc[grp & 1][i * 64 * NW + threadIdx.x] = snext[i];
+    };
+    auto step = [&](uint8_t* cur, const uint8_t* nxt, int ks, bool first) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < NF; ++i) {
             if (i + D < NF) read_b(cur, ks, i + D);
             if (i == NF - D) {
                 turn();
+                if (first) put((ks >> 2) + 1);
                 fill(cur, min(ks + 2, whole - 1));
             }
             if (i >= NF - D) read_b(nxt, ks + 1, i + D - NF);
@@ -260,15 +271,6 @@ void mm8_tile_kernel(MM8 q)
         read_a(nxt, ks + 1, 0);
     };
 
-    const int last = (k_end - 1) >> 2;
-    auto ask = [&](int grp) {
-#pragma unroll
-        for (int i = 0; i < SR; ++i) snext[i] = ((const uint32_t*)sp[i])[min(grp, last)];
-    };
-    auto put = [&](int grp) {
-#pragma unroll
-        for (int i = 0; i < SR; ++i) sc[grp & 1][i * 64 * NW + threadIdx.x] = snext[i];
-    };
     if (!SPLIT && (int)threadIdx.x < TN) bias[threadIdx.x] = n0 + threadIdx.x < q.N ? mm8_bias(q, n0 + threadIdx.x) : 0.f;      // (the workgroup meets before it is read)
     ask(k_first >> 2);                                                   // (k_first is a multiple of 4)
     put(k_first >> 2);
@@ -280,14 +282,14 @@ void mm8_tile_kernel(MM8 q)
         read_a(buf0, ks, 0);
 #pragma unroll
         for (int e = 0; e < D; ++e) read_b(buf0, ks, e);
-        // scales of the next four steps are asked for and put into LDS in every pair of steps, needed or not: no branch
+        // Scales of the next four steps are asked for and put into LDS in every pair of steps, needed or not: no branch.  (Put where the
+        // workgroup has just waited for its loads, and before it asks for more: anywhere else the compiler waits for those too.)
         for (; ks + 1 < whole; ks += 2) {
             ask((ks >> 2) + 1);
-            step(buf0, buf1, ks, 0);
-            put((ks >> 2) + 1);
-            step(buf1, buf0, ks + 1, 1);
+            step(buf0, buf1, ks, true);
+            step(buf1, buf0, ks + 1, false);
         }
-        if (ks < whole) step(buf0, buf1, ks, 0);
+        if (ks < whole) step(buf0, buf1, ks, false);
     }
     if (k_end > whole) {                                                 // a last step that K does not fill
         turn();
@@ -301,7 +303,7 @@ void mm8_tile_kernel(MM8 q)
             for (int j = 0; j < MF; ++j) acc[i][j] = mm8_mfma<FA, FB, EXACT>(b[i % R], a[0][j], acc[i][j], cb[i % R], ca[0][j]);
         }
     }
-    __builtin_amdgcn_s_waitcnt(0x0f70);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                     // (no load into LDS outlives the workgroup)
 
     const int64_t mw = m0 + wm * MF * 16 + r16, nw = n0 + wn * NF * 16 + 4 * G * g;
     if constexpr (SPLIT) mm8_part<NF, MF, G>(q, acc, mw, nw);
