@@ -98,9 +98,17 @@ def _rows_apart(t):
     return (t.shape[1] == 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1])
 
 
+_FAR = 1 << 23                                          # elements between rows that the products do not reach across
+
+
+def _near_rows(t):
+    """t, or a copy whose rows follow one another: for what the products read."""
+    return t if _rows_apart(t) and (t.shape[0] <= 1 or t.stride(0) < _FAR) else t.contiguous()
+
+
 def _ld(t):
     """Distance of rows in elements; of a single row, the columns it has."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 class Block8:
@@ -168,7 +176,7 @@ class Block8:
     def _aligned(self):
         """Itself, or a copy whose rows are whole, aligned 16 and 4 bytes (a single row's length does not matter)."""
         one = self.rows <= 1
-        if self._cp % 16 == 0 and self._sp % 4 == 0 and (one or (self._ldc % 16 == 0 and self._lds % 4 == 0)):
+        if self._cp % 16 == 0 and self._sp % 4 == 0 and (one or (self._ldc % 16 == 0 and self._lds % 4 == 0 and self._ldc < _FAR)):
             return self
         q = Block8._new(self.rows, self.cols, self._f, self.device)
         q.codes.view(torch.uint8).copy_(self.codes.view(torch.uint8))
@@ -275,8 +283,7 @@ def weight_grad(dy, q: Block8, dtype=torch.float32, bias_dtype=None, weight: boo
     _b8(q, "weight_grad checkpoint")
     assert dy.dim() == 2 and dy.shape[0] == q.rows and dy.shape[1] >= 1, (tuple(dy.shape), tuple(q.shape))
     _same_device(q._dev, dy)
-    if not _rows_apart(dy):
-        dy = dy.contiguous()
+    dy = _near_rows(dy)
     if weight:
         _dtype(dtype, "weight_grad")
     if bias_dtype is not None:

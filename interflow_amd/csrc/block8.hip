@@ -22,9 +22,10 @@ void quantize2_kernel(B8Rows q, B8Rows q2) {
 
 template <class T>
 __global__ __launch_bounds__(256)
-void quantize_t_kernel(B8Cols q) {
+void quantize_t_kernel(B8Cols q, int tiles) {
     __shared__ __attribute__((aligned(16))) uint8_t sm[B8_COLS_LDS];
-    b8_quantize_cols<T>(q, sm, blockIdx.x, blockIdx.y);
+    const int kb = blockIdx.x / tiles;
+    b8_quantize_cols<T>(q, sm, blockIdx.x - kb * tiles, kb);
 }
 
 // ------------------------------------------------------------------------------------------------ restore
@@ -214,9 +215,9 @@ extern "C" int ifl_block8_quantize(const void* x, int xtype, int64_t row_stride,
     hipStream_t st = (hipStream_t)stream;
     if (col_stride != 1) {
         const int64_t gx = (rows + 63) / 64;
-        IFL_CHECK_ARG(gx <= 0x7fffffff && KB <= 65535, IFL_ENOTSUP, "block8_quantize: transposed %lld x %lld", (long long)rows, (long long)cols);
+        IFL_CHECK_ARG(gx * KB <= 0x7fffffff, IFL_ENOTSUP, "block8_quantize: transposed %lld x %lld", (long long)rows, (long long)cols);
         const B8Cols q = {x, col_stride, codes, ldc, scales, lds, rows, (int)cols, b8_pad(cols, ldc), fmt};
-        B8_DISPATCH(xtype, hipLaunchKernelGGL(HIP_KERNEL_NAME(quantize_t_kernel<T>), dim3((unsigned)gx, KB), dim3(256), 0, st, q));
+        B8_DISPATCH(xtype, hipLaunchKernelGGL(HIP_KERNEL_NAME(quantize_t_kernel<T>), dim3((unsigned)(gx * KB)), dim3(256), 0, st, q, (int)gx));
         IFL_LAUNCH_CHECK();
         return 0;
     }

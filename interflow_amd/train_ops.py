@@ -368,9 +368,7 @@ class _Linear8(torch.autograd.Function):
         raw, w = ctx.saved_tensors
         shape, bias_dtype, f = ctx.meta
         need_x, need_w, need_b, _ = ctx.needs_input_grad
-        g = g.reshape(-1, w.shape[0])
-        if not block8._rows_apart(g):
-            g = g.contiguous()
+        g = block8._near_rows(g.reshape(-1, w.shape[0]))
         dx, dw, db = block8._linear_bwd(g, raw, w, need_x, need_w, bias_dtype if need_b else None, f)
         return dx if dx is None or len(shape) == 2 else dx.view(shape), dw, db, None
 

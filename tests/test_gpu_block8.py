@@ -409,6 +409,38 @@ def test_linear8_parts_of_the_gradient():
         assert not train_ops.linear8(full[0], full[1]).requires_grad
 
 
+def test_second_derivatives_are_refused():
+    g = gen(15)
+    x, w = rand(g, 8, 64).requires_grad_(), rand(g, 16, 64).requires_grad_()
+    r, b, l = (t.requires_grad_() for t in (torch.nn.functional.pad(rand(g, 1, 4, 4, 64), (0, 0, 1, 1, 1, 1)), rand(g, 64), rand(g, 64)))
+    for y, leaf in ((train_ops.linear8(x, w), x), (train_ops.an_relu8_ring(r, b, l)[0], r)):
+        d, = torch.autograd.grad((y * y).sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError):
+            d.sum().backward()
+
+
+def test_rows_far_apart():
+    """Rows of gradients and codes further apart than the products reach, and single rows with such a stride."""
+    g = gen(16)
+    far = (1 << 23) + 16
+    store = torch.zeros(2 * far + 64, dtype=torch.bfloat16, device="cuda")
+    dy = torch.as_strided(store, (3, 64), (far, 1))
+    dy.copy_(rand(g, 3, 64))
+    q = block8.quantize(rand(g, 3, 40))
+    assert torch.equal(block8.weight_grad(dy, q)[0], block8.weight_grad(dy.contiguous(), q)[0])
+    assert torch.equal(block8.weight_grad(dy[:1], block8.Block8(q.codes[:1], q.scales[:1]))[0],
+                       block8.weight_grad(dy[:1].contiguous(), block8.Block8(q.codes[:1].contiguous(), q.scales[:1]))[0])
+    p = block8.quantize(dy)
+    assert torch.equal(p.codes.float(), block8.quantize(dy.contiguous()).codes.float())
+    codes = torch.as_strided(store.view(torch.uint8).view(p.codes.dtype), (3, 64), (far, 1))
+    codes.view(torch.uint8).copy_(p.codes.view(torch.uint8))
+    w = block8.quantize(rand(g, 50, 64))
+    want = block8.matmul(p, w)
+    assert torch.equal(block8.matmul(block8.Block8(codes, p.scales), w), want)
+    assert torch.equal(block8.matmul(block8.Block8(codes[:1], p.scales[:1]), w), block8.matmul(block8.Block8(p.codes[:1], p.scales[:1]), w))
+    assert torch.equal(block8.linear(torch.as_strided(store, (1, 64), (far, 1), 8), w), block8.linear(store[8:72], w)[None])
+
+
 def test_linear8_refuses_a_changed_weight():
     g = gen(13)
     x, w = rand(g, 8, 64).requires_grad_(), rand(g, 16, 64).requires_grad_()
