@@ -88,14 +88,22 @@ def _size(what, *args):
     return fn(*args)
 
 
-def _scratch(n, dev):
-    """n bytes, or nothing."""
-    return torch.empty((n,), dtype=torch.uint8, device=dev) if n else None
+def _scratch(n, like):
+    """n bytes beside the tensor `like`, or nothing."""
+    return like.new_empty((n,), dtype=torch.uint8) if n else None
 
 
 def _rows_apart(t):
     """Columns contiguous and rows that do not overlap, as far as there are several."""
     return (t.shape[1] == 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1])
+
+
+def _rows_of(t, rows, cols):
+    """(t or a contiguous copy, distance of its rows) for a t whose columns may not be contiguous."""
+    rs, cs = t.stride()
+    if (cs == 1 or cols == 1) and (rows <= 1 or rs >= cols):
+        return t, rs if rows > 1 else cols
+    return t.contiguous(), cols
 
 
 _FAR = 1 << 23                                          # elements between rows that the products do not reach across
@@ -122,26 +130,28 @@ class Block8:
         f = _FMT_OF.get(codes.dtype)
         if f is None or scales.dtype != torch.float8_e8m0fnu:
             raise TypeError(f"Block8: codes in float8_e4m3fn or float8_e5m2 and scales in float8_e8m0fnu, got {codes.dtype} and {scales.dtype}")
-        assert codes.dim() == 2 and scales.dim() == 2 and codes.shape[1] >= 1, (tuple(codes.shape), tuple(scales.shape))
-        rows, cols = codes.shape
-        assert scales.shape == (rows, -(-cols // BLOCK)), (tuple(codes.shape), tuple(scales.shape))
-        self._dev = codes.get_device()
-        _same_device(self._dev, scales)
-        self._codes = codes = codes if _rows_apart(codes) else codes.contiguous()
-        self._scales = scales = scales if _rows_apart(scales) else scales.contiguous()
+        shape, blocks = codes.shape, scales.shape
+        assert len(shape) == 2 and len(blocks) == 2 and shape[1] >= 1, (tuple(shape), tuple(blocks))
+        rows, cols = shape
+        assert blocks[0] == rows and blocks[1] == (cols + 127) // 128, (tuple(shape), tuple(blocks))
+        self._dev = dev = codes.get_device()
+        if scales.get_device() != dev:
+            _same_device(dev, scales)
+        self._codes, self._ldc = codes, _ = _rows_of(codes, rows, cols)
+        self._scales, self._lds = scales, _ = _rows_of(scales, rows, blocks[1])
         self.rows, self.cols, self._f, self._raw = rows, cols, f, None
-        self._cp, self._ldc, self._sp, self._lds = codes.data_ptr(), _ld(codes), scales.data_ptr(), _ld(scales)
+        self._cp, self._sp = codes.data_ptr(), scales.data_ptr()
 
     @classmethod
-    def _new(cls, rows, cols, f, dev, raw=None):
-        """Room for rows x cols: one allocation, codes in rows of whole 16 bytes and behind them scales in rows of whole 4, which is
-        what the product's wide loads want."""
+    def _new(cls, rows, cols, f, like):
+        """Room for rows x cols beside the tensor `like`: one allocation, codes in rows of whole 16 bytes and behind them scales in rows
+        of whole 4, which is what the product's wide loads want."""
         q = cls.__new__(cls)
         ldc, lds = (cols + 15) // 16 * 16, (cols + 511) // 512 * 4
-        q._raw = raw = torch.empty((rows * (ldc + lds),), dtype=torch.uint8, device=dev) if raw is None else raw
+        q._raw = raw = like.new_empty((rows * (ldc + lds),), dtype=torch.uint8)
         q.rows, q.cols, q._f, q._dev, q._codes, q._scales = rows, cols, f, raw.get_device(), None, None
-        q._cp, q._ldc, q._lds = raw.data_ptr(), ldc, lds
-        q._sp = q._cp + rows * ldc
+        q._cp = p = raw.data_ptr()
+        q._ldc, q._lds, q._sp = ldc, lds, p + rows * ldc
         return q
 
     @property
@@ -170,6 +180,10 @@ class Block8:
     def fmt(self):
         return "e5m2" if self._f else "e4m3"
 
+    def _like(self):
+        """A tensor on its device."""
+        return self._codes if self._raw is None else self._raw
+
     def __repr__(self):
         return f"Block8({self.rows} x {self.cols}, {self.fmt}, {self.device})"
 
@@ -178,7 +192,7 @@ class Block8:
         one = self.rows <= 1
         if self._cp % 16 == 0 and self._sp % 4 == 0 and (one or (self._ldc % 16 == 0 and self._lds % 4 == 0 and self._ldc < _FAR)):
             return self
-        q = Block8._new(self.rows, self.cols, self._f, self.device)
+        q = Block8._new(self.rows, self.cols, self._f, self._like())
         q.codes.view(torch.uint8).copy_(self.codes.view(torch.uint8))
         q.scales.view(torch.uint8).copy_(self.scales.view(torch.uint8))
         return q
@@ -194,15 +208,12 @@ def _up(n, k):
     return (n + k - 1) // k * k
 
 
-def _matrix(x):
-    """(x, row stride, column stride) of a 2-dimensional x as the library reads it: one of the strides is 1."""
-    rows, cols = x.shape
+def _matrix(x, rows, cols):
+    """(x, row stride, column stride) of x [rows, cols] as the library reads it: one of the strides is 1."""
     rs, cs = x.stride()
     if cs == 1 or cols == 1:
         return x, rs, 1
-    if rows == 1 and cs:
-        return x, 1, cs
-    if rs == 1 and cs:
+    if cs and (rs == 1 or rows == 1):
         return x, 1, cs
     return x.contiguous(), cols, 1
 
@@ -213,8 +224,8 @@ def quantize(x, fmt: str = "e4m3") -> Block8:
     f = _format(fmt, "quantize")
     assert x.dim() == 2 and x.shape[1] >= 1, tuple(x.shape)
     rows, cols = x.shape
-    x, rs, cs = _matrix(x)
-    q = Block8._new(rows, cols, f, x.device)
+    x, rs, cs = _matrix(x, rows, cols)
+    q = Block8._new(rows, cols, f, x)
     _call("ifl_block8_quantize", q._dev, x.data_ptr(), t, rs, cs, q._cp, q._ldc, q._sp, q._lds, rows, cols, f)
     return q
 
@@ -223,7 +234,7 @@ def dequantize(q: Block8, dtype=torch.float32) -> torch.Tensor:
     """The values [rows, cols] that `q` stands for, rounded once to `dtype` (float16 overflows to infinity above 65504)."""
     _b8(q, "dequantize")
     t = _dtype(dtype, "dequantize")
-    out = torch.empty((q.rows, q.cols), dtype=dtype, device=q.device)
+    out = q._like().new_empty((q.rows, q.cols), dtype=dtype)
     _call("ifl_block8_dequantize", q._dev, q._cp, q._ldc, q._sp, q._lds, q._f, None, out.data_ptr(), t, q.cols, q.rows, q.cols)
     return out
 
@@ -247,8 +258,8 @@ def matmul(a: Block8, b: Block8, bias=None, dtype=torch.bfloat16) -> torch.Tenso
     assert b._dev == dev, f"{a} and {b}"
     bias, bp, bt = _bias(bias, N, dev)
     t = _dtype(dtype, "matmul")
-    out = torch.empty((M, N), dtype=dtype, device=a.device)
-    scratch = _scratch(4 * _size("ifl_block8_matmul_scratch_floats", M, N, K, t), out.device)
+    out = a._like().new_empty((M, N), dtype=dtype)
+    scratch = _scratch(4 * _size("ifl_block8_matmul_scratch_floats", M, N, K, t), out)
     _call("ifl_block8_matmul", dev, a._cp, _up(a._ldc, 16), a._sp, _up(a._lds, 4), a._f, b._cp, _up(b._ldc, 16), b._sp, _up(b._lds, 4), b._f, bp, bt,
           out.data_ptr(), t, N, scratch.data_ptr() if scratch is not None else None, M, N, K)
     return out
@@ -263,14 +274,12 @@ def linear(x, w: Block8, bias=None) -> torch.Tensor:
     assert len(shape) >= 1 and shape[-1] == K and N >= 1, (tuple(shape), tuple(w.shape))
     dev = x.get_device()
     assert w._dev == dev, f"x on cuda:{dev}, weights {w}"
-    bias, bp, bt = _bias(bias, N, dev)
-    x2 = x if len(shape) == 2 else x.reshape(-1, K)
-    if not _rows_apart(x2):
-        x2 = x2.contiguous()
+    bias, bp, bt = _bias(bias, N, dev) if bias is not None else (None, None, 0)
+    x2, ldx = _rows_of(x if len(shape) == 2 else x.reshape(-1, K), x.numel() // K, K)
     M = x2.shape[0]
-    out = torch.empty((*shape[:-1], N), dtype=x.dtype, device=x.device)
-    scratch = _scratch(_size("ifl_block8_linear_scratch_bytes", M, N, K, t), out.device)
-    _call("ifl_block8_linear", dev, x2.data_ptr(), t, _ld(x2), w._cp, _up(w._ldc, 16), w._sp, _up(w._lds, 4), w._f, bp, bt, out.data_ptr(), N,
+    out = x.new_empty((M, N) if len(shape) == 2 else (*shape[:-1], N))
+    scratch = _scratch(_size("ifl_block8_linear_scratch_bytes", M, N, K, t), x)
+    _call("ifl_block8_linear", dev, x2.data_ptr(), t, ldx, w._cp, _up(w._ldc, 16), w._sp, _up(w._lds, 4), w._f, bp, bt, out.data_ptr(), N,
           scratch.data_ptr() if scratch is not None else None, M, N, K)
     return out
 
@@ -298,9 +307,9 @@ def _wgrad(dy, cp, ldc, sp, lds, f, K, chan, dtype, bias_dtype):
     """dy [M, N], contiguous columns; codes [M, K] and scales by their addresses and row strides; chan float32 [K] or None."""
     M, N = dy.shape
     dev = dy.get_device()
-    dw = torch.empty((N, K), dtype=dtype, device=dy.device) if dtype is not None else None
-    db = torch.empty((N,), dtype=bias_dtype, device=dy.device) if bias_dtype is not None else None
-    scratch = _scratch(4 * _size("ifl_block8_wgrad_scratch_floats", M, N, K if dw is not None else 0, _TYPE[dy.dtype]), dy.device)
+    dw = dy.new_empty((N, K), dtype=dtype) if dtype is not None else None
+    db = dy.new_empty((N,), dtype=bias_dtype) if bias_dtype is not None else None
+    scratch = _scratch(4 * _size("ifl_block8_wgrad_scratch_floats", M, N, K if dw is not None else 0, _TYPE[dy.dtype]), dy)
     _call("ifl_block8_wgrad", dev, dy.data_ptr(), _TYPE[dy.dtype], _ld(dy), cp, ldc, sp, lds, f, chan.data_ptr() if chan is not None else None,
           dw.data_ptr() if dw is not None else None, _TYPE[dtype] if dw is not None else 0, K, db.data_ptr() if db is not None else None,
           _TYPE[bias_dtype] if db is not None else 0, scratch.data_ptr() if scratch is not None else None, M, N, K if dw is not None else 0)
@@ -312,30 +321,38 @@ def _linear_fwd(x2, w, bias, keep: bool):
     """(y [M, N], x's 8-bit blocks as one tensor, if they are to be kept): quantize x and w along K and multiply."""
     M, K = x2.shape
     N = w.shape[0]
-    t, wt = _TYPE[x2.dtype], _TYPE[w.dtype]
-    x2, rs, cs = _matrix(x2)
-    w, wrs, wcs = _matrix(w)
-    bias, bp, bt = _bias(bias, N, x2.get_device())
-    y = torch.empty((M, N), dtype=x2.dtype, device=x2.device)
-    q = Block8._new(M, K, 0, x2.device)
-    scratch = _scratch(_size("ifl_linear8_fwd_scratch_bytes", M, N, K, t), x2.device)
-    _call("ifl_linear8_fwd", q._dev, x2.data_ptr(), t, rs, cs, w.data_ptr(), wt, wrs, wcs, bp, bt, q._cp, q._sp, y.data_ptr(),
+    t, wt, dev = _TYPE[x2.dtype], _TYPE[w.dtype], x2.get_device()
+    x2, rs, cs = _matrix(x2, M, K)
+    w, wrs, wcs = _matrix(w, N, K)
+    bias, bp, bt = _bias(bias, N, dev) if bias is not None else (None, None, 0)
+    y = x2.new_empty((M, N))
+    codes, scales = M * ((K + 15) // 16 * 16), M * ((K + 511) // 512 * 4)
+    raw = x2.new_empty((codes + scales,), dtype=torch.uint8)
+    scratch = x2.new_empty((_size("ifl_linear8_fwd_scratch_bytes", M, N, K, t),), dtype=torch.uint8)
+    cp = raw.data_ptr()
+    _call("ifl_linear8_fwd", dev, x2.data_ptr(), t, rs, cs, w.data_ptr(), wt, wrs, wcs, bp, bt, cp, cp + codes, y.data_ptr(),
           scratch.data_ptr(), M, N, K)
-    return y, q._raw if keep else None
+    return y, raw if keep else None
 
 
 def _linear_bwd(g, raw, w, need_x, need_w, bias_dtype, f):
     """(dx, dw, db) of `_linear_fwd`; g [M, N] contiguous columns, raw the kept blocks of x."""
     M, N = g.shape
     K = w.shape[1]
-    t, wt, dev = _TYPE[g.dtype], _TYPE[w.dtype], g.device
-    w, wrs, wcs = _matrix(w)
-    dx = torch.empty((M, K), dtype=g.dtype, device=dev) if need_x else None
-    dw = torch.empty((N, K), dtype=w.dtype, device=dev) if need_w else None
-    db = torch.empty((N,), dtype=bias_dtype, device=dev) if bias_dtype is not None else None
-    scratch = _scratch(_size("ifl_linear8_bwd_scratch_bytes", M, N, K, t, int(need_x), int(need_w)), dev)
-    cp = raw.data_ptr() if need_w else None
-    _call("ifl_linear8_bwd", g.get_device(), g.data_ptr(), t, _ld(g), cp, cp + M * _up(K, 16) if need_w else None, w.data_ptr(), wt, wrs, wcs, f,
-          dx.data_ptr() if need_x else None, dw.data_ptr() if need_w else None, db.data_ptr() if db is not None else None,
-          _TYPE[bias_dtype] if db is not None else 0, scratch.data_ptr(), M, N, K)
+    t, wt = _TYPE[g.dtype], _TYPE[w.dtype]
+    w, wrs, wcs = _matrix(w, N, K)
+    dx = dw = db = dxp = dwp = dbp = cp = sp = None
+    if need_x:
+        dx = g.new_empty((M, K))
+        dxp = dx.data_ptr()
+    if need_w:
+        dw = w.new_empty((N, K))
+        dwp, cp = dw.data_ptr(), raw.data_ptr()
+        sp = cp + M * ((K + 15) // 16 * 16)
+    if bias_dtype is not None:
+        db = g.new_empty((N,), dtype=bias_dtype)
+        dbp = db.data_ptr()
+    scratch = g.new_empty((_size("ifl_linear8_bwd_scratch_bytes", M, N, K, t, int(need_x), int(need_w)),), dtype=torch.uint8)
+    _call("ifl_linear8_bwd", g.get_device(), g.data_ptr(), t, _ld(g), cp, sp, w.data_ptr(), wt, wrs, wcs, f, dxp, dwp, dbp,
+          _TYPE[bias_dtype] if bias_dtype is not None else 0, scratch.data_ptr(), M, N, K)
     return dx, dw, db
