@@ -206,11 +206,13 @@ void mm8_tile_kernel(MM8 q)
     auto nrow = [](int f) { return 16 * G * (f / G) + 4 * (f % G); };
 
     // a thread's rows of the scales (threads past the tile's rows repeat one): n side first
-    const uint8_t* sp[SR];
+    const uint8_t *sp[SR], *sb = q.sb, *sa = q.sa;
+    int64_t lsb = q.lsb, lsa = q.lsa;
+    asm volatile("" : "+s"(sb), "+s"(sa), "+s"(lsb), "+s"(lsa));         // (arguments chosen between per lane would be loaded per lane)
 #pragma unroll
     for (int i = 0; i < SR; ++i) {
         const int r = i * 64 * NW + threadIdx.x;
-        sp[i] = r < TN ? q.sb + min(n0 + r, q.N - 1) * q.lsb : q.sa + min(m0 + (r - TN), q.M - 1) * q.lsa;
+        sp[i] = r < TN ? sb + min(n0 + r, q.N - 1) * lsb : sa + min(m0 + (r - TN), q.M - 1) * lsa;
     }
     uint32_t snext[SR];
 
@@ -271,12 +273,13 @@ void mm8_tile_kernel(MM8 q)
         read_a(nxt, ks + 1, 0);
     };
 
-    if (!SPLIT && (int)threadIdx.x < TN) bias[threadIdx.x] = n0 + threadIdx.x < q.N ? mm8_bias(q, n0 + threadIdx.x) : 0.f;      // (the workgroup meets before it is read)
-    ask(k_first >> 2);                                                   // (k_first is a multiple of 4)
-    put(k_first >> 2);
+    // the first step's codes, the first scales and the bias are asked for together: one wait for all of them
     int ks = k_first;
+    if (ks < whole) fill(buf0, ks);
+    ask(k_first >> 2);                                                   // (k_first is a multiple of 4)
+    if (!SPLIT && (int)threadIdx.x < TN) bias[threadIdx.x] = n0 + threadIdx.x < q.N ? mm8_bias(q, n0 + threadIdx.x) : 0.f;
+    put(k_first >> 2);
     if (ks < whole) {
-        fill(buf0, ks);
         turn();
         fill(buf1, min(ks + 1, whole - 1));
         read_a(buf0, ks, 0);
