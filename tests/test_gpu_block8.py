@@ -611,6 +611,63 @@ def test_a_checkpoints_logs_may_not_change_before_they_are_used():
         late.restore()
 
 
+# ------------------------------------------------------------------------------------------------ offsets beyond 32 bits
+BIG = (70001, 32768)                                                          # 2.3e9 values; the last rows lie behind 2^31
+
+
+def _big(dtype):
+    return torch.randn(BIG, generator=torch.Generator("cuda").manual_seed(60), device="cuda", dtype=dtype)
+
+
+def test_large_quantize_restore_and_products():
+    x = _big(torch.bfloat16)
+    q = block8.quantize(x)
+    tail, rows = x[-3:].clone(), slice(BIG[0] - 3, BIG[0])
+    want = block8.quantize(tail)
+    assert torch.equal(q.codes[rows].float(), want.codes.float()) and torch.equal(q.scales[rows].float(), want.scales.float())
+    assert torch.equal(block8.dequantize(q, torch.bfloat16)[rows], block8.dequantize(want, torch.bfloat16))
+    t = block8.quantize(x.t())                                                # its last block of columns: x's last rows
+    assert torch.equal(t.codes[-70:, -1].float(), block8.quantize(x[-(BIG[0] % 128):, -70:].t()).codes[:, -1].float())
+    del t
+    g = gen(61)
+    w = block8.quantize(rand(g, 64, BIG[1]))
+    v, u = R.of(want), R.of(w)
+    close(block8.matmul(q, w, dtype=torch.float32)[rows], v @ u.t(), BIG[1], v.abs() @ u.abs().t())
+    close(block8.linear(x, w)[rows], v @ u.t(), BIG[1], v.abs() @ u.abs().t(), product8=True)
+    dy = rand(g, BIG[0], 8, dtype=torch.bfloat16)
+    dw = block8.weight_grad(dy, q)[0][:, -5:]
+    cols = block8.dequantize(q, torch.bfloat16)[:, -5:].double()
+    close(dw, dy.double().t() @ cols, BIG[0], dy.double().abs().t() @ cols.abs())
+
+
+def test_large_results_and_gradients():
+    g = gen(62)
+    a, b = block8.quantize(rand(g, BIG[0], 128)), block8.quantize(rand(g, BIG[1], 128))
+    y = block8.matmul(a, b)
+    v, u = R.of(block8.Block8(a.codes[-3:], a.scales[-3:])), R.of(b)
+    close(y[-3:], v @ u.t(), 128, v.abs() @ u.abs().t(), product8=True)
+    del y
+    dy, q = _big(torch.float32), block8.quantize(rand(g, BIG[0], 8))
+    dw, db = block8.weight_grad(dy, q, bias_dtype=torch.float32)
+    cols, v = dy[:, -5:].double(), R.of(q)
+    close(dw[-5:], cols.t() @ v, BIG[0] + 1, cols.abs().t() @ v.abs())
+    close(db[-5:], cols.sum(0), BIG[0], cols.abs().sum(0))
+
+
+def test_large_an_relu8():
+    x = torch.randn(1, 1500, 1500, 1024, generator=torch.Generator("cuda").manual_seed(63), device="cuda")
+    bias, logs = rand(gen(64), 1024), 0.1 * rand(gen(65), 1024)
+    leaf = x.detach().requires_grad_()
+    y, ck = train_ops.an_relu8_ring(leaf, bias, logs)
+    small = x[:, -3:, -4:].contiguous()                                      # the last two inner pixels of the last inner row
+    ys, cs = train_ops.an_relu8_ring(small, bias, logs)
+    assert torch.equal(y[:, -2, -3:], ys[:, -2, -3:])
+    assert torch.equal(ck.codes[:, -2, -3:].float(), cs.codes[:, -2, -3:].float())
+    y.backward(x)
+    want = torch.where(ys[:, -2, -3:-1] > 0, small[:, -2, -3:-1] * logs.exp(), 0.0)
+    assert torch.allclose(leaf.grad[:, -2, -3:-1], want, rtol=2.0 ** -21, atol=0)
+
+
 # ------------------------------------------------------------------------------------------------ streams, graphs, two at once
 def test_on_another_stream_and_concurrently():
     g = gen(31)
