@@ -12,6 +12,7 @@
 // tiles repeats it, was the slower way: its arithmetic does not fit beside the matrix instructions (2048 x 2048 over 65536 rows,
 // bf16: 615 us with it, 390 without; float32: 1644 and 841).
 #include "block8.h"
+#include <math.h>
 
 namespace {
 
@@ -455,7 +456,9 @@ __global__ void fill_zero_kernel(TW* p, int64_t ld, int rows, int cols)
 // Tiles of 128 x 128, or 256 x 256 where there are 32 of them, an eighth of them at most lies past the edge, and a workgroup gets 48 steps.
 // Measured (bf16; 128 / 256): 1024 x 2048 x 2048 33.0 / 40.3 us, 4096 x 2048 x 2048 56.7 / 59.5, 16384 x 2048 x 2048 156 / 141, 2048 x
 // 4096 x 4096 90.2 / 71.9, 16384 x 1024 x 1024 60.8 / 64.0, 16384 x 64 x 2048 42.5 / 50.0.  The rows are split until the card is full
-// (one workgroup on a CU of the large tiles, two of the small ones), each with four steps at least.
+// (one workgroup on a CU of the large tiles, two of the small ones), each with four steps at least, but not further than pays: a part
+// costs 1.6 us for each million of dw's values (written and read), a step 0.4 us (512 x 2048 x 2048: 32.3 us in two parts, 21.0 in
+// one; 256 x 1024 x 1024: 19.4 in two, 15.1 in one).
 struct WPlan { int tile, split, steps, cs_parts, y_tpr_log; int64_t cs_rows, x_floats, y_floats, part_floats, cs_floats; bool in_place; };
 WPlan wg8_plan(int64_t M, int64_t N, int64_t K, int dytype, bool aligned)
 {
@@ -468,6 +471,8 @@ WPlan wg8_plan(int64_t M, int64_t N, int64_t K, int dytype, bool aligned)
     const int64_t full = p.tile == 256 ? 256 : 512;
     int64_t s = 4 * n >= 3 * full ? 1 : full / n;
     if (s > steps * terms / 4) s = steps * terms / 4;
+    const double best = sqrt(0.4 * (double)(steps * terms) / (1.6e-6 * (double)N * (double)(K > 0 ? K : 1)));
+    if ((double)s > best + 0.5) s = (int64_t)(best + 0.5);
     if (s > 256) s = 256;
     if (s < 1) s = 1;
     p.steps = (int)((steps + s - 1) / s);
