@@ -312,9 +312,10 @@ int ifl_coupling_bwd(const float* z, const float* dzout, const float* dld, const
  * code row from `cols` to the next multiple of 16 (or ldc) are written as zeros.  rows = 0 does nothing.
  * ifl_block8_dequantize: out[r * ldo + c] = code * 2^e (* chan[c] unless NULL), rounded once to otype.
  * ifl_block8_matmul: out[m * ldo + n] = sum_k A[m][k] B[n][k] + bias[n] (bias may be NULL), A [M][K] and B [N][K] in 8-bit blocks,
- * code rows 16-byte and scale rows 4-byte aligned (ld* multiples of 16, ls* of 4; a row's last 16 and 4 bytes are read whole); sums in float32, rounded once to otype
- * (IFL_T_F32: with 24-bit products; else from the 8-bit instructions, see matmul8.hip).  scratch:
- * ifl_block8_matmul_scratch_floats floats (NULL if 0).
+ * code rows 16-byte and scale rows 4-byte aligned (ld* multiples of 16, ls* of 4; a row's last 16 and 4 bytes are read whole); products
+ * exact unless an operand has bits below 2^-133, sums in float32, rounded once to otype.  IFL_P_8BIT or-ed to otype (to xtype of the
+ * calls below, and wherever that goes): a 16-bit result may come from the scaled 8-bit instructions, up to twice as fast, which among 8
+ * products drop what is below 2^-13 of the largest (matmul8.hip).  scratch: ifl_block8_matmul_scratch_floats floats (NULL if 0).
  * ifl_block8_linear: the same with the m side x [M][K] (IFL_T_*, columns contiguous) quantized to e4m3 on the way; out has x's
  * type.  scratch: ifl_block8_linear_scratch_bytes bytes, 16-byte aligned (NULL if 0).
  * ifl_block8_wgrad: dw[n * ldw + k] = chan[k] sum_m dy[m * ldy + n] A[m][k] (chan may be NULL) and db[n] = sum_m dy[m * ldy + n]; dw or
@@ -324,6 +325,7 @@ int ifl_coupling_bwd(const float* z, const float* dzout, const float* dld, const
  * float32), and partial sums.  M = 0 gives zeros.                                                                            */
 enum { IFL_T_F32 = 0, IFL_T_BF16 = 1, IFL_T_F16 = 2 };
 enum { IFL_Q_E4M3 = 0, IFL_Q_E5M2 = 1 };
+enum { IFL_P_8BIT = 0x100 };
 int ifl_block8_quantize(const void* x, int xtype, int64_t row_stride, int64_t col_stride, uint8_t* codes, int64_t ldc, uint8_t* scales,
                         int64_t lds, int64_t rows, int64_t cols, int fmt, void* stream);
 int ifl_block8_dequantize(const uint8_t* codes, int64_t ldc, const uint8_t* scales, int64_t lds, int fmt, const float* chan, void* out,

@@ -6,9 +6,15 @@ even.  A value is off by at most 2^-4 of itself (e5m2: 2^-3), or by 2^-10 2^e (2
 block's largest.  NaN stays NaN; infinity stays infinity in e5m2 and becomes NaN in e4m3; neither changes the other values.
 
 * `quantize` / `dequantize`  -- to and from 8-bit blocks
-* `matmul`                   -- A B^T of two such matrices on the scaled 8-bit matrix instructions, sums in float32
+* `matmul`                   -- A B^T of two such matrices on the matrix cores
 * `linear`                   -- a layer whose weights are kept in 8-bit blocks (serving); `train_ops.linear8` is its training form
 * `weight_grad`              -- dy^T A (and dy's column sums) from a checkpoint A
+
+What a product keeps: the codes times their scales are multiplied exactly and summed in float32, like the other matrix products here.
+With `exact=False` a bfloat16 or float16 result comes from the scaled 8-bit matrix instructions instead, which are up to twice as fast
+on large products and keep less: among 8 products they drop what is below 2^-13 of the largest.  A result is then off by 4e-5
+of itself in the 2-norm for activations with outliers (rounding to float16 adds 2e-4, to bfloat16 1.7e-3), by up to 7 2^-13 of the
+sum of its products' magnitudes, and where large products cancel, what they leave is lost.  float32 results are always exact.
 
 Everything runs on the current stream of the tensors' device; nothing synchronises, and calls may be captured into a graph.
 There is no CPU fallback."""
@@ -24,6 +30,7 @@ _get_device = torch._C._cuda_getDevice
 BLOCK = 128
 _FMT = {"e4m3": 0, "e5m2": 1}
 _FMT_OF = {torch.float8_e4m3fn: 0, torch.float8_e5m2: 1}
+_8BIT = 0x100                                           # or-ed to a result's type: products by the 8-bit instructions
 _TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -250,25 +257,29 @@ def _bias(bias, n, dev):
     return bias, bias.data_ptr(), t
 
 
-def matmul(a: Block8, b: Block8, bias=None, dtype=torch.bfloat16) -> torch.Tensor:
-    """a [M, K] times b [N, K]^T (+ bias [N]) -> [M, N] of `dtype`.  Formats may differ.  Sums are float32, rounded once."""
+def matmul(a: Block8, b: Block8, bias=None, dtype=torch.bfloat16, exact: bool = True) -> torch.Tensor:
+    """a [M, K] times b [N, K]^T (+ bias [N]) -> [M, N] of `dtype`.  Formats may differ.  Products are exact (operands' bits below
+    2^-133 aside) and sums float32, rounded once; `exact=False` allows a 16-bit result the 8-bit instructions, which keep less (above)."""
     a, b = _b8(a, "matmul a")._aligned(), _b8(b, "matmul b")._aligned()
     M, K, N, dev = a.rows, a.cols, b.rows, a._dev
     assert b.cols == K and N >= 1, (tuple(a.shape), tuple(b.shape))
     assert b._dev == dev, f"{a} and {b}"
     bias, bp, bt = _bias(bias, N, dev)
     t = _dtype(dtype, "matmul")
+    p = t if exact else t | _8BIT
     out = a._like().new_empty((M, N), dtype=dtype)
-    scratch = _scratch(4 * _size("ifl_block8_matmul_scratch_floats", M, N, K, t), out)
+    scratch = _scratch(4 * _size("ifl_block8_matmul_scratch_floats", M, N, K, p), out)
     _call("ifl_block8_matmul", dev, a._cp, _up(a._ldc, 16), a._sp, _up(a._lds, 4), a._f, b._cp, _up(b._ldc, 16), b._sp, _up(b._lds, 4), b._f, bp, bt,
-          out.data_ptr(), t, N, scratch.data_ptr() if scratch is not None else None, M, N, K)
+          out.data_ptr(), p, N, scratch.data_ptr() if scratch is not None else None, M, N, K)
     return out
 
 
-def linear(x, w: Block8, bias=None) -> torch.Tensor:
+def linear(x, w: Block8, bias=None, exact: bool = True) -> torch.Tensor:
     """x [..., K] (float32, bfloat16 or float16) through a layer whose weights w [N, K] are kept in 8-bit blocks: x is quantized
-    along its last dimension (e4m3) and multiplied -> [..., N] of x's type."""
+    along its last dimension (e4m3) and multiplied as in `matmul` (`exact` too) -> [..., N] of x's type."""
     t = _real(x, "linear input")
+    if not exact:
+        t |= _8BIT
     w = _b8(w, "linear weights")._aligned()
     shape, K, N = x.shape, w.cols, w.rows
     assert len(shape) >= 1 and shape[-1] == K and N >= 1, (tuple(shape), tuple(w.shape))
@@ -317,11 +328,13 @@ def _wgrad(dy, cp, ldc, sp, lds, f, K, chan, dtype, bias_dtype):
 
 
 # ------------------------------------------------------------------------------------------------ the layer in training
-def _linear_fwd(x2, w, bias, keep: bool):
+def _linear_fwd(x2, w, bias, keep: bool, exact: bool):
     """(y [M, N], x's 8-bit blocks as one tensor, if they are to be kept): quantize x and w along K and multiply."""
     M, K = x2.shape
     N = w.shape[0]
     t, wt, dev = _TYPE[x2.dtype], _TYPE[w.dtype], x2.get_device()
+    if not exact:
+        t |= _8BIT
     x2, rs, cs = _matrix(x2, M, K)
     w, wrs, wcs = _matrix(w, N, K)
     bias, bp, bt = _bias(bias, N, dev) if bias is not None else (None, None, 0)
@@ -335,11 +348,13 @@ def _linear_fwd(x2, w, bias, keep: bool):
     return y, raw if keep else None
 
 
-def _linear_bwd(g, raw, w, need_x, need_w, bias_dtype, f):
+def _linear_bwd(g, raw, w, need_x, need_w, bias_dtype, f, exact: bool):
     """(dx, dw, db) of `_linear_fwd`; g [M, N] contiguous columns, raw the kept blocks of x."""
     M, N = g.shape
     K = w.shape[1]
     t, wt = _TYPE[g.dtype], _TYPE[w.dtype]
+    if not exact:
+        t |= _8BIT
     w, wrs, wcs = _matrix(w, N, K)
     dx = dw = db = dxp = dwp = dbp = cp = sp = None
     if need_x:

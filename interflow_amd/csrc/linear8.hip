@@ -22,6 +22,8 @@ extern "C" int ifl_linear8_fwd(const void* x, int xtype, int64_t x_rs, int64_t x
                                const void* bias, int btype, uint8_t* codes, uint8_t* scales, void* y, void* scratch, int64_t M, int64_t N,
                                int64_t K, void* stream)
 {
+    const int otype = xtype;
+    xtype &= ~IFL_P_8BIT;
     IFL_CHECK_ARG(sizes_ok(M, N, K), IFL_EINVAL, "linear8_fwd: %lld x %lld x %lld", (long long)M, (long long)N, (long long)K);
     IFL_CHECK_ARG(b8_type_ok(xtype) && b8_type_ok(wtype) && (!bias || b8_type_ok(btype)), IFL_EINVAL, "linear8_fwd: element types");
     if (M == 0) return 0;
@@ -37,7 +39,7 @@ extern "C" int ifl_linear8_fwd(const void* x, int xtype, int64_t x_rs, int64_t x
         if (int rc = ifl_block8_quantize(x, xtype, x_rs, x_cs, codes, code_ld(K), scales, scale_ld(K), M, K, IFL_Q_E4M3, stream)) return rc;
         if (int rc = ifl_block8_quantize(w, wtype, w_rs, w_cs, wc, code_ld(K), ws, scale_ld(K), N, K, IFL_Q_E4M3, stream)) return rc;
     }
-    return ifl_block8_matmul(codes, code_ld(K), scales, scale_ld(K), IFL_Q_E4M3, wc, code_ld(K), ws, scale_ld(K), IFL_Q_E4M3, bias, btype, y, xtype, N, part,
+    return ifl_block8_matmul(codes, code_ld(K), scales, scale_ld(K), IFL_Q_E4M3, wc, code_ld(K), ws, scale_ld(K), IFL_Q_E4M3, bias, btype, y, otype, N, part,
                              M, N, K, stream);
 }
 
@@ -45,13 +47,15 @@ extern "C" int64_t ifl_linear8_bwd_scratch_bytes(int64_t M, int64_t N, int64_t K
 {
     if (!sizes_ok(M, N, K)) return 0;
     const int64_t a = need_dx ? block_bytes(M, N) + block_bytes(K, N) + up16(4 * ifl_block8_matmul_scratch_floats(M, K, N, xtype)) : 0;
-    return a + 4 * ifl_block8_wgrad_scratch_floats(M, N, need_dw ? K : 0, xtype) + 16;
+    return a + 4 * ifl_block8_wgrad_scratch_floats(M, N, need_dw ? K : 0, xtype & ~IFL_P_8BIT) + 16;
 }
 
 extern "C" int ifl_linear8_bwd(const void* dy, int xtype, int64_t ldy, const uint8_t* codes, const uint8_t* scales, const void* w, int wtype,
                                int64_t w_rs, int64_t w_cs, int gfmt, void* dx, void* dw, void* db, int dbtype, void* scratch, int64_t M,
                                int64_t N, int64_t K, void* stream)
 {
+    const int otype = xtype;
+    xtype &= ~IFL_P_8BIT;
     IFL_CHECK_ARG(sizes_ok(M, N, K), IFL_EINVAL, "linear8_bwd: %lld x %lld x %lld", (long long)M, (long long)N, (long long)K);
     IFL_CHECK_ARG(b8_type_ok(xtype) && b8_type_ok(wtype) && b8_fmt_ok(gfmt) && (!db || b8_type_ok(dbtype)), IFL_EINVAL, "linear8_bwd: types");
     IFL_CHECK_ARG(M == 0 || (dy && (w || !dx) && ((codes && scales) || !dw)), IFL_EINVAL, "linear8_bwd: null pointer");
@@ -62,7 +66,7 @@ extern "C" int ifl_linear8_bwd(const void* dy, int xtype, int64_t ldy, const uin
     const bool sums = dw || db;
     uint8_t *gc = at, *gs = gc + up16(M * code_ld(N)), *wc = gc + block_bytes(M, N), *ws = wc + up16(K * code_ld(N));
     float* part = (float*)(wc + block_bytes(K, N));
-    if (dx) at = (uint8_t*)part + up16(4 * ifl_block8_matmul_scratch_floats(M, K, N, xtype));
+    if (dx) at = (uint8_t*)part + up16(4 * ifl_block8_matmul_scratch_floats(M, K, N, otype));
     // (w^T has rows of w's columns: next to each other in memory as a rule)
     const bool together = dx && sums && w_cs == 1;
     const B8Quant quant = {gc, gs, code_ld(N), scale_ld(N), gfmt,
@@ -74,7 +78,7 @@ extern "C" int ifl_linear8_bwd(const void* dy, int xtype, int64_t ldy, const uin
         if (int rc = sums ? gradients(1) : ifl_block8_quantize(dy, xtype, ldy, 1, gc, code_ld(N), gs, scale_ld(N), M, N, gfmt, stream)) return rc;
         if (!together)
             if (int rc = ifl_block8_quantize(w, wtype, w_cs, w_rs, wc, code_ld(N), ws, scale_ld(N), K, N, IFL_Q_E4M3, stream)) return rc;
-        if (int rc = ifl_block8_matmul(gc, code_ld(N), gs, scale_ld(N), gfmt, wc, code_ld(N), ws, scale_ld(N), IFL_Q_E4M3, nullptr, 0, dx, xtype, K, part, M, K, N, stream)) return rc;
+        if (int rc = ifl_block8_matmul(gc, code_ld(N), gs, scale_ld(N), gfmt, wc, code_ld(N), ws, scale_ld(N), IFL_Q_E4M3, nullptr, 0, dx, otype, K, part, M, K, N, stream)) return rc;
     }
     return sums ? gradients(dx ? 2 : 3) : 0;
 }

@@ -1,16 +1,17 @@
-// matmul8.hip -- C[m][n] = sum_k A[m][k] B[n][k] (+ bias[n]) over rows in 8-bit blocks (block8.h), on the scaled 8-bit matrix
-// instructions of gfx950: v_mfma_scale_f32_16x16x128_f8f6f4 multiplies 16 x 128 by 128 x 16 codes and takes one E8M0 byte per row
-// and 32 values.  A block of 128 is one instruction deep, so every scale is applied by the instruction, exactly, and sums are
-// held in float32.
+// matmul8.hip -- C[m][n] = sum_k A[m][k] B[n][k] (+ bias[n]) over rows in 8-bit blocks (block8.h), in one of two ways:
+//
+// Exact (the default, and all float32 results): the codes times their scales, exact in bf16 (what is below its smallest step, 2^-133,
+// aside), go through v_mfma_f32_16x16x32_bf16, which keeps 24 bits.
+//
+// By the scaled 8-bit instructions, where the caller allows a 16-bit result that (IFL_P_8BIT): v_mfma_scale_f32_16x16x128_f8f6f4
+// multiplies 16 x 128 by 128 x 16 codes and takes one E8M0 byte per row and 32 values.  A block of 128 is one instruction deep, so
+// every scale is applied by the instruction, exactly, and what it returns is summed in float32.  But within 8 products it drops what is
+// below 2^-13 of the largest (measured): a result is off by up to 7 2^-13 of sum |a b|, and in the 2-norm by 4.1e-5 of itself for
+// activations with outliers and spread, 1.5e-5 for normal values (K = 4096).  Rounding to float16 adds 2.1e-4, to bfloat16 1.7e-3; but
+// where large products cancel, what they leave is lost.  Twice the rate: 8192 x 8192 x 4096 bf16 240 us, exact 451.
 //
 // Operands: the instruction's first is B (the n side) and its second A (the m side), so that a lane ends up with four
 // neighbouring n of one m: a contiguous store.
-//
-// What the 8-bit instructions keep: within 8 products they drop what is below 2^-13 of the largest (measured), so a result is off
-// by about 1.5e-5 of itself (2-norm; 1.7e-5 of sum |a b| at most in random data, 7 2^-13 of it at worst) -- a thirtieth of what
-// rounding it to float16 costs and a hundredth of bfloat16's.  A float32 result would show it: for that the codes times their
-// scales, exact in bf16 (what is below its smallest step, 2^-133, aside), go through v_mfma_f32_16x16x32_bf16, which keeps 24 bits, at half
-// the rate.
 //
 // Lane l gives row l % 16 and 32 of the 128 values; which 32 is free as long
 // as both operands agree (all of a block share a scale): 16 bytes from 16 (l / 16) and 16 from 64 + 16 (l / 16).
@@ -129,11 +130,11 @@ __device__ __forceinline__ void mm8_part(const MM8& q, const f32x4 (&acc)[NF][MF
 //
 // Workgroups go to the 8 XCDs in turn; an XCD takes a contiguous run of tiles, in groups of 8 along m, so that the 32 tiles
 // it works on at a time share rows of both operands in its own L2.
-template <int TN, int TM, int WN, int WM, int FA, int FB, bool EXACT, bool SPLIT>
+template <int TN, int TM, int WN, int WM, int FA, int FB, bool EXACT, bool SPLIT, int G>
 __global__ __launch_bounds__(64 * WN * WM, 1)
 void mm8_tile_kernel(MM8 q)
 {
-    constexpr int NW = WN * WM, NF = TN / WN / 16, MF = TM / WM / 16, G = EXACT ? 1 : 2;
+    constexpr int NW = WN * WM, NF = TN / WN / 16, MF = TM / WM / 16;
     constexpr int CH = (TN + TM) * 8, PER = CH / (64 * NW);              // 16-byte pieces of a step, per thread
     constexpr int D = 1, R = 2 * D;                                          // n-fragments read ahead, and the registers they rotate through
     static_assert(NF % R == 0 && D < R, "");
@@ -312,7 +313,7 @@ void mm8_tile_kernel(MM8 q)
     if constexpr (SPLIT) mm8_part<NF, MF, G>(q, acc, mw, nw);
     else {
         const float* bs = bias + wn * NF * 16 + 4 * G * g;
-        if constexpr (EXACT) mm8_results<float, NF, MF, G>(q, acc, mw, nw, bs);
+        if constexpr (G == 1) mm8_results<float, NF, MF, G>(q, acc, mw, nw, bs);
         else if (q.otype == IFL_T_BF16) mm8_results<__bf16, NF, MF, G>(q, acc, mw, nw, bs);
         else mm8_results<_Float16, NF, MF, G>(q, acc, mw, nw, bs);
     }
@@ -429,7 +430,7 @@ void mm8_skinny_kernel(MM8 q)
         for (int w = 1; w < SK_WAVES; ++w) t += red[w][i];
         if (m < q.M && nn < q.N) {
             t += mm8_bias(q, nn);
-            if constexpr (EXACT) ((float*)q.out)[m * q.ldo + nn] = t;
+            if (q.otype == IFL_T_F32) ((float*)q.out)[m * q.ldo + nn] = t;
             else if (q.otype == IFL_T_BF16) ((__bf16*)q.out)[m * q.ldo + nn] = (__bf16)t;
             else ((_Float16*)q.out)[m * q.ldo + nn] = (_Float16)t;
         }
@@ -438,15 +439,17 @@ void mm8_skinny_kernel(MM8 q)
 
 // ------------------------------------------------------------------------------------------------ which of them
 // Few rows: the skinny kernel.  Else the tile that costs least.  With n tiles on a CU, halfway between the busiest one's and the mean, a
-// product takes in us at K = 2048 about 2 + 4.4 n in tiles of 64 x 64, 7 + 10.5 n of 128 x 128, 4 + 34 n of 256 x 256; the second terms grow with
-// K (float32 results 1.6 times that, and at most 128: their fragments are held as bf16).  Measured, 64 / 128 / 256: 1024 x 2048 10.7 / 16.2 /
+// product takes in us at K = 2048 about 2 + 4.4 n in tiles of 64 x 64, 7 + 10.5 n of 128 x 128, 4 + 34 n of 256 x 256 by the 8-bit instructions;
+// the second terms grow with K, and are all about 1.6 times that where products are exact: one rule serves both.  Measured, 64 / 128 / 256,
+// exact, bf16: 1024 x 2048 18.1 / 25.9 / 55.7, 2048 x 2048 31.0 / 27.4 / 57.3, 16384 x 512 51.4 / 38.4 / 59.1, 3584 x 3584 78.7 / 68.8 / 60.2, 8192 x
+// 2048 98.2 / 70.9 / 61.9, 5000 x 1000 35.2 / 37.1; by the 8-bit instructions 1024 x 2048 10.7 / 16.2 /
 // 30.7, 2048 x 2048 18.5 / 18.4 / 33, 16384 x 512 35.6 / 25.5 / 33.8, 3584 x 3584 52.8 / 43.4 / 36.3, 8192 x 2048 69.2 / 47.7 / 39.0, 5000 x 1000
 // 24.9 / 22.6, and at K = 4096 48.1 / 37.7.  A product of few tiles and a long K is split along K.
 // The skinny kernel quantizes the m side itself where that is at most 32768 values: then it is the faster way, in a graph (1 x 2048 x
 // 2048: 3.5 us, 6.9 with a launch for it; 16 x 2048 x 2048: 6.2 and 7.3) and out of one (9 and 13.6).
 bool mm8_own(int64_t M, int64_t K) { return M <= 16 && M * K <= 32768; }
 struct Plan { int kind, tile, split, ksteps; };
-Plan mm8_plan(int64_t M, int64_t N, int64_t K, int otype)
+Plan mm8_plan(int64_t M, int64_t N, int64_t K)
 {
     Plan p = {0, 0, 1, 0};
     if (M <= 32) { p.kind = M <= 16 ? 1 : 2; return p; }
@@ -457,7 +460,7 @@ Plan mm8_plan(int64_t M, int64_t N, int64_t K, int otype)
     };
     const double c64 = cost(64, 2, 4.4), c128 = cost(128, 7, 10.5), c256 = cost(256, 4, 34);
     p.tile = c64 <= c128 ? 64 : 128;
-    if (otype != IFL_T_F32 && c256 < c64 && c256 < c128) p.tile = 256;
+    if (c256 < c64 && c256 < c128) p.tile = 256;
     const int64_t n = tiles(p.tile), steps = (K + B8_BLK - 1) / B8_BLK;
     if (p.tile == 64 && n <= 128 && steps >= 8) {
         int64_t s = 256 / n;
@@ -469,15 +472,18 @@ Plan mm8_plan(int64_t M, int64_t N, int64_t K, int otype)
     return p;
 }
 
+// whether a result of this type, perhaps with IFL_P_8BIT, gets exact products
+bool mm8_exact(int otype) { return otype != (IFL_T_BF16 | IFL_P_8BIT) && otype != (IFL_T_F16 | IFL_P_8BIT); }
+
 template <int FA, int FB>
-int mm8_launch(MM8 q, const Plan& p, hipStream_t st)
+int mm8_launch(MM8 q, const Plan& p, bool exact, hipStream_t st)
 {
     const bool f32 = q.otype == IFL_T_F32;
     if (p.kind) {
         const dim3 grid((unsigned)((q.N + 15) / 16)), block(64 * SK_WAVES);
 #define MM8_SK(MF, EX) hipLaunchKernelGGL(HIP_KERNEL_NAME(mm8_skinny_kernel<MF, FA, FB, EX, false, float>), grid, block, 0, st, q)
-        if (p.kind == 1) { if (f32) MM8_SK(1, true); else MM8_SK(1, false); }
-        else { if (f32) MM8_SK(2, true); else MM8_SK(2, false); }
+        if (p.kind == 1) { if (exact) MM8_SK(1, true); else MM8_SK(1, false); }
+        else { if (exact) MM8_SK(2, true); else MM8_SK(2, false); }
         IFL_LAUNCH_CHECK();
         return 0;
     }
@@ -486,11 +492,11 @@ int mm8_launch(MM8 q, const Plan& p, hipStream_t st)
     q.per_xcd = (q.tiles_m * q.tiles_n + 7) / 8;
     q.split = p.split; q.ksteps = p.ksteps;
     const dim3 grid(8 * q.per_xcd, p.split);
-#define MM8_TILE(T, WN, WM, EX, SP) hipLaunchKernelGGL(HIP_KERNEL_NAME(mm8_tile_kernel<T, T, WN, WM, FA, FB, EX, SP>), grid, dim3(64 * WN * WM), 0, st, q)
-    if (p.tile == 256) MM8_TILE(256, 2, 4, false, false);
-    else if (p.tile == 128) { if (f32) MM8_TILE(128, 2, 2, true, false); else MM8_TILE(128, 2, 2, false, false); }
-    else if (p.split == 1) { if (f32) MM8_TILE(64, 2, 2, true, false); else MM8_TILE(64, 2, 2, false, false); }
-    else { if (f32) MM8_TILE(64, 2, 2, true, true); else MM8_TILE(64, 2, 2, false, true); }
+#define MM8_TILE(T, WN, WM, EX, SP, G) hipLaunchKernelGGL(HIP_KERNEL_NAME(mm8_tile_kernel<T, T, WN, WM, FA, FB, EX, SP, G>), grid, dim3(64 * WN * WM), 0, st, q)
+    if (p.tile == 256) { if (f32) MM8_TILE(256, 2, 4, true, false, 1); else if (exact) MM8_TILE(256, 2, 4, true, false, 2); else MM8_TILE(256, 2, 4, false, false, 2); }
+    else if (p.tile == 128) { if (f32) MM8_TILE(128, 2, 2, true, false, 1); else if (exact) MM8_TILE(128, 2, 2, true, false, 2); else MM8_TILE(128, 2, 2, false, false, 2); }
+    else if (p.split == 1) { if (f32) MM8_TILE(64, 2, 2, true, false, 1); else if (exact) MM8_TILE(64, 2, 2, true, false, 2); else MM8_TILE(64, 2, 2, false, false, 2); }
+    else { if (exact) MM8_TILE(64, 2, 2, true, true, 1); else MM8_TILE(64, 2, 2, false, true, 2); }
     IFL_LAUNCH_CHECK();
     if (p.split > 1) {
         const dim3 jg((unsigned)((q.N + 255) / 256), (unsigned)q.M);
@@ -518,10 +524,10 @@ int mm8_check(int64_t M, int64_t N, int64_t K, const uint8_t* b, int64_t ldb, co
 
 }  // namespace
 
-extern "C" int64_t ifl_block8_matmul_scratch_floats(int64_t M, int64_t N, int64_t K, int otype)
+extern "C" int64_t ifl_block8_matmul_scratch_floats(int64_t M, int64_t N, int64_t K, int)
 {
     if (M < 1 || N < 1 || K < 1) return 0;
-    const Plan p = mm8_plan(M, N, K, otype);
+    const Plan p = mm8_plan(M, N, K);
     return p.split > 1 ? p.split * M * N : 0;
 }
 
@@ -529,6 +535,8 @@ extern "C" int ifl_block8_matmul(const uint8_t* a, int64_t lda, const uint8_t* s
                                  const uint8_t* sb, int64_t lsb, int fb, const void* bias, int btype, void* out, int otype, int64_t ldo,
                                  float* scratch, int64_t M, int64_t N, int64_t K, void* stream)
 {
+    const bool exact = mm8_exact(otype);
+    otype &= ~IFL_P_8BIT;
     IFL_CHECK_ARG(b8_fmt_ok(fa) && b8_fmt_ok(fb), IFL_EINVAL, "block8_matmul: formats %d, %d", fa, fb);
     if (int rc = mm8_check(M, N, K, b, ldb, sb, lsb, bias, btype, out, otype, ldo)) return rc;
     if (M == 0) return 0;
@@ -537,16 +545,16 @@ extern "C" int ifl_block8_matmul(const uint8_t* a, int64_t lda, const uint8_t* s
     IFL_CHECK_ARG(lda % 16 == 0 && (uintptr_t)a % 16 == 0 && lsa % 4 == 0 && (uintptr_t)sa % 4 == 0, IFL_EINVAL,
                   "block8_matmul: codes in rows of whole, aligned 16 bytes, scales of whole, aligned 4");
     IFL_CHECK_ARG(lda < (1 << 23), IFL_ENOTSUP, "block8_matmul: rows of %lld bytes", (long long)lda);
-    const Plan p = mm8_plan(M, N, K, otype);
+    const Plan p = mm8_plan(M, N, K);
     IFL_CHECK_ARG(p.split == 1 || scratch, IFL_EINVAL, "block8_matmul: no scratch");
     MM8 q = {};
     q.a = a; q.b = b; q.sa = sa; q.sb = sb; q.lda = lda; q.ldb = ldb; q.lsa = lsa; q.lsb = lsb; q.bias = bias; q.btype = btype;
     q.out = out; q.otype = otype; q.ldo = ldo; q.M = M; q.N = N; q.K = (int)K; q.part = scratch;
     hipStream_t st = (hipStream_t)stream;
-    if (fa == 0 && fb == 0) return mm8_launch<0, 0>(q, p, st);
-    if (fa == 0) return mm8_launch<0, 1>(q, p, st);
-    if (fb == 0) return mm8_launch<1, 0>(q, p, st);
-    return mm8_launch<1, 1>(q, p, st);
+    if (fa == 0 && fb == 0) return mm8_launch<0, 0>(q, p, exact, st);
+    if (fa == 0) return mm8_launch<0, 1>(q, p, exact, st);
+    if (fb == 0) return mm8_launch<1, 0>(q, p, exact, st);
+    return mm8_launch<1, 1>(q, p, exact, st);
 }
 
 extern "C" int64_t ifl_block8_linear_scratch_bytes(int64_t M, int64_t N, int64_t K, int otype)
@@ -560,6 +568,9 @@ extern "C" int ifl_block8_linear(const void* x, int xtype, int64_t ldx, const ui
                                  const void* bias, int btype, void* out, int64_t ldo, void* scratch, int64_t M, int64_t N, int64_t K,
                                  void* stream)
 {
+    const bool exact = mm8_exact(xtype);
+    const int otype = xtype;
+    xtype &= ~IFL_P_8BIT;
     IFL_CHECK_ARG(b8_fmt_ok(fb) && b8_type_ok(xtype), IFL_EINVAL, "block8_linear: types");
     if (int rc = mm8_check(M, N, K, b, ldb, sb, lsb, bias, btype, out, xtype, ldo)) return rc;
     if (M == 0) return 0;
@@ -571,10 +582,11 @@ extern "C" int ifl_block8_linear(const void* x, int xtype, int64_t ldx, const ui
         q.M = M; q.N = N; q.K = (int)K; q.x = x; q.ldx = ldx;
         const int KB = ifl_cdiv((int)K, B8_BLK), sm = (int)M * KB * B8_BLK + (int)M * KB;
         const dim3 grid((unsigned)((N + 15) / 16)), block(64 * SK_WAVES);
+#define MM8_OWN2(FB, EX, TX) hipLaunchKernelGGL(HIP_KERNEL_NAME(mm8_skinny_kernel<1, 0, FB, EX, true, TX>), grid, block, sm, st, q)
 #define MM8_OWN(FB) do { \
-            if (xtype == IFL_T_F32) hipLaunchKernelGGL(HIP_KERNEL_NAME(mm8_skinny_kernel<1, 0, FB, true, true, float>), grid, block, sm, st, q); \
-            else if (xtype == IFL_T_BF16) hipLaunchKernelGGL(HIP_KERNEL_NAME(mm8_skinny_kernel<1, 0, FB, false, true, __bf16>), grid, block, sm, st, q); \
-            else hipLaunchKernelGGL(HIP_KERNEL_NAME(mm8_skinny_kernel<1, 0, FB, false, true, _Float16>), grid, block, sm, st, q); } while (0)
+            if (xtype == IFL_T_F32) MM8_OWN2(FB, true, float); \
+            else if (xtype == IFL_T_BF16) { if (exact) MM8_OWN2(FB, true, __bf16); else MM8_OWN2(FB, false, __bf16); } \
+            else if (exact) MM8_OWN2(FB, true, _Float16); else MM8_OWN2(FB, false, _Float16); } while (0)
         if (fb == 0) MM8_OWN(0); else MM8_OWN(1);
         IFL_LAUNCH_CHECK();
         return 0;
@@ -585,5 +597,5 @@ extern "C" int ifl_block8_linear(const void* x, int xtype, int64_t ldx, const ui
     uint8_t* scales = codes + M * lda;
     float* part = (float*)(scales + M * lsa);                            // (both sizes are multiples of 4)
     if (int rc = ifl_block8_quantize(x, xtype, ldx, 1, codes, lda, scales, lsa, M, K, IFL_Q_E4M3, stream)) return rc;
-    return ifl_block8_matmul(codes, lda, scales, lsa, IFL_Q_E4M3, b, ldb, sb, lsb, fb, bias, btype, out, xtype, ldo, part, M, N, K, stream);
+    return ifl_block8_matmul(codes, lda, scales, lsa, IFL_Q_E4M3, b, ldb, sb, lsb, fb, bias, btype, out, otype, ldo, part, M, N, K, stream);
 }

@@ -355,35 +355,36 @@ class _Linear8(torch.autograd.Function):
     """y = Q(x) Q(w)^T + bias; the backward has Q(x) for a checkpoint (block8.py)."""
 
     @staticmethod
-    def forward(ctx, x, w, bias, f):
+    def forward(ctx, x, w, bias, f, exact):
         shape = x.shape
-        y, raw = block8._linear_fwd(x if len(shape) == 2 else x.reshape(-1, shape[-1]), w, bias, ctx.needs_input_grad[1])
+        y, raw = block8._linear_fwd(x if len(shape) == 2 else x.reshape(-1, shape[-1]), w, bias, ctx.needs_input_grad[1], exact)
         ctx.save_for_backward(raw, w)
-        ctx.meta = (shape, bias.dtype if bias is not None else None, f)
+        ctx.meta = (shape, bias.dtype if bias is not None else None, f, exact)
         return y if len(shape) == 2 else y.view(*shape[:-1], w.shape[0])
 
     @staticmethod
     @_once
     def backward(ctx, g):
         raw, w = ctx.saved_tensors
-        shape, bias_dtype, f = ctx.meta
-        need_x, need_w, need_b, _ = ctx.needs_input_grad
+        shape, bias_dtype, f, exact = ctx.meta
+        need_x, need_w, need_b, _, _ = ctx.needs_input_grad
         g = block8._near_rows(g.reshape(-1, w.shape[0]))
-        dx, dw, db = block8._linear_bwd(g, raw, w, need_x, need_w, bias_dtype if need_b else None, f)
-        return dx if dx is None or len(shape) == 2 else dx.view(shape), dw, db, None
+        dx, dw, db = block8._linear_bwd(g, raw, w, need_x, need_w, bias_dtype if need_b else None, f, exact)
+        return dx if dx is None or len(shape) == 2 else dx.view(shape), dw, db, None, None
 
 
-def linear8(x, weight, bias=None, grad_fmt: str = "e4m3"):
-    """x [..., K] times weight [N, K]^T (+ bias [N]) -> [..., N] in x's type, on the 8-bit matrix cores, with gradients.
+def linear8(x, weight, bias=None, grad_fmt: str = "e4m3", exact: bool = True):
+    """x [..., K] times weight [N, K]^T (+ bias [N]) -> [..., N] in x's type, of operands in 8-bit blocks, with gradients.
     Forward: x and weight are quantized along K in blocks of 128 (e4m3); x's 8-bit blocks are the checkpoint.  Backward: dx is the
     product of the quantized gradient (`grad_fmt`, along N) and the weight quantized along N; dw multiplies the gradient as it is
-    with the checkpoint (exact products); the bias' gradient is the gradient's column sum.  Sums are float32.  x and the gradient
-    float32, bfloat16 or float16; weight and bias each any of them (a float32 master weight under bfloat16 activations)."""
+    with the checkpoint (exact products); the bias' gradient is the gradient's column sum.  Products are exact and sums float32;
+    `exact=False` allows a 16-bit y and dx the 8-bit matrix instructions, which are faster and keep less (see `block8`).  x and the
+    gradient float32, bfloat16 or float16; weight and bias each any of them (a float32 master weight under bfloat16 activations)."""
     block8._real(x, "linear8 input")
     block8._real(weight, "linear8 weight")
     assert x.dim() >= 1 and weight.dim() == 2 and x.shape[-1] == weight.shape[1] and weight.numel() > 0, (tuple(x.shape), tuple(weight.shape))
     block8._same_device(x.get_device(), weight)
-    return _Linear8.apply(x, weight, bias, block8._format(grad_fmt, "linear8 grad_fmt"))
+    return _Linear8.apply(x, weight, bias, block8._format(grad_fmt, "linear8 grad_fmt"), bool(exact))
 
 
 class _Coupling(torch.autograd.Function):
