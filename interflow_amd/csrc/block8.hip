@@ -40,7 +40,9 @@ void dequantize_kernel(const uint8_t* __restrict__ codes, int64_t ldc, const uin
     const int rpb = 256 >> tpr_log;
     const int64_t step = (int64_t)gridDim.x * rpb;
     for (int64_t r0 = (int64_t)blockIdx.x * rpb + (threadIdx.x >> tpr_log); r0 < rows; r0 += U * step) {
-        for (int c = ((threadIdx.x & ((1 << tpr_log) - 1)) + (blockIdx.y << tpr_log)) * 8; c < cols; c += 8 * gridDim.y << tpr_log) {
+        // (counted in groups of 8 columns: columns themselves, up to 2^31 of them, would wrap at the last step)
+        for (int i8 = (threadIdx.x & ((1 << tpr_log) - 1)) + (blockIdx.y << tpr_log); i8 < (cols + 7) / 8; i8 += gridDim.y << tpr_log) {
+            const int c = i8 * 8;
             i32x2 w[U];
             int sb[U];
 #pragma unroll
