@@ -42,13 +42,23 @@ struct WG8 {
 
 // The next of the bf16 terms whose sum is a value, as a float with 16 low zero bits: its leading 8 significant bits; x becomes what is
 // left.  What is not finite is the first term alone.  (FIRST; of bf16 the first term is the value.)
-template <bool FIRST, class T>
-__device__ __forceinline__ uint32_t wg8_term(float& x) {
+// ALL: no term of a value that is not 0 is 0, for a checkpoint with infinities (e5m2), which a zero term would turn into NaN: where
+// nothing would be left, the last of a term's 8 bits is; the sum stays exact.  (Bits below 2^-133 are lost in this too: gradients below
+// 2^-117 may give NaN there.)  An infinite gradient is infinite in all terms.
+template <bool FIRST, bool ALL, class T>
+__device__ __forceinline__ uint32_t wg8_term(float& x, bool last) {
     if constexpr (sizeof(T) == 2 && !__is_same(T, _Float16)) return __float_as_uint(x);
     if (FIRST) x = __builtin_canonicalizef(x);                           // (a NaN has a high bit set)
-    const uint32_t t = __float_as_uint(x) & 0xffff0000u;
-    x -= __uint_as_float(t);
-    if (FIRST) x = x == x ? x : 0.f;
+    uint32_t t = __float_as_uint(x) & 0xffff0000u;
+    float left = x - __uint_as_float(t);
+    if constexpr (ALL) {
+        if (!last) {
+            t -= (min(t << 1, 1u) & ~min(__float_as_uint(left) << 1, 1u)) << 16;         // (in numbers: as branches it took 200 registers more)
+            left = x - __uint_as_float(t);
+        }
+        left = left == left ? left : x;
+    } else if (FIRST) left = left == left ? left : 0.f;
+    x = left;
     return t;
 }
 
@@ -97,7 +107,7 @@ __device__ __forceinline__ int wg8_row(int gg, int e) { return (gg >> 2) * 32 + 
 // 8-bit blocks as well.  The next x_blocks restore codes.  The others take up to 256 columns of cs_rows rows of dy, with column
 // sums on the way that are joined in LDS in a fixed order, and dy's terms, if the product does not read it in place.  (16384 x 2048,
 // both operands, bf16: 30 us; with dy's blocks 43, 25 more on its own; with 2048 x 2048 weights 47, 19 more on their own.)
-template <class T, int NP, bool QUANT, class TW>
+template <class T, int NP, bool QUANT, bool ALL, class TW>
 __global__ __launch_bounds__(256, NP > 1 ? 2 : 3)
 void wgrad8_prepare_kernel(WG8 q)
 {
@@ -201,8 +211,8 @@ void wgrad8_prepare_kernel(WG8 q)
                 for (int i = 0; i < 8; ++i)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const uint32_t lo = k ? wg8_term<false, T>(v[2 * e][i]) : wg8_term<true, T>(v[2 * e][i]);
-                        const uint32_t hi = k ? wg8_term<false, T>(v[2 * e + 1][i]) : wg8_term<true, T>(v[2 * e + 1][i]);
+                        const uint32_t lo = k ? wg8_term<false, ALL, T>(v[2 * e][i], k == NP - 1) : wg8_term<true, ALL, T>(v[2 * e][i], k == NP - 1);
+                        const uint32_t hi = k ? wg8_term<false, ALL, T>(v[2 * e + 1][i], k == NP - 1) : wg8_term<true, ALL, T>(v[2 * e + 1][i], k == NP - 1);
                         t[i][e] = (int)__builtin_amdgcn_perm(hi, lo, 0x07060302u);       // the high halves
                         __builtin_amdgcn_sched_barrier(0);
                     }
@@ -570,8 +580,9 @@ int b8_wgrad(int todo, const B8Quant* quant, const void* dy, int dytype, int64_t
         }
         const dim3 pg((unsigned)(q.w_blocks + q.x_blocks + y_blocks));
 #define WG8_P(TY, NP) do { \
-            if (!quant) hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_prepare_kernel<TY, NP, false, float>), pg, dim3(256), 0, st, q); \
-            else B8_DISPATCH(quant->wtype, hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_prepare_kernel<TY, NP, true, T>), pg, dim3(256), 0, st, q)); \
+            if (!quant && fmt == IFL_Q_E5M2) hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_prepare_kernel<TY, NP, false, (NP > 1), float>), pg, dim3(256), 0, st, q); \
+            else if (!quant) hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_prepare_kernel<TY, NP, false, false, float>), pg, dim3(256), 0, st, q); \
+            else B8_DISPATCH(quant->wtype, hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_prepare_kernel<TY, NP, true, false, T>), pg, dim3(256), 0, st, q)); \
         } while (0)
         if (dytype == IFL_T_F32) WG8_P(float, 3); else if (dytype == IFL_T_F16) WG8_P(_Float16, 2); else WG8_P(__bf16, 1);
         IFL_LAUNCH_CHECK();
