@@ -1,0 +1,14 @@
+"""How the library is compiled: no GPU and no compiler run needed."""
+import os
+import subprocess
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def test_no_source_is_compiled_with_packed_float32():
+    lines = subprocess.run(["make", "-n", "-B", "-C", os.path.join(ROOT, "interflow_amd", "csrc")], check=True, capture_output=True, text=True).stdout.splitlines()
+    compiles = [line for line in lines if " -c " in line]
+    sources = [f for f in os.listdir(os.path.join(ROOT, "interflow_amd", "csrc")) if f.endswith(".hip")]
+    assert len(compiles) == len(sources)
+    for line in compiles:
+        assert "-Xclang -target-feature -Xclang -packed-fp32-ops" in line, line

@@ -8,7 +8,7 @@ mkdir -p gpurun_exp/obj_$SUFFIX
 objs=""
 for f in api layout pointwise conv1 conv1x conv3 conv3w convg rrdb train_glue train_fused; do
   if [[ " $FILES " == *" $f "* ]]; then
-    /opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -ffp-contract=off $EXTRA -c interflow_amd/csrc/$f.hip -o gpurun_exp/obj_$SUFFIX/$f.o &
+    /opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -ffp-contract=off -Xclang -target-feature -Xclang -packed-fp32-ops $EXTRA -c interflow_amd/csrc/$f.hip -o gpurun_exp/obj_$SUFFIX/$f.o &
     objs="$objs gpurun_exp/obj_$SUFFIX/$f.o"
   else
     objs="$objs interflow_amd/csrc/$f.o"
