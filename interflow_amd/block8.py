@@ -24,9 +24,6 @@ import torch
 
 from . import hip
 
-_raw_stream = torch._C._cuda_getCurrentRawStream        # (a current_stream() object costs a small call more than its launch)
-_get_device = torch._C._cuda_getDevice
-
 BLOCK = 128
 _FMT = {"e4m3": 0, "e5m2": 1}
 _FMT_OF = {torch.float8_e4m3fn: 0, torch.float8_e5m2: 1}
@@ -71,6 +68,12 @@ def _same_device(dev, *ts):
 
 
 _fns = {}
+_raw_stream = _get_device = None                        # torch's own, bound at the first call: a build of torch without a GPU lacks them
+
+
+def _bind():
+    global _raw_stream, _get_device                     # (a current_stream() object costs a small call more than its launch)
+    _raw_stream, _get_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
 def _call(what, dev, *args):
@@ -78,6 +81,8 @@ def _call(what, dev, *args):
     fn = _fns.get(what)
     if fn is None:
         fn = _fns[what] = getattr(hip.lib(), what)
+    if _get_device is None:
+        _bind()
     if _get_device() == dev:
         rc = fn(*args, _raw_stream(dev))
     else:
