@@ -133,7 +133,8 @@ def _ld(t):
 
 class Block8:
     """A matrix in 8-bit blocks: `codes` [rows, cols] (torch.float8_e4m3fn or float8_e5m2) and `scales` [rows, ceil(cols / 128)]
-    (torch.float8_e8m0fnu), columns contiguous, rows any distance apart.  Made by `quantize`, or from tensors of that form."""
+    (torch.float8_e8m0fnu), columns contiguous, rows any distance apart.  Made by `quantize`, or from tensors of that form, which
+    every call reads as they then are."""
     __slots__ = ("rows", "cols", "_f", "_dev", "_raw", "_codes", "_scales", "_cp", "_ldc", "_sp", "_lds")
 
     def __init__(self, codes, scales):
@@ -149,10 +150,8 @@ class Block8:
         self._dev = dev = codes.get_device()
         if scales.get_device() != dev:
             _same_device(dev, scales)
-        self._codes, self._ldc = codes, _ = _rows_of(codes, rows, cols)
-        self._scales, self._lds = scales, _ = _rows_of(scales, rows, blocks[1])
+        self._codes, self._scales = codes, scales
         self.rows, self.cols, self._f, self._raw = rows, cols, f, None
-        self._cp, self._sp = codes.data_ptr(), scales.data_ptr()
 
     @classmethod
     def _new(cls, rows, cols, f, like):
@@ -196,18 +195,37 @@ class Block8:
         """A tensor on its device."""
         return self._codes if self._raw is None else self._raw
 
+    def _now(self):
+        """Itself, with the addresses and strides that its tensors have now (their owner may have given them other memory); or a
+        copy, if their columns are not contiguous."""
+        if self._raw is not None:
+            return self
+        codes, scales, rows, cols = self._codes, self._scales, self.rows, self.cols
+        blocks = (cols + 127) // 128
+        if codes.shape != (rows, cols) or scales.shape != (rows, blocks) or codes.get_device() != self._dev or scales.get_device() != self._dev:
+            raise RuntimeError(f"{self}: its tensors were given another shape or device: {tuple(codes.shape)} on {codes.device}, {tuple(scales.shape)} on {scales.device}")
+        if not (_rows_apart(codes) and _rows_apart(scales)):
+            return self._copy()
+        self._cp, self._ldc, self._sp, self._lds = codes.data_ptr(), _ld(codes), scales.data_ptr(), _ld(scales)
+        return self
+
+    def _copy(self):
+        """The same in memory of its own, rows whole 16 and 4 bytes."""
+        q = Block8._new(self.rows, self.cols, self._f, self._like())
+        q.codes.view(torch.uint8).copy_(self.codes.view(torch.uint8))
+        q.scales.view(torch.uint8).copy_(self.scales.view(torch.uint8))
+        return q
+
     def __repr__(self):
         return f"Block8({self.rows} x {self.cols}, {self.fmt}, {self.device})"
 
     def _aligned(self):
         """Itself, or a copy whose rows are whole, aligned 16 and 4 bytes (a single row's length does not matter)."""
+        self = self._now()
         one = self.rows <= 1
         if self._cp % 16 == 0 and self._sp % 4 == 0 and (one or (self._ldc % 16 == 0 and self._lds % 4 == 0 and self._ldc < _FAR)):
             return self
-        q = Block8._new(self.rows, self.cols, self._f, self._like())
-        q.codes.view(torch.uint8).copy_(self.codes.view(torch.uint8))
-        q.scales.view(torch.uint8).copy_(self.scales.view(torch.uint8))
-        return q
+        return self._copy()
 
 
 def _b8(q, name):
@@ -244,7 +262,7 @@ def quantize(x, fmt: str = "e4m3") -> Block8:
 
 def dequantize(q: Block8, dtype=torch.float32) -> torch.Tensor:
     """The values [rows, cols] that `q` stands for, rounded once to `dtype` (float16 overflows to infinity above 65504)."""
-    _b8(q, "dequantize")
+    q = _b8(q, "dequantize")._now()
     t = _dtype(dtype, "dequantize")
     out = q._like().new_empty((q.rows, q.cols), dtype=dtype)
     _call("ifl_block8_dequantize", q._dev, q._cp, q._ldc, q._sp, q._lds, q._f, None, out.data_ptr(), t, q.cols, q.rows, q.cols)
@@ -315,8 +333,10 @@ def weight_grad(dy, q: Block8, dtype=torch.float32, bias_dtype=None, weight: boo
         _dtype(bias_dtype, "weight_grad")
     if not weight and bias_dtype is None:
         return None, None
-    q = q._aligned() if weight else q
-    return _wgrad(dy, q._cp, _up(q._ldc, 16), q._sp, q._lds, q._f, q.cols, None, dtype if weight else None, bias_dtype)
+    if not weight:
+        return _wgrad(dy, None, 0, None, 0, 0, 0, None, None, bias_dtype)
+    q = q._aligned()
+    return _wgrad(dy, q._cp, _up(q._ldc, 16), q._sp, q._lds, q._f, q.cols, None, dtype, bias_dtype)
 
 
 def _wgrad(dy, cp, ldc, sp, lds, f, K, chan, dtype, bias_dtype):
