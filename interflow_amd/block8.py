@@ -219,8 +219,10 @@ class Block8:
     def __repr__(self):
         return f"Block8({self.rows} x {self.cols}, {self.fmt}, {self.device})"
 
-    def _aligned(self):
-        """Itself, or a copy whose rows are whole, aligned 16 and 4 bytes (a single row's length does not matter)."""
+    def aligned(self):
+        """Itself, or a copy whose rows are whole, aligned 16 and 4 bytes, as `quantize` makes them (a single row's length does not
+        matter).  `matmul`, `linear` and `weight_grad` make such a copy in every call that needs one: of weights built from tensors of
+        other layouts (scales of 5 bytes a row, say) keep this one instead."""
         self = self._now()
         one = self.rows <= 1
         if self._cp % 16 == 0 and self._sp % 4 == 0 and (one or (self._ldc % 16 == 0 and self._lds % 4 == 0 and self._ldc < _FAR)):
@@ -283,7 +285,7 @@ def _bias(bias, n, dev):
 def matmul(a: Block8, b: Block8, bias=None, dtype=torch.bfloat16, exact: bool = True) -> torch.Tensor:
     """a [M, K] times b [N, K]^T (+ bias [N]) -> [M, N] of `dtype`.  Formats may differ.  Products are exact (operands' bits below
     2^-133 aside) and sums float32, rounded once; `exact=False` allows a 16-bit result the 8-bit instructions, which keep less (above)."""
-    a, b = _b8(a, "matmul a")._aligned(), _b8(b, "matmul b")._aligned()
+    a, b = _b8(a, "matmul a").aligned(), _b8(b, "matmul b").aligned()
     M, K, N, dev = a.rows, a.cols, b.rows, a._dev
     assert b.cols == K and N >= 1, (tuple(a.shape), tuple(b.shape))
     assert b._dev == dev, f"{a} and {b}"
@@ -303,7 +305,7 @@ def linear(x, w: Block8, bias=None, exact: bool = True) -> torch.Tensor:
     t = _real(x, "linear input")
     if not exact:
         t |= _8BIT
-    w = _b8(w, "linear weights")._aligned()
+    w = _b8(w, "linear weights").aligned()
     shape, K, N = x.shape, w.cols, w.rows
     assert len(shape) >= 1 and shape[-1] == K and N >= 1, (tuple(shape), tuple(w.shape))
     dev = x.get_device()
@@ -335,7 +337,7 @@ def weight_grad(dy, q: Block8, dtype=torch.float32, bias_dtype=None, weight: boo
         return None, None
     if not weight:
         return _wgrad(dy, None, 0, None, 0, 0, 0, None, None, bias_dtype)
-    q = q._aligned()
+    q = q.aligned()
     return _wgrad(dy, q._cp, _up(q._ldc, 16), q._sp, q._lds, q._f, q.cols, None, dtype, bias_dtype)
 
 

@@ -54,3 +54,18 @@ def test_tensors_of_another_shape_are_refused():
     for call in (lambda: block8.dequantize(p), lambda: block8.matmul(p, w), lambda: block8.matmul(w, p), lambda: block8.linear(rand(12, 5, 300), p), lambda: block8.weight_grad(dy, p)):
         with pytest.raises(RuntimeError):
             call()
+
+
+@pytest.mark.parametrize("cols", [640, 150])
+def test_aligned_once(cols):
+    """Weights whose rows are not whole 16 and 4 bytes: their aligned form gives the same results and is not copied again."""
+    w, x = block8.quantize(rand(13, 40, cols)), rand(14, 20, cols)
+    p = block8.Block8(w.codes.contiguous(), w.scales.contiguous())
+    a = p.aligned()
+    assert a is not p and a.aligned() is a and w.aligned() is w
+    assert torch.equal(a.codes.view(torch.uint8), p.codes.view(torch.uint8)) and torch.equal(a.scales.view(torch.uint8), p.scales.view(torch.uint8))
+    assert torch.equal(block8.linear(x, a), block8.linear(x, p)) and torch.equal(block8.linear(x, a), block8.linear(x, w))
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_stats()["allocation.all.allocated"]
+    block8.linear(x[:1], a)
+    assert torch.cuda.memory_stats()["allocation.all.allocated"] == before + 1          # (its result; the launch quantizes the row itself)
