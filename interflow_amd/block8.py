@@ -375,6 +375,12 @@ def _linear_fwd(x2, w, bias, keep: bool, exact: bool):
     return y, raw if keep else None
 
 
+def _backward_reaches(N, K, need_x, need_w, need_b):
+    """Refuses a layer that the forward pass takes and the backward pass does not, before either."""
+    if need_x and N > (1 << 23) - 16 or (need_w or need_b) and N > 0x3fffff or need_w and K > 0x3fffff:
+        raise NotImplementedError(f"linear8: gradients of a weight of {N} x {K}")
+
+
 def _linear_bwd(g, raw, w, need_x, need_w, bias_dtype, f, exact: bool):
     """(dx, dw, db) of `_linear_fwd`; g [M, N] contiguous columns, raw the kept blocks of x."""
     M, N = g.shape

@@ -8,6 +8,8 @@ int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
 int64_t code_ld(int64_t cols) { return up16(cols); }
 int64_t scale_ld(int64_t cols) { return (cols + 511) / 512 * 4; }
 int64_t block_bytes(int64_t rows, int64_t cols) { return up16(rows * code_ld(cols)) + up16(rows * scale_ld(cols)); }
+// what the products and the weight gradient take: looked at before anything is launched
+constexpr int64_t PRODUCT_ROWS = 0x3fffffff, PRODUCT_LD = 1 << 23, WGRAD_COLS = 0x3fffff;
 bool sizes_ok(int64_t M, int64_t N, int64_t K) { return M >= 0 && N >= 1 && K >= 1 && M < ((int64_t)1 << 40) && N < ((int64_t)1 << 30) && K < ((int64_t)1 << 30); }
 
 }  // namespace
@@ -26,6 +28,7 @@ extern "C" int ifl_linear8_fwd(const void* x, int xtype, int64_t x_rs, int64_t x
     xtype &= ~IFL_P_8BIT;
     IFL_CHECK_ARG(sizes_ok(M, N, K), IFL_EINVAL, "linear8_fwd: %lld x %lld x %lld", (long long)M, (long long)N, (long long)K);
     IFL_CHECK_ARG(b8_type_ok(xtype) && b8_type_ok(wtype) && (!bias || b8_type_ok(btype)), IFL_EINVAL, "linear8_fwd: element types");
+    IFL_CHECK_ARG(M <= PRODUCT_ROWS && N <= PRODUCT_ROWS && code_ld(K) < PRODUCT_LD, IFL_ENOTSUP, "linear8_fwd: %lld x %lld x %lld", (long long)M, (long long)N, (long long)K);
     if (M == 0) return 0;
     IFL_CHECK_ARG(x && w && codes && scales && y, IFL_EINVAL, "linear8_fwd: null pointer");
     IFL_CHECK_ARG(w_rs == 1 || w_cs == 1 || N == 1, IFL_EINVAL, "linear8_fwd: strides of w");
@@ -58,6 +61,8 @@ extern "C" int ifl_linear8_bwd(const void* dy, int xtype, int64_t ldy, const uin
     xtype &= ~IFL_P_8BIT;
     IFL_CHECK_ARG(sizes_ok(M, N, K), IFL_EINVAL, "linear8_bwd: %lld x %lld x %lld", (long long)M, (long long)N, (long long)K);
     IFL_CHECK_ARG(b8_type_ok(xtype) && b8_type_ok(wtype) && b8_fmt_ok(gfmt) && (!db || b8_type_ok(dbtype)), IFL_EINVAL, "linear8_bwd: types");
+    IFL_CHECK_ARG(M <= PRODUCT_ROWS && (!dx || (K <= PRODUCT_ROWS && code_ld(N) < PRODUCT_LD)) && (!(dw || db) || (N <= WGRAD_COLS && ldy < PRODUCT_LD)) && (!dw || K <= WGRAD_COLS),
+                  IFL_ENOTSUP, "linear8_bwd: %lld x %lld x %lld, rows of dy %lld apart", (long long)M, (long long)N, (long long)K, (long long)ldy);
     IFL_CHECK_ARG(M == 0 || (dy && (w || !dx) && ((codes && scales) || !dw)), IFL_EINVAL, "linear8_bwd: null pointer");
     IFL_CHECK_ARG(M <= 1 || ldy >= N, IFL_EINVAL, "linear8_bwd: rows of dy %lld apart", (long long)ldy);
     IFL_CHECK_ARG(!dx || w_rs == 1 || w_cs == 1 || K == 1, IFL_EINVAL, "linear8_bwd: strides of w");

@@ -357,6 +357,8 @@ class _Linear8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias, f, exact):
         shape = x.shape
+        if w.shape[0] > 0x3fffff or w.shape[1] > 0x3fffff:
+            block8._backward_reaches(*w.shape, *ctx.needs_input_grad[:3])
         y, raw = block8._linear_fwd(x if len(shape) == 2 else x.reshape(-1, shape[-1]), w, bias, ctx.needs_input_grad[1], exact)
         ctx.save_for_backward(raw, w)
         ctx.meta = (shape, bias.dtype if bias is not None else None, f, exact)

@@ -125,3 +125,30 @@ def test_library_refuses(call, args):
 def test_library_refuses_channel_counts(C):
     with pytest.raises(NotImplementedError):
         hip.check(hip.lib().ifl_an_relu8_fwd(16, 16, 16, 16, 16, 16, 1, 4, 4, C, None), "ifl_an_relu8_fwd")
+
+
+BIG = 1 << 30
+
+
+@pytest.mark.parametrize("call, args", [
+    # (sizes that a later step would refuse, after the first had run)
+    ("ifl_linear8_fwd", (16, 0, 64, 1, 16, 0, 64, 1, None, 0, 16, 16, 16, 16, BIG, 8, 64, None)),
+    ("ifl_linear8_fwd", (16, 0, 64, 1, 16, 0, 64, 1, None, 0, 16, 16, 16, 16, 4, 8, 1 << 23, None)),
+    ("ifl_linear8_bwd", (16, 0, 8, 16, 16, 16, 0, 64, 1, 0, 16, None, None, 0, 16, BIG, 8, 64, None)),
+    ("ifl_linear8_bwd", (16, 0, 1 << 23, 16, 16, 16, 0, 64, 1, 0, 16, None, None, 0, 16, 4, 1 << 23, 64, None)),
+    ("ifl_linear8_bwd", (16, 0, 1 << 22, 16, 16, 16, 0, 64, 1, 0, 16, 16, None, 0, 16, 4, 1 << 22, 64, None)),
+    ("ifl_linear8_bwd", (16, 0, 8, 16, 16, 16, 0, 64, 1, 0, 16, 16, None, 0, 16, 4, 8, 1 << 22, None)),
+    ("ifl_linear8_bwd", (16, 0, 1 << 23, 16, 16, 16, 0, 64, 1, 0, 16, None, 16, 0, 16, 4, 8, 64, None)),
+])
+def test_layer_refuses_before_any_launch(call, args):
+    with pytest.raises(NotImplementedError):
+        hip.check(getattr(hip.lib(), call)(*args), call)
+
+
+def test_layer_refuses_what_its_backward_pass_would():
+    for sizes, need in (((1 << 23, 8), (1, 0, 0)), ((1 << 22, 8), (0, 1, 0)), ((1 << 22, 8), (0, 0, 1)), ((8, 1 << 22), (0, 1, 0))):
+        with pytest.raises(NotImplementedError):
+            block8._backward_reaches(*sizes, *need)
+    block8._backward_reaches((1 << 22) - 1, (1 << 22) - 1, 1, 1, 1)
+    block8._backward_reaches(8, 1 << 22, 1, 0, 1)
+    block8._backward_reaches((1 << 23) - 16, 1 << 22, 1, 0, 0)
