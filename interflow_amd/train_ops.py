@@ -244,14 +244,14 @@ class Checkpoint8:
     """An activation of `an_relu8_ring` in 8 bits: values v in 8-bit blocks (block8: e4m3, a scale per pixel and 128 channels) and
     the factor per channel that makes them y = v exp(logs).  codes [B, h+2, w+2, C], scales [B, h+2, w+2, ceil(C / 128)], chan [C].
     `raw` is both in one tensor of bytes, codes first."""
-    __slots__ = ("raw", "shape", "_chan", "_logs", "_version")
+    __slots__ = ("raw", "shape", "_chan", "_made", "_logs", "_version")
 
     def __init__(self, raw, shape, chan=None, logs=None):
-        self.raw, self.shape, self._chan, self._logs = raw, shape, chan, logs
+        self.raw, self.shape, self._chan, self._made, self._logs = raw, shape, chan, None, logs
         if logs is not None:
             self._version = None if logs.is_inference() else logs._version
             if self._version is None:
-                self._chan = torch.exp(logs.reshape(-1).float())
+                self._make_chan()
 
     @staticmethod
     def room(shape, like):
@@ -266,12 +266,25 @@ class Checkpoint8:
     def scales(self):
         return self.raw[self.shape.numel():].view(torch.float8_e8m0fnu).view(*self.shape[:3], -1)
 
+    def _make_chan(self):
+        """The factors, kept with the event behind them; but not what a capture makes: that has values in the graph's replays only."""
+        chan = torch.exp(self._logs.detach().reshape(-1).float())
+        if not torch.cuda.is_current_stream_capturing():
+            stream = torch.cuda.current_stream(chan.device)
+            self._chan, self._made = chan, (stream, stream.record_event())
+        return chan
+
     @property
     def chan(self):
         if self._chan is None:
-            if self._logs._version != self._version:
+            if self._version is not None and self._logs._version != self._version:
                 raise RuntimeError("an activation checkpoint's logs were changed in place before its channel factors were first used")
-            self._chan = torch.exp(self._logs.detach().reshape(-1).float())
+            return self._make_chan()
+        if self._made is not None and not torch.cuda.is_current_stream_capturing():          # (a capture begins behind all work)
+            here = torch.cuda.current_stream(self._chan.device)
+            if here != self._made[0]:
+                here.wait_event(self._made[1])
+                self._chan.record_stream(here)
         return self._chan
 
     def _where(self):
