@@ -42,9 +42,9 @@ struct WG8 {
 
 // The next of the bf16 terms whose sum is a value, as a float with 16 low zero bits: its leading 8 significant bits; x becomes what is
 // left.  What is not finite is the first term alone.  (FIRST; of bf16 the first term is the value.)
-// ALL: no term of a value that is not 0 is 0, for a checkpoint with infinities (e5m2), which a zero term would turn into NaN: where
-// nothing would be left, the last of a term's 8 bits is; the sum stays exact.  (Bits below 2^-133 are lost in this too: gradients below
-// 2^-117 may give NaN there.)  An infinite gradient is infinite in all terms.
+// ALL: no term of a value that is not 0 is 0, for a checkpoint with infinities (e5m2), which a zero term would turn into NaN.  Where
+// nothing is left 2^-110 + 2^-126 is, two terms more, or 2^-126 after the second: at most 2^-33 of the value, which is under what
+// the sums keep and leaves exact ones exact.  Values below 2^-77 go without (there an infinity may still become NaN).
 template <bool FIRST, bool ALL, class T>
 __device__ __forceinline__ uint32_t wg8_term(float& x, bool last) {
     if constexpr (sizeof(T) == 2 && !__is_same(T, _Float16)) return __float_as_uint(x);
@@ -52,11 +52,9 @@ __device__ __forceinline__ uint32_t wg8_term(float& x, bool last) {
     uint32_t t = __float_as_uint(x) & 0xffff0000u;
     float left = x - __uint_as_float(t);
     if constexpr (ALL) {
-        if (!last) {
-            t -= (min(t << 1, 1u) & ~min(__float_as_uint(left) << 1, 1u)) << 16;         // (in numbers: as branches it took 200 registers more)
-            left = x - __uint_as_float(t);
-        }
-        left = left == left ? left : x;
+        const float more = FIRST ? 0x1p-110f + 0x1p-126f : 0x1p-126f, least = FIRST ? 0x1p-77f : 0x1p-100f;
+        // (what is left of a value of at least `least` is more than `more`, or nothing; of an infinity it is NaN, which the maximum drops)
+        if (!last) left = copysignf(fmaxf(fabsf(left), fabsf(x) >= least ? more : 0.f), x);
     } else if (FIRST) left = left == left ? left : 0.f;
     x = left;
     return t;

@@ -49,3 +49,12 @@ def test_terms_of_a_gradient_are_exact_beside_infinities(dtype):
     dy = torch.ldexp(torch.trunc(f * 2.0 ** bits.float()), e - bits).clamp(-32752, 32752)         # 0 to 23 significant bits, finite in float16 (infinity times the zeros of q is NaN)
     dy = dy.to(DT[dtype]).cuda()
     assert torch.equal(block8.weight_grad(dy, q)[0], 2 * dy.t().float())
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+def test_whole_numbers_beside_infinities(dtype):
+    """Sums that float32 holds stay exact under an e5m2 checkpoint: what makes its terms all non-zero is below what a sum keeps."""
+    M, N, K, g = 700, 60, 90, gen(4)
+    dy = torch.randint(-9, 10, (M, N), generator=g).to(DT[dtype]).cuda()
+    x = torch.randint(-3, 4, (M, K), generator=g).float().cuda()
+    assert torch.equal(block8.weight_grad(dy, block8.quantize(x, "e5m2"))[0].double(), dy.double().t() @ x.double())
