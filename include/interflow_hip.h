@@ -341,6 +341,10 @@ int64_t ifl_block8_wgrad_scratch_floats(int64_t M, int64_t N, int64_t K, int dyt
 int ifl_block8_wgrad(const void* dy, int dytype, int64_t ldy, const uint8_t* codes, int64_t ldc, const uint8_t* scales, int64_t lds,
                      int fmt, const float* chan, void* dw, int dwtype, int64_t ldw, void* db, int dbtype, float* scratch, int64_t M,
                      int64_t N, int64_t K, void* stream);
+/* Which kernel a size goes to: its tile (ifl_block8_matmul: 16 or 32 rows at once, or a square of 64, 128 or 256) and, from bit 16
+ * on, the parts that its sum is split into.  0 for sizes that are none.                                                 */
+int ifl_block8_matmul_plan(int64_t M, int64_t N, int64_t K);
+int ifl_block8_wgrad_plan(int64_t M, int64_t N, int64_t K, int dytype);
 /* The layer y = Q(x) Q(w)^T + bias in training, one call per direction.  Forward: x [M][K] and w [N][K] (element (r, c) at
  * r *_rs + c *_cs, one of the two 1) are quantized along K (e4m3); codes [M][K rounded up to 16] and scales [M][ceil(K / 512) * 4]
  * receive x's blocks, the checkpoint; y [M][N] of x's type.  Backward, from dy [M][N] (x's type, columns contiguous): dx [M][K] =

@@ -531,6 +531,13 @@ extern "C" int64_t ifl_block8_matmul_scratch_floats(int64_t M, int64_t N, int64_
     return p.split > 1 ? p.split * M * N : 0;
 }
 
+extern "C" int ifl_block8_matmul_plan(int64_t M, int64_t N, int64_t K)
+{
+    if (M < 1 || N < 1 || K < 1) return 0;
+    const Plan p = mm8_plan(M, N, K);
+    return (p.kind ? 16 * p.kind : p.tile) | p.split << 16;
+}
+
 extern "C" int ifl_block8_matmul(const uint8_t* a, int64_t lda, const uint8_t* sa, int64_t lsa, int fa, const uint8_t* b, int64_t ldb,
                                  const uint8_t* sb, int64_t lsb, int fb, const void* bias, int btype, void* out, int otype, int64_t ldo,
                                  float* scratch, int64_t M, int64_t N, int64_t K, void* stream)

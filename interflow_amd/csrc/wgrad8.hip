@@ -513,6 +513,13 @@ extern "C" int64_t ifl_block8_wgrad_scratch_floats(int64_t M, int64_t N, int64_t
     return p.x_floats + p.y_floats + p.part_floats + p.cs_floats;
 }
 
+extern "C" int ifl_block8_wgrad_plan(int64_t M, int64_t N, int64_t K, int dytype)
+{
+    if (M < 1 || N < 1 || K < 1 || !b8_type_ok(dytype)) return 0;
+    const WPlan p = wg8_plan(M, N, K, dytype, false);
+    return p.tile | p.split << 16;
+}
+
 extern "C" int ifl_block8_wgrad(const void* dy, int dytype, int64_t ldy, const uint8_t* codes, int64_t ldc, const uint8_t* scales,
                                 int64_t lds, int fmt, const float* chan, void* dw, int dwtype, int64_t ldw, void* db, int dbtype,
                                 float* scratch, int64_t M, int64_t N, int64_t K, void* stream)

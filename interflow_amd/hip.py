@@ -151,6 +151,10 @@ def lib():
     L.ifl_block8_wgrad_scratch_floats.argtypes = [ll, ll, ll, c_int]
     L.ifl_block8_wgrad_scratch_floats.restype = ll
     L.ifl_block8_wgrad.argtypes = [vp, c_int, ll, vp, ll, vp, ll, c_int, vp, vp, c_int, ll, vp, c_int, vp, ll, ll, ll, vp]
+    L.ifl_block8_matmul_plan.argtypes = [ll, ll, ll]
+    L.ifl_block8_matmul_plan.restype = c_int
+    L.ifl_block8_wgrad_plan.argtypes = [ll, ll, ll, c_int]
+    L.ifl_block8_wgrad_plan.restype = c_int
     L.ifl_linear8_fwd.argtypes = [vp, c_int, ll, ll, vp, c_int, ll, ll, vp, c_int, vp, vp, vp, vp, ll, ll, ll, vp]
     L.ifl_linear8_fwd_scratch_bytes.argtypes = [ll, ll, ll, c_int]
     L.ifl_linear8_fwd_scratch_bytes.restype = ll
@@ -187,6 +191,7 @@ EXPORTS = ("ifl_version", "ifl_last_error", "ifl_step_param_floats", "ifl_step_f
            "ifl_train_bulk_conv1", "ifl_wino4_tiles", "ifl_wino4_kmajor", "ifl_wino4_dw", "ifl_conv2d_wgrad_batched", "ifl_conv2d_batched",
            "ifl_block8_quantize", "ifl_block8_dequantize", "ifl_block8_matmul", "ifl_block8_matmul_scratch_floats",
            "ifl_block8_linear", "ifl_block8_linear_scratch_bytes", "ifl_block8_wgrad_scratch_floats", "ifl_block8_wgrad",
+           "ifl_block8_matmul_plan", "ifl_block8_wgrad_plan",
            "ifl_linear8_fwd", "ifl_linear8_fwd_scratch_bytes", "ifl_linear8_bwd", "ifl_linear8_bwd_scratch_bytes",
            "ifl_an_relu8_blocks", "ifl_an_relu8_fwd", "ifl_an_relu8_bwd")
 
