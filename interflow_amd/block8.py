@@ -3,7 +3,7 @@
 Format (csrc/block8.h): a row's values in blocks of 128 (the last may be shorter).  A block has one power-of-two scale 2^e, e the
 smallest integer >= -126 with max |x| <= F 2^e (F = 448 for e4m3, 57344 for e5m2), and its codes are x 2^-e rounded to nearest
 even.  A value is off by at most 2^-4 of itself (e5m2: 2^-3), or by 2^-10 2^e (2^-17 2^e) where it is that small beside its
-block's largest.  NaN stays NaN; infinity stays infinity in e5m2 and becomes NaN in e4m3; neither changes the other values.
+block's largest; from 0.97 2^128 on (e5m2: 0.94 2^128) it rounds up to 2^128, which is infinity.  NaN stays NaN; infinity stays infinity in e5m2 and becomes NaN in e4m3; neither changes the other values.
 
 * `quantize` / `dequantize`  -- to and from 8-bit blocks
 * `matmul`                   -- A B^T of two such matrices on the matrix cores

@@ -242,7 +242,8 @@ def an_relu_ring(x_ring, bias, logs):
 
 class Checkpoint8:
     """An activation of `an_relu8_ring` in 8 bits: values v in 8-bit blocks (block8: e4m3, a scale per pixel and 128 channels) and
-    the factor per channel that makes them y = v exp(logs).  codes [B, h+2, w+2, C], scales [B, h+2, w+2, ceil(C / 128)], chan [C].
+    the factor per channel that makes them y = v exp(logs).  A v is off by at most 2^-4 of itself, or by 2^-10 of its block's scale
+    2^e where it is that small; a positive v that would round to zero is 2^-9 2^e instead, always upward.  codes [B, h+2, w+2, C], scales [B, h+2, w+2, ceil(C / 128)], chan [C].
     `raw` is both in one tensor of bytes, codes first."""
     __slots__ = ("raw", "shape", "_chan", "_made", "_logs", "_version")
 
