@@ -32,12 +32,14 @@ _checkpoint8 = [os.environ.get("IFL_CHECKPOINT8", "0") == "1"]
 
 def set_activation_checkpoints(bits=None) -> int:
     """How gradient-enabled passes keep the coupling networks' hidden activations for the backward pass: 32 (default) as float32,
-    8 in 8-bit blocks with a scale per pixel and 128 channels (`train_ops.an_relu8_ring`; environment IFL_CHECKPOINT8=1).  With 8
-    a pass is evaluated layer by layer and keeps 65 bytes per pixel and hidden layer instead of 512 (the level drivers hold their
-    activations in float32 arenas); outputs and the gradients of everything a network's input depends on are those of the float32
-    path, the weight, `logs` and conditioning-weight gradients behind a checkpoint are those of its values: each within 2^-4 of the
-    activation, or, where that is small beside the largest of its pixel's 128 channels (2^e, the block's scale, is 1/448 to 1/224
-    of that one), within 2^-10 2^e, and within 2^-9 2^e above it where it would round to zero: a positive activation stays one.  `None` only queries.  Takes effect for passes that start afterwards.  Returns the previous setting."""
+    8 in 8-bit blocks with a scale per pixel and 128 channels (`train_ops.an_relu8_ring`; environment IFL_CHECKPOINT8=1).
+    8 trades time for memory: a pass is evaluated layer by layer, without the level drivers and their float32 arenas, and keeps 65
+    bytes per pixel and hidden layer instead of 512 (eight 160 x 160 patches: 1.3 GB and 68 ms a step; the drivers 7.7 GB and 21 ms).
+    Outputs and the gradients of everything a network's input depends on are those of the float32 path; the weight, `logs` and
+    conditioning-weight gradients behind a checkpoint are those of its values: each within 2^-4 of the activation, or, where that is
+    small beside the largest of its pixel's 128 channels (2^e, the block's scale, is 1/448 to 1/224 of that one), within 2^-10 2^e, and
+    within 2^-9 2^e above it where it would round to zero: a positive activation stays one.
+    `None` only queries.  Takes effect for passes that start afterwards.  Returns the previous setting."""
     prev = 8 if _checkpoint8[0] else 32
     if bits is not None:
         if bits not in (8, 32):
