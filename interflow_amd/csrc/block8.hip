@@ -121,6 +121,8 @@ void an_relu8_fwd_kernel(const float* __restrict__ x, float* __restrict__ y, uin
 
 // dx = g s [code != 0];  part[blk][0:C] = sum g [..], part[blk][C:2C] = sum g v8 over the block's pixels (both still without
 // the factor s, which the reduction applies).  A block walks a contiguous range of pixels; a thread keeps its 8 channels.
+// Sums of 16 pixels are joined, then those sums, then the threads' in four rows: what is added up in one row stays short, and with it the
+// rounding (700 x 700 x 1024: at most 47 2^-24 of the magnitudes' sum; in one row after the other 58 2^-24 were seen).
 __global__ __launch_bounds__(256)
 void an_relu8_bwd_kernel(const float* __restrict__ g, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                          const float* __restrict__ logs, float* __restrict__ dx, float* __restrict__ part, uint32_t npx,
@@ -134,6 +136,8 @@ void an_relu8_bwd_kernel(const float* __restrict__ g, const uint8_t* __restrict_
     for (int i = 0; i < 8; ++i) { sg[i] = sv[i] = 0.f; s[i] = expf(logs[c + i]); }
     const uint32_t end = min(npx, (blockIdx.x + 1) * px_per_block);
     if (pl < ppb) {
+        float tg[8] = {}, tv[8] = {};
+        int row = 0;
         for (uint32_t p = blockIdx.x * px_per_block + pl; p < end; p += ppb) {
             const uint32_t line = p / (uint32_t)w2, px = p - line * w2, py = line % (uint32_t)h2;
             const bool inside = px > 0 && px < (uint32_t)w2 - 1 && py > 0 && py < (uint32_t)h2 - 1;
@@ -148,21 +152,30 @@ void an_relu8_bwd_kernel(const float* __restrict__ g, const uint8_t* __restrict_
             for (int i = 0; i < 8; ++i) {
                 const float e = v[i] == 0.f ? 0.f : d[i];
                 r[i] = e * s[i];
-                sg[i] += e;
-                sv[i] = fmaf(e, v[i] * sc, sv[i]);
+                tg[i] += e;
+                tv[i] = fmaf(e, v[i] * sc, tv[i]);
             }
             b8_store8<float>(dx + o, 8, r);
+            if (++row == 16) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) { sg[i] += tg[i]; sv[i] += tv[i]; tg[i] = tv[i] = 0.f; }
+                row = 0;
+            }
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) { sm[(pl * 2) * C + c + i] = sg[i]; sm[(pl * 2 + 1) * C + c + i] = sv[i]; }
+        for (int i = 0; i < 8; ++i) { sm[(pl * 2) * C + c + i] = sg[i] + tg[i]; sm[(pl * 2 + 1) * C + c + i] = sv[i] + tv[i]; }
     }
     __syncthreads();
     for (int k = threadIdx.x; k < 2 * C; k += 256) {
-        float t = 0.f;
-        for (int i = 0; i < ppb; ++i) t += sm[i * 2 * C + k];
-        part[(int64_t)blockIdx.x * 2 * C + k] = t;
+        float t[4] = {};
+        for (int i = 0; i < ppb; i += 4)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { const float v = sm[min(i + e, ppb - 1) * 2 * C + k]; t[e] += i + e < ppb ? v : 0.f; }
+        part[(int64_t)blockIdx.x * 2 * C + k] = (t[0] + t[1]) + (t[2] + t[3]);
     }
 }
+
+constexpr int AN8_BLOCKS = 1024;                                         // most blocks (partial sums) of the backward pass
 
 // out[k] = exp(logs[k mod C]) sum over blocks of part[blk][k].  Workgroup = 16 k, 64 threads to each, which take every 64th block and
 // meet in LDS in a fixed order: a thread's loads are all under way together (979 blocks of 128: 4.8 us; a wave to each k, whose
@@ -173,20 +186,28 @@ void an_relu8_reduce_kernel(const float* __restrict__ part, int nblk, const floa
 {
     __shared__ float red[64][17];
     const int i = threadIdx.x & 15, r = threadIdx.x >> 4, k = blockIdx.x * 16 + i;       // (2 C is a multiple of 16)
-    float t = 0.f;
-#pragma unroll 8
-    for (int b = r; b < nblk; b += 64) t += part[(int64_t)b * 2 * C + k];
+    float q[4] = {};
+    float v[AN8_BLOCKS / 64];
+#pragma unroll
+    for (int e = 0; e < AN8_BLOCKS / 64; ++e) v[e] = part[(int64_t)min(r + 64 * e, nblk - 1) * 2 * C + k];
+#pragma unroll
+    for (int e = 0; e < AN8_BLOCKS / 64; ++e) q[e & 3] += r + 64 * e < nblk ? v[e] : 0.f;
+    float t = (q[0] + q[1]) + (q[2] + q[3]);
+    auto pairs = [](const float (&u)[8]) { return ((u[0] + u[4]) + (u[2] + u[6])) + ((u[1] + u[5]) + (u[3] + u[7])); };
     red[r][i] = t;
     __syncthreads();
     if (r < 8) {
+        float u[8];
 #pragma unroll
-        for (int e = 1; e < 8; ++e) t += red[r + 8 * e][i];
-        red[r][i] = t;
+        for (int e = 0; e < 8; ++e) u[e] = red[r + 8 * e][i];
+        red[r][i] = pairs(u);
     }
     __syncthreads();
     if (r == 0) {
+        float u[8];
 #pragma unroll
-        for (int e = 1; e < 8; ++e) t += red[e][i];
+        for (int e = 0; e < 8; ++e) u[e] = red[e][i];
+        t = pairs(u);
         const int c = k < C ? k : k - C;
         (k < C ? dbias : dlogs)[c] = t * expf(logs[c]);
     }
@@ -212,8 +233,6 @@ B8Rows rows_job(const void* x, int64_t rs, uint8_t* codes, int64_t ldc, uint8_t*
     if (grid > 65536) grid = 65536;
     return {x, rs, codes, ldc, scales, lds, rows, (int)cols, b8_pad(cols, ldc), kgl, fmt, (int)grid, (int)share_rows(grid, (KB + (1 << kgl) - 1) >> kgl)};
 }
-
-constexpr int AN8_BLOCKS = 1024;                                         // most blocks (partial sums) of the backward pass
 
 }  // namespace
 
