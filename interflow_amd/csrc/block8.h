@@ -316,6 +316,9 @@ static inline bool b8_fmt_ok(int f) { return f == IFL_Q_E4M3 || f == IFL_Q_E5M2;
 int b8_quantize2(const void* x, int xtype, int64_t x_rs, const void* w, int wtype, int64_t w_rs, uint8_t* xc, uint8_t* xs, uint8_t* wc, uint8_t* ws,
                  int64_t ldc, int64_t lds, int64_t M, int64_t N, int64_t K, void* stream);
 
+// whether a product of these sizes, M from 0 on, N and K from 1 on, fits a launch
+bool b8_matmul_fits(int64_t M, int64_t N, int64_t K);
+
 // ifl_block8_wgrad in two steps for the layer whose other product needs dy in 8-bit blocks, and its weights along their columns: 1
 // prepares (and quantizes dy, if told where to, and w, if there is one), 2 multiplies and joins, 3 both.
 struct B8Quant { uint8_t *codes, *scales; int64_t ldc, lds; int fmt; B8Cols w; int wtype; };

@@ -250,7 +250,7 @@ extern "C" int ifl_block8_quantize(const void* x, int xtype, int64_t row_stride,
     hipStream_t st = (hipStream_t)stream;
     if (col_stride != 1) {
         const int64_t gx = (rows + 63) / 64;
-        IFL_CHECK_ARG(gx * KB <= 0x7fffffff, IFL_ENOTSUP, "block8_quantize: transposed %lld x %lld", (long long)rows, (long long)cols);
+        IFL_CHECK_ARG(gx < 1 << 24 && gx * KB < 1 << 24, IFL_ENOTSUP, "block8_quantize: transposed %lld x %lld", (long long)rows, (long long)cols);
         const B8Cols q = {x, col_stride, codes, ldc, scales, lds, rows, (int)cols, b8_pad(cols, ldc), fmt};
         B8_DISPATCH(xtype, hipLaunchKernelGGL(HIP_KERNEL_NAME(quantize_t_kernel<T>), dim3((unsigned)(gx * KB)), dim3(256), 0, st, q, (int)gx));
         IFL_LAUNCH_CHECK();

@@ -28,7 +28,7 @@ extern "C" int ifl_linear8_fwd(const void* x, int xtype, int64_t x_rs, int64_t x
     xtype &= ~IFL_P_8BIT;
     IFL_CHECK_ARG(sizes_ok(M, N, K), IFL_EINVAL, "linear8_fwd: %lld x %lld x %lld", (long long)M, (long long)N, (long long)K);
     IFL_CHECK_ARG(b8_type_ok(xtype) && b8_type_ok(wtype) && (!bias || b8_type_ok(btype)), IFL_EINVAL, "linear8_fwd: element types");
-    IFL_CHECK_ARG(M <= PRODUCT_ROWS && N <= PRODUCT_ROWS && code_ld(K) < PRODUCT_LD, IFL_ENOTSUP, "linear8_fwd: %lld x %lld x %lld", (long long)M, (long long)N, (long long)K);
+    IFL_CHECK_ARG(M <= PRODUCT_ROWS && N <= PRODUCT_ROWS && code_ld(K) < PRODUCT_LD && b8_matmul_fits(M, N, K), IFL_ENOTSUP, "linear8_fwd: %lld x %lld x %lld", (long long)M, (long long)N, (long long)K);
     if (M == 0) return 0;
     IFL_CHECK_ARG(x && w && codes && scales && y, IFL_EINVAL, "linear8_fwd: null pointer");
     IFL_CHECK_ARG(w_rs == 1 || w_cs == 1 || N == 1, IFL_EINVAL, "linear8_fwd: strides of w");
@@ -61,7 +61,7 @@ extern "C" int ifl_linear8_bwd(const void* dy, int xtype, int64_t ldy, const uin
     xtype &= ~IFL_P_8BIT;
     IFL_CHECK_ARG(sizes_ok(M, N, K), IFL_EINVAL, "linear8_bwd: %lld x %lld x %lld", (long long)M, (long long)N, (long long)K);
     IFL_CHECK_ARG(b8_type_ok(xtype) && b8_type_ok(wtype) && b8_fmt_ok(gfmt) && (!db || b8_type_ok(dbtype)), IFL_EINVAL, "linear8_bwd: types");
-    IFL_CHECK_ARG(M <= PRODUCT_ROWS && (!dx || (K <= PRODUCT_ROWS && code_ld(N) < PRODUCT_LD)) && (!(dw || db) || (N <= WGRAD_COLS && ldy < PRODUCT_LD)) && (!dw || K <= WGRAD_COLS),
+    IFL_CHECK_ARG(M <= PRODUCT_ROWS && (!dx || (K <= PRODUCT_ROWS && code_ld(N) < PRODUCT_LD && b8_matmul_fits(M, K, N))) && (!(dw || db) || (N <= WGRAD_COLS && ldy < PRODUCT_LD)) && (!dw || K <= WGRAD_COLS),
                   IFL_ENOTSUP, "linear8_bwd: %lld x %lld x %lld, rows of dy %lld apart", (long long)M, (long long)N, (long long)K, (long long)ldy);
     IFL_CHECK_ARG(M == 0 || (dy && (w || !dx) && ((codes && scales) || !dw)), IFL_EINVAL, "linear8_bwd: null pointer");
     IFL_CHECK_ARG(M <= 1 || ldy >= N, IFL_EINVAL, "linear8_bwd: rows of dy %lld apart", (long long)ldy);

@@ -506,12 +506,21 @@ int mm8_launch(MM8 q, const Plan& p, bool exact, hipStream_t st)
     return 0;
 }
 
+// a launch has fewer than 2^32 threads
+bool mm8_fits(int64_t M, int64_t N, int64_t K)
+{
+    if (M < 1) return true;
+    const Plan p = mm8_plan(M, N, K);
+    const int64_t blocks = p.kind ? (N + 15) / 16 : ((M + p.tile - 1) / p.tile) * ((N + p.tile - 1) / p.tile) + 7;
+    return blocks < (int64_t)1 << (p.kind ? 22 : p.tile == 256 ? 23 : 24);
+}
+
 int mm8_check(int64_t M, int64_t N, int64_t K, const uint8_t* b, int64_t ldb, const uint8_t* sb, int64_t lsb, const void* bias, int btype,
               const void* out, int otype, int64_t ldo)
 {
     IFL_CHECK_ARG(b8_type_ok(otype) && (!bias || b8_type_ok(btype)), IFL_EINVAL, "block8 product: element types");
     IFL_CHECK_ARG(M >= 0 && N >= 1 && K >= 1, IFL_EINVAL, "block8 product: %lld x %lld x %lld", (long long)M, (long long)N, (long long)K);
-    IFL_CHECK_ARG(K <= 0x7ffffc00 && M <= 0x3fffffff && N <= 0x3fffffff, IFL_ENOTSUP, "block8 product: %lld x %lld x %lld", (long long)M, (long long)N, (long long)K);
+    IFL_CHECK_ARG(K <= 0x7ffffc00 && M <= 0x3fffffff && N <= 0x3fffffff && mm8_fits(M, N, K), IFL_ENOTSUP, "block8 product: %lld x %lld x %lld", (long long)M, (long long)N, (long long)K);
     if (M == 0) return 0;
     const int KB = ifl_cdiv((int)K, B8_BLK);
     IFL_CHECK_ARG(b && sb && out, IFL_EINVAL, "block8 product: null pointer");
@@ -523,6 +532,8 @@ int mm8_check(int64_t M, int64_t N, int64_t K, const uint8_t* b, int64_t ldb, co
 }
 
 }  // namespace
+
+bool b8_matmul_fits(int64_t M, int64_t N, int64_t K) { return mm8_fits(M, N, K); }
 
 extern "C" int64_t ifl_block8_matmul_scratch_floats(int64_t M, int64_t N, int64_t K, int)
 {

@@ -152,3 +152,17 @@ def test_layer_refuses_what_its_backward_pass_would():
     block8._backward_reaches((1 << 22) - 1, (1 << 22) - 1, 1, 1, 1)
     block8._backward_reaches(8, 1 << 22, 1, 0, 1)
     block8._backward_reaches((1 << 23) - 16, 1 << 22, 1, 0, 0)
+
+
+@pytest.mark.parametrize("call, args", [
+    # (more than 2^32 threads)
+    ("ifl_block8_matmul", (16, 64, 16, 4, 0, 16, 64, 16, 4, 0, None, 0, 16, 0, 1 << 26, None, 1, 1 << 26, 64, None)),
+    ("ifl_block8_matmul", (16, 64, 16, 4, 0, 16, 64, 16, 4, 0, None, 0, 16, 0, 1 << 17, None, 1 << 23, 1 << 17, 64, None)),
+    ("ifl_block8_linear", (16, 0, 64, 16, 64, 16, 4, 0, None, 0, 16, 1 << 26, 16, 1, 1 << 26, 64, None)),
+    ("ifl_linear8_fwd", (16, 0, 64, 1, 16, 0, 64, 1, None, 0, 16, 16, 16, 16, 4, 1 << 26, 64, None)),
+    ("ifl_linear8_bwd", (16, 0, 64, 16, 16, 16, 0, 64, 1, 0, 16, None, None, 0, 16, 4, 64, 1 << 26, None)),
+    ("ifl_block8_quantize", (16, 0, 1, 1 << 30, 16, 16, 16, 4, 1 << 30, 2, 0, None)),
+])
+def test_library_refuses_what_no_launch_holds(call, args):
+    with pytest.raises(NotImplementedError):
+        hip.check(getattr(hip.lib(), call)(*args), call)
