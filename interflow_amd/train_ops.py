@@ -197,7 +197,11 @@ def conv2d_ring(srcs, real_channels, weight, bias=None, checkpoints=None):
     if checkpoints is not None:
         assert len(checkpoints) == len(srcs)
         for s, ck in zip(srcs, checkpoints):
-            assert ck is None or tuple(ck.shape) == tuple(s.shape), (tuple(ck.shape), tuple(s.shape))
+            if ck is None:
+                continue
+            if not isinstance(ck, Checkpoint8):
+                raise TypeError(f"conv2d_ring checkpoints: expected a Checkpoint8 or None, got {type(ck).__name__}")
+            assert tuple(ck.shape) == tuple(s.shape) and ck.raw.device == s.device, (tuple(ck.shape), ck.raw.device, tuple(s.shape), s.device)
     return _ConvRing.apply(weight, bias, tuple(real_channels), checkpoints, *srcs)
 
 

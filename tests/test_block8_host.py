@@ -166,3 +166,14 @@ def test_layer_refuses_what_its_backward_pass_would():
 def test_library_refuses_what_no_launch_holds(call, args):
     with pytest.raises(NotImplementedError):
         hip.check(getattr(hip.lib(), call)(*args), call)
+
+
+def test_convolution_refuses_what_is_no_checkpoint_of_its_source():
+    x, w = torch.zeros(1, 6, 6, 32), torch.zeros(8, 32, 1, 1)
+    ck = train_ops.Checkpoint8(train_ops.Checkpoint8.room(x.shape, x), x.shape, torch.ones(32))
+    for bad in (x, 8, "e4m3"):
+        with pytest.raises(TypeError):
+            train_ops.conv2d_ring([x], [32], w, checkpoints=[bad])
+    for bad in ([], [ck, ck], [train_ops.Checkpoint8(ck.raw, torch.Size((1, 6, 5, 32)), torch.ones(32))], [train_ops.Checkpoint8(ck.raw.to("meta"), x.shape, torch.ones(32))]):
+        with pytest.raises(AssertionError):
+            train_ops.conv2d_ring([x], [32], w, checkpoints=bad)
