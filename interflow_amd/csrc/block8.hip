@@ -178,8 +178,8 @@ void an_relu8_bwd_kernel(const float* __restrict__ g, const uint8_t* __restrict_
 constexpr int AN8_BLOCKS = 1024;                                         // most blocks (partial sums) of the backward pass
 
 // out[k] = exp(logs[k mod C]) sum over blocks of part[blk][k].  Workgroup = 16 k, 64 threads to each, which take every 64th block and
-// meet in LDS in a fixed order: a thread's loads are all under way together (979 blocks of 128: 4.8 us; a wave to each k, whose
-// lanes read far apart, 7.0).
+// meet in LDS in a fixed order: a thread's loads are all under way together (979 blocks of 128: 3.9 to 4.7 us; a loop over them 4.8; a
+// wave to each k, whose lanes read far apart, 7.0).
 __global__ __launch_bounds__(1024)
 void an_relu8_reduce_kernel(const float* __restrict__ part, int nblk, const float* __restrict__ logs, float* __restrict__ dbias,
                             float* __restrict__ dlogs, int C)
@@ -187,11 +187,14 @@ void an_relu8_reduce_kernel(const float* __restrict__ part, int nblk, const floa
     __shared__ float red[64][17];
     const int i = threadIdx.x & 15, r = threadIdx.x >> 4, k = blockIdx.x * 16 + i;       // (2 C is a multiple of 16)
     float q[4] = {};
-    float v[AN8_BLOCKS / 64];
+    if (nblk <= 64) q[0] = r < nblk ? part[(int64_t)r * 2 * C + k] : 0.f;
+    else {
+        float v[AN8_BLOCKS / 64];
 #pragma unroll
-    for (int e = 0; e < AN8_BLOCKS / 64; ++e) v[e] = part[(int64_t)min(r + 64 * e, nblk - 1) * 2 * C + k];
+        for (int e = 0; e < AN8_BLOCKS / 64; ++e) v[e] = part[(int64_t)min(r + 64 * e, nblk - 1) * 2 * C + k];
 #pragma unroll
-    for (int e = 0; e < AN8_BLOCKS / 64; ++e) q[e & 3] += r + 64 * e < nblk ? v[e] : 0.f;
+        for (int e = 0; e < AN8_BLOCKS / 64; ++e) q[e & 3] += r + 64 * e < nblk ? v[e] : 0.f;
+    }
     float t = (q[0] + q[1]) + (q[2] + q[3]);
     auto pairs = [](const float (&u)[8]) { return ((u[0] + u[4]) + (u[2] + u[6])) + ((u[1] + u[5]) + (u[3] + u[7])); };
     red[r][i] = t;

@@ -78,3 +78,19 @@ def test_8bit_instructions_on_request(M, N, K, dtype):
     assert bool(((block8.linear(x, b, exact=False).double() - ref).abs() <= tol).all())
     y = train_ops.linear8(x, vb.float(), exact=False)
     assert bool(((y.double() - qx @ R.values(vb).t()).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("M", [5, 100, 2040])
+@pytest.mark.parametrize("ea, eb", [(-110, 60), (100, -126), (-60, -60), (60, 60), (-126, 126)])
+def test_products_of_far_scales(M, ea, eb):
+    """Whole numbers times powers of two near the ends of the range: exact as long as float32 has every partial sum, that is where the
+    products' magnitudes add up to less than 2^128 (at 2^60 times 2^60: to less than 256)."""
+    g = gen(M)
+    K = 264 if M < 2000 else 1500
+    a, b = torch.randint(-3, 4, (M, K), generator=g).float().cuda(), torch.randint(-3, 4, (M, K), generator=g).float().cuda()
+    p, q = block8.quantize(a * 2.0 ** ea), block8.quantize(b * 2.0 ** eb)
+    assert torch.equal(R.of(p), a.double() * 2.0 ** ea)
+    ref = (a.double() @ b.double().t()) * 2.0 ** (ea + eb)
+    held = (a.double().abs() @ b.double().abs().t()) * 2.0 ** (ea + eb) < 2.0 ** 128
+    got = block8.matmul(p, q, dtype=torch.float32).double()
+    assert torch.equal(torch.where(held, got, 0.0), torch.where(held, ref, 0.0)) and (bool(held.all()) or ea + eb == 120)
