@@ -8,7 +8,9 @@
 // every scale is applied by the instruction, exactly, and what it returns is summed in float32.  But within 8 products it drops what is
 // below 2^-13 of the largest (measured): a result is off by up to 7 2^-13 of sum |a b|, and in the 2-norm by 4.1e-5 of itself for
 // activations with outliers and spread, 1.5e-5 for normal values (K = 4096).  Rounding to float16 adds 2.1e-4, to bfloat16 1.7e-3; but
-// where large products cancel, what they leave is lost.  Twice the rate: 8192 x 8192 x 4096 bf16 240 us, exact 451.
+// where large products cancel, what they leave is lost.  Twice the rate: 8192 x 8192 x 4096 bf16 237 us, exact 444 (1.24 PFLOP/s; a large
+// bf16 library product on this card 1.34); 16384 x 2048 x 2048 67 and 121, 512 x 2048 x 2048 7.0 and 11.8, 1 x 4096 x 4096 4.9 and 5.1.  Times
+// quoted below are of the 8-bit instructions unless they say exact or float32: what they compare is the same for both.
 //
 // Operands: the instruction's first is B (the n side) and its second A (the m side), so that a lane ends up with four
 // neighbouring n of one m: a contiguous store.
@@ -126,7 +128,7 @@ __device__ __forceinline__ void mm8_part(const MM8& q, const f32x4 (&acc)[NF][MF
 // Waves WN x WM; a wave has NF x MF fragments of 16 x 16.  Row r of n-fragment f is row 16 G (f / G) + 4 G (r / 4) + 4 (f % G) +
 // r % 4 of the wave's: so the four values a lane gets from each of G fragments are 4 G neighbours of one output row, and 16 bytes
 // (G = 2 for 16-bit results, 1 for float32): four lanes' stores fill 64 bytes of a row.  With twice as many neighbours to a lane each
-// store left gaps for the next (16384 x 2048 x 2048: 69.3 us instead of 67.3, float32 169 instead of 144).
+// store left gaps for the next (16384 x 2048 x 2048: 69.3 us instead of 67.3, float32 in tiles of 128 169 instead of 144).
 //
 // Workgroups go to the 8 XCDs in turn; an XCD takes a contiguous run of tiles, in groups of 8 along m, so that the 32 tiles
 // it works on at a time share rows of both operands in its own L2.
@@ -446,7 +448,7 @@ void mm8_skinny_kernel(MM8 q)
 // 30.7, 2048 x 2048 18.5 / 18.4 / 33, 16384 x 512 35.6 / 25.5 / 33.8, 3584 x 3584 52.8 / 43.4 / 36.3, 8192 x 2048 69.2 / 47.7 / 39.0, 5000 x 1000
 // 24.9 / 22.6, and at K = 4096 48.1 / 37.7.  A product of few tiles and a long K is split along K.
 // The skinny kernel quantizes the m side itself where that is at most 32768 values: then it is the faster way, in a graph (1 x 2048 x
-// 2048: 3.5 us, 6.9 with a launch for it; 16 x 2048 x 2048: 6.2 and 7.3) and out of one (9 and 13.6).
+// 2048: 3.5 us, 6.9 with a launch for it; 16 x 2048 x 2048: 5.8 and 7.3, exact too) and out of one (9 and 13.6).
 bool mm8_own(int64_t M, int64_t K) { return M <= 16 && M * K <= 32768; }
 struct Plan { int kind, tile, split, ksteps; };
 Plan mm8_plan(int64_t M, int64_t N, int64_t K)
