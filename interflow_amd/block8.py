@@ -202,11 +202,16 @@ class Block8:
             return self
         codes, scales, rows, cols = self._codes, self._scales, self.rows, self.cols
         blocks = (cols + 127) // 128
-        if codes.shape != (rows, cols) or scales.shape != (rows, blocks) or codes.get_device() != self._dev or scales.get_device() != self._dev:
+        dev, (cr, cc), (sr, sc) = self._dev, codes.stride(), scales.stride()
+        if codes.shape != (rows, cols) or scales.shape != (rows, blocks) or codes.get_device() != dev or scales.get_device() != dev:
             raise RuntimeError(f"{self}: its tensors were given another shape or device: {tuple(codes.shape)} on {codes.device}, {tuple(scales.shape)} on {scales.device}")
-        if not (_rows_apart(codes) and _rows_apart(scales)):
+        if cc != 1 and cols > 1 or sc != 1 and blocks > 1:
             return self._copy()
-        self._cp, self._ldc, self._sp, self._lds = codes.data_ptr(), _ld(codes), scales.data_ptr(), _ld(scales)
+        if rows <= 1:
+            cr, sr = cols, blocks
+        elif cr < cols or sr < blocks:
+            return self._copy()
+        self._cp, self._ldc, self._sp, self._lds = codes.data_ptr(), cr, scales.data_ptr(), sr
         return self
 
     def _copy(self):
