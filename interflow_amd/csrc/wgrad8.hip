@@ -42,22 +42,23 @@ struct WG8 {
 
 // The next of the bf16 terms whose sum is a value, as a float with 16 low zero bits: its leading 8 significant bits; x becomes what is
 // left.  What is not finite is the first term alone.  (FIRST; of bf16 the first term is the value.)
-// ALL: no term of a value that is not 0 is 0, for a checkpoint with infinities (e5m2), which a zero term would turn into NaN.  Where
-// nothing is left 2^-110 + 2^-126 is, two terms more, or 2^-126 after the second: at most 2^-33 of the value, which is under what
-// the sums keep and leaves exact ones exact.  Values below 2^-77 go without (there an infinity may still become NaN).
-template <bool FIRST, bool ALL, class T>
-__device__ __forceinline__ uint32_t wg8_term(float& x, bool last) {
+template <bool FIRST, class T>
+__device__ __forceinline__ uint32_t wg8_term(float& x) {
     if constexpr (sizeof(T) == 2 && !__is_same(T, _Float16)) return __float_as_uint(x);
     if (FIRST) x = __builtin_canonicalizef(x);                           // (a NaN has a high bit set)
-    uint32_t t = __float_as_uint(x) & 0xffff0000u;
-    float left = x - __uint_as_float(t);
-    if constexpr (ALL) {
-        const float more = FIRST ? 0x1p-110f + 0x1p-126f : 0x1p-126f, least = FIRST ? 0x1p-77f : 0x1p-100f;
-        // (what is left of a value of at least `least` is more than `more`, or nothing; of an infinity it is NaN, which the maximum drops)
-        if (!last) left = copysignf(fmaxf(fabsf(left), fabsf(x) >= least ? more : 0.f), x);
-    } else if (FIRST) left = left == left ? left : 0.f;
-    x = left;
+    const uint32_t t = __float_as_uint(x) & 0xffff0000u;
+    x -= __uint_as_float(t);
+    if (FIRST) x = x == x ? x : 0.f;
     return t;
+}
+
+// Two bf16 values, zeros in place of infinities.  An infinity of a checkpoint meets the first term of a gradient only: the others may be zero,
+// and infinity times zero is NaN.
+__device__ __forceinline__ uint32_t wg8_finite2(uint32_t w) {
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    const u16x2 other = __builtin_bit_cast(u16x2, (w & 0x7fff7fffu) ^ 0x7f807f80u);      // 0 where it is one
+    const u16x2 keep = (u16x2)0 - __builtin_elementwise_min(other, (u16x2)1);
+    return w & __builtin_bit_cast(uint32_t, keep);
 }
 
 template <class TW>
@@ -105,7 +106,7 @@ __device__ __forceinline__ int wg8_row(int gg, int e) { return (gg >> 2) * 32 + 
 // 8-bit blocks as well.  The next x_blocks restore codes.  The others take up to 256 columns of cs_rows rows of dy, with column
 // sums on the way that are joined in LDS in a fixed order, and dy's terms, if the product does not read it in place.  (16384 x 2048,
 // both operands, bf16: 30 us; with dy's blocks 43, 25 more on its own; with 2048 x 2048 weights 47, 19 more on their own.)
-template <class T, int NP, bool QUANT, bool ALL, class TW>
+template <class T, int NP, bool QUANT, class TW>
 __global__ __launch_bounds__(256, NP > 1 ? 2 : 3)
 void wgrad8_prepare_kernel(WG8 q)
 {
@@ -209,8 +210,8 @@ void wgrad8_prepare_kernel(WG8 q)
                 for (int i = 0; i < 8; ++i)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const uint32_t lo = k ? wg8_term<false, ALL, T>(v[2 * e][i], k == NP - 1) : wg8_term<true, ALL, T>(v[2 * e][i], k == NP - 1);
-                        const uint32_t hi = k ? wg8_term<false, ALL, T>(v[2 * e + 1][i], k == NP - 1) : wg8_term<true, ALL, T>(v[2 * e + 1][i], k == NP - 1);
+                        const uint32_t lo = k ? wg8_term<false, T>(v[2 * e][i]) : wg8_term<true, T>(v[2 * e][i]);
+                        const uint32_t hi = k ? wg8_term<false, T>(v[2 * e + 1][i]) : wg8_term<true, T>(v[2 * e + 1][i]);
                         t[i][e] = (int)__builtin_amdgcn_perm(hi, lo, 0x07060302u);       // the high halves
                         __builtin_amdgcn_sched_barrier(0);
                     }
@@ -247,7 +248,7 @@ void wgrad8_prepare_kernel(WG8 q)
 // all workgroups ask for at the same time take to come from memory.
 template <int V> struct Int { static constexpr int value = V; };
 
-template <int NP, bool TR, int TN, int TK, int WN, int WK>
+template <int NP, bool TR, bool INF, int TN, int TK, int WN, int WK>
 __global__ __launch_bounds__(64 * WN * WK)
 void wgrad8_kernel(WG8 q)
 {
@@ -337,6 +338,15 @@ void wgrad8_kernel(WG8 q)
         if constexpr (PL.value == 0) {
 #pragma unroll
             for (int f = 0; f < KF; ++f) x[f] = *(const bf16x8*)(xs + rx * XB + xa + f * 256);
+        }
+        if constexpr (INF && PL.value == 1) {                            // (the terms after the first share what this leaves)
+#pragma unroll
+            for (int f = 0; f < KF; ++f) {
+                i32x4 w = __builtin_bit_cast(i32x4, x[f]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = (int)wg8_finite2((uint32_t)w[e]);
+                x[f] = __builtin_bit_cast(bf16x8, w);
+            }
         }
         // the next step's loads have come: those of the two behind it are newer
         constexpr int NEWER = YP * 2 + XP * (((PL.value + 2) % NP == 0) + (P3 == 0));
@@ -585,9 +595,8 @@ int b8_wgrad(int todo, const B8Quant* quant, const void* dy, int dytype, int64_t
         }
         const dim3 pg((unsigned)(q.w_blocks + q.x_blocks + y_blocks));
 #define WG8_P(TY, NP) do { \
-            if (!quant && fmt == IFL_Q_E5M2) hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_prepare_kernel<TY, NP, false, (NP > 1), float>), pg, dim3(256), 0, st, q); \
-            else if (!quant) hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_prepare_kernel<TY, NP, false, false, float>), pg, dim3(256), 0, st, q); \
-            else B8_DISPATCH(quant->wtype, hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_prepare_kernel<TY, NP, true, false, T>), pg, dim3(256), 0, st, q)); \
+            if (!quant) hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_prepare_kernel<TY, NP, false, float>), pg, dim3(256), 0, st, q); \
+            else B8_DISPATCH(quant->wtype, hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_prepare_kernel<TY, NP, true, T>), pg, dim3(256), 0, st, q)); \
         } while (0)
         if (dytype == IFL_T_F32) WG8_P(float, 3); else if (dytype == IFL_T_F16) WG8_P(_Float16, 2); else WG8_P(__bf16, 1);
         IFL_LAUNCH_CHECK();
@@ -598,9 +607,11 @@ int b8_wgrad(int todo, const B8Quant* quant, const void* dy, int dytype, int64_t
         q.tiles_k = (int)((K + p.tile - 1) / p.tile);
         q.per_xcd = (q.tiles_n * q.tiles_k * p.split + 7) / 8;
         const dim3 grid(8 * q.per_xcd);
+        const bool inf = fmt == IFL_Q_E5M2;                                // (only that format has infinities)
+#define WG8_L(NP, TR, INF, T, WN, WK) hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_kernel<NP, TR, INF, T, T, WN, WK>), grid, dim3(64 * WN * WK), 0, st, q)
 #define WG8_K(NP, TR) do { \
-        if (p.tile == 256) hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_kernel<NP, TR, 256, 256, 4, 2>), grid, dim3(512), 0, st, q); \
-        else hipLaunchKernelGGL(HIP_KERNEL_NAME(wgrad8_kernel<NP, TR, 128, 128, 2, 2>), grid, dim3(256), 0, st, q); \
+        if (p.tile == 256) { if (inf) WG8_L(NP, TR, (NP > 1), 256, 4, 2); else WG8_L(NP, TR, false, 256, 4, 2); } \
+        else if (inf) WG8_L(NP, TR, (NP > 1), 128, 2, 2); else WG8_L(NP, TR, false, 128, 2, 2); \
     } while (0)
         if (dytype == IFL_T_F32) WG8_K(3, false); else if (dytype == IFL_T_F16) WG8_K(2, false);
         else if (p.in_place) WG8_K(1, true); else WG8_K(1, false);

@@ -58,3 +58,15 @@ def test_whole_numbers_beside_infinities(dtype):
     dy = torch.randint(-9, 10, (M, N), generator=g).to(DT[dtype]).cuda()
     x = torch.randint(-3, 4, (M, K), generator=g).float().cuda()
     assert torch.equal(block8.weight_grad(dy, block8.quantize(x, "e5m2"))[0].double(), dy.double().t() @ x.double())
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("fmt", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("M", [2, 7, 33])
+def test_sums_that_cancel_are_zero(M, fmt, dtype):
+    g = gen(M)
+    dy = torch.randint(-2, 3, (M, 60), generator=g).to(DT[dtype]).cuda()
+    x = torch.randint(-2, 3, (M, 90), generator=g).float().cuda()
+    ref = dy.double().t() @ x.double()
+    assert int(((ref == 0) & ((dy != 0).double().t() @ (x != 0).double() > 0)).sum()) > 100
+    assert torch.equal(block8.weight_grad(dy, block8.quantize(x, fmt))[0].double(), ref)
