@@ -52,13 +52,14 @@ __device__ __forceinline__ uint32_t wg8_term(float& x) {
     return t;
 }
 
-// Two bf16 values, zeros in place of infinities.  An infinity of a checkpoint meets the first term of a gradient only: the others may be zero,
-// and infinity times zero is NaN.
+// Two bf16 values, the largest finite one in place of infinities.  An infinity of a checkpoint meets the first term of a gradient only: the
+// others may be zero, and infinity times zero is NaN; what they give instead has the first one's sign.  (As unsigned numbers negative
+// infinities are above all else but NaN, as signed ones positive ones are.)
 __device__ __forceinline__ uint32_t wg8_finite2(uint32_t w) {
     typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-    const u16x2 other = __builtin_bit_cast(u16x2, (w & 0x7fff7fffu) ^ 0x7f807f80u);      // 0 where it is one
-    const u16x2 keep = (u16x2)0 - __builtin_elementwise_min(other, (u16x2)1);
-    return w & __builtin_bit_cast(uint32_t, keep);
+    typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
+    const u16x2 u = __builtin_elementwise_min(__builtin_bit_cast(u16x2, w), (u16x2)(uint16_t)0xff7f);
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(i16x2, u), (i16x2)(int16_t)0x7f7f));
 }
 
 template <class TW>
