@@ -203,8 +203,10 @@ class Block8:
         codes, scales, rows, cols = self._codes, self._scales, self.rows, self.cols
         blocks = (cols + 127) // 128
         dev, (cr, cc), (sr, sc) = self._dev, codes.stride(), scales.stride()
-        if codes.shape != (rows, cols) or scales.shape != (rows, blocks) or codes.get_device() != dev or scales.get_device() != dev:
-            raise RuntimeError(f"{self}: its tensors were given another shape or device: {tuple(codes.shape)} on {codes.device}, {tuple(scales.shape)} on {scales.device}")
+        if codes.shape != (rows, cols) or scales.shape != (rows, blocks) or codes.get_device() != dev or scales.get_device() != dev \
+                or _FMT_OF.get(codes.dtype) != self._f or scales.dtype != torch.float8_e8m0fnu:
+            raise RuntimeError(f"{self}: its tensors were given another shape, type or device: {tuple(codes.shape)} {codes.dtype} on {codes.device}, "
+                               f"{tuple(scales.shape)} {scales.dtype} on {scales.device}")
         if cc != 1 and cols > 1 or sc != 1 and blocks > 1:
             return self._copy()
         if rows <= 1:

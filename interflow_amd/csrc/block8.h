@@ -6,8 +6,8 @@
 //     code = x 2^-e rounded to nearest even.
 // A power of two costs a floating code no precision, is exact to apply and to undo (a code times its scale is exact in bf16),
 // makes codes independent of how they were computed, and is what the scaled matrix instructions take (one byte per row and
-// 32 values).  |x| 2^-e <= F, so rounding never saturates; but next to float32's largest it rounds up to 2^128 (e4m3 from 248 2^120 on,
-// e5m2 from 30720 2^113), which is restored as infinity.  NaN has the code NaN; infinity keeps its sign in e5m2 and is NaN in
+// 32 values).  |x| 2^-e <= F, so rounding never saturates; but next to float32's largest it rounds up to 2^128 (e4m3 from 0.96875 2^128 on,
+// e5m2 from 0.9375 2^128), which is restored as infinity.  NaN has the code NaN; infinity keeps its sign in e5m2 and is NaN in
 // e4m3, which has none; neither takes part in m, so the other values of the block are what they would be without it.
 #pragma once
 #include "ifl_common.h"

@@ -69,3 +69,12 @@ def test_aligned_once(cols):
     before = torch.cuda.memory_stats()["allocation.all.allocated"]
     block8.linear(x[:1], a)
     assert torch.cuda.memory_stats()["allocation.all.allocated"] == before + 1          # (its result; the launch quantizes the row itself)
+
+
+def test_tensors_of_another_type_are_refused():
+    q = block8.quantize(rand(15, 30, 300))
+    codes, scales = q.codes.clone(), q.scales.clone()
+    p = block8.Block8(codes, scales)
+    codes.data = codes.view(torch.uint8).view(torch.float8_e5m2)
+    with pytest.raises(RuntimeError):
+        block8.dequantize(p)
