@@ -330,7 +330,7 @@ def linear(x, w: Block8, bias=None, exact: bool = True) -> torch.Tensor:
 def weight_grad(dy, q: Block8, dtype=torch.float32, bias_dtype=None, weight: bool = True):
     """(dw, db): dy [M, N]^T times the checkpoint q [M, K] -> dw [N, K] of `dtype` (None unless `weight`), and dy's column sums
     [N] of `bias_dtype` (None without one).  Products are exact (operands' bits below 2^-133 aside) and sums float32, in an order
-    that depends on the sizes only.  Both operands pass through scratch as bfloat16 terms: 2 bytes per code, 2 to 6 per gradient."""
+    that depends on the sizes only; an infinity of an e5m2 checkpoint gives infinities of its and the gradients' sign.  Both operands pass through scratch as bfloat16 terms: 2 bytes per code, 2 to 6 per gradient."""
     _real(dy, "weight_grad dy")
     _b8(q, "weight_grad checkpoint")
     assert dy.dim() == 2 and dy.shape[0] == q.rows and dy.shape[1] >= 1, (tuple(dy.shape), tuple(q.shape))
